@@ -22,7 +22,7 @@ STATUS_NAMES = {
 }
 
 # GgmlDType codes (fuel-ir/src/quantized.rs:36-76)
-F32, F16, Q8_0, Q4K, Q6K, Q8K = 0, 1, 8, 12, 14, 15
+F32, F16, Q8_0, Q4K, Q6K, Q8K, BF16 = 0, 1, 8, 12, 14, 15, 30
 
 
 class FuelRocmError(RuntimeError):
@@ -31,6 +31,18 @@ class FuelRocmError(RuntimeError):
     def __init__(self, status: int, msg: str):
         super().__init__(f"{STATUS_NAMES.get(status, status)}: {msg}")
         self.status = status
+
+
+class PagedKv(C.Structure):
+    """frq_paged_kv"""
+    _fields_ = [("dtype", C.c_int), ("n_pages", C.c_size_t), ("page_size", C.c_size_t), ("n_kv_heads", C.c_size_t),
+                ("head_dim", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class PagedBatch(C.Structure):
+    """frq_paged_batch"""
+    _fields_ = [("n_seqs", C.c_size_t), ("max_pages", C.c_size_t), ("rows", C.c_size_t), ("max_kv_len", C.c_size_t),
+                ("page_table", C.c_void_p), ("kv_len", C.c_void_p), ("row_start", C.c_void_p)]
 
 
 # Every exported symbol of include/fuel_rocm.h with its ctypes signature.
@@ -91,6 +103,10 @@ SIGNATURES = {
     "frq_swiglu_rows": (_i32, [_vp, _sz, _sz, _vp, _sz, _vp, _sz]),
     "frq_add": (_i32, [_vp, _sz, _vp, _vp]),
     "frq_gather_rows": (_i32, [_vp, _vp, _sz, _sz, _vp, _sz, _vp]),
+    "frq_paged_append": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz]),
+    "frq_paged_attention_workspace": (_sz, [_vp, _vp, _sz]),
+    "frq_paged_attention_decode": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, C.c_float, _vp, _sz, _vp, _sz]),
+    "frq_paged_attention_prefill": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, C.c_float, _vp, _sz, _vp, _sz]),
     "frq_block_isums": (_i32, [_vp, _i32, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
     "frq_fill_random_bits": (_i32, [_vp, _vp, _sz, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32]),
     "frq_fill_normal": (_i32, [_vp, _vp, _sz, C.c_uint64, C.c_uint32, C.c_float, C.c_float]),

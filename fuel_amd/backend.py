@@ -285,6 +285,88 @@ def qmatmul_f32_rocm_wrapper(inputs: Sequence[RocmStorage], outputs: Sequence[Ro
                             C.c_void_p(out.ptr), out.nbytes))
 
 
+# ---- a batch of sequences over a paged KV cache ----
+
+def _ptr(x) -> int:
+    """Device address of a RocmStorage, or the address itself (None: null)."""
+    return x.ptr if isinstance(x, RocmStorage) else int(x or 0)
+
+
+class PagedKvCache:
+    """Pools of KV pages [n_pages, n_kv_heads, page_size, head_dim] that a batch
+    of sequences shares (frq_paged_kv).  dtype: F16 or BF16.  k, v: device
+    addresses or storages of the caller's own pools; otherwise zeroed ones are
+    allocated."""
+
+    def __init__(self, dev: RocmDevice, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 dtype: int = N.F16, k=None, v=None):
+        if (k is None) != (v is None):
+            raise FuelRocmError(N.FRQ_INVALID, "PagedKvCache: k and v go together")
+        self.dev = dev
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = n_pages, page_size, n_kv_heads, head_dim
+        self.dtype = dtype
+        if k is None:
+            shape = (n_pages, n_kv_heads, page_size, head_dim)
+            k, v = dev.alloc(shape, np.uint16), dev.alloc(shape, np.uint16)
+            for s in (k, v):
+                check(lib().frq_memset(dev.handle, C.c_void_p(s.ptr), 0, s.nbytes))
+        self.k, self.v = k, v
+        self.struct = N.PagedKv(dtype, n_pages, page_size, n_kv_heads, head_dim, _ptr(k), _ptr(v))
+        self.ref = C.byref(self.struct)
+
+
+class PagedBatch:
+    """The sequences of a call and its packed rows (frq_paged_batch): page_table
+    [n_seqs, max_pages], kv_len [n_seqs] and row_start [n_seqs + 1] (None: one
+    row a sequence) are int32 in device memory, as storages or addresses."""
+
+    def __init__(self, page_table, kv_len, n_seqs: int, max_pages: int, rows: int | None = None, row_start=None,
+                 max_kv_len: int = 0):
+        self.n_seqs, self.max_pages, self.max_kv_len = n_seqs, max_pages, max_kv_len
+        self.rows = n_seqs if rows is None else rows
+        self.page_table, self.kv_len, self.row_start = page_table, kv_len, row_start
+        self.struct = N.PagedBatch(n_seqs, max_pages, self.rows, max_kv_len, _ptr(page_table), _ptr(kv_len),
+                                   _ptr(row_start))
+        self.ref = C.byref(self.struct)
+
+
+def paged_append(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, k, v, q_out, ldq: int = 0,
+                 ldk: int = 0, ldv: int = 0, ldqo: int = 0, rope_cos=None, rope_sin=None, rope_rows: int = 0) -> None:
+    """RoPE of the packed q and k rows (type dtype), rotated q to q_out, k and v
+    into the cache at each row's position (frq_paged_append).  Operands are
+    storages or device addresses; a leading dimension of 0 stands for packed
+    rows; rope_cos / rope_sin are [rope_rows, head_dim] f32 tables."""
+    wide, narrow = n_heads * cache.head_dim, cache.n_kv_heads * cache.head_dim
+    check(lib().frq_paged_append(cache.dev.handle, cache.ref, batch.ref, dtype, n_heads, _ptr(q), ldq or wide, _ptr(k),
+                                 ldk or narrow, _ptr(v), ldv or narrow, _ptr(rope_cos), _ptr(rope_sin), rope_rows,
+                                 _ptr(q_out), ldqo or wide))
+
+
+def paged_attention_workspace(cache: PagedKvCache, batch: PagedBatch, n_heads: int) -> int:
+    """Bytes of scratch the paged attention calls need for this batch."""
+    return int(lib().frq_paged_attention_workspace(cache.ref, batch.ref, n_heads))
+
+
+def _paged_attention(fn, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo) -> None:
+    wide = n_heads * cache.head_dim
+    check(fn(cache.dev.handle, cache.ref, batch.ref, dtype, n_heads, _ptr(q), ldq or wide, scale,
+             work.ptr if work is not None else None, work.nbytes if work is not None else 0, _ptr(out), ldo or wide))
+
+
+def paged_attention_decode(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
+                           work: RocmStorage | None = None, ldq: int = 0, ldo: int = 0) -> None:
+    """Attention of one new token per sequence over its cached rows
+    (frq_paged_attention_decode); work: paged_attention_workspace() bytes."""
+    _paged_attention(lib().frq_paged_attention_decode, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo)
+
+
+def paged_attention_prefill(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
+                            work: RocmStorage | None = None, ldq: int = 0, ldo: int = 0) -> None:
+    """Causal attention of packed prompt rows over the cache
+    (frq_paged_attention_prefill); work: paged_attention_workspace() bytes."""
+    _paged_attention(lib().frq_paged_attention_prefill, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo)
+
+
 # ---- synthetic inputs ----
 
 def fill_normal(dev: RocmDevice, shape, seed: int, stream: int, mean: float = 0.0, std: float = 1.0) -> RocmStorage:

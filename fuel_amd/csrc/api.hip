@@ -1422,6 +1422,156 @@ int frq_argmax_embed(frq_device* dev, const float* logits, size_t vocab, const f
     return FRQ_OK;
 }
 
+// ---- paged KV cache ----
+
+namespace {
+
+// The structs of a paged call as the kernels take them, or a refusal.
+int paged_args(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b, size_t n_heads, PagedKv* kvo,
+               PagedRows* ro) {
+    if (!kv || !b) return fail(FRQ_INVALID, "%s: null cache or batch", who);
+    if (kv->dtype != GGML_F16 && kv->dtype != GGML_BF16)
+        return fail(FRQ_UNSUPPORTED, "%s: cache dtype %d (supported: f16, bf16)", who, kv->dtype);
+    if (kv->head_dim != 64 && kv->head_dim != 128)
+        return fail(FRQ_UNSUPPORTED, "%s: head_dim=%zu (supported: 64, 128)", who, kv->head_dim);
+    const size_t ps = kv->page_size;
+    if (ps < 16 || ps > 1024 || (ps & (ps - 1)))
+        return fail(FRQ_UNSUPPORTED, "%s: page_size=%zu (a power of two, 16 .. 1024)", who, ps);
+    const size_t imax = 0x7fffffff;
+    if (kv->n_pages == 0 || kv->n_pages > imax || kv->n_kv_heads == 0 || kv->n_kv_heads > 65535)
+        return fail(FRQ_INVALID, "%s: n_pages=%zu n_kv_heads=%zu", who, kv->n_pages, kv->n_kv_heads);
+    if (n_heads == 0 || n_heads > 65535 || n_heads % kv->n_kv_heads)
+        return fail(FRQ_INVALID, "%s: n_heads=%zu is no multiple of n_kv_heads=%zu (up to 65535)", who, n_heads,
+                    kv->n_kv_heads);
+    if (b->n_seqs > imax / n_heads || b->rows > imax / n_heads - b->n_seqs)
+        return fail(FRQ_UNSUPPORTED, "%s: n_seqs=%zu rows=%zu n_heads=%zu", who, b->n_seqs, b->rows, n_heads);
+    if (!b->row_start && b->rows != b->n_seqs)
+        return fail(FRQ_INVALID, "%s: rows=%zu, n_seqs=%zu without row_start", who, b->rows, b->n_seqs);
+    if (b->max_pages > imax / ps) return fail(FRQ_UNSUPPORTED, "%s: max_pages=%zu page_size=%zu", who, b->max_pages, ps);
+    const size_t cap = b->max_pages * ps;
+    if (b->max_kv_len > cap)
+        return fail(FRQ_INVALID, "%s: max_kv_len=%zu > max_pages * page_size = %zu", who, b->max_kv_len, cap);
+    int log_ps = 4;
+    while (((size_t)1 << log_ps) < ps) log_ps++;
+    *kvo = PagedKv{kv->k, kv->v, (int)kv->n_pages, log_ps, (int)kv->n_kv_heads};
+    *ro = PagedRows{b->page_table, b->kv_len, b->row_start, (int)b->n_seqs, (int)b->max_pages, (int)b->rows,
+                    (int)(b->max_kv_len ? b->max_kv_len : cap)};
+    return FRQ_OK;
+}
+
+int paged_buffers(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b) {
+    if (!kv->k || !kv->v || !b->kv_len || (b->max_pages && !b->page_table))
+        return fail(FRQ_INVALID, "%s: null cache, page_table or kv_len", who);
+    if (!aligned16(kv->k) || !aligned16(kv->v)) return fail(FRQ_MISALIGNED, "%s: pages not 16-byte aligned", who);
+    if (!aligned4(b->page_table) || !aligned4(b->kv_len) || !aligned4(b->row_start))
+        return fail(FRQ_MISALIGNED, "%s: page_table, kv_len or row_start not 4-byte aligned", who);
+    return FRQ_OK;
+}
+
+// A row operand of `width` elements of type dtype, ld elements apart.
+int paged_operand(const char* who, const char* name, int dtype, const void* p, size_t width, size_t ld) {
+    const size_t size = dtype == GGML_F32 ? 4 : 2;
+    if (!p) return fail(FRQ_INVALID, "%s: null %s", who, name);
+    if (ld < width || ld > 0x7fffffff) return fail(FRQ_INVALID, "%s: %s rows %zu apart, %zu wide", who, name, ld, width);
+    if (!aligned16(p) || ld * size % 16)
+        return fail(FRQ_MISALIGNED, "%s: %s must be 16-byte aligned, its rows a multiple of 16 bytes apart", who, name);
+    return FRQ_OK;
+}
+
+int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
+                    size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes, void* out,
+                    size_t ldo) {
+    int rc;
+    PagedAttendArgs a{};
+    if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
+    if (!paged_types(kv->dtype, dtype))
+        return fail(FRQ_UNSUPPORTED, "%s: dtype %d over a cache of dtype %d", who, dtype, kv->dtype);
+    const bool none = b->n_seqs == 0 || b->rows == 0;
+    const size_t need = frq_paged_attention_workspace(kv, b, n_heads);
+    if (!none && work_bytes < need)
+        return fail(FRQ_WORKSPACE, "%s: workspace %zu < %zu bytes", who, work_bytes, need);
+    if (!none && need && !work) return fail(FRQ_INVALID, "%s: null workspace", who);
+    if (!none && need && !aligned16(work)) return fail(FRQ_MISALIGNED, "%s: work not 16-byte aligned", who);
+    if (!none && (rc = paged_buffers(who, kv, b))) return rc;
+    if (!none && (rc = paged_operand(who, "q", dtype, q, n_heads * kv->head_dim, ldq))) return rc;
+    if (!none && (rc = paged_operand(who, "out", dtype, out, n_heads * kv->head_dim, ldo))) return rc;
+    DevGuard guard(dev);
+    if ((rc = use_device(dev)) || none) return rc;
+    a.n_heads = (int)n_heads;
+    a.q = q;
+    a.ldq = (int)ldq;
+    a.scale = scale;
+    a.out = out;
+    a.ldo = (int)ldo;
+    HIP_TRY(launch_paged_attend(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
+    return FRQ_OK;
+}
+
+}  // namespace
+
+int frq_paged_append(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype, size_t n_heads,
+                     const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv,
+                     const float* rope_cos, const float* rope_sin, size_t rope_rows, void* q_out, size_t ldqo) {
+    const char* who = "paged_append";
+    int rc;
+    PagedAppendArgs a{};
+    if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
+    if (!paged_types(kv->dtype, dtype))
+        return fail(FRQ_UNSUPPORTED, "%s: dtype %d into a cache of dtype %d", who, dtype, kv->dtype);
+    const bool none = b->n_seqs == 0 || b->rows == 0;
+    if (!none && (rc = paged_buffers(who, kv, b))) return rc;
+    if (!q != !q_out) return fail(FRQ_INVALID, "%s: q and q_out go together", who);
+    if (!rope_cos != !rope_sin) return fail(FRQ_INVALID, "%s: rope_cos and rope_sin go together", who);
+    if (rope_cos && (rope_rows == 0 || rope_rows > 0x7fffffff))
+        return fail(FRQ_INVALID, "%s: rope_rows=%zu", who, rope_rows);
+    if (!aligned16(rope_cos) || !aligned16(rope_sin))
+        return fail(FRQ_MISALIGNED, "%s: rope tables not 16-byte aligned", who);
+    const size_t hd = kv->head_dim, kw = kv->n_kv_heads * hd;
+    if (!none && q && (rc = paged_operand(who, "q", dtype, q, n_heads * hd, ldq))) return rc;
+    if (!none && q && (rc = paged_operand(who, "q_out", dtype, q_out, n_heads * hd, ldqo))) return rc;
+    if (!none && (rc = paged_operand(who, "k", dtype, k, kw, ldk))) return rc;
+    if (!none && (rc = paged_operand(who, "v", dtype, v, kw, ldv))) return rc;
+    DevGuard guard(dev);
+    if ((rc = use_device(dev)) || none) return rc;
+    a.n_heads = (int)n_heads;
+    a.q = q;
+    a.ldq = (int)ldq;
+    a.k = k;
+    a.ldk = (int)ldk;
+    a.v = v;
+    a.ldv = (int)ldv;
+    a.cos = rope_cos;
+    a.sin = rope_sin;
+    a.rope_rows = (int)rope_rows;
+    a.q_out = q_out;
+    a.ldqo = (int)ldqo;
+    HIP_TRY(launch_paged_append(kv->dtype, dtype, (int)hd, a, dev->stream));
+    return FRQ_OK;
+}
+
+size_t frq_paged_attention_workspace(const frq_paged_kv* kv, const frq_paged_batch* b, size_t n_heads) {
+    PagedKv k;
+    PagedRows r;
+    if (paged_args("paged_attention_workspace", kv, b, n_heads, &k, &r)) return 0;
+    return 0;
+}
+
+int frq_paged_attention_decode(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
+                               size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes,
+                               void* out, size_t ldo) {
+    if (b && b->row_start)
+        return fail(FRQ_INVALID, "paged_attention_decode: one row a sequence (row_start must be NULL)");
+    return paged_attention("paged_attention_decode", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes, out,
+                           ldo);
+}
+
+int frq_paged_attention_prefill(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
+                                size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes,
+                                void* out, size_t ldo) {
+    return paged_attention("paged_attention_prefill", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes, out,
+                           ldo);
+}
+
 int frq_fill_random_bits(frq_device* dev, uint32_t* y, size_t n, uint64_t start, uint64_t seed, uint32_t base,
                          uint32_t stream) {
     DevGuard guard(dev);

@@ -19,7 +19,7 @@ constexpr int Q6K_BYTES = 210;
 constexpr int Q8K_BYTES = 292;
 
 // GgmlDType codes (fuel-ir/src/quantized.rs:36-76).
-enum : int { GGML_F32 = 0, GGML_F16 = 1, GGML_Q8_0 = 8, GGML_Q4K = 12, GGML_Q6K = 14, GGML_Q8K = 15 };
+enum : int { GGML_F32 = 0, GGML_F16 = 1, GGML_Q8_0 = 8, GGML_Q4K = 12, GGML_Q6K = 14, GGML_Q8K = 15, GGML_BF16 = 30 };
 
 __device__ __forceinline__ float f16_to_f32(uint32_t bits) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "common.hpp"
+#include "paged.hpp"
 
 namespace frq {
 
@@ -257,5 +258,37 @@ hipError_t launch_swiglu_rows(const float* gu, int ldgu, int M, int f, float* h,
 hipError_t launch_add_rows(const float* x, float* y, size_t n, hipStream_t s);
 hipError_t launch_gather_rows(const float* table, int rows, int dim, const int* ids, int M, float* out,
                               hipStream_t s);
+
+// paged.hip: operators of a batch of sequences over a paged KV cache.  dtype is
+// the type of q, k, v and the outputs, kv_dtype the cache's; hd 64 or 128.
+bool paged_types(int kv_dtype, int dtype);
+struct PagedAppendArgs {
+    PagedKv kv;
+    PagedRows rows;
+    int n_heads;
+    const void* q;  // null: keys and values only
+    int ldq;
+    const void* k;
+    int ldk;
+    const void* v;
+    int ldv;
+    const float* cos;  // null: no rotation
+    const float* sin;
+    int rope_rows;
+    void* q_out;
+    int ldqo;
+};
+hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppendArgs& p, hipStream_t s);
+struct PagedAttendArgs {
+    PagedKv kv;
+    PagedRows rows;
+    int n_heads;
+    const void* q;
+    int ldq;
+    float scale;
+    void* out;
+    int ldo;
+};
+hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 
 }  // namespace frq

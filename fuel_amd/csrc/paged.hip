@@ -1,0 +1,464 @@
+// Operators of a batch of sequences over a paged KV cache (paged.hpp):
+//
+//   append     RoPE of the packed q and k rows (rotate-half with the f32
+//              tables, as rope_append_rows), k and v rounded once to the
+//              cache's type and written at each row's position
+//   attention  of packed rows over the cache rows 0 .. each row's position,
+//              n_heads / kv_heads query heads to a KV head
+//
+// Attention, one wavefront and 16 query rows of one KV head.  A sequence's
+// rows and the G = n_heads / kv_heads query heads of a KV head are one list of
+// n * G query rows (row i is head i % G of packed row i / G), so that grouped
+// heads fill the MFMA's columns and share the K and V loads.  For 32 keys at a
+// time:
+//   S^T (keys x rows) = K . Q^T on v_mfma_f32_16x16x32, two groups of 16 keys.
+//     The C layout leaves lane 16 g + r keys 4g + i (i < 4) of each group for
+//     row r: with both groups its 8 values of the PV product's k index, in an
+//     order that V's loads follow.  P never moves between lanes.
+//   p = e^(s - m), running maximum m and sum l per row (l per lane until the end)
+//   O^T (dims x rows) += V^T . P^T: tile t takes the dims VW * r + t, so that
+//     lane 16 g + r's loads of its 8 keys, VW dims from VW * r, hold the A
+//     operand of all VW tiles, put together by byte permutes.
+// f32 activations: q and p are split into parts of the cache's type (2 of f16,
+// 3 of bf16), which keeps products and sums at f32's precision.  f16 parts
+// take q scaled by a power of two per row (exact) so that no part leaves f16's
+// range.  16-bit activations: q as it is, p in two parts; their products cost
+// nothing here, where K and V bytes are the bound, and one part would add a
+// rounding as large as the output's own.
+// p carries a factor 2^PA_SHIFT, which l carries too: f16 parts of the many
+// small p of a long context keep steps of 2^-24 / 2^15 of the largest p
+// (2^15 < f16's largest, 65504).
+#include <hip/hip_runtime.h>
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "paged.hpp"
+
+namespace frq {
+
+namespace {
+
+constexpr int PA_WAVES = 4;
+constexpr float PA_SHIFT = 15.0f;
+
+template <class E, class T, int HD>
+struct Rows16 {
+    using P = PgElem<E>;
+    using v8 = typename P::v8;
+    static constexpr bool WIDE = std::is_same<T, float>::value;
+    static constexpr int NQ = WIDE ? P::SPLIT : 1;
+    static constexpr int NP = WIDE ? P::SPLIT : 2;
+    static constexpr int KS = HD / 32, VW = HD / 16;
+
+    v8 q[NQ][KS];
+    float factor;  // score = S^T * factor, in units of log2
+    int limit;     // the row's position; -1: it sees nothing
+    pg_f4 o[VW];
+    float m, l;
+
+    struct Block {
+        uint4 k[2][KS];
+        uint32_t v[8][VW / 2];
+    };
+
+    // Lane 16 g + r takes row r: dims 32 t + 8 g + e of x (null: a row of zeros).
+    __device__ void load_q(const T* x, float scale) {
+        const int g = (threadIdx.x & 63) >> 4;
+        float f[KS][8];
+#pragma unroll
+        for (int t = 0; t < KS; t++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[t][e] = 0.0f;
+        if (x) {
+#pragma unroll
+            for (int t = 0; t < KS; t++) {
+                T raw[8];
+                __builtin_memcpy(raw, __builtin_assume_aligned(x + 32 * t + 8 * g, 16), sizeof raw);
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[t][e] = (float)raw[e];
+            }
+        }
+        factor = fabsf(scale) * 1.4426950408889634f;
+        if (scale < 0.0f) {  // (the maximum is taken of scores with a positive factor)
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[t][e] = -f[t][e];
+        }
+        if constexpr (WIDE && std::is_same<E, _Float16>::value) {
+            float a = 0.0f;
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) a = fmaxf(a, fabsf(f[t][e]));
+            a = fmaxf(a, __shfl_xor(a, 16));
+            a = fmaxf(a, __shfl_xor(a, 32));
+            // (a row with an infinite value keeps it; its scores are no numbers anyway)
+            const int ex = a > 0.0f && a < __builtin_inff() ? min(120, max(-120, __builtin_amdgcn_frexp_expf(a))) : 0;
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) f[t][e] = __builtin_amdgcn_ldexpf(f[t][e], -ex);
+            factor = __builtin_amdgcn_ldexpf(factor, ex);
+        }
+#pragma unroll
+        for (int t = 0; t < KS; t++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float rest = f[t][e];
+#pragma unroll
+                for (int p = 0; p < NQ; p++) {
+                    q[p][t][e] = (E)rest;
+                    rest -= (float)q[p][t][e];
+                }
+            }
+    }
+
+    __device__ void start() {
+#pragma unroll
+        for (int t = 0; t < VW; t++) o[t] = pg_f4{0.f, 0.f, 0.f, 0.f};
+        // (a finite floor: a row that has seen nothing yet keeps m = -1e30, l = 0, o = 0)
+        m = -1e30f;
+        l = 0.0f;
+    }
+
+    // The loads of 32 keys: group a's 16 rows start at ka[a] / va[a].
+    __device__ void load(Block& b, const E* const (&ka)[2], const E* const (&va)[2]) const {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+                b.k[a][t] = *reinterpret_cast<const uint4*>(ka[a] + r * HD + 32 * t + 8 * g);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                __builtin_memcpy(b.v[4 * a + i], __builtin_assume_aligned(va[a] + (4 * g + i) * HD + VW * r, 2 * VW),
+                                 2 * VW);
+        }
+    }
+
+    // 32 keys from j0.  MASK: some key is past a row's position, past the
+    // sequence's length kv, or in a page that is none (bad).
+    template <bool MASK>
+    __device__ void step(Block& b, int j0, int kv, const bool (&bad)[2], const E* const (&va)[2]) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        float s[8], top = -__builtin_inff();
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            pg_f4 st = pg_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int p = NQ - 1; p >= 0; p--) st = P::mfma16(__builtin_bit_cast(v8, b.k[a][t]), q[p][t], st);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float v = st[i] * factor;
+                if constexpr (MASK) {
+                    if (bad[a]) v = pg_nan();
+                    if (j0 + 16 * a + 4 * g + i > limit) v = -__builtin_inff();
+                }
+                s[4 * a + i] = v;
+                top = fmaxf(top, v);
+            }
+        }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float mn = fmaxf(m, top);
+        const float c = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before: l = o = 0)
+        m = mn;
+        l *= c;
+        v8 pp[NP];
+        float pf[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            pf[i] = __builtin_amdgcn_exp2f(s[i] - mn + PA_SHIFT);
+            l += pf[i];
+            float rest = pf[i];
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                pp[p][i] = (E)rest;
+                rest -= (float)pp[p][i];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < VW; t++) o[t] *= c;
+        if constexpr (MASK) {
+            // keys that no row of the sequence may see: their rows hold anything
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const bool none = bad[i >> 2] || j0 + 16 * (i >> 2) + 4 * g + (i & 3) >= kv;
+#pragma unroll
+                for (int w = 0; w < VW / 2; w++) {
+                    if (none) b.v[i][w] = 0;
+                    odd |= pg_word_inf<E>(b.v[i][w]);
+                }
+            }
+            if (__any(odd)) {
+                // an infinite or NaN value in a key that some rows do not see:
+                // 0 * inf must not reach those rows, so each row adds only its own keys
+                for (int j = 0; j < 32; j++) {
+                    float p = pf[0];
+#pragma unroll
+                    for (int i = 1; i < 8; i++) p = (j >> 4) * 4 + (j & 3) == i ? pf[i] : p;
+                    p = __shfl(p, r + 16 * ((j >> 2) & 3));
+                    if (j0 + j <= limit) {
+                        const E* row = (j < 16 ? va[0] : va[1]) + (j & 15) * HD + 4 * VW * g;
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+#pragma unroll
+                            for (int t = 0; t < VW; t++) o[t][i] = fmaf(p, (float)row[VW * i + t], o[t][i]);
+                    }
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < VW; t++) {
+            const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;  // high or low halves of two words
+            uint4 a;
+            a.x = __builtin_amdgcn_perm(b.v[1][t >> 1], b.v[0][t >> 1], sel);
+            a.y = __builtin_amdgcn_perm(b.v[3][t >> 1], b.v[2][t >> 1], sel);
+            a.z = __builtin_amdgcn_perm(b.v[5][t >> 1], b.v[4][t >> 1], sel);
+            a.w = __builtin_amdgcn_perm(b.v[7][t >> 1], b.v[6][t >> 1], sel);
+#pragma unroll
+            for (int p = NP - 1; p >= 0; p--) o[t] = P::mfma16(__builtin_bit_cast(v8, a), pp[p], o[t]);
+        }
+    }
+
+    // The row's sum over the four lanes that share it.
+    __device__ void finish() {
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+    }
+};
+
+// The walk of one wavefront over keys [j0, j1) (j0 a multiple of 32) of a
+// sequence for the 16 rows of `a`: no row sees a key >= j1.
+template <class E, class T, int HD>
+__device__ void pa_walk(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int max_pages, int head, int j0,
+                        int j1, int kv, int all_see) {
+    const E* ka[2];
+    const E* va[2];
+    bool bad[2];
+    typename Rows16<E, T, HD>::Block b;
+    for (; j0 < j1; j0 += 32) {
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int j = j0 + 16 * g;
+            // (a group past the length has no page: its keys are masked)
+            const int page = j < kv ? table[j >> c.log_ps] : 0;
+            bad[g] = (unsigned)page >= (unsigned)c.n_pages;
+            const size_t at = (((size_t)(bad[g] ? 0 : page) * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1));
+            ka[g] = static_cast<const E*>(c.k) + at * HD;
+            va[g] = static_cast<const E*>(c.v) + at * HD;
+        }
+        a.load(b, ka, va);
+        if (j0 + 31 <= all_see && !bad[0] && !bad[1])
+            a.template step<false>(b, j0, kv, bad, va);
+        else
+            a.template step<true>(b, j0, kv, bad, va);
+    }
+}
+
+// One workgroup: 16 query rows of one KV head, workgroup tile * kv_heads + head
+// of the batch's tiles; its wavefronts take contiguous quarters of the keys and are
+// merged through LDS in wavefront order.
+template <class E, class T, int HD>
+__global__ __launch_bounds__(64 * PA_WAVES) void paged_attend_kernel(PagedKv c, PagedRows b, int grp,
+                                                                     const T* __restrict__ q, int ldq, float scale,
+                                                                     T* __restrict__ out, int ldo) {
+    using A = Rows16<E, T, HD>;
+    constexpr int NO = 4 * A::VW;
+    __shared__ float s_o[PA_WAVES - 1][NO][64];
+    __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int head = blockIdx.x % c.kv_heads;
+    int tile;
+    const int s = pg_find(b.n_seqs, blockIdx.x / c.kv_heads, [&](int i) { return (pg_seq(b, i).n * grp + 15) / 16; }, tile);
+    if (s >= b.n_seqs) return;
+    const PgSeq sq = pg_seq(b, s);
+    const int n = sq.n * grp, i0 = 16 * tile;
+    const int i = min(i0 + r, n - 1);
+    const int row = sq.row0 + i / grp, h = head * grp + i % grp;
+    A a;
+    a.load_q(q + (size_t)row * ldq + (size_t)h * HD, scale);
+    a.limit = sq.kv - sq.n + i / grp;
+    a.start();
+    const int first = sq.kv - sq.n + i0 / grp;                        // the tile's first and last positions
+    const int last = sq.kv - sq.n + min(i0 + 15, n - 1) / grp;
+    const int blocks = last >= 0 ? last / 32 + 1 : 0, per = (blocks + PA_WAVES - 1) / PA_WAVES;
+    pa_walk<E, T, HD>(a, c, b.table + (size_t)s * b.max_pages, b.max_pages, head, 32 * w * per,
+                      min(last + 1, 32 * (w + 1) * per), sq.kv, first);
+    a.finish();
+    if (w > 0) {
+#pragma unroll
+        for (int t = 0; t < A::VW; t++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) s_o[w - 1][4 * t + k][lane] = a.o[t][k];
+    }
+    if (g == 0) {
+        s_m[w][r] = a.m;
+        s_l[w][r] = a.l;
+    }
+    __syncthreads();
+    if (w == 0 && i0 + r < n) {
+        float mx = s_m[0][r], l = 0.0f, wt[PA_WAVES];
+#pragma unroll
+        for (int v = 1; v < PA_WAVES; v++) mx = fmaxf(mx, s_m[v][r]);
+#pragma unroll
+        for (int v = 0; v < PA_WAVES; v++) {
+            wt[v] = __builtin_amdgcn_exp2f(s_m[v][r] - mx);
+            l += s_l[v][r] * wt[v];
+        }
+        const float inv = 1.0f / l;
+        T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            T res[A::VW];
+#pragma unroll
+            for (int t = 0; t < A::VW; t++) {
+                float x = a.o[t][k] * wt[0];
+#pragma unroll
+                for (int v = 1; v < PA_WAVES; v++) x = fmaf(s_o[v - 1][4 * t + k][lane], wt[v], x);
+                x = sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : x * inv;
+                res[t] = (T)x;
+            }
+            __builtin_memcpy(__builtin_assume_aligned(dst + A::VW * k, 8), res, sizeof res);
+        }
+    }
+}
+
+// The rows of a batch by binary search over row_start: the last sequence that
+// starts at or before `row`, or -1 if the row is in none.
+__device__ __forceinline__ int pg_row_seq(const PagedRows& b, int row) {
+    if (!b.row_start) return row < b.n_seqs ? row : -1;
+    int lo = 0, hi = b.n_seqs;  // starts[lo] <= row < starts[hi], if the row is in any
+    if (b.row_start[0] > row || b.row_start[b.n_seqs] <= row) return -1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (b.row_start[mid] <= row) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+constexpr int AP_WG = 256;
+
+// One packed row a workgroup.  y[i] = x[i] cos[i] - x[i + HD/2] sin[i],
+// y[i + HD/2] = x[i + HD/2] cos[i + HD/2] + x[i] sin[i + HD/2] (rope_f32,
+// byte_kernels.rs:1885-1964): two products and a sum in f32, rounded once.
+template <class E, class T, int HD>
+__global__ __launch_bounds__(AP_WG) void paged_append_kernel(PagedKv c, PagedRows b, int n_heads,
+                                                             const T* __restrict__ q, int ldq,
+                                                             const T* __restrict__ k, int ldk,
+                                                             const T* __restrict__ v, int ldv,
+                                                             const float* __restrict__ cs, const float* __restrict__ sn,
+                                                             int rope_rows, T* q_out, int ldqo) {
+    const int row = blockIdx.x;
+    const int s = pg_row_seq(b, row);
+    if (s < 0) return;
+    const PgSeq sq = pg_seq(b, s);
+    if (row < sq.row0 || row >= sq.row0 + sq.n) return;
+    const int pos = sq.kv - sq.n + (row - sq.row0);
+    const bool bad = sq.bad || (cs && pos >= rope_rows);
+    const int page = bad || pos < 0 ? -1 : b.table[(size_t)s * b.max_pages + (pos >> c.log_ps)];
+    const bool put = (unsigned)page < (unsigned)c.n_pages;
+    const int slot = pos & ((1 << c.log_ps) - 1);
+    constexpr int HALF = HD / 2;
+    for (int e = threadIdx.x; e < (n_heads + c.kv_heads) * HALF; e += AP_WG) {
+        const int h = e / HALF, i = e % HALF;
+        const bool is_q = h < n_heads;
+        if (is_q ? !q : !put) continue;
+        const T* x = is_q ? q + (size_t)row * ldq + h * HD : k + (size_t)row * ldk + (h - n_heads) * HD;
+        const float lo = (float)x[i], hi = (float)x[i + HALF];
+        float a = lo, z = hi;
+        if (cs && pos >= 0 && !bad) {
+            const float* ct = cs + (size_t)pos * HD;
+            const float* st = sn + (size_t)pos * HD;
+            a = lo * ct[i] - hi * st[i];
+            z = hi * ct[i + HALF] + lo * st[i + HALF];
+        }
+        if (is_q) {
+            if (bad) a = z = pg_nan();
+            else if (pos < 0) a = z = 0.0f;
+            T* y = q_out + (size_t)row * ldqo + h * HD;
+            y[i] = (T)a;
+            y[i + HALF] = (T)z;
+        } else {
+            E* y = static_cast<E*>(c.k) + ((((size_t)page * c.kv_heads + (h - n_heads)) << c.log_ps) + slot) * HD;
+            y[i] = (E)a;
+            y[i + HALF] = (E)z;
+        }
+    }
+    if (!put) return;
+    for (int e = threadIdx.x; e < c.kv_heads * HD; e += AP_WG) {
+        const int h = e / HD, i = e % HD;
+        static_cast<E*>(c.v)[((((size_t)page * c.kv_heads + h) << c.log_ps) + slot) * HD + i] =
+            (E)(float)v[(size_t)row * ldv + e];
+    }
+}
+
+// Calls f.template operator()<E, T, HD>() for the types of a call.
+template <class F>
+hipError_t with_types(int kv_dtype, int dtype, int hd, F f) {
+    const bool h64 = hd == 64;
+    if (kv_dtype == GGML_F16 && dtype == GGML_F32)
+        return h64 ? f.template run<_Float16, float, 64>() : f.template run<_Float16, float, 128>();
+    if (kv_dtype == GGML_F16 && dtype == GGML_F16)
+        return h64 ? f.template run<_Float16, _Float16, 64>() : f.template run<_Float16, _Float16, 128>();
+    if (kv_dtype == GGML_BF16 && dtype == GGML_F32)
+        return h64 ? f.template run<__bf16, float, 64>() : f.template run<__bf16, float, 128>();
+    if (kv_dtype == GGML_BF16 && dtype == GGML_BF16)
+        return h64 ? f.template run<__bf16, __bf16, 64>() : f.template run<__bf16, __bf16, 128>();
+    return hipErrorInvalidValue;
+}
+
+struct AppendCall {
+    const PagedAppendArgs& p;
+    hipStream_t s;
+    template <class E, class T, int HD>
+    hipError_t run() const {
+        hipLaunchKernelGGL((paged_append_kernel<E, T, HD>), dim3(p.rows.rows), dim3(AP_WG), 0, s, p.kv, p.rows,
+                           p.n_heads, static_cast<const T*>(p.q), p.ldq, static_cast<const T*>(p.k), p.ldk,
+                           static_cast<const T*>(p.v), p.ldv, p.cos, p.sin, p.rope_rows, static_cast<T*>(p.q_out),
+                           p.ldqo);
+        return hipGetLastError();
+    }
+};
+
+struct AttendCall {
+    const PagedAttendArgs& p;
+    hipStream_t s;
+    template <class E, class T, int HD>
+    hipError_t run() const {
+        const int grp = p.n_heads / p.kv.kv_heads;
+        // a bound on the tiles: each sequence's last may be partly empty
+        const long tiles = p.rows.row_start ? (long)p.rows.rows * grp / 16 + p.rows.n_seqs
+                                            : (long)p.rows.n_seqs * ((grp + 15) / 16);
+        hipLaunchKernelGGL((paged_attend_kernel<E, T, HD>), dim3((unsigned)(tiles * p.kv.kv_heads)),
+                           dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp, static_cast<const T*>(p.q), p.ldq, p.scale,
+                           static_cast<T*>(p.out), p.ldo);
+        return hipGetLastError();
+    }
+};
+
+}  // namespace
+
+bool paged_types(int kv_dtype, int dtype) {
+    return (kv_dtype == GGML_F16 && (dtype == GGML_F32 || dtype == GGML_F16)) ||
+           (kv_dtype == GGML_BF16 && (dtype == GGML_F32 || dtype == GGML_BF16));
+}
+
+hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppendArgs& p, hipStream_t s) {
+    if (p.rows.rows <= 0) return hipSuccess;
+    return with_types(kv_dtype, dtype, hd, AppendCall{p, s});
+}
+
+hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
+    if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
+    return with_types(kv_dtype, dtype, hd, AttendCall{p, s});
+}
+
+}  // namespace frq

@@ -1,0 +1,125 @@
+// The paged KV cache: argument views and the device helpers its kernels share
+// (paged.hip, paged_prefill.hip).
+//
+// Cache: k and v are [n_pages][kv_heads][page_size][HD] f16 or bf16, so the
+// rows of one head in one page are contiguous (16 rows of 128 are 4 KiB).
+// Sequence s keeps position j in page table[s * max_pages + j / page_size],
+// row j % page_size.  page_size is a power of two >= 16: 16 keys from a
+// multiple of 16 never cross a page.
+//
+// Packed rows: row_start[s] .. row_start[s + 1] - 1 are sequence s's (row s
+// alone without a row_start); the last of them stands at position
+// kv_len[s] - 1, the ones before it at the positions before.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace frq {
+
+struct PagedKv {
+    void* k;
+    void* v;
+    int n_pages;
+    int log_ps;
+    int kv_heads;
+};
+
+struct PagedRows {
+    const int* table;
+    const int* kv_len;
+    const int* row_start;  // null: one row a sequence
+    int n_seqs;
+    int max_pages;
+    int rows;
+    int cap;  // kv_len beyond it is no length (<= max_pages * page_size)
+};
+
+#ifdef __HIPCC__
+
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef float pg_f2 __attribute__((ext_vector_type(2)));
+
+// Vector types, conversions and MFMAs of a cache element type.
+template <class E>
+struct PgElem;
+template <>
+struct PgElem<_Float16> {
+    typedef _Float16 v8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 v2 __attribute__((ext_vector_type(2)));
+    static constexpr uint32_t INF = 0x7c007c00u;  // exponent bits of both halves of a word
+    static constexpr int SPLIT = 2;               // parts that hold an f32 to 2^-22
+    __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct PgElem<__bf16> {
+    typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
+    static constexpr uint32_t INF = 0x7f807f80u;
+    static constexpr int SPLIT = 3;  // 8 significant bits each: an f32 to 2^-24
+    __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// Whether a word holds an infinite or NaN half.
+template <class E>
+__device__ __forceinline__ bool pg_word_inf(uint32_t w) {
+    const uint32_t t = ~w & PgElem<E>::INF;
+    return (t & 0xffffu) == 0 || (t >> 16) == 0;
+}
+
+__device__ __forceinline__ float pg_nan() { return __builtin_nanf(""); }
+
+// A sequence as the kernels see it.  n = 0 where row_start is no range of
+// rows; bad where kv_len is no length (its rows' results are NaN).
+struct PgSeq {
+    int row0, n, kv;
+    bool bad;
+};
+__device__ __forceinline__ PgSeq pg_seq(const PagedRows& b, int s) {
+    PgSeq q;
+    q.row0 = s;
+    q.n = 1;
+    if (b.row_start) {
+        q.row0 = b.row_start[s];
+        const int end = b.row_start[s + 1];
+        q.n = q.row0 >= 0 && end <= b.rows && end > q.row0 ? end - q.row0 : 0;
+    }
+    q.kv = b.kv_len[s];
+    q.bad = q.kv < 0 || q.kv > b.cap;
+    if (q.bad) q.kv = 0;
+    return q;
+}
+
+// The sequence that holds unit `at` of the batch, where sequence s has
+// units(s) >= 0 of them one after another: s and the unit's number in it, or
+// s = n_seqs past the last.  Every lane of a wavefront takes part (64
+// sequences a step); the result is wave-uniform.
+template <class F>
+__device__ __forceinline__ int pg_find(int n_seqs, int at, F units, int& in_seq) {
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+        const int u = s0 + lane < n_seqs ? units(s0 + lane) : 0;
+        int sum = u;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int up = __shfl_up(sum, off);
+            if (lane >= off) sum += up;
+        }
+        const uint64_t past = __ballot(base + sum > at);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            in_seq = at - base - __builtin_amdgcn_readlane(sum - u, l);
+            return s0 + l;
+        }
+        base += __builtin_amdgcn_readlane(sum, 63);
+    }
+    in_seq = 0;
+    return n_seqs;
+}
+
+#endif  // __HIPCC__
+
+}  // namespace frq

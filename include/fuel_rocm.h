@@ -53,7 +53,8 @@ enum {
     FRQ_Q8_0 = 8,
     FRQ_Q4K = 12,
     FRQ_Q6K = 14,
-    FRQ_Q8K = 15
+    FRQ_Q8K = 15,
+    FRQ_BF16 = 30
 };
 
 typedef struct frq_device frq_device;
@@ -330,6 +331,86 @@ int frq_gather_rows(frq_device *dev, const float *table_dev, size_t rows, size_t
 int frq_argmax_embed(frq_device *dev, const float *logits_dev, size_t vocab, const float *table_dev, size_t dim,
                      int32_t *tokens_dev, size_t tokens_cap, const int32_t *prompt_len_dev, int32_t *pos_dev,
                      float *x_dev);
+
+/* ---- a batch of sequences over a paged KV cache ----
+ * The cache a server keeps for many sequences at once (the reference's block
+ * pools, fuel-core/src/kv_block_pool*.rs): k and v are pools of pages
+ * [n_pages, n_kv_heads, page_size, head_dim], f16 or bf16 (dtype FRQ_F16 or
+ * FRQ_BF16), 16-byte aligned; page_size is a power of two from 16 to 1024,
+ * head_dim 64 or 128.  n_heads query heads are a multiple of n_kv_heads:
+ * query head h reads KV head h / (n_heads / n_kv_heads). */
+typedef struct frq_paged_kv {
+    int dtype;
+    size_t n_pages, page_size, n_kv_heads, head_dim;
+    void *k, *v;
+} frq_paged_kv;
+/* The sequences of a call and its packed rows, in device memory:
+ *   page_table [n_seqs, max_pages]: page of positions i * page_size ..
+ *   kv_len [n_seqs]: tokens of each sequence, this call's rows included
+ *   row_start [n_seqs + 1], non-decreasing: sequence s has the rows
+ *     row_start[s] .. row_start[s + 1] - 1; NULL: row s alone (rows = n_seqs)
+ * rows is the number of rows of the call's q, k, v and outputs.  max_kv_len
+ * is the caller's bound on kv_len (at most max_pages * page_size; 0 stands
+ * for that): work is divided by it, so a near bound helps short contexts, and
+ * a captured call gives the largest it will be replayed with.
+ * The last row of sequence s stands at position kv_len[s] - 1, the rows before
+ * it at the positions before.  What the device finds:
+ *   kv_len[s] = 0, or fewer than its rows: a row before position 0 sees
+ *     nothing, its results are zeros and nothing of it is appended (the empty
+ *     slots of a padded batch)
+ *   kv_len[s] < 0 or > max_kv_len: the rows' results are NaN, nothing is
+ *     appended
+ *   a page outside [0, n_pages) among a row's keys: its results are NaN; in
+ *     an append the row is not stored
+ *   row_start[s] .. row_start[s + 1] no range within [0, rows]: the sequence
+ *     has no rows
+ *   rows before row_start[0] or from row_start[n_seqs] on: left as they were
+ * Cache rows beyond a sequence's length, and keys a row does not see, may hold
+ * anything (NaN included) without effect on it. */
+typedef struct frq_paged_batch {
+    size_t n_seqs, max_pages, rows, max_kv_len;
+    const int32_t *page_table, *kv_len, *row_start;
+} frq_paged_batch;
+/* RoPE of the rows' q and k and the append of k and v (frq_rope_append_rows
+ * for a batch): q [rows, n_heads * head_dim], k and v [rows, n_kv_heads *
+ * head_dim] of type dtype, rows ldq, ldk, ldv elements apart (the three may be
+ * parts of one projection's output).  q and k are rotated (rope_f32
+ * rotate-half, byte_kernels.rs:1885-1964) by the rows `position` of the
+ * [rope_rows, head_dim] tables; rotated q goes to q_out (which may be q), k and
+ * v to their page.  f32 arithmetic, one rounding to q_out's or the cache's
+ * type.  A position >= rope_rows: NaN in q_out, nothing appended.  rope_cos
+ * and rope_sin NULL: no rotation.  q and q_out NULL: k and v only.  Two rows
+ * must not name the same page and position.  dtype: FRQ_F32 or the cache's
+ * type.  Pointers 16-byte aligned, rows a multiple of 16 bytes apart.
+ * Asynchronous, allocates nothing. */
+int frq_paged_append(frq_device *dev, const frq_paged_kv *kv, const frq_paged_batch *batch, int dtype, size_t n_heads,
+                     const void *q_dev, size_t ldq, const void *k_dev, size_t ldk, const void *v_dev, size_t ldv,
+                     const float *rope_cos_dev, const float *rope_sin_dev, size_t rope_rows, void *q_out_dev,
+                     size_t ldqo);
+/* Bytes of scratch that the two attention calls below need for a batch (0:
+ * none, or arguments that they refuse); it depends on the sizes of the
+ * structs alone.  No initialization needed; calls that may overlap need one
+ * each. */
+size_t frq_paged_attention_workspace(const frq_paged_kv *kv, const frq_paged_batch *batch, size_t n_heads);
+/* Attention of one new token per sequence (row_start NULL): row s of q
+ * [n_seqs, n_heads * head_dim] over the sequence's cache rows 0 .. kv_len[s]
+ * - 1, out = softmax((q . k_j) * scale) . v_j per head, the new token's own
+ * key and value appended before (frq_paged_append).  q and out are of type
+ * dtype (FRQ_F32, or the cache's type), rows ldq and ldo elements apart.
+ * Scores, softmax and sums are f32, f32 operands keep f32's precision.
+ * Alignment as frq_paged_append, work 16-byte aligned.  Asynchronous,
+ * allocates nothing; the same call gives the same bits. */
+int frq_paged_attention_decode(frq_device *dev, const frq_paged_kv *kv, const frq_paged_batch *batch, int dtype,
+                               size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
+                               size_t work_bytes, void *out_dev, size_t ldo);
+/* Causal attention of packed rows (whole prompts, or chunks whose earlier part
+ * is cached): each row over the cache rows 0 .. its position, arguments as
+ * frq_paged_attention_decode; the batch's own keys and values are appended
+ * before.  With 16-bit operands the softmax weights are rounded to that type
+ * for the product with V (their sum is not). */
+int frq_paged_attention_prefill(frq_device *dev, const frq_paged_kv *kv, const frq_paged_batch *batch, int dtype,
+                                size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
+                                size_t work_bytes, void *out_dev, size_t ldo);
 
 /* ---- integer taps (build-internal parity probes; no reference counterpart) ----
  * Quantize rows of f32 activations into fuel's activation blocks
