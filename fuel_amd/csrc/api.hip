@@ -1478,7 +1478,7 @@ int paged_operand(const char* who, const char* name, int dtype, const void* p, s
     return FRQ_OK;
 }
 
-int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
+int paged_attention(const char* who, bool decode, frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
                     size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes, void* out,
                     size_t ldo) {
     int rc;
@@ -1486,6 +1486,8 @@ int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, co
     if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
     if (!paged_types(kv->dtype, dtype))
         return fail(FRQ_UNSUPPORTED, "%s: dtype %d over a cache of dtype %d", who, dtype, kv->dtype);
+    if (decode && !paged_decode_fits(a.kv, a.rows, (int)n_heads))
+        return fail(FRQ_UNSUPPORTED, "%s: n_seqs=%zu of up to %d tokens", who, b->n_seqs, a.rows.cap);
     const bool none = b->n_seqs == 0 || b->rows == 0;
     const size_t need = frq_paged_attention_workspace(kv, b, n_heads);
     if (!none && work_bytes < need)
@@ -1503,7 +1505,8 @@ int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, co
     a.scale = scale;
     a.out = out;
     a.ldo = (int)ldo;
-    HIP_TRY(launch_paged_attend(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
+    a.work = work;
+    HIP_TRY((decode ? launch_paged_decode : launch_paged_attend)(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
     return FRQ_OK;
 }
 
@@ -1553,7 +1556,7 @@ size_t frq_paged_attention_workspace(const frq_paged_kv* kv, const frq_paged_bat
     PagedKv k;
     PagedRows r;
     if (paged_args("paged_attention_workspace", kv, b, n_heads, &k, &r)) return 0;
-    return 0;
+    return r.row_start ? 0 : paged_decode_work_bytes(k, r, (int)n_heads, (int)kv->head_dim);
 }
 
 int frq_paged_attention_decode(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
@@ -1561,15 +1564,15 @@ int frq_paged_attention_decode(frq_device* dev, const frq_paged_kv* kv, const fr
                                void* out, size_t ldo) {
     if (b && b->row_start)
         return fail(FRQ_INVALID, "paged_attention_decode: one row a sequence (row_start must be NULL)");
-    return paged_attention("paged_attention_decode", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes, out,
-                           ldo);
+    return paged_attention("paged_attention_decode", true, dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
+                           out, ldo);
 }
 
 int frq_paged_attention_prefill(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
                                 size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes,
                                 void* out, size_t ldo) {
-    return paged_attention("paged_attention_prefill", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes, out,
-                           ldo);
+    return paged_attention("paged_attention_prefill", false, dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
+                           out, ldo);
 }
 
 int frq_fill_random_bits(frq_device* dev, uint32_t* y, size_t n, uint64_t start, uint64_t seed, uint32_t base,

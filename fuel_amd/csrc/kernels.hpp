@@ -288,7 +288,13 @@ struct PagedAttendArgs {
     float scale;
     void* out;
     int ldo;
+    void* work;
 };
+// One row a sequence: units over all workgroups, cut sequences joined (work of
+// paged_decode_work_bytes()); paged_decode_fits: their count fits an int.
+bool paged_decode_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
+size_t paged_decode_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
+hipError_t launch_paged_decode(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 
 }  // namespace frq

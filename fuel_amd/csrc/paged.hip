@@ -41,6 +41,16 @@ namespace {
 constexpr int PA_WAVES = 4;
 constexpr float PA_SHIFT = 15.0f;
 
+// The largest of the four lanes 16 g + r of a row, in all four.
+__device__ __forceinline__ float pg_row_max(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const float w = fmaxf(__builtin_bit_cast(float, (uint32_t)a[0]), __builtin_bit_cast(float, (uint32_t)a[1]));
+    const uint32_t x = __builtin_bit_cast(uint32_t, w);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)b[0]), __builtin_bit_cast(float, (uint32_t)b[1]));
+}
+
 template <class E, class T, int HD>
 struct Rows16 {
     using P = PgElem<E>;
@@ -56,9 +66,11 @@ struct Rows16 {
     pg_f4 o[VW];
     float m, l;
 
-    struct Block {
-        uint4 k[2][KS];
-        uint32_t v[8][VW / 2];
+    struct KeyRegs {
+        uint4 w[2][KS];
+    };
+    struct ValueRegs {
+        uint32_t w[8][VW / 2];
     };
 
     // Lane 16 g + r takes row r: dims 32 t + 8 g + e of x (null: a row of zeros).
@@ -123,57 +135,67 @@ struct Rows16 {
     }
 
     // The loads of 32 keys: group a's 16 rows start at ka[a] / va[a].
-    __device__ void load(Block& b, const E* const (&ka)[2], const E* const (&va)[2]) const {
+    __device__ static void load_k(KeyRegs& k, const E* const (&ka)[2]) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int a = 0; a < 2; a++) {
+        for (int a = 0; a < 2; a++)
 #pragma unroll
-            for (int t = 0; t < KS; t++)
-                b.k[a][t] = *reinterpret_cast<const uint4*>(ka[a] + r * HD + 32 * t + 8 * g);
+            for (int t = 0; t < KS; t++) k.w[a][t] = *reinterpret_cast<const uint4*>(ka[a] + r * HD + 32 * t + 8 * g);
+    }
+    __device__ static void load_v(ValueRegs& v, const E* const (&va)[2]) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int a = 0; a < 2; a++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                __builtin_memcpy(b.v[4 * a + i], __builtin_assume_aligned(va[a] + (4 * g + i) * HD + VW * r, 2 * VW),
+                __builtin_memcpy(v.w[4 * a + i], __builtin_assume_aligned(va[a] + (4 * g + i) * HD + VW * r, 2 * VW),
                                  2 * VW);
-        }
     }
 
-    // 32 keys from j0.  MASK: some key is past a row's position, past the
-    // sequence's length kv, or in a page that is none (bad).
+    // Which keys of a block of 32 from j0 a row sees: none past its position,
+    // past the sequence's length kv or in a page that is none (bad: NaN).
+    struct Mask {
+        int j0, kv;
+        bool bad[2];
+    };
+
+    // The block's scores in log2 units: s[4 a + i] of key 16 a + 4 g + i.
     template <bool MASK>
-    __device__ void step(Block& b, int j0, int kv, const bool (&bad)[2], const E* const (&va)[2]) {
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        float s[8], top = -__builtin_inff();
+    __device__ void scores(const KeyRegs& k, const Mask& mk, float (&s)[8]) const {
+        const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
         for (int a = 0; a < 2; a++) {
             pg_f4 st = pg_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < KS; t++)
 #pragma unroll
-                for (int p = NQ - 1; p >= 0; p--) st = P::mfma16(__builtin_bit_cast(v8, b.k[a][t]), q[p][t], st);
+                for (int p = NQ - 1; p >= 0; p--) st = P::mfma16(__builtin_bit_cast(v8, k.w[a][t]), q[p][t], st);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 float v = st[i] * factor;
                 if constexpr (MASK) {
-                    if (bad[a]) v = pg_nan();
-                    if (j0 + 16 * a + 4 * g + i > limit) v = -__builtin_inff();
+                    if (mk.bad[a]) v = pg_nan();
+                    if (mk.j0 + 16 * a + 4 * g + i > limit) v = -__builtin_inff();
                 }
                 s[4 * a + i] = v;
-                top = fmaxf(top, v);
             }
         }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float mn = fmaxf(m, top);
+    }
+
+    // Weights of the block's scores (s becomes them), maximum and sums renewed.
+    __device__ void weights(float (&s)[8], v8 (&pp)[NP]) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
+        const float mn = fmaxf(m, pg_row_max(top));
         const float c = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before: l = o = 0)
         m = mn;
         l *= c;
-        v8 pp[NP];
-        float pf[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            pf[i] = __builtin_amdgcn_exp2f(s[i] - mn + PA_SHIFT);
-            l += pf[i];
-            float rest = pf[i];
+            s[i] = __builtin_amdgcn_exp2f(s[i] - mn + PA_SHIFT);
+            l += s[i];
+            float rest = s[i];
 #pragma unroll
             for (int p = 0; p < NP; p++) {
                 pp[p][i] = (E)rest;
@@ -182,47 +204,56 @@ struct Rows16 {
         }
 #pragma unroll
         for (int t = 0; t < VW; t++) o[t] *= c;
-        if constexpr (MASK) {
-            // keys that no row of the sequence may see: their rows hold anything
-            bool odd = false;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const bool none = bad[i >> 2] || j0 + 16 * (i >> 2) + 4 * g + (i & 3) >= kv;
-#pragma unroll
-                for (int w = 0; w < VW / 2; w++) {
-                    if (none) b.v[i][w] = 0;
-                    odd |= pg_word_inf<E>(b.v[i][w]);
-                }
-            }
-            if (__any(odd)) {
-                // an infinite or NaN value in a key that some rows do not see:
-                // 0 * inf must not reach those rows, so each row adds only its own keys
-                for (int j = 0; j < 32; j++) {
-                    float p = pf[0];
-#pragma unroll
-                    for (int i = 1; i < 8; i++) p = (j >> 4) * 4 + (j & 3) == i ? pf[i] : p;
-                    p = __shfl(p, r + 16 * ((j >> 2) & 3));
-                    if (j0 + j <= limit) {
-                        const E* row = (j < 16 ? va[0] : va[1]) + (j & 15) * HD + 4 * VW * g;
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int t = 0; t < VW; t++) o[t][i] = fmaf(p, (float)row[VW * i + t], o[t][i]);
-                    }
-                }
-                return;
-            }
-        }
+    }
+
+    __device__ void product(const ValueRegs& v, const v8 (&pp)[NP]) {
 #pragma unroll
         for (int t = 0; t < VW; t++) {
             const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;  // high or low halves of two words
             uint4 a;
-            a.x = __builtin_amdgcn_perm(b.v[1][t >> 1], b.v[0][t >> 1], sel);
-            a.y = __builtin_amdgcn_perm(b.v[3][t >> 1], b.v[2][t >> 1], sel);
-            a.z = __builtin_amdgcn_perm(b.v[5][t >> 1], b.v[4][t >> 1], sel);
-            a.w = __builtin_amdgcn_perm(b.v[7][t >> 1], b.v[6][t >> 1], sel);
+            a.x = __builtin_amdgcn_perm(v.w[1][t >> 1], v.w[0][t >> 1], sel);
+            a.y = __builtin_amdgcn_perm(v.w[3][t >> 1], v.w[2][t >> 1], sel);
+            a.z = __builtin_amdgcn_perm(v.w[5][t >> 1], v.w[4][t >> 1], sel);
+            a.w = __builtin_amdgcn_perm(v.w[7][t >> 1], v.w[6][t >> 1], sel);
 #pragma unroll
             for (int p = NP - 1; p >= 0; p--) o[t] = P::mfma16(__builtin_bit_cast(v8, a), pp[p], o[t]);
+        }
+    }
+
+    // Keys that no row of the sequence may see: their rows hold anything.
+    // Whether an infinite or NaN value is left.
+    __device__ static bool clear(ValueRegs& v, const Mask& mk) {
+        const int g = (threadIdx.x & 63) >> 4;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const bool none = mk.bad[i >> 2] || mk.j0 + 16 * (i >> 2) + 4 * g + (i & 3) >= mk.kv;
+#pragma unroll
+            for (int w = 0; w < VW / 2; w++) {
+                if (none) v.w[i][w] = 0;
+                odd |= pg_word_inf<E>(v.w[i][w]);
+            }
+        }
+        return odd;
+    }
+
+    // The product with V where a value in a key that some rows do not see is
+    // infinite or NaN: 0 * inf must not reach those rows, so each row adds
+    // only its own keys.
+    __device__ void product_seen(const float (&w)[8], const Mask& mk, const E* const (&va)[2]) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+        for (int j = 0; j < 32; j++) {
+            float p = w[0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) p = (j >> 4) * 4 + (j & 3) == i ? w[i] : p;
+            p = __shfl(p, r + 16 * ((j >> 2) & 3));
+            if (mk.j0 + j <= limit) {
+                const E* row = (j < 16 ? va[0] : va[1]) + (j & 15) * HD + 4 * VW * g;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int t = 0; t < VW; t++) o[t][i] = fmaf(p, (float)row[VW * i + t], o[t][i]);
+            }
         }
     }
 
@@ -236,28 +267,40 @@ struct Rows16 {
 // The walk of one wavefront over keys [j0, j1) (j0 a multiple of 32) of a
 // sequence for the 16 rows of `a`: no row sees a key >= j1.
 template <class E, class T, int HD>
-__device__ void pa_walk(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int max_pages, int head, int j0,
-                        int j1, int kv, int all_see) {
-    const E* ka[2];
-    const E* va[2];
-    bool bad[2];
-    typename Rows16<E, T, HD>::Block b;
+__device__ void pa_walk(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int head, int j0, int j1, int kv,
+                        int all_see) {
+    using A = Rows16<E, T, HD>;
+    typename A::KeyRegs kr;
+    typename A::ValueRegs vr;
     for (; j0 < j1; j0 += 32) {
+        typename A::Mask mk{j0, kv, {false, false}};
+        const E* ka[2];
+        const E* va[2];
 #pragma unroll
         for (int g = 0; g < 2; g++) {
             const int j = j0 + 16 * g;
             // (a group past the length has no page: its keys are masked)
             const int page = j < kv ? table[j >> c.log_ps] : 0;
-            bad[g] = (unsigned)page >= (unsigned)c.n_pages;
-            const size_t at = (((size_t)(bad[g] ? 0 : page) * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1));
+            mk.bad[g] = (unsigned)page >= (unsigned)c.n_pages;
+            const size_t at =
+                (((size_t)(mk.bad[g] ? 0 : page) * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1));
             ka[g] = static_cast<const E*>(c.k) + at * HD;
             va[g] = static_cast<const E*>(c.v) + at * HD;
         }
-        a.load(b, ka, va);
-        if (j0 + 31 <= all_see && !bad[0] && !bad[1])
-            a.template step<false>(b, j0, kv, bad, va);
-        else
-            a.template step<true>(b, j0, kv, bad, va);
+        A::load_k(kr, ka);
+        A::load_v(vr, va);
+        float s[8];
+        typename A::v8 pp[A::NP];
+        if (j0 + 31 <= all_see && !mk.bad[0] && !mk.bad[1]) {
+            a.template scores<false>(kr, mk, s);
+            a.weights(s, pp);
+            a.product(vr, pp);
+        } else {
+            a.template scores<true>(kr, mk, s);
+            a.weights(s, pp);
+            if (__any(A::clear(vr, mk))) a.product_seen(s, mk, va);
+            else a.product(vr, pp);
+        }
     }
 }
 
@@ -289,7 +332,7 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attend_kernel(PagedKv c, 
     const int first = sq.kv - sq.n + i0 / grp;                        // the tile's first and last positions
     const int last = sq.kv - sq.n + min(i0 + 15, n - 1) / grp;
     const int blocks = last >= 0 ? last / 32 + 1 : 0, per = (blocks + PA_WAVES - 1) / PA_WAVES;
-    pa_walk<E, T, HD>(a, c, b.table + (size_t)s * b.max_pages, b.max_pages, head, 32 * w * per,
+    pa_walk<E, T, HD>(a, c, b.table + (size_t)s * b.max_pages, head, 32 * w * per,
                       min(last + 1, 32 * (w + 1) * per), sq.kv, first);
     a.finish();
     if (w > 0) {
@@ -328,6 +371,239 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attend_kernel(PagedKv c, 
             __builtin_memcpy(__builtin_assume_aligned(dst + A::VW * k, 8), res, sizeof res);
         }
     }
+}
+
+// ---- one new token per sequence ----
+//
+// The keys of all sequences and KV heads are one list of units of PD_UNIT keys
+// (head by head, within a head sequence by sequence), cut into equal
+// contiguous ranges, one per workgroup: a batch of very different lengths
+// keeps every CU busy to the end, and the host needs to know no length.  A
+// range covers the end of one sequence, some whole ones and the start of
+// another; whole ones are written out, the cut pieces (at most two a
+// workgroup) leave their sums in the workspace for paged_join_kernel.
+constexpr int PD_UNIT = 32 * PA_WAVES;
+constexpr int PD_WGS = 512;  // two a CU, all resident at once
+
+// Slot of a cut piece: o [16][HD] (unnormalized), m [16], l [16].
+constexpr int pd_slot(int hd) { return 16 * hd + 32; }
+
+// Units of a sequence; one without keys has one, which writes its rows.
+__device__ __forceinline__ int pd_units(const PagedRows& b, int s) {
+    const int kv = b.kv_len[s];
+    return kv <= 0 || kv > b.cap ? 1 : (kv + PD_UNIT - 1) / PD_UNIT;
+}
+__device__ __forceinline__ int pd_total(const PagedRows& b) {
+    int sum = 0;
+    for (int s = threadIdx.x & 63; s < b.n_seqs; s += 64) sum += pd_units(b, s);
+    return wave_sum_i(sum);
+}
+// Of n_wgs <= total workgroups, w's range starts at unit w * total / n_wgs: none is empty.
+__device__ __forceinline__ int pd_start(int w, int total, int n_wgs) { return (int)((long)w * total / n_wgs); }
+// The workgroup whose range holds unit u: the largest w with pd_start(w) <= u.
+__device__ __forceinline__ int pd_owner(int u, int total, int n_wgs) {
+    return (int)((((long)u + 1) * n_wgs - 1) / total);
+}
+
+// One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of 32;
+// j1 too, or kv).  The next block's keys are loaded as soon as this one's
+// scores are formed, its values as soon as this one's product is: one or the
+// other is in flight all the time, in one set of registers each (two sets
+// spill at HD 128).  The page ids of 1024 keys are one load, lane i holding
+// the page of group i.
+template <class E, class T, int HD>
+__device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int head, int j0,
+                                        int j1, int kv) {
+    using A = Rows16<E, T, HD>;
+    const int lane = threadIdx.x & 63;
+    while (j0 < j1) {
+        const int end = min(j1, j0 + 1024);
+        const int jl = j0 + 16 * lane;
+        const int id = jl < kv ? table[jl >> c.log_ps] : 0;
+        const bool off = (unsigned)id >= (unsigned)c.n_pages;
+        if (__any(off && jl < end)) a.l = pg_nan();  // a page that is none, and every row sees its keys
+        const int page = off ? 0 : id;
+        auto rows = [&](const void* pool, int blk, const E* (&at)[2]) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int g = 2 * blk + i, p = __builtin_amdgcn_readlane(page, g);
+                at[i] = static_cast<const E*>(pool) + ((((size_t)p * c.kv_heads + head) << c.log_ps) +
+                                                       ((j0 + 16 * g) & ((1 << c.log_ps) - 1))) * HD;
+            }
+        };
+        const int last = (end - j0 + 31) / 32 - 1;
+        const E* at[2];
+        typename A::KeyRegs kr;
+        typename A::ValueRegs vr;
+        float s[8];
+        typename A::v8 pp[A::NP];
+        typename A::Mask mk{j0 + 32 * last, kv, {false, false}};
+        rows(c.k, 0, at);
+        A::load_k(kr, at);
+        rows(c.v, 0, at);
+        A::load_v(vr, at);
+        for (int i = 0; i < last; i++) {
+            a.template scores<false>(kr, mk, s);
+            rows(c.k, i + 1, at);
+            A::load_k(kr, at);
+            a.weights(s, pp);
+            a.product(vr, pp);
+            rows(c.v, i + 1, at);
+            A::load_v(vr, at);
+        }
+        if (mk.j0 + 32 <= kv) {
+            a.template scores<false>(kr, mk, s);
+        } else {
+            a.template scores<true>(kr, mk, s);
+            A::clear(vr, mk);
+        }
+        a.weights(s, pp);
+        a.product(vr, pp);
+        j0 = end;
+    }
+}
+
+template <class E, class T, int HD>
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv c, PagedRows b, int grp, int tiles,
+                                                                        const T* __restrict__ q, int ldq, float scale,
+                                                                        T* __restrict__ out, int ldo,
+                                                                        float* __restrict__ part) {
+    using A = Rows16<E, T, HD>;
+    constexpr int NO = 4 * A::VW;
+    __shared__ float s_o[PA_WAVES - 1][NO][64];
+    __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int units = pd_total(b), heads = c.kv_heads * tiles, total = units * heads;
+    const int n_wgs = min((int)gridDim.x, total);
+    if ((int)blockIdx.x >= n_wgs) return;
+    const int begin = pd_start(blockIdx.x, total, n_wgs), stop = pd_start(blockIdx.x + 1, total, n_wgs);
+    int vh = begin / units, u;
+    int s = pg_find(b.n_seqs, begin - vh * units, [&](int i) { return pd_units(b, i); }, u);
+    for (int at = begin; at < stop;) {
+        const int n = pd_units(b, s), m = min(n - u, stop - at);  // units u .. u + m - 1 of sequence s
+        const PgSeq sq = pg_seq(b, s);
+        const int head = vh / tiles, h0 = (vh % tiles) * 16, rows = min(16, grp - h0);
+        const int h = head * grp + h0 + min(r, rows - 1);
+        A a;
+        a.load_q(q + (size_t)s * ldq + (size_t)h * HD, scale);
+        a.limit = sq.kv - 1;
+        a.start();
+        const int k0 = u * PD_UNIT, k1 = min(sq.kv, (u + m) * PD_UNIT);
+        const int per = ((k1 - k0 + 31) / 32 + PA_WAVES - 1) / PA_WAVES;
+        pd_walk<E, T, HD>(a, c, b.table + (size_t)s * b.max_pages, head, k0 + 32 * w * per,
+                          min(k1, k0 + 32 * (w + 1) * per), sq.kv);
+        a.finish();
+        if (w > 0) {
+#pragma unroll
+            for (int t = 0; t < A::VW; t++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) s_o[w - 1][4 * t + k][lane] = a.o[t][k];
+        }
+        if (g == 0) {
+            s_m[w][r] = a.m;
+            s_l[w][r] = a.l;
+        }
+        __syncthreads();
+        if (w == 0 && r < rows) {
+            float mx = s_m[0][r], l = 0.0f, wt[PA_WAVES];
+#pragma unroll
+            for (int v = 1; v < PA_WAVES; v++) mx = fmaxf(mx, s_m[v][r]);
+#pragma unroll
+            for (int v = 0; v < PA_WAVES; v++) {
+                wt[v] = __builtin_amdgcn_exp2f(s_m[v][r] - mx);
+                l += s_l[v][r] * wt[v];
+            }
+            const bool whole = m == n;
+            float* slot = part + ((size_t)2 * blockIdx.x + (at != begin)) * pd_slot(HD);
+            const float inv = whole ? 1.0f / l : 1.0f;
+            T* dst = out + (size_t)s * ldo + (size_t)h * HD + 4 * A::VW * g;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float x[A::VW];
+#pragma unroll
+                for (int t = 0; t < A::VW; t++) {
+                    x[t] = a.o[t][k] * wt[0];
+#pragma unroll
+                    for (int v = 1; v < PA_WAVES; v++) x[t] = fmaf(s_o[v - 1][4 * t + k][lane], wt[v], x[t]);
+                    x[t] = sq.bad ? pg_nan() : sq.kv == 0 ? 0.0f : x[t] * inv;
+                }
+                if (whole) {
+                    T y[A::VW];
+#pragma unroll
+                    for (int t = 0; t < A::VW; t++) y[t] = (T)x[t];
+                    __builtin_memcpy(__builtin_assume_aligned(dst + A::VW * k, 8), y, sizeof y);
+                } else {
+                    __builtin_memcpy(__builtin_assume_aligned(slot + r * HD + A::VW * (4 * g + k), 16), x, sizeof x);
+                }
+            }
+            if (!whole && g == 0) {
+                slot[16 * HD + r] = mx;
+                slot[16 * HD + 16 + r] = l;
+            }
+        }
+        at += m;
+        u = 0;
+        if (++s == b.n_seqs) {
+            s = 0;
+            vh++;
+        }
+        if (at < stop) __syncthreads();  // the merge's LDS is read
+    }
+}
+
+// Joins the pieces of a cut sequence: workgroup (w, i) takes row i of the
+// sequence that begins in range w and goes on past it, if there is one, with
+// PJ_GROUPS threads per dim that each add every PJ_GROUPS-th piece.
+constexpr int PJ_GROUPS = 4;
+template <class T, int HD>
+__global__ __launch_bounds__(PJ_GROUPS * HD) void paged_join_kernel(PagedRows b, int kv_heads, int grp, int tiles,
+                                                                    const float* __restrict__ part,
+                                                                    T* __restrict__ out, int ldo) {
+    __shared__ float s_o[PJ_GROUPS][HD], s_l[PJ_GROUPS], s_m[PJ_GROUPS];
+    const int w0 = blockIdx.x, r = blockIdx.y;
+    const int units = pd_total(b), total = units * kv_heads * tiles;
+    const int n_wgs = min((int)gridDim.x, total);
+    if (w0 >= n_wgs) return;
+    const int begin = pd_start(w0, total, n_wgs), stop = pd_start(w0 + 1, total, n_wgs);
+    const int vh = (stop - 1) / units;
+    int u;
+    const int s = pg_find(b.n_seqs, stop - 1 - vh * units, [&](int i) { return pd_units(b, i); }, u);
+    const int n = pd_units(b, s), first = stop - 1 - u;  // the sequence's first unit
+    if (first < begin || first + n == stop) return;
+    const int h0 = (vh % tiles) * 16;
+    if (r >= min(16, grp - h0)) return;
+    const int w1 = pd_owner(first + n - 1, total, n_wgs);
+    const int d = threadIdx.x % HD, p = threadIdx.x / HD;
+    const float* row = part + r * HD + d;
+    const float* stat = part + 16 * HD + r;
+    float M = -1e30f, L = 0.0f, O = 0.0f;
+    for (int w = w0 + p; w <= w1; w += PJ_GROUPS) {
+        const size_t slot = (size_t)(2 * w + (w == w0 && first != begin)) * pd_slot(HD);
+        const float o = row[slot], m = stat[slot], l = stat[slot + 16];
+        const float mn = fmaxf(M, m), f = __builtin_amdgcn_exp2f(M - mn), e = __builtin_amdgcn_exp2f(m - mn);
+        M = mn;
+        L = fmaf(l, e, L * f);
+        O = fmaf(o, e, O * f);
+    }
+    s_o[p][d] = O;
+    if (d == 0) {
+        s_l[p] = L;
+        s_m[p] = M;
+    }
+    __syncthreads();
+    if (p) return;
+    float mx = s_m[0];
+#pragma unroll
+    for (int i = 1; i < PJ_GROUPS; i++) mx = fmaxf(mx, s_m[i]);
+    L = O = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PJ_GROUPS; i++) {
+        const float e = __builtin_amdgcn_exp2f(s_m[i] - mx);
+        L = fmaf(s_l[i], e, L);
+        O = fmaf(s_o[i][d], e, O);
+    }
+    out[(size_t)s * ldo + (size_t)(vh / tiles * grp + h0 + r) * HD + d] = (T)(O / L);
 }
 
 // The rows of a batch by binary search over row_start: the last sequence that
@@ -444,7 +720,44 @@ struct AttendCall {
     }
 };
 
+// How many workgroups a decode takes: a range each, no more than the units that
+// lengths up to cap can have.
+int pd_wgs(const PagedRows& r, int heads) {
+    const long units = (long)r.n_seqs * ((r.cap + PD_UNIT - 1) / PD_UNIT > 0 ? (r.cap + PD_UNIT - 1) / PD_UNIT : 1);
+    return units * heads < PD_WGS ? (int)(units * heads) : PD_WGS;
+}
+
+struct DecodeCall {
+    const PagedAttendArgs& p;
+    hipStream_t s;
+    template <class E, class T, int HD>
+    hipError_t run() const {
+        const int grp = p.n_heads / p.kv.kv_heads, tiles = (grp + 15) / 16;
+        const int wgs = pd_wgs(p.rows, p.kv.kv_heads * tiles);
+        hipLaunchKernelGGL((paged_decode_kernel<E, T, HD>), dim3(wgs), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp,
+                           tiles, static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo,
+                           static_cast<float*>(p.work));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess || p.rows.cap <= PD_UNIT) return e;  // (one unit a sequence: none is cut)
+        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(wgs, grp < 16 ? grp : 16), dim3(PJ_GROUPS * HD), 0, s,
+                           p.rows, p.kv.kv_heads, grp, tiles, static_cast<const float*>(p.work),
+                           static_cast<T*>(p.out), p.ldo);
+        return hipGetLastError();
+    }
+};
+
 }  // namespace
+
+size_t paged_decode_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    if (r.cap <= PD_UNIT || r.n_seqs == 0) return 0;
+    const int grp = n_heads / kv.kv_heads;
+    return (size_t)2 * pd_wgs(r, kv.kv_heads * ((grp + 15) / 16)) * pd_slot(hd) * sizeof(float);
+}
+
+bool paged_decode_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {
+    const long units = (long)r.n_seqs * (r.cap / PD_UNIT + 1);
+    return units * kv.kv_heads * ((n_heads / kv.kv_heads + 15) / 16) <= 0x7fffffff;
+}
 
 bool paged_types(int kv_dtype, int dtype) {
     return (kv_dtype == GGML_F16 && (dtype == GGML_F32 || dtype == GGML_F16)) ||
@@ -454,6 +767,11 @@ bool paged_types(int kv_dtype, int dtype) {
 hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0) return hipSuccess;
     return with_types(kv_dtype, dtype, hd, AppendCall{p, s});
+}
+
+hipError_t launch_paged_decode(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
+    if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
+    return with_types(kv_dtype, dtype, hd, DecodeCall{p, s});
 }
 
 hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {

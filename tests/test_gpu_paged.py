@@ -86,7 +86,8 @@ class Case:
             want, A, B, V = R.attend(qs, k, v, pos, scale)
             tol = R.bound(want, A, B, V, max(1, int(self.kv[s])), self.D, self.act, self.cache, not self.decode)
             g = got[r0:r0 + n, :w].reshape(want.shape)
-            assert np.isfinite(g).all(), (s, np.argwhere(~np.isfinite(g))[:3])
+            gone = np.argwhere(~np.isfinite(g))
+            assert not len(gone), (s, gone[:3])
             err = np.abs(g - want)
             worst = max(worst, float(np.linalg.norm(err) / max(np.linalg.norm(want), 1e-30)))
             bad = np.argwhere(err > tol)
