@@ -319,7 +319,8 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attend_kernel(PagedKv c, 
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int head = blockIdx.x % c.kv_heads;
     int tile;
-    const int s = pg_find(b.n_seqs, blockIdx.x / c.kv_heads, [&](int i) { return (pg_seq(b, i).n * grp + 15) / 16; }, tile);
+    const auto units = [&](int i) { return (pg_seq(b, i).n * grp + 15) / 16; };
+    const int s = PgUnits(b.n_seqs, units).find(b.n_seqs, blockIdx.x / c.kv_heads, units, tile);
     if (s >= b.n_seqs) return;
     const PgSeq sq = pg_seq(b, s);
     const int n = sq.n * grp, i0 = 16 * tile;
@@ -385,18 +386,20 @@ __global__ __launch_bounds__(64 * PA_WAVES) void paged_attend_kernel(PagedKv c, 
 constexpr int PD_UNIT = 32 * PA_WAVES;
 constexpr int PD_WGS = 512;  // two a CU, all resident at once
 
-// Slot of a cut piece: o [16][HD] (unnormalized), m [16], l [16].
+// The workspace: two slots a workgroup, o [16][HD] (unnormalized), m [16],
+// l [16] of a cut piece; then what each workgroup leaves to be joined.
 constexpr int pd_slot(int hd) { return 16 * hd + 32; }
+struct PdJoin {
+    int s;     // sequence, or -1: none of the workgroup's is cut behind it
+    int vh;    // row tile of a KV head
+    int last;  // workgroup of the sequence's last piece
+    int slot;  // of its first piece
+};
 
 // Units of a sequence; one without keys has one, which writes its rows.
 __device__ __forceinline__ int pd_units(const PagedRows& b, int s) {
     const int kv = b.kv_len[s];
     return kv <= 0 || kv > b.cap ? 1 : (kv + PD_UNIT - 1) / PD_UNIT;
-}
-__device__ __forceinline__ int pd_total(const PagedRows& b) {
-    int sum = 0;
-    for (int s = threadIdx.x & 63; s < b.n_seqs; s += 64) sum += pd_units(b, s);
-    return wave_sum_i(sum);
 }
 // Of n_wgs <= total workgroups, w's range starts at unit w * total / n_wgs: none is empty.
 __device__ __forceinline__ int pd_start(int w, int total, int n_wgs) { return (int)((long)w * total / n_wgs); }
@@ -467,19 +470,24 @@ template <class E, class T, int HD>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv c, PagedRows b, int grp, int tiles,
                                                                         const T* __restrict__ q, int ldq, float scale,
                                                                         T* __restrict__ out, int ldo,
-                                                                        float* __restrict__ part) {
+                                                                        float* __restrict__ part,
+                                                                        PdJoin* __restrict__ joins) {
     using A = Rows16<E, T, HD>;
     constexpr int NO = 4 * A::VW;
     __shared__ float s_o[PA_WAVES - 1][NO][64];
     __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int units = pd_total(b), heads = c.kv_heads * tiles, total = units * heads;
-    const int n_wgs = min((int)gridDim.x, total);
-    if ((int)blockIdx.x >= n_wgs) return;
+    const auto units_of = [&](int i) { return pd_units(b, i); };
+    const PgUnits pu(b.n_seqs, units_of);
+    const int units = pu.total, total = units * c.kv_heads * tiles, n_wgs = min((int)gridDim.x, total);
+    if ((int)blockIdx.x >= n_wgs) {
+        if (joins && threadIdx.x == 0) joins[blockIdx.x].s = -1;
+        return;
+    }
     const int begin = pd_start(blockIdx.x, total, n_wgs), stop = pd_start(blockIdx.x + 1, total, n_wgs);
     int vh = begin / units, u;
-    int s = pg_find(b.n_seqs, begin - vh * units, [&](int i) { return pd_units(b, i); }, u);
+    int s = pu.find(b.n_seqs, begin - vh * units, units_of, u);
     for (int at = begin; at < stop;) {
         const int n = pd_units(b, s), m = min(n - u, stop - at);  // units u .. u + m - 1 of sequence s
         const PgSeq sq = pg_seq(b, s);
@@ -543,6 +551,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv 
             }
         }
         at += m;
+        if (at == stop && joins && threadIdx.x == 0) {
+            const bool cut = u == 0 && m < n;  // begins here, ends in a later range
+            joins[blockIdx.x] = {cut ? s : -1, vh, cut ? pd_owner(at - m + n - 1, total, n_wgs) : 0,
+                                 2 * (int)blockIdx.x + (at - m != begin)};
+        }
         u = 0;
         if (++s == b.n_seqs) {
             s = 0;
@@ -552,39 +565,53 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv 
     }
 }
 
-// Joins the pieces of a cut sequence: workgroup (w, i) takes row i of the
-// sequence that begins in range w and goes on past it, if there is one, with
-// PJ_GROUPS threads per dim that each add every PJ_GROUPS-th piece.
-constexpr int PJ_GROUPS = 4;
+// Joins the pieces of cut sequences: workgroup (w, r) takes row r of the one
+// that workgroup w of the decode left, if it left one.  HD / 4 threads a piece,
+// PJ_WG / (HD / 4) groups of them with every such piece each, PJ_STEP pieces a
+// step: the loads of 64 pieces (one sequence over all workgroups, 8 KV heads)
+// are one memory round trip.
+constexpr int PJ_WG = 256;
+constexpr int PJ_STEP = 8;
 template <class T, int HD>
-__global__ __launch_bounds__(PJ_GROUPS * HD) void paged_join_kernel(PagedRows b, int kv_heads, int grp, int tiles,
-                                                                    const float* __restrict__ part,
-                                                                    T* __restrict__ out, int ldo) {
-    __shared__ float s_o[PJ_GROUPS][HD], s_l[PJ_GROUPS], s_m[PJ_GROUPS];
-    const int w0 = blockIdx.x, r = blockIdx.y;
-    const int units = pd_total(b), total = units * kv_heads * tiles;
-    const int n_wgs = min((int)gridDim.x, total);
-    if (w0 >= n_wgs) return;
-    const int begin = pd_start(w0, total, n_wgs), stop = pd_start(w0 + 1, total, n_wgs);
-    const int vh = (stop - 1) / units;
-    int u;
-    const int s = pg_find(b.n_seqs, stop - 1 - vh * units, [&](int i) { return pd_units(b, i); }, u);
-    const int n = pd_units(b, s), first = stop - 1 - u;  // the sequence's first unit
-    if (first < begin || first + n == stop) return;
-    const int h0 = (vh % tiles) * 16;
-    if (r >= min(16, grp - h0)) return;
-    const int w1 = pd_owner(first + n - 1, total, n_wgs);
-    const int d = threadIdx.x % HD, p = threadIdx.x / HD;
-    const float* row = part + r * HD + d;
+__global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PdJoin* __restrict__ joins,
+                                                           const float* __restrict__ part, int grp, int tiles,
+                                                           T* __restrict__ out, int ldo) {
+    constexpr int TH = HD / 4, GROUPS = PJ_WG / TH;
+    __shared__ pg_f4 s_o[GROUPS][TH];
+    __shared__ float s_l[GROUPS], s_m[GROUPS];
+    const PdJoin j = joins[blockIdx.x];
+    const int r = blockIdx.y, h0 = (j.vh % tiles) * 16;
+    if (j.s < 0 || r >= min(16, grp - h0)) return;
+    const int d = threadIdx.x % TH, p = threadIdx.x / TH, w0 = blockIdx.x;
+    const float* row = part + r * HD + 4 * d;
     const float* stat = part + 16 * HD + r;
-    float M = -1e30f, L = 0.0f, O = 0.0f;
-    for (int w = w0 + p; w <= w1; w += PJ_GROUPS) {
-        const size_t slot = (size_t)(2 * w + (w == w0 && first != begin)) * pd_slot(HD);
-        const float o = row[slot], m = stat[slot], l = stat[slot + 16];
-        const float mn = fmaxf(M, m), f = __builtin_amdgcn_exp2f(M - mn), e = __builtin_amdgcn_exp2f(m - mn);
+    float M = -1e30f, L = 0.0f;
+    pg_f4 O = pg_f4{0.f, 0.f, 0.f, 0.f};
+    for (int w = w0 + p; w <= j.last; w += GROUPS * PJ_STEP) {
+        pg_f4 o[PJ_STEP];
+        float m[PJ_STEP], l[PJ_STEP], mn = M;
+#pragma unroll
+        for (int i = 0; i < PJ_STEP; i++) {  // (past the last: the last again, with weight 0)
+            const int wi = min(w + i * GROUPS, j.last);
+            const size_t slot = (size_t)(wi == w0 ? j.slot : 2 * wi) * pd_slot(HD);
+            o[i] = *reinterpret_cast<const pg_f4*>(row + slot);
+            m[i] = stat[slot];
+            l[i] = stat[slot + 16];
+        }
+#pragma unroll
+        for (int i = 0; i < PJ_STEP; i++) mn = fmaxf(mn, m[i]);
+        const float f = __builtin_amdgcn_exp2f(M - mn);
         M = mn;
-        L = fmaf(l, e, L * f);
-        O = fmaf(o, e, O * f);
+        L *= f;
+        O *= f;
+#pragma unroll
+        for (int i = 0; i < PJ_STEP; i++) {
+            if (w + i * GROUPS > j.last) break;
+            const float e = __builtin_amdgcn_exp2f(m[i] - mn);
+            L = fmaf(l[i], e, L);
+#pragma unroll
+            for (int k = 0; k < 4; k++) O[k] = fmaf(o[i][k], e, O[k]);
+        }
     }
     s_o[p][d] = O;
     if (d == 0) {
@@ -595,15 +622,22 @@ __global__ __launch_bounds__(PJ_GROUPS * HD) void paged_join_kernel(PagedRows b,
     if (p) return;
     float mx = s_m[0];
 #pragma unroll
-    for (int i = 1; i < PJ_GROUPS; i++) mx = fmaxf(mx, s_m[i]);
-    L = O = 0.0f;
+    for (int i = 1; i < GROUPS; i++) mx = fmaxf(mx, s_m[i]);
+    L = 0.0f;
+    O = pg_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < PJ_GROUPS; i++) {
+    for (int i = 0; i < GROUPS; i++) {
         const float e = __builtin_amdgcn_exp2f(s_m[i] - mx);
         L = fmaf(s_l[i], e, L);
-        O = fmaf(s_o[i][d], e, O);
+        const pg_f4 o = s_o[i][d];
+#pragma unroll
+        for (int k = 0; k < 4; k++) O[k] = fmaf(o[k], e, O[k]);
     }
-    out[(size_t)s * ldo + (size_t)(vh / tiles * grp + h0 + r) * HD + d] = (T)(O / L);
+    T y[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) y[k] = (T)(O[k] / L);
+    __builtin_memcpy(__builtin_assume_aligned(out + (size_t)j.s * ldo + (size_t)(j.vh / tiles * grp + h0 + r) * HD + 4 * d, 8),
+                     y, sizeof y);
 }
 
 // The rows of a batch by binary search over row_start: the last sequence that
@@ -734,14 +768,16 @@ struct DecodeCall {
     hipError_t run() const {
         const int grp = p.n_heads / p.kv.kv_heads, tiles = (grp + 15) / 16;
         const int wgs = pd_wgs(p.rows, p.kv.kv_heads * tiles);
+        const bool cuts = p.rows.cap > PD_UNIT;  // (one unit a sequence: none is cut)
+        float* part = static_cast<float*>(p.work);
+        PdJoin* joins = cuts ? reinterpret_cast<PdJoin*>(part + (size_t)2 * wgs * pd_slot(HD)) : nullptr;
         hipLaunchKernelGGL((paged_decode_kernel<E, T, HD>), dim3(wgs), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp,
-                           tiles, static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo,
-                           static_cast<float*>(p.work));
+                           tiles, static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part,
+                           joins);
         const hipError_t e = hipGetLastError();
-        if (e != hipSuccess || p.rows.cap <= PD_UNIT) return e;  // (one unit a sequence: none is cut)
-        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(wgs, grp < 16 ? grp : 16), dim3(PJ_GROUPS * HD), 0, s,
-                           p.rows, p.kv.kv_heads, grp, tiles, static_cast<const float*>(p.work),
-                           static_cast<T*>(p.out), p.ldo);
+        if (e != hipSuccess || !cuts) return e;
+        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(wgs, grp < 16 ? grp : 16), dim3(PJ_WG), 0, s, joins, part,
+                           grp, tiles, static_cast<T*>(p.out), p.ldo);
         return hipGetLastError();
     }
 };
@@ -751,7 +787,7 @@ struct DecodeCall {
 size_t paged_decode_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     if (r.cap <= PD_UNIT || r.n_seqs == 0) return 0;
     const int grp = n_heads / kv.kv_heads;
-    return (size_t)2 * pd_wgs(r, kv.kv_heads * ((grp + 15) / 16)) * pd_slot(hd) * sizeof(float);
+    return pd_wgs(r, kv.kv_heads * ((grp + 15) / 16)) * (2 * pd_slot(hd) * sizeof(float) + sizeof(PdJoin));
 }
 
 bool paged_decode_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {

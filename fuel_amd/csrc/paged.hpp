@@ -92,33 +92,60 @@ __device__ __forceinline__ PgSeq pg_seq(const PagedRows& b, int s) {
     return q;
 }
 
-// The sequence that holds unit `at` of the batch, where sequence s has
-// units(s) >= 0 of them one after another: s and the unit's number in it, or
-// s = n_seqs past the last.  Every lane of a wavefront takes part (64
-// sequences a step); the result is wave-uniform.
-template <class F>
-__device__ __forceinline__ int pg_find(int n_seqs, int at, F units, int& in_seq) {
-    const int lane = threadIdx.x & 63;
-    int base = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
-        const int u = s0 + lane < n_seqs ? units(s0 + lane) : 0;
-        int sum = u;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int up = __shfl_up(sum, off);
-            if (lane >= off) sum += up;
-        }
-        const uint64_t past = __ballot(base + sum > at);
-        if (past) {
-            const int l = __builtin_ctzll(past);
-            in_seq = at - base - __builtin_amdgcn_readlane(sum - u, l);
-            return s0 + l;
-        }
-        base += __builtin_amdgcn_readlane(sum, 63);
-    }
-    in_seq = 0;
-    return n_seqs;
+// Sums of v over lanes 0 .. the own one, by DPP (a chain of lane shuffles takes
+// ten times as long).
+__device__ __forceinline__ int pg_scan(int v) {
+#define FRQ_DPP_ADD(ctrl, rmask) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rmask, 0xF, false)
+    FRQ_DPP_ADD(0x111, 0xF);  // row_shr 1, 2, 4, 8: sums within each 16-lane row
+    FRQ_DPP_ADD(0x112, 0xF);
+    FRQ_DPP_ADD(0x114, 0xF);
+    FRQ_DPP_ADD(0x118, 0xF);
+    FRQ_DPP_ADD(0x142, 0xA);  // row_bcast:15 -> rows 1, 3 add the row before
+    FRQ_DPP_ADD(0x143, 0xC);  // row_bcast:31 -> rows 2, 3 add rows 0 + 1
+#undef FRQ_DPP_ADD
+    return v;
 }
+
+// The units of a batch's sequences, units(s) >= 0 of sequence s one after
+// another, as one wavefront sees them; the first 64 sequences' stay in
+// registers.  Every lane takes part, results are wave-uniform.
+struct PgUnits {
+    int own, sum;  // lane l: sequence l's units, and those of 0 .. l
+    int total;
+
+    template <class F>
+    __device__ __forceinline__ PgUnits(int n_seqs, F units) {
+        const int lane = threadIdx.x & 63;
+        own = lane < n_seqs ? units(lane) : 0;
+        sum = pg_scan(own);
+        total = __builtin_amdgcn_readlane(sum, 63);
+        for (int s0 = 64; s0 < n_seqs; s0 += 64)
+            total += __builtin_amdgcn_readlane(pg_scan(s0 + lane < n_seqs ? units(s0 + lane) : 0), 63);
+    }
+
+    // The sequence that holds unit `at`, and the unit's number in it; n_seqs
+    // past the last.
+    template <class F>
+    __device__ __forceinline__ int find(int n_seqs, int at, F units, int& in_seq) const {
+        const int lane = threadIdx.x & 63;
+        int base = 0, u = own, s = sum;
+        for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+            if (s0) {
+                u = s0 + lane < n_seqs ? units(s0 + lane) : 0;
+                s = pg_scan(u);
+            }
+            const uint64_t past = __ballot(base + s > at);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                in_seq = at - base - __builtin_amdgcn_readlane(s - u, l);
+                return s0 + l;
+            }
+            base += __builtin_amdgcn_readlane(s, 63);
+        }
+        in_seq = 0;
+        return n_seqs;
+    }
+};
 
 #endif  // __HIPCC__
 
