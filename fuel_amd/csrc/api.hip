@@ -1506,7 +1506,7 @@ int paged_attention(const char* who, bool decode, frq_device* dev, const frq_pag
     a.out = out;
     a.ldo = (int)ldo;
     a.work = work;
-    HIP_TRY((decode ? launch_paged_decode : launch_paged_attend)(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
+    HIP_TRY((decode ? launch_paged_decode : launch_paged_prefill)(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
     return FRQ_OK;
 }
 

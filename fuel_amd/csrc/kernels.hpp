@@ -295,6 +295,8 @@ struct PagedAttendArgs {
 bool paged_decode_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
 size_t paged_decode_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
 hipError_t launch_paged_decode(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
+// Packed rows: paged_prefill.hip.
+hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 
 }  // namespace frq

@@ -710,21 +710,6 @@ __global__ __launch_bounds__(AP_WG) void paged_append_kernel(PagedKv c, PagedRow
     }
 }
 
-// Calls f.template operator()<E, T, HD>() for the types of a call.
-template <class F>
-hipError_t with_types(int kv_dtype, int dtype, int hd, F f) {
-    const bool h64 = hd == 64;
-    if (kv_dtype == GGML_F16 && dtype == GGML_F32)
-        return h64 ? f.template run<_Float16, float, 64>() : f.template run<_Float16, float, 128>();
-    if (kv_dtype == GGML_F16 && dtype == GGML_F16)
-        return h64 ? f.template run<_Float16, _Float16, 64>() : f.template run<_Float16, _Float16, 128>();
-    if (kv_dtype == GGML_BF16 && dtype == GGML_F32)
-        return h64 ? f.template run<__bf16, float, 64>() : f.template run<__bf16, float, 128>();
-    if (kv_dtype == GGML_BF16 && dtype == GGML_BF16)
-        return h64 ? f.template run<__bf16, __bf16, 64>() : f.template run<__bf16, __bf16, 128>();
-    return hipErrorInvalidValue;
-}
-
 struct AppendCall {
     const PagedAppendArgs& p;
     hipStream_t s;
@@ -802,17 +787,17 @@ bool paged_types(int kv_dtype, int dtype) {
 
 hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0) return hipSuccess;
-    return with_types(kv_dtype, dtype, hd, AppendCall{p, s});
+    return paged_with_types(kv_dtype, dtype, hd, AppendCall{p, s});
 }
 
 hipError_t launch_paged_decode(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
-    return with_types(kv_dtype, dtype, hd, DecodeCall{p, s});
+    return paged_with_types(kv_dtype, dtype, hd, DecodeCall{p, s});
 }
 
 hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
-    return with_types(kv_dtype, dtype, hd, AttendCall{p, s});
+    return paged_with_types(kv_dtype, dtype, hd, AttendCall{p, s});
 }
 
 }  // namespace frq

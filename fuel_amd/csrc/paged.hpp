@@ -17,6 +17,8 @@
 
 #include <type_traits>
 
+#include "common.hpp"
+
 namespace frq {
 
 struct PagedKv {
@@ -146,6 +148,21 @@ struct PgUnits {
         return n_seqs;
     }
 };
+
+// Calls f.run<E, T, HD>() for the types of a call.
+template <class F>
+hipError_t paged_with_types(int kv_dtype, int dtype, int hd, F f) {
+    const bool h64 = hd == 64;
+    if (kv_dtype == GGML_F16 && dtype == GGML_F32)
+        return h64 ? f.template run<_Float16, float, 64>() : f.template run<_Float16, float, 128>();
+    if (kv_dtype == GGML_F16 && dtype == GGML_F16)
+        return h64 ? f.template run<_Float16, _Float16, 64>() : f.template run<_Float16, _Float16, 128>();
+    if (kv_dtype == GGML_BF16 && dtype == GGML_F32)
+        return h64 ? f.template run<__bf16, float, 64>() : f.template run<__bf16, float, 128>();
+    if (kv_dtype == GGML_BF16 && dtype == GGML_BF16)
+        return h64 ? f.template run<__bf16, __bf16, 64>() : f.template run<__bf16, __bf16, 128>();
+    return hipErrorInvalidValue;
+}
 
 #endif  // __HIPCC__
 

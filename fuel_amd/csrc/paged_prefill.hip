@@ -1,0 +1,378 @@
+// Causal attention of packed prompt rows over a paged KV cache (paged.hpp).
+//
+// A sequence's rows and the G = n_heads / kv_heads query heads of a KV head are
+// one list of n * G query rows, as in paged.hip; a workgroup takes PF_ROWS of
+// them, 32 a wavefront, and walks the keys in tiles of 64 that it stages in LDS,
+// shared by its four wavefronts: the next tile's LDS DMA runs while a tile is
+// worked, one barrier a tile.
+//   S^T (keys x rows) = K . Q^T on v_mfma_f32_32x32x16: the C layout leaves lane
+//     32 h + n keys 8 i + 4 h + (0..3) of row n, which is what the second
+//     product takes as its B operand, in a key order that V's reads follow: P
+//     never moves between lanes.
+//   O^T (dims x rows) += V^T . P^T: V^T comes out of the row-major V tile by the
+//     transposing LDS read (ds_read_b64_tr_b16).
+// LDS rows are kept unpadded (the DMA writes them in lane order); the DMA's
+// source addresses permute the 16-byte chunks of a row instead, so that the
+// rows one read touches fall in different banks.
+// The running maximum is renewed only when a row's scores pass it by 2^PF_LAZY:
+// the weights stay below 2^(PF_SHIFT + PF_LAZY) = 2^15, in f16's range, and the
+// sums and the output share the factor whatever it is.
+// 16-bit activations: p is rounded to the cache's type for the second product
+// (a relative 2^-11 or 2^-8 of each weight at most, the output's own rounding;
+// the sum l takes p as it is).  A second part, as the decode keeps, would cost
+// half as many matrix instructions again, which are the bound here.  f32
+// activations: q and p in parts that keep f32's precision.
+#include <hip/hip_runtime.h>
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "paged.hpp"
+
+namespace frq {
+
+namespace {
+
+constexpr int PF_WAVES = 4;
+constexpr int PF_KEYS = 64;
+constexpr float PF_SHIFT = 8.0f, PF_LAZY = 7.0f;
+
+typedef float pf_f16 __attribute__((ext_vector_type(16)));
+typedef short pf_s4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ pf_f16 pf_mfma(PgElem<_Float16>::v8 a, PgElem<_Float16>::v8 b, pf_f16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ pf_f16 pf_mfma(PgElem<__bf16>::v8 a, PgElem<__bf16>::v8 b, pf_f16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// 64 lanes' 16 bytes from base + voff to LDS address lds + 16 * lane.  Written
+// in assembly so that the compiler does not wait for it before every LDS read
+// (it cannot tell the tile being filled from the one being read): the kernel
+// waits itself.  The wait states cover M0 and a base that a lane read made.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void pf_dma(const void* base, uint32_t voff, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds)
+                 : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ uint32_t pf_lds(const void* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) uint8_t*)p;
+}
+__device__ __forceinline__ pf_s4 pf_read_tr(const uint8_t* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pf_s4*)p);
+}
+
+__device__ __forceinline__ float pf_other_half(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? (uint32_t)a[0] : (uint32_t)a[1]);
+}
+
+template <class E, class T, int HD>
+struct PrefillTile {
+    using P = PgElem<E>;
+    using v8 = typename P::v8;
+    static constexpr bool WIDE = std::is_same<T, float>::value;
+    static constexpr int NP = WIDE ? P::SPLIT : 1;
+    static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
+    static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
+    static constexpr int RPI = 512 / HD, NI = HD / 32;  // rows a DMA instruction, instructions a wavefront and tile
+    static constexpr int ROWS = 32 * PF_WAVES;
+};
+
+template <class E, class T, int HD>
+__global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv c, PagedRows b, int grp,
+                                                                         const T* __restrict__ q, int ldq, float scale,
+                                                                         T* __restrict__ out, int ldo) {
+    using X = PrefillTile<E, T, HD>;
+    using v8 = typename X::v8;
+    __shared__ __align__(1024) uint8_t s_k[2][X::TILE], s_v[2][X::TILE];
+    __shared__ uint32_t s_odd[2];
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int head = blockIdx.x % c.kv_heads;
+    // the tiles with the most keys first: the last ones of each sequence
+    const auto units = [&](int i) { return (int)(((long)pg_seq(b, i).n * grp + X::ROWS - 1) / X::ROWS); };
+    const PgUnits pu(b.n_seqs, units);
+    const int unit = pu.total - 1 - (int)(blockIdx.x / c.kv_heads);
+    if (unit < 0) return;
+    int tile;
+    const int s = pu.find(b.n_seqs, unit, units, tile);
+    const PgSeq sq = pg_seq(b, s);
+    const int rows = sq.n * grp, i0 = tile * X::ROWS;
+    const int mine = min(i0 + 32 * w + n, rows - 1);
+    const int row = sq.row0 + mine / grp, qh = head * grp + mine % grp;
+    const int pos0 = sq.kv - sq.n;
+    const int limit = pos0 + mine / grp;
+    // first and last position of the workgroup's and of this wavefront's rows
+    const int wg_first = pos0 + i0 / grp, wg_last = pos0 + min(i0 + X::ROWS - 1, rows - 1) / grp;
+    const int first = pos0 + min(i0 + 32 * w, rows - 1) / grp;
+    const int last = i0 + 32 * w < rows ? pos0 + min(i0 + 32 * w + 31, rows - 1) / grp : -1;
+    const int tiles = wg_last >= 0 ? wg_last / PF_KEYS + 1 : 0;
+
+    // Q^T, the B operand: dims 16 t + 8 h + e of row n
+    v8 qf[X::NP][X::KS];
+    float factor = fabsf(scale) * 1.4426950408889634f;
+    {
+        const T* x = q + (size_t)row * ldq + (size_t)qh * HD;
+        float f[X::KS][8], a = 0.0f;
+#pragma unroll
+        for (int t = 0; t < X::KS; t++) {
+            T raw[8];
+            __builtin_memcpy(raw, __builtin_assume_aligned(x + 16 * t + 8 * h, 16), sizeof raw);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                f[t][e] = scale < 0.0f ? -(float)raw[e] : (float)raw[e];
+                a = fmaxf(a, fabsf(f[t][e]));
+            }
+        }
+        int ex = 0;
+        if constexpr (X::WIDE && std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
+            a = fmaxf(a, pf_other_half(a));
+            if (a > 0.0f && a < __builtin_inff()) ex = min(120, max(-120, __builtin_amdgcn_frexp_expf(a)));
+            factor = __builtin_amdgcn_ldexpf(factor, ex);
+        }
+#pragma unroll
+        for (int t = 0; t < X::KS; t++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                float rest = __builtin_amdgcn_ldexpf(f[t][e], -ex);
+#pragma unroll
+                for (int p = 0; p < X::NP; p++) {
+                    qf[p][t][e] = (E)rest;
+                    rest -= (float)qf[p][t][e];
+                }
+            }
+    }
+
+    pf_f16 o[X::DT];
+#pragma unroll
+    for (int d = 0; d < X::DT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+    float m = -1e30f, l = 0.0f;
+
+    // DMA source offsets: chunk pc of LDS row r holds the row's chunk pc ^ (r & 7)
+    // of K, pc ^ 2 (r & 3) of V
+    constexpr int CPR = HD / 8;
+    const int dr = w * X::RPI + lane / CPR, pc = lane % CPR;
+    const uint32_t koff = (lane / CPR) * X::ROW + 16 * (pc ^ (dr & 7));
+    const uint32_t voff = (lane / CPR) * X::ROW + 16 * (pc ^ (2 * (dr & 3)));
+    const int* table = b.table + (size_t)s * b.max_pages;
+    // page ids of 64 groups of 16 keys, lane i that of group i from key id0 on
+    int id0 = 0, id = 0;
+    auto fetch_ids = [&](int j0) {
+        id0 = j0;
+        const int j = j0 + 16 * lane;
+        id = j < sq.kv ? table[j >> c.log_ps] : 0;
+    };
+    auto issue = [&](int t) {
+        const int j0 = t * PF_KEYS;
+        if (j0 - id0 >= 1024) fetch_ids(j0);
+#pragma unroll
+        for (int i = 0; i < X::NI; i++) {
+            const int r0 = (i * PF_WAVES + w) * X::RPI;
+            int page = __builtin_amdgcn_readlane(id, (j0 - id0 + r0) >> 4);
+            if ((unsigned)page >= (unsigned)c.n_pages) page = 0;
+            const size_t at = ((((size_t)page * c.kv_heads + head) << c.log_ps) + ((j0 + r0) & ((1 << c.log_ps) - 1))) * X::ROW;
+            const uint32_t to = (i * PF_WAVES + w) * 1024;
+            pf_dma(static_cast<const uint8_t*>(c.k) + at, koff, pf_lds(s_k[t & 1]) + to);
+            pf_dma(static_cast<const uint8_t*>(c.v) + at, voff, pf_lds(s_v[t & 1]) + to);
+        }
+    };
+    // LDS read offsets of this lane: K row n (+ 32), chunks 2 t + h; V rows
+    // 4 h + (lane / 4) % 4 (+ 16 k + 8 j), dims 16 ((lane / 16) % 2) + 4 (lane % 4) (+ 32 d)
+    const uint32_t kbase = n * X::ROW + 16 * (h ^ (n & 7));
+    const int vr = (lane >> 2) & 3;
+    const uint32_t vbase = (4 * h + vr) * X::ROW + 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ (2 * vr)) + 8 * (lane & 1);
+
+    if (tiles) {
+        fetch_ids(0);
+        issue(0);
+    }
+    for (int t = 0; t < tiles; t++) {
+        const int j0 = t * PF_KEYS;
+        // tile t landed, in every wavefront, and tile t - 1 is read
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        // pages that are none, one bit a group of 16 keys
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < PF_KEYS / 16; i++)
+            bad |= (uint32_t)((unsigned)__builtin_amdgcn_readlane(id, ((j0 - id0) >> 4) + i) >= (unsigned)c.n_pages) << i;
+        const bool masked = j0 + PF_KEYS - 1 > wg_first || bad;
+        uint64_t odd = 0;
+        if (masked) {
+            // rows of V that are no keys are cleared, so are infinite and NaN
+            // values, whose keys are noted: 0 * inf must not reach the rows
+            // that do not see them
+            if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+            __syncthreads();
+            for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
+                const int r = ch / CPR;
+                uint4* at = reinterpret_cast<uint4*>(s_v[t & 1]) + ch;
+                const uint4 u = *at;
+                uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                const bool none = j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1);
+                bool hit = false;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (pg_word_inf<E>(x[k])) {
+                        hit = true;
+                        x[k] = 0;
+                    }
+                }
+                if (none || hit) *at = none ? make_uint4(0, 0, 0, 0) : make_uint4(x[0], x[1], x[2], x[3]);
+                if (hit && !none) atomicOr(&s_odd[r >> 5], 1u << (r & 31));
+            }
+            __syncthreads();
+            odd = (uint64_t)s_odd[1] << 32 | s_odd[0];
+        }
+        const int id_now = id, id0_now = id0;
+        if (t + 1 < tiles) issue(t + 1);
+        if (j0 > last) continue;
+
+        const uint8_t* kt = s_k[t & 1];
+        const uint8_t* vt = s_v[t & 1];
+        pf_f16 st[2];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) st[a][i] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < X::KS; k++) {
+                const v8 kf = *reinterpret_cast<const v8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
+#pragma unroll
+                for (int p = X::NP - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
+            }
+        }
+        const bool mask = j0 + PF_KEYS - 1 > first || bad;
+        if (mask) {
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int r = 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h;
+                    if ((bad >> (r >> 4)) & 1) st[a][i] = pg_nan();
+                    if (j0 + r > limit) st[a][i] = -__builtin_inff();
+                }
+        }
+        float top = st[0][0];
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
+        top = fmaxf(top, pf_other_half(top)) * factor;
+        if (__any(top > m + PF_LAZY)) {
+            const float mn = fmaxf(m, top);
+            const float f = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before)
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < X::DT; d++) o[d] *= f;
+        }
+        const float ms = m - PF_SHIFT;
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) st[a][i] = fmaf(st[a][i], factor, -ms);
+        if (mask) {  // (again: a factor of 0 would make NaN of -inf)
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (j0 + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h > limit) st[a][i] = -__builtin_inff();
+        }
+        v8 pp[X::NP][4];
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                st[a][i] = __builtin_amdgcn_exp2f(st[a][i]);
+                l += st[a][i];
+                float rest = st[a][i];
+#pragma unroll
+                for (int p = 0; p < X::NP; p++) {
+                    pp[p][2 * a + (i >> 3)][i & 7] = (E)rest;
+                    rest -= (float)pp[p][2 * a + (i >> 3)][i & 7];
+                }
+            }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int d = 0; d < X::DT; d++) {
+                const uint8_t* at = vt + 16 * k * X::ROW + (vbase ^ (64 * d));
+                const pf_s4 lo = pf_read_tr(at), hi = pf_read_tr(at + 8 * X::ROW);
+                const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                for (int p = X::NP - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
+            }
+        if (masked) {
+            for (; odd; odd &= odd - 1) {  // the cleared values, for the rows that see them
+                const int r = __builtin_ctzll(odd);
+                float p = 0.0f;
+#pragma unroll
+                for (int a = 0; a < 2; a++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (32 * a + (i & 3) + 8 * (i >> 2) == (r & ~4)) p = st[a][i];
+                const float q2 = pf_other_half(p);
+                p = ((r >> 2) & 1) == h ? p : q2;
+                const int page = __builtin_amdgcn_readlane(id_now, (j0 - id0_now + r) >> 4);
+                const E* src = static_cast<const E*>(c.v) +
+                               ((((size_t)page * c.kv_heads + head) << c.log_ps) + ((j0 + r) & ((1 << c.log_ps) - 1))) * HD;
+                if (j0 + r > limit) continue;
+#pragma unroll
+                for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float v = (float)src[32 * d + (i & 3) + 8 * (i >> 2) + 4 * h];
+                        if (!(fabsf(v) < __builtin_inff())) o[d][i] = fmaf(p, v, o[d][i]);
+                    }
+            }
+        }
+    }
+    l += pf_other_half(l);
+    if (i0 + 32 * w + n >= rows) return;
+    const float inv = 1.0f / l;
+    T* dst = out + (size_t)row * ldo + (size_t)qh * HD + 4 * h;
+#pragma unroll
+    for (int d = 0; d < X::DT; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            T y[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float x = o[d][4 * g + i] * inv;
+                y[i] = (T)(sq.bad ? pg_nan() : limit < 0 ? 0.0f : x);
+            }
+            __builtin_memcpy(__builtin_assume_aligned(dst + 32 * d + 8 * g, 8), y, sizeof y);
+        }
+}
+
+struct PrefillCall {
+    const PagedAttendArgs& p;
+    hipStream_t s;
+    template <class E, class T, int HD>
+    hipError_t run() const {
+        const int grp = p.n_heads / p.kv.kv_heads;
+        // a bound on the tiles: each sequence's last may be partly empty
+        const long tiles = (long)p.rows.rows * grp / PrefillTile<E, T, HD>::ROWS + p.rows.n_seqs;
+        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD>), dim3((unsigned)(tiles * p.kv.kv_heads)),
+                           dim3(64 * PF_WAVES), 0, s, p.kv, p.rows, grp, static_cast<const T*>(p.q), p.ldq, p.scale,
+                           static_cast<T*>(p.out), p.ldo);
+        return hipGetLastError();
+    }
+};
+
+}  // namespace
+
+hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
+    if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
+    return paged_with_types(kv_dtype, dtype, hd, PrefillCall{p, s});
+}
+
+}  // namespace frq
