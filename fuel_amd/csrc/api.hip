@@ -1478,7 +1478,12 @@ int paged_operand(const char* who, const char* name, int dtype, const void* p, s
     return FRQ_OK;
 }
 
-int paged_attention(const char* who, bool decode, frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
+// Which attention kernel a call takes.
+bool paged_takes_rows16(const PagedKv& kv, const PagedRows& r, int n_heads) {
+    return !r.row_start || (long)r.rows * n_heads <= (long)r.n_seqs * kv.kv_heads * 32 || (long)r.rows * n_heads <= 8192;
+}
+
+int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
                     size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes, void* out,
                     size_t ldo) {
     int rc;
@@ -1486,7 +1491,8 @@ int paged_attention(const char* who, bool decode, frq_device* dev, const frq_pag
     if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
     if (!paged_types(kv->dtype, dtype))
         return fail(FRQ_UNSUPPORTED, "%s: dtype %d over a cache of dtype %d", who, dtype, kv->dtype);
-    if (decode && !paged_decode_fits(a.kv, a.rows, (int)n_heads))
+    const bool rows16 = paged_takes_rows16(a.kv, a.rows, (int)n_heads);
+    if (rows16 && !paged_rows16_fits(a.kv, a.rows, (int)n_heads))
         return fail(FRQ_UNSUPPORTED, "%s: n_seqs=%zu of up to %d tokens", who, b->n_seqs, a.rows.cap);
     const bool none = b->n_seqs == 0 || b->rows == 0;
     const size_t need = frq_paged_attention_workspace(kv, b, n_heads);
@@ -1506,7 +1512,7 @@ int paged_attention(const char* who, bool decode, frq_device* dev, const frq_pag
     a.out = out;
     a.ldo = (int)ldo;
     a.work = work;
-    HIP_TRY((decode ? launch_paged_decode : launch_paged_prefill)(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
+    HIP_TRY((rows16 ? launch_paged_rows16 : launch_paged_prefill)(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
     return FRQ_OK;
 }
 
@@ -1556,7 +1562,7 @@ size_t frq_paged_attention_workspace(const frq_paged_kv* kv, const frq_paged_bat
     PagedKv k;
     PagedRows r;
     if (paged_args("paged_attention_workspace", kv, b, n_heads, &k, &r)) return 0;
-    return r.row_start ? 0 : paged_decode_work_bytes(k, r, (int)n_heads, (int)kv->head_dim);
+    return paged_takes_rows16(k, r, (int)n_heads) ? paged_rows16_work_bytes(k, r, (int)n_heads, (int)kv->head_dim) : 0;
 }
 
 int frq_paged_attention_decode(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
@@ -1564,14 +1570,14 @@ int frq_paged_attention_decode(frq_device* dev, const frq_paged_kv* kv, const fr
                                void* out, size_t ldo) {
     if (b && b->row_start)
         return fail(FRQ_INVALID, "paged_attention_decode: one row a sequence (row_start must be NULL)");
-    return paged_attention("paged_attention_decode", true, dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
+    return paged_attention("paged_attention_decode", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
                            out, ldo);
 }
 
 int frq_paged_attention_prefill(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
                                 size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes,
                                 void* out, size_t ldo) {
-    return paged_attention("paged_attention_prefill", false, dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
+    return paged_attention("paged_attention_prefill", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
                            out, ldo);
 }
 

@@ -290,13 +290,12 @@ struct PagedAttendArgs {
     int ldo;
     void* work;
 };
-// One row a sequence: units over all workgroups, cut sequences joined (work of
-// paged_decode_work_bytes()); paged_decode_fits: their count fits an int.
-bool paged_decode_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
-size_t paged_decode_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
-hipError_t launch_paged_decode(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
-// Packed rows: paged_prefill.hip.
+// Few rows a sequence: 16-row tiles, the keys over all workgroups, cut tiles
+// joined (work of paged_rows16_work_bytes()); fits: the units are an int.
+bool paged_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
+size_t paged_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
+hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
+// paged_prefill.hip: many rows a sequence, 128-row tiles.
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
-hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 
 }  // namespace frq

@@ -264,159 +264,35 @@ struct Rows16 {
     }
 };
 
-// The walk of one wavefront over keys [j0, j1) (j0 a multiple of 32) of a
-// sequence for the 16 rows of `a`: no row sees a key >= j1.
-template <class E, class T, int HD>
-__device__ void pa_walk(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int head, int j0, int j1, int kv,
-                        int all_see) {
-    using A = Rows16<E, T, HD>;
-    typename A::KeyRegs kr;
-    typename A::ValueRegs vr;
-    for (; j0 < j1; j0 += 32) {
-        typename A::Mask mk{j0, kv, {false, false}};
-        const E* ka[2];
-        const E* va[2];
-#pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const int j = j0 + 16 * g;
-            // (a group past the length has no page: its keys are masked)
-            const int page = j < kv ? table[j >> c.log_ps] : 0;
-            mk.bad[g] = (unsigned)page >= (unsigned)c.n_pages;
-            const size_t at =
-                (((size_t)(mk.bad[g] ? 0 : page) * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1));
-            ka[g] = static_cast<const E*>(c.k) + at * HD;
-            va[g] = static_cast<const E*>(c.v) + at * HD;
-        }
-        A::load_k(kr, ka);
-        A::load_v(vr, va);
-        float s[8];
-        typename A::v8 pp[A::NP];
-        if (j0 + 31 <= all_see && !mk.bad[0] && !mk.bad[1]) {
-            a.template scores<false>(kr, mk, s);
-            a.weights(s, pp);
-            a.product(vr, pp);
-        } else {
-            a.template scores<true>(kr, mk, s);
-            a.weights(s, pp);
-            if (__any(A::clear(vr, mk))) a.product_seen(s, mk, va);
-            else a.product(vr, pp);
-        }
-    }
-}
-
-// One workgroup: 16 query rows of one KV head, workgroup tile * kv_heads + head
-// of the batch's tiles; its wavefronts take contiguous quarters of the keys and are
-// merged through LDS in wavefront order.
-template <class E, class T, int HD>
-__global__ __launch_bounds__(64 * PA_WAVES) void paged_attend_kernel(PagedKv c, PagedRows b, int grp,
-                                                                     const T* __restrict__ q, int ldq, float scale,
-                                                                     T* __restrict__ out, int ldo) {
-    using A = Rows16<E, T, HD>;
-    constexpr int NO = 4 * A::VW;
-    __shared__ float s_o[PA_WAVES - 1][NO][64];
-    __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int head = blockIdx.x % c.kv_heads;
-    int tile;
-    const auto units = [&](int i) { return (pg_seq(b, i).n * grp + 15) / 16; };
-    const int s = PgUnits(b.n_seqs, units).find(b.n_seqs, blockIdx.x / c.kv_heads, units, tile);
-    if (s >= b.n_seqs) return;
-    const PgSeq sq = pg_seq(b, s);
-    const int n = sq.n * grp, i0 = 16 * tile;
-    const int i = min(i0 + r, n - 1);
-    const int row = sq.row0 + i / grp, h = head * grp + i % grp;
-    A a;
-    a.load_q(q + (size_t)row * ldq + (size_t)h * HD, scale);
-    a.limit = sq.kv - sq.n + i / grp;
-    a.start();
-    const int first = sq.kv - sq.n + i0 / grp;                        // the tile's first and last positions
-    const int last = sq.kv - sq.n + min(i0 + 15, n - 1) / grp;
-    const int blocks = last >= 0 ? last / 32 + 1 : 0, per = (blocks + PA_WAVES - 1) / PA_WAVES;
-    pa_walk<E, T, HD>(a, c, b.table + (size_t)s * b.max_pages, head, 32 * w * per,
-                      min(last + 1, 32 * (w + 1) * per), sq.kv, first);
-    a.finish();
-    if (w > 0) {
-#pragma unroll
-        for (int t = 0; t < A::VW; t++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) s_o[w - 1][4 * t + k][lane] = a.o[t][k];
-    }
-    if (g == 0) {
-        s_m[w][r] = a.m;
-        s_l[w][r] = a.l;
-    }
-    __syncthreads();
-    if (w == 0 && i0 + r < n) {
-        float mx = s_m[0][r], l = 0.0f, wt[PA_WAVES];
-#pragma unroll
-        for (int v = 1; v < PA_WAVES; v++) mx = fmaxf(mx, s_m[v][r]);
-#pragma unroll
-        for (int v = 0; v < PA_WAVES; v++) {
-            wt[v] = __builtin_amdgcn_exp2f(s_m[v][r] - mx);
-            l += s_l[v][r] * wt[v];
-        }
-        const float inv = 1.0f / l;
-        T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            T res[A::VW];
-#pragma unroll
-            for (int t = 0; t < A::VW; t++) {
-                float x = a.o[t][k] * wt[0];
-#pragma unroll
-                for (int v = 1; v < PA_WAVES; v++) x = fmaf(s_o[v - 1][4 * t + k][lane], wt[v], x);
-                x = sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : x * inv;
-                res[t] = (T)x;
-            }
-            __builtin_memcpy(__builtin_assume_aligned(dst + A::VW * k, 8), res, sizeof res);
-        }
-    }
-}
-
-// ---- one new token per sequence ----
+// ---- few rows a sequence ----
 //
-// The keys of all sequences and KV heads are one list of units of PD_UNIT keys
-// (head by head, within a head sequence by sequence), cut into equal
-// contiguous ranges, one per workgroup: a batch of very different lengths
-// keeps every CU busy to the end, and the host needs to know no length.  A
-// range covers the end of one sequence, some whole ones and the start of
-// another; whole ones are written out, the cut pieces (at most two a
-// workgroup) leave their sums in the workspace for paged_join_kernel.
+// The query rows of a sequence and KV head in tiles of 16, and for each tile
+// the sequence's keys in units of `unit` keys, are one list (head by head,
+// within a head sequence by sequence, tile by tile), cut into equal contiguous
+// ranges, one per workgroup: a batch of very different lengths keeps every CU
+// busy to the end, and the host needs to know no length.  A range covers the
+// end of one tile, some whole ones and the start of another; whole ones are
+// written out, the cut pieces (at most two a workgroup) leave their sums in
+// the workspace for paged_join_kernel.
 constexpr int PD_UNIT = 32 * PA_WAVES;
-constexpr int PD_WGS = 512;  // two a CU, all resident at once
+// Workgroups a CU that the registers allow, all resident at once.
+constexpr int pd_per_cu(int hd) { return hd == 64 ? 3 : 2; }
+constexpr int pd_wgs(int hd) { return 256 * pd_per_cu(hd); }
 
-// The workspace: two slots a workgroup, o [16][HD] (unnormalized), m [16],
-// l [16] of a cut piece; then what each workgroup leaves to be joined.
-constexpr int pd_slot(int hd) { return 16 * hd + 32; }
-struct PdJoin {
-    int s;     // sequence, or -1: none of the workgroup's is cut behind it
-    int vh;    // row tile of a KV head
-    int last;  // workgroup of the sequence's last piece
-    int slot;  // of its first piece
-};
+// Tiles of a sequence, and units of each; one without keys has one unit, which
+// writes its rows.
+__device__ __forceinline__ int pd_tiles(const PgSeq& q, int grp) { return (q.n * grp + 15) >> 4; }
+__device__ __forceinline__ int pd_units(const PgSeq& q, int unit) { return q.kv <= unit ? 1 : (q.kv + unit - 1) / unit; }
 
-// Units of a sequence; one without keys has one, which writes its rows.
-__device__ __forceinline__ int pd_units(const PagedRows& b, int s) {
-    const int kv = b.kv_len[s];
-    return kv <= 0 || kv > b.cap ? 1 : (kv + PD_UNIT - 1) / PD_UNIT;
-}
-// Of n_wgs <= total workgroups, w's range starts at unit w * total / n_wgs: none is empty.
-__device__ __forceinline__ int pd_start(int w, int total, int n_wgs) { return (int)((long)w * total / n_wgs); }
-// The workgroup whose range holds unit u: the largest w with pd_start(w) <= u.
-__device__ __forceinline__ int pd_owner(int u, int total, int n_wgs) {
-    return (int)((((long)u + 1) * n_wgs - 1) / total);
-}
-
-// One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of 32;
-// j1 too, or kv).  The next block's keys are loaded as soon as this one's
-// scores are formed, its values as soon as this one's product is: one or the
-// other is in flight all the time, in one set of registers each (two sets
-// spill at HD 128).  The page ids of 1024 keys are one load, lane i holding
-// the page of group i.
+// One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of 32).
+// The next block's keys are loaded as soon as this one's scores are formed, its
+// values as soon as this one's product is: one or the other is in flight all
+// the time, in one set of registers each (two sets spill at HD 128).  The page
+// ids of 1024 keys are one load, lane i holding the page of group i.  Every row
+// sees the keys up to all_see.
 template <class E, class T, int HD>
 __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int head, int j0,
-                                        int j1, int kv) {
+                                        int j1, int kv, int all_see) {
     using A = Rows16<E, T, HD>;
     const int lane = threadIdx.x & 63;
     while (j0 < j1) {
@@ -424,7 +300,7 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
         const int jl = j0 + 16 * lane;
         const int id = jl < kv ? table[jl >> c.log_ps] : 0;
         const bool off = (unsigned)id >= (unsigned)c.n_pages;
-        if (__any(off && jl < end)) a.l = pg_nan();  // a page that is none, and every row sees its keys
+        const uint64_t none = __ballot(off && jl < end);  // groups whose page is none
         const int page = off ? 0 : id;
         auto rows = [&](const void* pool, int blk, const E* (&at)[2]) {
 #pragma unroll
@@ -440,12 +316,32 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
         typename A::ValueRegs vr;
         float s[8];
         typename A::v8 pp[A::NP];
-        typename A::Mask mk{j0 + 32 * last, kv, {false, false}};
         rows(c.k, 0, at);
         A::load_k(kr, at);
         rows(c.v, 0, at);
         A::load_v(vr, at);
-        for (int i = 0; i < last; i++) {
+        for (int i = 0;; i++) {
+            const int j = j0 + 32 * i;
+            const uint32_t bad = (uint32_t)(none >> (2 * i)) & 3;
+            const typename A::Mask mk{j, kv, {(bad & 1) != 0, (bad & 2) != 0}};
+            const bool mask = j + 31 > all_see || bad;
+            if (i == last || mask) {  // (apart from the loop's body, which keeps its loads in flight)
+                if (mask) a.template scores<true>(kr, mk, s);
+                else a.template scores<false>(kr, mk, s);
+                a.weights(s, pp);
+                if (mask && __any(A::clear(vr, mk))) {
+                    rows(c.v, i, at);
+                    a.product_seen(s, mk, at);
+                } else {
+                    a.product(vr, pp);
+                }
+                if (i == last) break;
+                rows(c.k, i + 1, at);
+                A::load_k(kr, at);
+                rows(c.v, i + 1, at);
+                A::load_v(vr, at);
+                continue;
+            }
             a.template scores<false>(kr, mk, s);
             rows(c.k, i + 1, at);
             A::load_k(kr, at);
@@ -454,53 +350,58 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
             rows(c.v, i + 1, at);
             A::load_v(vr, at);
         }
-        if (mk.j0 + 32 <= kv) {
-            a.template scores<false>(kr, mk, s);
-        } else {
-            a.template scores<true>(kr, mk, s);
-            A::clear(vr, mk);
-        }
-        a.weights(s, pp);
-        a.product(vr, pp);
         j0 = end;
     }
 }
 
 template <class E, class T, int HD>
-__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv c, PagedRows b, int grp, int tiles,
+__global__ __launch_bounds__(64 * PA_WAVES, pd_per_cu(HD)) void paged_rows16_kernel(PagedKv c, PagedRows b, int grp, int unit,
                                                                         const T* __restrict__ q, int ldq, float scale,
                                                                         T* __restrict__ out, int ldo,
                                                                         float* __restrict__ part,
-                                                                        PdJoin* __restrict__ joins) {
+                                                                        PgJoin* __restrict__ joins) {
     using A = Rows16<E, T, HD>;
     constexpr int NO = 4 * A::VW;
     __shared__ float s_o[PA_WAVES - 1][NO][64];
     __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const auto units_of = [&](int i) { return pd_units(b, i); };
+    const auto units_of = [&](int i) {
+        const PgSeq sq = pg_seq(b, i);
+        return pd_tiles(sq, grp) * pd_units(sq, unit);
+    };
     const PgUnits pu(b.n_seqs, units_of);
-    const int units = pu.total, total = units * c.kv_heads * tiles, n_wgs = min((int)gridDim.x, total);
+    const int units = pu.total, total = units * c.kv_heads, n_wgs = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= n_wgs) {
-        if (joins && threadIdx.x == 0) joins[blockIdx.x].s = -1;
+        if (joins && threadIdx.x == 0) joins[blockIdx.x].rows = 0;
         return;
     }
-    const int begin = pd_start(blockIdx.x, total, n_wgs), stop = pd_start(blockIdx.x + 1, total, n_wgs);
-    int vh = begin / units, u;
-    int s = pu.find(b.n_seqs, begin - vh * units, units_of, u);
+    const int begin = pg_start(blockIdx.x, total, n_wgs), stop = pg_start(blockIdx.x + 1, total, n_wgs);
+    int head = (unsigned)begin / (unsigned)units, u;
+    int s = pu.find(b.n_seqs, begin - head * units, units_of, u);
     for (int at = begin; at < stop;) {
-        const int n = pd_units(b, s), m = min(n - u, stop - at);  // units u .. u + m - 1 of sequence s
         const PgSeq sq = pg_seq(b, s);
-        const int head = vh / tiles, h0 = (vh % tiles) * 16, rows = min(16, grp - h0);
-        const int h = head * grp + h0 + min(r, rows - 1);
+        const int all = sq.n * grp, nt = pd_tiles(sq, grp), n = pd_units(sq, unit);
+        if (nt == 0) {  // (a sequence without rows)
+            u = 0;
+            if (++s == b.n_seqs) {
+                s = 0;
+                head++;
+            }
+            continue;
+        }
+        const int tile = u / n, u0 = u - tile * n, m = min(n - u0, stop - at);  // units u0 .. u0 + m - 1 of the tile
+        const int i0 = 16 * tile, i = min(i0 + r, all - 1), pos0 = sq.kv - sq.n;
+        const int row = sq.row0 + i / grp, h = head * grp + i % grp;
         A a;
-        a.load_q(q + (size_t)s * ldq + (size_t)h * HD, scale);
-        a.limit = sq.kv - 1;
+        a.load_q(q + (size_t)row * ldq + (size_t)h * HD, scale);
+        a.limit = pos0 + i / grp;
         a.start();
-        const int k0 = u * PD_UNIT, k1 = min(sq.kv, (u + m) * PD_UNIT);
+        const int first = pos0 + i0 / grp, seen = pos0 + min(i0 + 15, all - 1) / grp + 1;  // keys that some row sees
+        const int k0 = u0 * unit, k1 = max(k0, min(seen, (u0 + m) * unit));
         const int per = ((k1 - k0 + 31) / 32 + PA_WAVES - 1) / PA_WAVES;
         pd_walk<E, T, HD>(a, c, b.table + (size_t)s * b.max_pages, head, k0 + 32 * w * per,
-                          min(k1, k0 + 32 * (w + 1) * per), sq.kv);
+                          min(k1, k0 + 32 * (w + 1) * per), sq.kv, first);
         a.finish();
         if (w > 0) {
 #pragma unroll
@@ -513,7 +414,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv 
             s_l[w][r] = a.l;
         }
         __syncthreads();
-        if (w == 0 && r < rows) {
+        const bool whole = m == n;
+        if (w == 0 && i0 + r < all) {
             float mx = s_m[0][r], l = 0.0f, wt[PA_WAVES];
 #pragma unroll
             for (int v = 1; v < PA_WAVES; v++) mx = fmaxf(mx, s_m[v][r]);
@@ -522,10 +424,9 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv 
                 wt[v] = __builtin_amdgcn_exp2f(s_m[v][r] - mx);
                 l += s_l[v][r] * wt[v];
             }
-            const bool whole = m == n;
-            float* slot = part + ((size_t)2 * blockIdx.x + (at != begin)) * pd_slot(HD);
+            float* slot = part + ((size_t)2 * blockIdx.x + (at != begin)) * pg_slot(16, HD);
             const float inv = whole ? 1.0f / l : 1.0f;
-            T* dst = out + (size_t)s * ldo + (size_t)h * HD + 4 * A::VW * g;
+            T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 float x[A::VW];
@@ -534,7 +435,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv 
                     x[t] = a.o[t][k] * wt[0];
 #pragma unroll
                     for (int v = 1; v < PA_WAVES; v++) x[t] = fmaf(s_o[v - 1][4 * t + k][lane], wt[v], x[t]);
-                    x[t] = sq.bad ? pg_nan() : sq.kv == 0 ? 0.0f : x[t] * inv;
+                    x[t] *= inv;
+                    if (whole) x[t] = sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : x[t];
                 }
                 if (whole) {
                     T y[A::VW];
@@ -551,40 +453,41 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_decode_kernel(PagedKv 
             }
         }
         at += m;
-        if (at == stop && joins && threadIdx.x == 0) {
-            const bool cut = u == 0 && m < n;  // begins here, ends in a later range
-            joins[blockIdx.x] = {cut ? s : -1, vh, cut ? pd_owner(at - m + n - 1, total, n_wgs) : 0,
-                                 2 * (int)blockIdx.x + (at - m != begin)};
-        }
-        u = 0;
-        if (++s == b.n_seqs) {
-            s = 0;
-            vh++;
+        if (at == stop && joins && threadIdx.x == 0)
+            joins[blockIdx.x] = pg_join(u0 == 0 && !whole, min(16, all - i0), sq, head, i0, at - m + n - 1, total,
+                                        n_wgs, 2 * blockIdx.x + (at - m != begin));
+        u += m;
+        if (u == nt * n) {
+            u = 0;
+            if (++s == b.n_seqs) {
+                s = 0;
+                head++;
+            }
         }
         if (at < stop) __syncthreads();  // the merge's LDS is read
     }
 }
 
-// Joins the pieces of cut sequences: workgroup (w, r) takes row r of the one
-// that workgroup w of the decode left, if it left one.  HD / 4 threads a piece,
+// Joins the pieces of cut tiles: workgroup (w, r) takes row r of the one that
+// workgroup w left to be joined, if it left one.  HD / 4 threads a piece,
 // PJ_WG / (HD / 4) groups of them with every such piece each, PJ_STEP pieces a
 // step: the loads of 64 pieces (one sequence over all workgroups, 8 KV heads)
 // are one memory round trip.
 constexpr int PJ_WG = 256;
 constexpr int PJ_STEP = 8;
 template <class T, int HD>
-__global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PdJoin* __restrict__ joins,
-                                                           const float* __restrict__ part, int grp, int tiles,
+__global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins,
+                                                           const float* __restrict__ part, int tile_rows, int grp,
                                                            T* __restrict__ out, int ldo) {
     constexpr int TH = HD / 4, GROUPS = PJ_WG / TH;
     __shared__ pg_f4 s_o[GROUPS][TH];
     __shared__ float s_l[GROUPS], s_m[GROUPS];
-    const PdJoin j = joins[blockIdx.x];
-    const int r = blockIdx.y, h0 = (j.vh % tiles) * 16;
-    if (j.s < 0 || r >= min(16, grp - h0)) return;
+    const PgJoin j = joins[blockIdx.x];
+    const int r = blockIdx.y;
+    if (r >= j.rows) return;
     const int d = threadIdx.x % TH, p = threadIdx.x / TH, w0 = blockIdx.x;
     const float* row = part + r * HD + 4 * d;
-    const float* stat = part + 16 * HD + r;
+    const float* stat = part + tile_rows * HD + r;
     float M = -1e30f, L = 0.0f;
     pg_f4 O = pg_f4{0.f, 0.f, 0.f, 0.f};
     for (int w = w0 + p; w <= j.last; w += GROUPS * PJ_STEP) {
@@ -593,10 +496,10 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PdJoin* __restr
 #pragma unroll
         for (int i = 0; i < PJ_STEP; i++) {  // (past the last: the last again, with weight 0)
             const int wi = min(w + i * GROUPS, j.last);
-            const size_t slot = (size_t)(wi == w0 ? j.slot : 2 * wi) * pd_slot(HD);
+            const size_t slot = (size_t)(wi == w0 ? j.slot : 2 * wi) * pg_slot(tile_rows, HD);
             o[i] = *reinterpret_cast<const pg_f4*>(row + slot);
             m[i] = stat[slot];
-            l[i] = stat[slot + 16];
+            l[i] = stat[slot + tile_rows];
         }
 #pragma unroll
         for (int i = 0; i < PJ_STEP; i++) mn = fmaxf(mn, m[i]);
@@ -635,9 +538,9 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PdJoin* __restr
     }
     T y[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) y[k] = (T)(O[k] / L);
-    __builtin_memcpy(__builtin_assume_aligned(out + (size_t)j.s * ldo + (size_t)(j.vh / tiles * grp + h0 + r) * HD + 4 * d, 8),
-                     y, sizeof y);
+    for (int k = 0; k < 4; k++) y[k] = (T)(j.pos0 + (j.i0 + r) / grp < 0 ? 0.0f : O[k] / L);
+    const size_t to = j.row0 + (j.i0 + r) / grp, h = j.head * grp + (j.i0 + r) % grp;
+    __builtin_memcpy(__builtin_assume_aligned(out + to * ldo + h * HD + 4 * d, 8), y, sizeof y);
 }
 
 // The rows of a batch by binary search over row_start: the last sequence that
@@ -723,61 +626,55 @@ struct AppendCall {
     }
 };
 
-struct AttendCall {
+// Sizes of a call of the 16-row kernel: keys a unit, and workgroups (a range
+// each, no more than the units that lengths up to cap can have).  Calls with
+// tiles for every CU and up to PD_WHOLE keys are not cut: a second launch costs
+// more than the longer walk.
+constexpr int PD_WHOLE = 512;
+struct Rows16Plan {
+    int unit, wgs;
+    bool cut;
+};
+Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    const int grp = n_heads / kv.kv_heads;
+    const long tiles = pg_tiles_bound(r, grp, 16) * kv.kv_heads;
+    Rows16Plan p;
+    p.unit = tiles >= 256 && r.cap <= PD_WHOLE ? PD_WHOLE : PD_UNIT;
+    const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
+    p.cut = r.cap > p.unit;
+    p.wgs = (int)(units < pd_wgs(hd) || !p.cut ? units : pd_wgs(hd));
+    return p;
+}
+
+struct Rows16Call {
     const PagedAttendArgs& p;
     hipStream_t s;
     template <class E, class T, int HD>
     hipError_t run() const {
         const int grp = p.n_heads / p.kv.kv_heads;
-        // a bound on the tiles: each sequence's last may be partly empty
-        const long tiles = p.rows.row_start ? (long)p.rows.rows * grp / 16 + p.rows.n_seqs
-                                            : (long)p.rows.n_seqs * ((grp + 15) / 16);
-        hipLaunchKernelGGL((paged_attend_kernel<E, T, HD>), dim3((unsigned)(tiles * p.kv.kv_heads)),
-                           dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp, static_cast<const T*>(p.q), p.ldq, p.scale,
-                           static_cast<T*>(p.out), p.ldo);
-        return hipGetLastError();
-    }
-};
-
-// How many workgroups a decode takes: a range each, no more than the units that
-// lengths up to cap can have.
-int pd_wgs(const PagedRows& r, int heads) {
-    const long units = (long)r.n_seqs * ((r.cap + PD_UNIT - 1) / PD_UNIT > 0 ? (r.cap + PD_UNIT - 1) / PD_UNIT : 1);
-    return units * heads < PD_WGS ? (int)(units * heads) : PD_WGS;
-}
-
-struct DecodeCall {
-    const PagedAttendArgs& p;
-    hipStream_t s;
-    template <class E, class T, int HD>
-    hipError_t run() const {
-        const int grp = p.n_heads / p.kv.kv_heads, tiles = (grp + 15) / 16;
-        const int wgs = pd_wgs(p.rows, p.kv.kv_heads * tiles);
-        const bool cuts = p.rows.cap > PD_UNIT;  // (one unit a sequence: none is cut)
+        const Rows16Plan pl = rows16_plan(p.kv, p.rows, p.n_heads, HD);
         float* part = static_cast<float*>(p.work);
-        PdJoin* joins = cuts ? reinterpret_cast<PdJoin*>(part + (size_t)2 * wgs * pd_slot(HD)) : nullptr;
-        hipLaunchKernelGGL((paged_decode_kernel<E, T, HD>), dim3(wgs), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp,
-                           tiles, static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part,
-                           joins);
+        PgJoin* joins = pl.cut ? reinterpret_cast<PgJoin*>(part + (size_t)2 * pl.wgs * pg_slot(16, HD)) : nullptr;
+        hipLaunchKernelGGL((paged_rows16_kernel<E, T, HD>), dim3(pl.wgs), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp, pl.unit,
+                           static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
-        if (e != hipSuccess || !cuts) return e;
-        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(wgs, grp < 16 ? grp : 16), dim3(PJ_WG), 0, s, joins, part,
-                           grp, tiles, static_cast<T*>(p.out), p.ldo);
+        if (e != hipSuccess || !pl.cut) return e;
+        const int rows = p.rows.row_start || grp > 16 ? 16 : grp;
+        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(pl.wgs, rows), dim3(PJ_WG), 0, s, joins, part, 16, grp,
+                           static_cast<T*>(p.out), p.ldo);
         return hipGetLastError();
     }
 };
 
 }  // namespace
 
-size_t paged_decode_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
-    if (r.cap <= PD_UNIT || r.n_seqs == 0) return 0;
-    const int grp = n_heads / kv.kv_heads;
-    return pd_wgs(r, kv.kv_heads * ((grp + 15) / 16)) * (2 * pd_slot(hd) * sizeof(float) + sizeof(PdJoin));
+size_t paged_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    const Rows16Plan p = rows16_plan(kv, r, n_heads, hd);
+    return p.cut ? p.wgs * (2 * pg_slot(16, hd) * sizeof(float) + sizeof(PgJoin)) : 0;
 }
 
-bool paged_decode_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {
-    const long units = (long)r.n_seqs * (r.cap / PD_UNIT + 1);
-    return units * kv.kv_heads * ((n_heads / kv.kv_heads + 15) / 16) <= 0x7fffffff;
+bool paged_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {
+    return pg_tiles_bound(r, n_heads / kv.kv_heads, 16) * kv.kv_heads <= 0x7fffffff / (r.cap / PD_UNIT + 1);
 }
 
 bool paged_types(int kv_dtype, int dtype) {
@@ -790,14 +687,9 @@ hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppen
     return paged_with_types(kv_dtype, dtype, hd, AppendCall{p, s});
 }
 
-hipError_t launch_paged_decode(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
+hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
-    return paged_with_types(kv_dtype, dtype, hd, DecodeCall{p, s});
-}
-
-hipError_t launch_paged_attend(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
-    if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
-    return paged_with_types(kv_dtype, dtype, hd, AttendCall{p, s});
+    return paged_with_types(kv_dtype, dtype, hd, Rows16Call{p, s});
 }
 
 }  // namespace frq

@@ -39,6 +39,24 @@ struct PagedRows {
     int cap;  // kv_len beyond it is no length (<= max_pages * page_size)
 };
 
+// A bound on the tiles of tile_rows query rows that a batch's sequences have:
+// each one's last may be partly empty.
+inline long pg_tiles_bound(const PagedRows& r, int grp, int tile_rows) {
+    return r.row_start ? (long)r.rows * grp / tile_rows + r.n_seqs : (long)r.n_seqs * ((grp + tile_rows - 1) / tile_rows);
+}
+
+// Cut tiles.  Workgroups that share the keys of a tile of `rows` query rows
+// leave slots of floats in the workspace, two a workgroup: o [rows][hd]
+// (unnormalized), m [rows], l [rows]; and each a record of what is to be joined.
+constexpr size_t pg_slot(int rows, int hd) { return (size_t)rows * hd + 2 * rows; }
+struct PgJoin {
+    int rows;        // of the tile that begins in the workgroup's range and goes on past it; 0: none
+    int last, slot;  // workgroup of the tile's last piece; slot of its first
+    int row0, pos0;  // the sequence's first packed row, and its position
+    int head, i0;    // KV head, the tile's first query row
+    int pad;
+};
+
 #ifdef __HIPCC__
 
 typedef float pg_f4 __attribute__((ext_vector_type(4)));
@@ -148,6 +166,23 @@ struct PgUnits {
         return n_seqs;
     }
 };
+
+// Equal contiguous ranges of `total` units over n_wgs <= total workgroups: w's
+// starts at unit w * total / n_wgs, none is empty; and the one that holds unit u.
+__device__ __forceinline__ int pg_start(int w, int total, int n_wgs) {
+    if (n_wgs == total) return w;
+    // (in 32 bits: n_wgs is below 2^16 here)
+    const unsigned q = (unsigned)total / (unsigned)n_wgs, rest = (unsigned)total % (unsigned)n_wgs;
+    return w * (int)q + (int)((unsigned)w * rest / (unsigned)n_wgs);
+}
+__device__ __forceinline__ int pg_owner(int u, int total, int n_wgs) {
+    return (int)((((long)u + 1) * n_wgs - 1) / total);
+}
+__device__ __forceinline__ PgJoin pg_join(bool cut, int rows, const PgSeq& q, int head, int i0, int last_unit, int total,
+                                          int n_wgs, int slot) {
+    if (!cut) return PgJoin{};
+    return PgJoin{rows, pg_owner(last_unit, total, n_wgs), slot, q.row0, q.kv - q.n, head, i0, 0};
+}
 
 // Calls f.run<E, T, HD>() for the types of a call.
 template <class F>

@@ -80,6 +80,11 @@ struct PrefillTile {
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
     static constexpr int RPI = 512 / HD, NI = HD / 32;  // rows a DMA instruction, instructions a wavefront and tile
     static constexpr int ROWS = 32 * PF_WAVES;
+    // LDS chunk pc of row r holds the row's chunk pc ^ kswz(r) of K, pc ^ vswz(r)
+    // of V: the 16 rows by 16 bytes, and the 4 rows by 64, that a read touches at
+    // once lie in different ones of the 64 banks.
+    __device__ static __forceinline__ int kswz(int r) { return HD == 128 ? r & 15 : (r >> 1) & 7; }
+    __device__ static __forceinline__ int vswz(int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
 };
 
 template <class E, class T, int HD>
@@ -154,12 +159,11 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float m = -1e30f, l = 0.0f;
 
-    // DMA source offsets: chunk pc of LDS row r holds the row's chunk pc ^ (r & 7)
-    // of K, pc ^ 2 (r & 3) of V
+    // DMA source offsets
     constexpr int CPR = HD / 8;
     const int dr = w * X::RPI + lane / CPR, pc = lane % CPR;
-    const uint32_t koff = (lane / CPR) * X::ROW + 16 * (pc ^ (dr & 7));
-    const uint32_t voff = (lane / CPR) * X::ROW + 16 * (pc ^ (2 * (dr & 3)));
+    const uint32_t koff = (lane / CPR) * X::ROW + 16 * (pc ^ X::kswz(dr));
+    const uint32_t voff = (lane / CPR) * X::ROW + 16 * (pc ^ X::vswz(dr));
     const int* table = b.table + (size_t)s * b.max_pages;
     // page ids of 64 groups of 16 keys, lane i that of group i from key id0 on
     int id0 = 0, id = 0;
@@ -184,9 +188,9 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
     };
     // LDS read offsets of this lane: K row n (+ 32), chunks 2 t + h; V rows
     // 4 h + (lane / 4) % 4 (+ 16 k + 8 j), dims 16 ((lane / 16) % 2) + 4 (lane % 4) (+ 32 d)
-    const uint32_t kbase = n * X::ROW + 16 * (h ^ (n & 7));
+    const uint32_t kbase = n * X::ROW + 16 * (h ^ X::kswz(n));
     const int vr = (lane >> 2) & 3;
-    const uint32_t vbase = (4 * h + vr) * X::ROW + 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ (2 * vr)) + 8 * (lane & 1);
+    const uint32_t vbase = (4 * h + vr) * X::ROW + 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ X::vswz(vr)) + 8 * (lane & 1);
 
     if (tiles) {
         fetch_ids(0);
