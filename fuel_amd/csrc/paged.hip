@@ -67,10 +67,11 @@ struct Rows16 {
     float m, l;
 
     struct KeyRegs {
-        uint4 w[2][KS];
+        pg_u4 w[2][KS];
     };
+    typedef uint32_t ValueWord __attribute__((ext_vector_type(VW / 2)));
     struct ValueRegs {
-        uint32_t w[8][VW / 2];
+        ValueWord w[8];
     };
 
     // Lane 16 g + r takes row r: dims 32 t + 8 g + e of x (null: a row of zeros).
@@ -134,22 +135,28 @@ struct Rows16 {
         l = 0.0f;
     }
 
-    // The loads of 32 keys: group a's 16 rows start at ka[a] / va[a].
+    // The loads of 32 keys: group a's 16 rows start at ka[a] / va[a].  ONCE:
+    // nothing else of the call reads them, so they go past the caches.
+    template <bool ONCE, class W>
+    __device__ static W load(const E* p) {
+        return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const W*>(p)) : *reinterpret_cast<const W*>(p);
+    }
+    template <bool ONCE>
     __device__ static void load_k(KeyRegs& k, const E* const (&ka)[2]) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int a = 0; a < 2; a++)
 #pragma unroll
-            for (int t = 0; t < KS; t++) k.w[a][t] = *reinterpret_cast<const uint4*>(ka[a] + r * HD + 32 * t + 8 * g);
+            for (int t = 0; t < KS; t++) k.w[a][t] = load<ONCE, pg_u4>(ka[a] + r * HD + 32 * t + 8 * g);
     }
+    template <bool ONCE>
     __device__ static void load_v(ValueRegs& v, const E* const (&va)[2]) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int a = 0; a < 2; a++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                __builtin_memcpy(v.w[4 * a + i], __builtin_assume_aligned(va[a] + (4 * g + i) * HD + VW * r, 2 * VW),
-                                 2 * VW);
+                v.w[4 * a + i] = load<ONCE, ValueWord>(va[a] + (4 * g + i) * HD + VW * r);
     }
 
     // Which keys of a block of 32 from j0 a row sees: none past its position,
@@ -275,9 +282,7 @@ struct Rows16 {
 // written out, the cut pieces (at most two a workgroup) leave their sums in
 // the workspace for paged_join_kernel.
 constexpr int PD_UNIT = 32 * PA_WAVES;
-// Workgroups a CU that the registers allow, all resident at once.
-constexpr int pd_per_cu(int hd) { return hd == 64 ? 3 : 2; }
-constexpr int pd_wgs(int hd) { return 256 * pd_per_cu(hd); }
+constexpr int PD_WGS = 512;  // two a CU, all resident at once
 
 // Tiles of a sequence, and units of each; one without keys has one unit, which
 // writes its rows.
@@ -290,7 +295,7 @@ __device__ __forceinline__ int pd_units(const PgSeq& q, int unit) { return q.kv 
 // the time, in one set of registers each (two sets spill at HD 128).  The page
 // ids of 1024 keys are one load, lane i holding the page of group i.  Every row
 // sees the keys up to all_see.
-template <class E, class T, int HD>
+template <class E, class T, int HD, bool ONCE>
 __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int head, int j0,
                                         int j1, int kv, int all_see) {
     using A = Rows16<E, T, HD>;
@@ -317,9 +322,9 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
         float s[8];
         typename A::v8 pp[A::NP];
         rows(c.k, 0, at);
-        A::load_k(kr, at);
+        A::template load_k<ONCE>(kr, at);
         rows(c.v, 0, at);
-        A::load_v(vr, at);
+        A::template load_v<ONCE>(vr, at);
         for (int i = 0;; i++) {
             const int j = j0 + 32 * i;
             const uint32_t bad = (uint32_t)(none >> (2 * i)) & 3;
@@ -337,25 +342,25 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
                 }
                 if (i == last) break;
                 rows(c.k, i + 1, at);
-                A::load_k(kr, at);
+                A::template load_k<ONCE>(kr, at);
                 rows(c.v, i + 1, at);
-                A::load_v(vr, at);
+                A::template load_v<ONCE>(vr, at);
                 continue;
             }
             a.template scores<false>(kr, mk, s);
             rows(c.k, i + 1, at);
-            A::load_k(kr, at);
+            A::template load_k<ONCE>(kr, at);
             a.weights(s, pp);
             a.product(vr, pp);
             rows(c.v, i + 1, at);
-            A::load_v(vr, at);
+            A::template load_v<ONCE>(vr, at);
         }
         j0 = end;
     }
 }
 
-template <class E, class T, int HD>
-__global__ __launch_bounds__(64 * PA_WAVES, pd_per_cu(HD)) void paged_rows16_kernel(PagedKv c, PagedRows b, int grp, int unit,
+template <class E, class T, int HD, bool ONCE>
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv c, PagedRows b, int grp, int unit,
                                                                         const T* __restrict__ q, int ldq, float scale,
                                                                         T* __restrict__ out, int ldo,
                                                                         float* __restrict__ part,
@@ -400,7 +405,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, pd_per_cu(HD)) void paged_rows16_ker
         const int first = pos0 + i0 / grp, seen = pos0 + min(i0 + 15, all - 1) / grp + 1;  // keys that some row sees
         const int k0 = u0 * unit, k1 = max(k0, min(seen, (u0 + m) * unit));
         const int per = ((k1 - k0 + 31) / 32 + PA_WAVES - 1) / PA_WAVES;
-        pd_walk<E, T, HD>(a, c, b.table + (size_t)s * b.max_pages, head, k0 + 32 * w * per,
+        pd_walk<E, T, HD, ONCE>(a, c, b.table + (size_t)s * b.max_pages, head, k0 + 32 * w * per,
                           min(k1, k0 + 32 * (w + 1) * per), sq.kv, first);
         a.finish();
         if (w > 0) {
@@ -471,9 +476,10 @@ __global__ __launch_bounds__(64 * PA_WAVES, pd_per_cu(HD)) void paged_rows16_ker
 // Joins the pieces of cut tiles: workgroup (w, r) takes row r of the one that
 // workgroup w left to be joined, if it left one.  HD / 4 threads a piece,
 // PJ_WG / (HD / 4) groups of them with every such piece each, PJ_STEP pieces a
-// step: the loads of 64 pieces (one sequence over all workgroups, 8 KV heads)
-// are one memory round trip.
-constexpr int PJ_WG = 256;
+// step, whose loads are one memory round trip.  (256 threads: 1.3 us less where
+// one sequence of 131071 is joined of 64 pieces, 2.6 us more for 128 sequences,
+// where most workgroups find little to join.)
+constexpr int PJ_WG = 128;
 constexpr int PJ_STEP = 8;
 template <class T, int HD>
 __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins,
@@ -635,14 +641,14 @@ struct Rows16Plan {
     int unit, wgs;
     bool cut;
 };
-Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads) {
     const int grp = n_heads / kv.kv_heads;
     const long tiles = pg_tiles_bound(r, grp, 16) * kv.kv_heads;
     Rows16Plan p;
     p.unit = tiles >= 256 && r.cap <= PD_WHOLE ? PD_WHOLE : PD_UNIT;
     const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
     p.cut = r.cap > p.unit;
-    p.wgs = (int)(units < pd_wgs(hd) || !p.cut ? units : pd_wgs(hd));
+    p.wgs = (int)(units < PD_WGS || !p.cut ? units : PD_WGS);
     return p;
 }
 
@@ -652,10 +658,16 @@ struct Rows16Call {
     template <class E, class T, int HD>
     hipError_t run() const {
         const int grp = p.n_heads / p.kv.kv_heads;
-        const Rows16Plan pl = rows16_plan(p.kv, p.rows, p.n_heads, HD);
+        const Rows16Plan pl = rows16_plan(p.kv, p.rows, p.n_heads);
         float* part = static_cast<float*>(p.work);
         PgJoin* joins = pl.cut ? reinterpret_cast<PgJoin*>(part + (size_t)2 * pl.wgs * pg_slot(16, HD)) : nullptr;
-        hipLaunchKernelGGL((paged_rows16_kernel<E, T, HD>), dim3(pl.wgs), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp, pl.unit,
+        // Past the caches where one tile reads its keys alone and the batch's may
+        // exceed the 256 MB last-level cache (537 MB 103.9 -> 92.8 us, 201 MB 55.6
+        // -> 50.5; what the cache still holds of 82 MB it would lose, 26.8 -> 29.1)
+        const double bytes = (double)p.rows.n_seqs * p.rows.cap * p.kv.kv_heads * HD * 4;
+        const auto kernel = !p.rows.row_start && grp <= 16 && bytes > 256e6 ? paged_rows16_kernel<E, T, HD, true>
+                                                           : paged_rows16_kernel<E, T, HD, false>;
+        hipLaunchKernelGGL(kernel, dim3(pl.wgs), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp, pl.unit,
                            static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !pl.cut) return e;
@@ -669,7 +681,7 @@ struct Rows16Call {
 }  // namespace
 
 size_t paged_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
-    const Rows16Plan p = rows16_plan(kv, r, n_heads, hd);
+    const Rows16Plan p = rows16_plan(kv, r, n_heads);
     return p.cut ? p.wgs * (2 * pg_slot(16, hd) * sizeof(float) + sizeof(PgJoin)) : 0;
 }
 

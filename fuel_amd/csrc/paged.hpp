@@ -60,7 +60,7 @@ struct PgJoin {
 #ifdef __HIPCC__
 
 typedef float pg_f4 __attribute__((ext_vector_type(4)));
-typedef float pg_f2 __attribute__((ext_vector_type(2)));
+typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));
 
 // Vector types, conversions and MFMAs of a cache element type.
 template <class E>
