@@ -549,73 +549,125 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
     __builtin_memcpy(__builtin_assume_aligned(out + to * ldo + h * HD + 4 * d, 8), y, sizeof y);
 }
 
-// The rows of a batch by binary search over row_start: the last sequence that
-// starts at or before `row`, or -1 if the row is in none.
+// The last sequence that starts at or before packed row `row`, or -1 if none
+// does or the row lies behind them all: a search in steps of 64 (one load a
+// lane, one vote).  Wave-uniform.
 __device__ __forceinline__ int pg_row_seq(const PagedRows& b, int row) {
-    if (!b.row_start) return row < b.n_seqs ? row : -1;
-    int lo = 0, hi = b.n_seqs;  // starts[lo] <= row < starts[hi], if the row is in any
-    if (b.row_start[0] > row || b.row_start[b.n_seqs] <= row) return -1;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (b.row_start[mid] <= row) lo = mid;
-        else hi = mid;
+    if (!b.row_start) return row;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = b.n_seqs + 1;  // the answer is the last of lo .. lo + n - 1 that starts at or before row
+    for (;;) {
+        const int step = (n + 63) >> 6, at = lane * step;
+        const bool le = at < n && b.row_start[lo + at] <= row;
+        const uint64_t v = __ballot(le);
+        if (!v) return -1;
+        const int k = 63 - __builtin_clzll(v);
+        lo += k * step;
+        if (step == 1) break;
+        n = min(step, n - k * step);
     }
-    return lo;
+    return lo < b.n_seqs ? lo : -1;  // (row_start[n_seqs] <= row: behind the last)
 }
 
+// Append.  Workgroups (row, y): the row's work in chunks, AP_WG of them a
+// workgroup and turn: 8 pairs (elements i .. i + 7 and i + HD / 2 ..) of a head
+// of q or k, or 8 elements of v, each 16 or 32 bytes a lane.
+//   y[i] = x[i] cos[i] - x[i + HD/2] sin[i],
+//   y[i + HD/2] = x[i + HD/2] cos[i + HD/2] + x[i] sin[i + HD/2]
+// (rope_f32, byte_kernels.rs:1885-1964): two products and a sum in f32, rounded
+// once.  A thread's chunks are the same part of different heads, so it reads
+// its part of the position's table rows once.  A chunk's loads need the row
+// alone and go out before the row's sequence and position are known.
 constexpr int AP_WG = 256;
-
-// One packed row a workgroup.  y[i] = x[i] cos[i] - x[i + HD/2] sin[i],
-// y[i + HD/2] = x[i + HD/2] cos[i + HD/2] + x[i] sin[i + HD/2] (rope_f32,
-// byte_kernels.rs:1885-1964): two products and a sum in f32, rounded once.
+constexpr int AP_FEW = 2048;
 template <class E, class T, int HD>
 __global__ __launch_bounds__(AP_WG) void paged_append_kernel(PagedKv c, PagedRows b, int n_heads,
-                                                             const T* __restrict__ q, int ldq,
-                                                             const T* __restrict__ k, int ldk,
+                                                             const T* q, int ldq, const T* __restrict__ k, int ldk,
                                                              const T* __restrict__ v, int ldv,
                                                              const float* __restrict__ cs, const float* __restrict__ sn,
                                                              int rope_rows, T* q_out, int ldqo) {
-    const int row = blockIdx.x;
+    constexpr int HALF = HD / 2, CP = HALF / 8;  // chunks of a head
+    const int row = blockIdx.x, nq = q ? n_heads : 0;
+    const int turned = CP * (nq + c.kv_heads), all = turned + 2 * CP * c.kv_heads;
+    const int stride = AP_WG * gridDim.y;  // (a multiple of CP)
+    int e = AP_WG * blockIdx.y + threadIdx.x;
+    const int i = 8 * (e % CP);
+    T lo[8], hi[8];
+    auto fetch = [&] {
+        if (e < turned) {
+            const int h = e / CP;
+            const T* x = h < nq ? q + (size_t)row * ldq + h * HD : k + (size_t)row * ldk + (h - nq) * HD;
+            __builtin_memcpy(lo, __builtin_assume_aligned(x + i, 16), sizeof lo);
+            __builtin_memcpy(hi, __builtin_assume_aligned(x + i + HALF, 16), sizeof hi);
+        } else if (e < all) {
+            __builtin_memcpy(lo, __builtin_assume_aligned(v + (size_t)row * ldv + 8 * (e - turned), 16), sizeof lo);
+        }
+    };
+    fetch();
     const int s = pg_row_seq(b, row);
     if (s < 0) return;
     const PgSeq sq = pg_seq(b, s);
     if (row < sq.row0 || row >= sq.row0 + sq.n) return;
     const int pos = sq.kv - sq.n + (row - sq.row0);
-    const bool bad = sq.bad || (cs && pos >= rope_rows);
-    const int page = bad || pos < 0 ? -1 : b.table[(size_t)s * b.max_pages + (pos >> c.log_ps)];
-    const bool put = (unsigned)page < (unsigned)c.n_pages;
-    const int slot = pos & ((1 << c.log_ps) - 1);
-    constexpr int HALF = HD / 2;
-    for (int e = threadIdx.x; e < (n_heads + c.kv_heads) * HALF; e += AP_WG) {
-        const int h = e / HALF, i = e % HALF;
-        const bool is_q = h < n_heads;
-        if (is_q ? !q : !put) continue;
-        const T* x = is_q ? q + (size_t)row * ldq + h * HD : k + (size_t)row * ldk + (h - n_heads) * HD;
-        const float lo = (float)x[i], hi = (float)x[i + HALF];
-        float a = lo, z = hi;
-        if (cs && pos >= 0 && !bad) {
-            const float* ct = cs + (size_t)pos * HD;
-            const float* st = sn + (size_t)pos * HD;
-            a = lo * ct[i] - hi * st[i];
-            z = hi * ct[i + HALF] + lo * st[i + HALF];
-        }
-        if (is_q) {
-            if (bad) a = z = pg_nan();
-            else if (pos < 0) a = z = 0.0f;
-            T* y = q_out + (size_t)row * ldqo + h * HD;
-            y[i] = (T)a;
-            y[i + HALF] = (T)z;
-        } else {
-            E* y = static_cast<E*>(c.k) + ((((size_t)page * c.kv_heads + (h - n_heads)) << c.log_ps) + slot) * HD;
-            y[i] = (E)a;
-            y[i + HALF] = (E)z;
-        }
+    const bool bad = sq.bad || (cs && pos >= rope_rows), seen = pos >= 0 && !bad;
+    const int page = seen ? b.table[(size_t)s * b.max_pages + (pos >> c.log_ps)] : -1;
+    float cl[8], ch[8], sl[8], sh[8];
+    if (cs && seen && e < turned) {
+        const float *ct = cs + (size_t)pos * HD + i, *st = sn + (size_t)pos * HD + i;
+        __builtin_memcpy(cl, __builtin_assume_aligned(ct, 16), sizeof cl);
+        __builtin_memcpy(ch, __builtin_assume_aligned(ct + HALF, 16), sizeof ch);
+        __builtin_memcpy(sl, __builtin_assume_aligned(st, 16), sizeof sl);
+        __builtin_memcpy(sh, __builtin_assume_aligned(st + HALF, 16), sizeof sh);
     }
-    if (!put) return;
-    for (int e = threadIdx.x; e < c.kv_heads * HD; e += AP_WG) {
-        const int h = e / HD, i = e % HD;
-        static_cast<E*>(c.v)[((((size_t)page * c.kv_heads + h) << c.log_ps) + slot) * HD + i] =
-            (E)(float)v[(size_t)row * ldv + e];
+    const bool put = (unsigned)page < (unsigned)c.n_pages;
+    const size_t at = (((size_t)(put ? page : 0) * c.kv_heads) << c.log_ps) + (pos & ((1 << c.log_ps) - 1));
+    auto cache_row = [&](void* pool, int h) { return static_cast<E*>(pool) + (at + ((size_t)h << c.log_ps)) * HD; };
+    for (; e < all; e += stride, fetch()) {
+        if (e >= turned) {
+            if (!put) continue;
+            const int x = 8 * (e - turned);
+            E y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = (E)(float)lo[j];
+            __builtin_memcpy(__builtin_assume_aligned(cache_row(c.v, x / HD) + x % HD, 16), y, sizeof y);
+            continue;
+        }
+        const int h = e / CP;
+        float a[8], z[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            a[j] = (float)lo[j];
+            z[j] = (float)hi[j];
+        }
+        if (cs && seen) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float x = a[j], y = z[j];
+                a[j] = x * cl[j] - y * sl[j];
+                z[j] = y * ch[j] + x * sh[j];
+            }
+        }
+        if (h < nq) {
+            T y[8], x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                y[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : a[j]);
+                x[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : z[j]);
+            }
+            T* to = q_out + (size_t)row * ldqo + h * HD + i;
+            __builtin_memcpy(__builtin_assume_aligned(to, 16), y, sizeof y);
+            __builtin_memcpy(__builtin_assume_aligned(to + HALF, 16), x, sizeof x);
+        } else if (put) {
+            E y[8], x[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                y[j] = (E)a[j];
+                x[j] = (E)z[j];
+            }
+            E* to = cache_row(c.k, h - nq) + i;
+            __builtin_memcpy(__builtin_assume_aligned(to, 16), y, sizeof y);
+            __builtin_memcpy(__builtin_assume_aligned(to + HALF, 16), x, sizeof x);
+        }
     }
 }
 
@@ -624,7 +676,10 @@ struct AppendCall {
     hipStream_t s;
     template <class E, class T, int HD>
     hipError_t run() const {
-        hipLaunchKernelGGL((paged_append_kernel<E, T, HD>), dim3(p.rows.rows), dim3(AP_WG), 0, s, p.kv, p.rows,
+        // one chunk a thread while that does not fill the chip
+        const int chunks = HD / 16 * ((p.q ? p.n_heads : 0) + 3 * p.kv.kv_heads), parts = (chunks + AP_WG - 1) / AP_WG;
+        const int y = (long)p.rows.rows * parts <= AP_FEW ? parts : 1;
+        hipLaunchKernelGGL((paged_append_kernel<E, T, HD>), dim3(p.rows.rows, y), dim3(AP_WG), 0, s, p.kv, p.rows,
                            p.n_heads, static_cast<const T*>(p.q), p.ldq, static_cast<const T*>(p.k), p.ldk,
                            static_cast<const T*>(p.v), p.ldv, p.cos, p.sin, p.rope_rows, static_cast<T*>(p.q_out),
                            p.ldqo);
