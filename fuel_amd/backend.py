@@ -289,6 +289,8 @@ def qmatmul_f32_rocm_wrapper(inputs: Sequence[RocmStorage], outputs: Sequence[Ro
 
 def _ptr(x) -> int:
     """Device address of a RocmStorage, or the address itself (None: null)."""
+    if type(x) is int:
+        return x
     return x.ptr if isinstance(x, RocmStorage) else int(x or 0)
 
 

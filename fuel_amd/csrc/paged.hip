@@ -371,11 +371,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
     __shared__ float s_m[PA_WAVES][16], s_l[PA_WAVES][16];
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const auto units_of = [&](int i) {
-        const PgSeq sq = pg_seq(b, i);
-        return pd_tiles(sq, grp) * pd_units(sq, unit);
-    };
-    const PgUnits pu(b.n_seqs, units_of);
+    const auto units_of = [&](const PgSeq& x) { return pd_tiles(x, grp) * pd_units(x, unit); };
+    PgUnits<decltype(units_of)> pu(b, units_of, !b.row_start && b.cap <= unit ? (grp + 15) >> 4 : 0);
     const int units = pu.total, total = units * c.kv_heads, n_wgs = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= n_wgs) {
         if (joins && threadIdx.x == 0) joins[blockIdx.x].rows = 0;
@@ -383,9 +380,9 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
     }
     const int begin = pg_start(blockIdx.x, total, n_wgs), stop = pg_start(blockIdx.x + 1, total, n_wgs);
     int head = (unsigned)begin / (unsigned)units, u;
-    int s = pu.find(b.n_seqs, begin - head * units, units_of, u);
+    int s = pu.find(begin - head * units, u);
     for (int at = begin; at < stop;) {
-        const PgSeq sq = pg_seq(b, s);
+        const PgSeq sq = pu.get(s);
         const int all = sq.n * grp, nt = pd_tiles(sq, grp), n = pd_units(sq, unit);
         if (nt == 0) {  // (a sequence without rows)
             u = 0;
@@ -473,79 +470,79 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
     }
 }
 
-// Joins the pieces of cut tiles: workgroup (w, r) takes row r of the one that
-// workgroup w left to be joined, if it left one.  HD / 4 threads a piece,
-// PJ_WG / (HD / 4) groups of them with every such piece each, PJ_STEP pieces a
-// step, whose loads are one memory round trip.  (256 threads: 1.3 us less where
-// one sequence of 131071 is joined of 64 pieces, 2.6 us more for 128 sequences,
-// where most workgroups find little to join.)
-constexpr int PJ_WG = 128;
+// Joins the pieces of cut tiles: workgroup (w, y) takes rows PJ_ROWS y .. of the
+// one that workgroup w left to be joined, if it left one.  HD / 4 threads a row,
+// as many groups of such threads as there is room for with every so many-th
+// piece each, PJ_STEP pieces a step, whose loads are one memory round trip.
+constexpr int PJ_WG = 256;
+constexpr int PJ_ROWS = 4;
 constexpr int PJ_STEP = 8;
 template <class T, int HD>
 __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins,
                                                            const float* __restrict__ part, int tile_rows, int grp,
                                                            T* __restrict__ out, int ldo) {
-    constexpr int TH = HD / 4, GROUPS = PJ_WG / TH;
-    __shared__ pg_f4 s_o[GROUPS][TH];
-    __shared__ float s_l[GROUPS], s_m[GROUPS];
+    constexpr int TH = HD / 4;
+    __shared__ pg_f4 s_o[PJ_WG];
+    __shared__ float s_l[PJ_WG / TH], s_m[PJ_WG / TH];
     const PgJoin j = joins[blockIdx.x];
-    const int r = blockIdx.y;
-    if (r >= j.rows) return;
-    const int d = threadIdx.x % TH, p = threadIdx.x / TH, w0 = blockIdx.x;
+    const int r0 = PJ_ROWS * blockIdx.y, rows = min(PJ_ROWS, j.rows - r0);
+    if (rows <= 0) return;
+    const int groups = (unsigned)(PJ_WG / TH) / (unsigned)rows, w0 = blockIdx.x;
+    const int d = threadIdx.x % TH, x = threadIdx.x / TH, p = (unsigned)x / (unsigned)rows, r = r0 + x - p * rows;
     const float* row = part + r * HD + 4 * d;
     const float* stat = part + tile_rows * HD + r;
     float M = -1e30f, L = 0.0f;
     pg_f4 O = pg_f4{0.f, 0.f, 0.f, 0.f};
-    for (int w = w0 + p; w <= j.last; w += GROUPS * PJ_STEP) {
-        pg_f4 o[PJ_STEP];
-        float m[PJ_STEP], l[PJ_STEP], mn = M;
+    if (p < groups) {
+        for (int w = w0 + p; w <= j.last; w += groups * PJ_STEP) {
+            pg_f4 o[PJ_STEP];
+            float m[PJ_STEP], l[PJ_STEP], mn = M;
 #pragma unroll
-        for (int i = 0; i < PJ_STEP; i++) {  // (past the last: the last again, with weight 0)
-            const int wi = min(w + i * GROUPS, j.last);
-            const size_t slot = (size_t)(wi == w0 ? j.slot : 2 * wi) * pg_slot(tile_rows, HD);
-            o[i] = *reinterpret_cast<const pg_f4*>(row + slot);
-            m[i] = stat[slot];
-            l[i] = stat[slot + tile_rows];
+            for (int i = 0; i < PJ_STEP; i++) {  // (past the last: the last again, with weight 0)
+                const int wi = min(w + i * groups, j.last);
+                const size_t slot = (size_t)(wi == w0 ? j.slot : 2 * wi) * pg_slot(tile_rows, HD);
+                o[i] = *reinterpret_cast<const pg_f4*>(row + slot);
+                m[i] = stat[slot];
+                l[i] = stat[slot + tile_rows];
+            }
+#pragma unroll
+            for (int i = 0; i < PJ_STEP; i++) mn = fmaxf(mn, m[i]);
+            const float f = __builtin_amdgcn_exp2f(M - mn);
+            M = mn;
+            L *= f;
+            O *= f;
+#pragma unroll
+            for (int i = 0; i < PJ_STEP; i++) {
+                const float e = w + i * groups <= j.last ? __builtin_amdgcn_exp2f(m[i] - mn) : 0.0f;
+                L = fmaf(l[i], e, L);
+#pragma unroll
+                for (int k = 0; k < 4; k++) O[k] = fmaf(o[i][k], e, O[k]);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < PJ_STEP; i++) mn = fmaxf(mn, m[i]);
-        const float f = __builtin_amdgcn_exp2f(M - mn);
-        M = mn;
-        L *= f;
-        O *= f;
-#pragma unroll
-        for (int i = 0; i < PJ_STEP; i++) {
-            if (w + i * GROUPS > j.last) break;
-            const float e = __builtin_amdgcn_exp2f(m[i] - mn);
-            L = fmaf(l[i], e, L);
-#pragma unroll
-            for (int k = 0; k < 4; k++) O[k] = fmaf(o[i][k], e, O[k]);
+        s_o[threadIdx.x] = O;
+        if (d == 0) {
+            s_l[x] = L;
+            s_m[x] = M;
         }
-    }
-    s_o[p][d] = O;
-    if (d == 0) {
-        s_l[p] = L;
-        s_m[p] = M;
     }
     __syncthreads();
     if (p) return;
-    float mx = s_m[0];
-#pragma unroll
-    for (int i = 1; i < GROUPS; i++) mx = fmaxf(mx, s_m[i]);
+    float mx = -1e30f;
+    for (int i = 0; i < groups; i++) mx = fmaxf(mx, s_m[i * rows + x]);
     L = 0.0f;
     O = pg_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < GROUPS; i++) {
-        const float e = __builtin_amdgcn_exp2f(s_m[i] - mx);
-        L = fmaf(s_l[i], e, L);
-        const pg_f4 o = s_o[i][d];
+    for (int i = 0; i < groups; i++) {
+        const float e = __builtin_amdgcn_exp2f(s_m[i * rows + x] - mx);
+        L = fmaf(s_l[i * rows + x], e, L);
+        const pg_f4 o = s_o[(i * rows + x) * TH + d];
 #pragma unroll
         for (int k = 0; k < 4; k++) O[k] = fmaf(o[k], e, O[k]);
     }
+    const int at = (unsigned)(j.i0 + r) / (unsigned)grp;
+    const size_t to = j.row0 + at, h = j.head * grp + (j.i0 + r - at * grp);
     T y[4];
 #pragma unroll
-    for (int k = 0; k < 4; k++) y[k] = (T)(j.pos0 + (j.i0 + r) / grp < 0 ? 0.0f : O[k] / L);
-    const size_t to = j.row0 + (j.i0 + r) / grp, h = j.head * grp + (j.i0 + r) % grp;
+    for (int k = 0; k < 4; k++) y[k] = (T)(j.pos0 + at < 0 ? 0.0f : O[k] / L);
     __builtin_memcpy(__builtin_assume_aligned(out + to * ldo + h * HD + 4 * d, 8), y, sizeof y);
 }
 
@@ -727,7 +724,8 @@ struct Rows16Call {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !pl.cut) return e;
         const int rows = p.rows.row_start || grp > 16 ? 16 : grp;
-        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(pl.wgs, rows), dim3(PJ_WG), 0, s, joins, part, 16, grp,
+        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(pl.wgs, (rows + PJ_ROWS - 1) / PJ_ROWS), dim3(PJ_WG), 0, s,
+                           joins, part, 16, grp,
                            static_cast<T*>(p.out), p.ldo);
         return hipGetLastError();
     }

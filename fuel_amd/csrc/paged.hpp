@@ -126,44 +126,78 @@ __device__ __forceinline__ int pg_scan(int v) {
     return v;
 }
 
-// The units of a batch's sequences, units(s) >= 0 of sequence s one after
-// another, as one wavefront sees them; the first 64 sequences' stay in
-// registers.  Every lane takes part, results are wave-uniform.
+// Where the units of a batch's sequences lie, units(PgSeq) >= 0 of them one
+// sequence after another, and 64 of its sequences in a wavefront's registers.
+// Every lane takes part, results are wave-uniform.  Lane l adds up the
+// sequences [l share, (l + 1) share), whose loads do not wait for each other;
+// a lookup then loads one share: two memory round trips for any n_seqs <= 4096.
+// each: every sequence has so many units (0: not known), and none is loaded
+// before the lookup.
+template <class F>
 struct PgUnits {
-    int own, sum;  // lane l: sequence l's units, and those of 0 .. l
-    int total;
+    const PagedRows& b;
+    F units;
+    PgSeq own;  // lane l: sequence s0 + l
+    int s0, share, sum, total, each;
 
-    template <class F>
-    __device__ __forceinline__ PgUnits(int n_seqs, F units) {
-        const int lane = threadIdx.x & 63;
-        own = lane < n_seqs ? units(lane) : 0;
-        sum = pg_scan(own);
-        total = __builtin_amdgcn_readlane(sum, 63);
-        for (int s0 = 64; s0 < n_seqs; s0 += 64)
-            total += __builtin_amdgcn_readlane(pg_scan(s0 + lane < n_seqs ? units(s0 + lane) : 0), 63);
+    __device__ __forceinline__ void load(int base) {
+        const int s = base + (int)(threadIdx.x & 63);
+        s0 = base;
+        own = PgSeq{0, 0, 0, false};
+        if (s < b.n_seqs) own = pg_seq(b, s);
     }
-
-    // The sequence that holds unit `at`, and the unit's number in it; n_seqs
-    // past the last.
-    template <class F>
-    __device__ __forceinline__ int find(int n_seqs, int at, F units, int& in_seq) const {
-        const int lane = threadIdx.x & 63;
-        int base = 0, u = own, s = sum;
-        for (int s0 = 0; s0 < n_seqs; s0 += 64) {
-            if (s0) {
-                u = s0 + lane < n_seqs ? units(s0 + lane) : 0;
-                s = pg_scan(u);
-            }
-            const uint64_t past = __ballot(base + s > at);
-            if (past) {
-                const int l = __builtin_ctzll(past);
-                in_seq = at - base - __builtin_amdgcn_readlane(s - u, l);
-                return s0 + l;
-            }
-            base += __builtin_amdgcn_readlane(s, 63);
+    __device__ __forceinline__ int mine() const { return s0 + (int)(threadIdx.x & 63) < b.n_seqs ? units(own) : 0; }
+    __device__ __forceinline__ PgUnits(const PagedRows& rows, F f, int each_ = 0) : b(rows), units(f), each(each_) {
+        share = (b.n_seqs + 63) >> 6;
+        if (each) {
+            s0 = -64;
+            total = b.n_seqs * each;
+            return;
         }
-        in_seq = 0;
-        return n_seqs;
+        int v = 0;
+        if (share == 1) {
+            load(0);
+            v = mine();
+        } else {
+            s0 = -64;
+            const int from = share * (int)(threadIdx.x & 63), to = min(b.n_seqs, from + share);
+#pragma unroll 4
+            for (int s = from; s < to; s++) v += units(pg_seq(b, s));
+        }
+        sum = pg_scan(v);
+        total = __builtin_amdgcn_readlane(sum, 63);
+    }
+    // The sequence that holds unit at < total, and the unit's number in it.
+    __device__ __forceinline__ int find(int at, int& in_seq) {
+        if (each) {
+            const int s = (unsigned)at / (unsigned)each;
+            in_seq = at - s * each;
+            return s;
+        }
+        int l = __builtin_ctzll(__ballot(sum > at)), base = l * share;
+        if (share == 1) {
+            in_seq = at - (l ? __builtin_amdgcn_readlane(sum, l - 1) : 0);
+            return l;
+        }
+        at -= l ? __builtin_amdgcn_readlane(sum, l - 1) : 0;
+        for (;; base += 64) {
+            load(base);
+            const int u = mine(), v = pg_scan(u);
+            const uint64_t past = __ballot(v > at);
+            if (past) {
+                l = __builtin_ctzll(past);
+                in_seq = at - __builtin_amdgcn_readlane(v - u, l);
+                return base + l;
+            }
+            at -= __builtin_amdgcn_readlane(v, 63);
+        }
+    }
+    // Sequence s < n_seqs.
+    __device__ __forceinline__ PgSeq get(int s) {
+        if (s < s0 || s >= s0 + 64) load(s);
+        const int l = s - s0;
+        return PgSeq{__builtin_amdgcn_readlane(own.row0, l), __builtin_amdgcn_readlane(own.n, l),
+                     __builtin_amdgcn_readlane(own.kv, l), __builtin_amdgcn_readlane((int)own.bad, l) != 0};
     }
 };
 

@@ -98,14 +98,15 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int head = blockIdx.x % c.kv_heads;
-    // the tiles with the most keys first: the last ones of each sequence
-    const auto units = [&](int i) { return (int)(((long)pg_seq(b, i).n * grp + X::ROWS - 1) / X::ROWS); };
-    const PgUnits pu(b.n_seqs, units);
+    const auto units = [&](const PgSeq& x) { return (int)(((long)x.n * grp + X::ROWS - 1) / X::ROWS); };
+    PgUnits<decltype(units)> pu(b, units);
+    // the last tiles of the sequences, which walk the most keys, first (sorted
+    // over all sequences 3 % more: neighbours share a sequence's keys)
     const int unit = pu.total - 1 - (int)(blockIdx.x / c.kv_heads);
     if (unit < 0) return;
     int tile;
-    const int s = pu.find(b.n_seqs, unit, units, tile);
-    const PgSeq sq = pg_seq(b, s);
+    const int s = pu.find(unit, tile);
+    const PgSeq sq = pu.get(s);
     const int rows = sq.n * grp, i0 = tile * X::ROWS;
     const int mine = min(i0 + 32 * w + n, rows - 1);
     const int row = sq.row0 + mine / grp, qh = head * grp + mine % grp;
