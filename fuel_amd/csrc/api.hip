@@ -1562,7 +1562,8 @@ size_t frq_paged_attention_workspace(const frq_paged_kv* kv, const frq_paged_bat
     PagedKv k;
     PagedRows r;
     if (paged_args("paged_attention_workspace", kv, b, n_heads, &k, &r)) return 0;
-    return paged_takes_rows16(k, r, (int)n_heads) ? paged_rows16_work_bytes(k, r, (int)n_heads, (int)kv->head_dim) : 0;
+    return (paged_takes_rows16(k, r, (int)n_heads) ? paged_rows16_work_bytes : paged_prefill_work_bytes)(
+        k, r, (int)n_heads, (int)kv->head_dim);
 }
 
 int frq_paged_attention_decode(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,

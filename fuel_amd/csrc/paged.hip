@@ -704,6 +704,14 @@ Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads) {
     return p;
 }
 
+template <class T, int HD>
+hipError_t join(const PgJoin* joins, const float* part, int wgs, int tile_rows, int rows, int grp, void* out, int ldo,
+                hipStream_t s) {
+    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(wgs, (rows + PJ_ROWS - 1) / PJ_ROWS), dim3(PJ_WG), 0, s, joins, part,
+                       tile_rows, grp, static_cast<T*>(out), ldo);
+    return hipGetLastError();
+}
+
 struct Rows16Call {
     const PagedAttendArgs& p;
     hipStream_t s;
@@ -723,11 +731,7 @@ struct Rows16Call {
                            static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !pl.cut) return e;
-        const int rows = p.rows.row_start || grp > 16 ? 16 : grp;
-        hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(pl.wgs, (rows + PJ_ROWS - 1) / PJ_ROWS), dim3(PJ_WG), 0, s,
-                           joins, part, 16, grp,
-                           static_cast<T*>(p.out), p.ldo);
-        return hipGetLastError();
+        return join<T, HD>(joins, part, pl.wgs, 16, p.rows.row_start || grp > 16 ? 16 : grp, grp, p.out, p.ldo, s);
     }
 };
 
@@ -750,6 +754,14 @@ bool paged_types(int kv_dtype, int dtype) {
 hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0) return hipSuccess;
     return paged_with_types(kv_dtype, dtype, hd, AppendCall{p, s});
+}
+
+hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, int tile_rows, int rows,
+                             int grp, void* out, int ldo, hipStream_t s) {
+    const auto run = dtype == GGML_F32   ? (hd == 64 ? join<float, 64> : join<float, 128>)
+                     : dtype == GGML_F16 ? (hd == 64 ? join<_Float16, 64> : join<_Float16, 128>)
+                                         : (hd == 64 ? join<__bf16, 64> : join<__bf16, 128>);
+    return run(joins, part, wgs, tile_rows, rows, grp, out, ldo, s);
 }
 
 hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {

@@ -87,26 +87,70 @@ struct PrefillTile {
     __device__ static __forceinline__ int vswz(int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
 };
 
-template <class E, class T, int HD>
+// A workgroup takes one tile of query rows, or with CUT an equal contiguous
+// range of all tiles' key tiles (head by head, sequence by sequence, tile by
+// tile), as the 16-row kernel does: where a batch has fewer tiles than fill the
+// chip and many keys each.  Tiles that a range cuts leave their sums in the
+// workspace.
+constexpr int PF_WGS = 512;  // two a CU
+
+template <class E, class T, int HD, bool CUT>
 __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv c, PagedRows b, int grp,
                                                                          const T* __restrict__ q, int ldq, float scale,
-                                                                         T* __restrict__ out, int ldo) {
+                                                                         T* __restrict__ out, int ldo,
+                                                                         float* __restrict__ part,
+                                                                         PgJoin* __restrict__ joins) {
     using X = PrefillTile<E, T, HD>;
     using v8 = typename X::v8;
     __shared__ __align__(1024) uint8_t s_k[2][X::TILE], s_v[2][X::TILE];
     __shared__ uint32_t s_odd[2];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int head = blockIdx.x % c.kv_heads;
-    const auto units = [&](const PgSeq& x) { return (int)(((long)x.n * grp + X::ROWS - 1) / X::ROWS); };
+    // key tiles of a sequence's tiles of rows (one where it has no keys)
+    const auto key_tiles = [&](const PgSeq& x) { return x.kv <= PF_KEYS ? 1 : (x.kv + PF_KEYS - 1) / PF_KEYS; };
+    const auto units = [&](const PgSeq& x) {
+        const int row_tiles = (int)(((long)x.n * grp + X::ROWS - 1) / X::ROWS);
+        return CUT ? row_tiles * key_tiles(x) : row_tiles;
+    };
     PgUnits<decltype(units)> pu(b, units);
-    // the last tiles of the sequences, which walk the most keys, first (sorted
-    // over all sequences 3 % more: neighbours share a sequence's keys)
-    const int unit = pu.total - 1 - (int)(blockIdx.x / c.kv_heads);
-    if (unit < 0) return;
-    int tile;
-    const int s = pu.find(unit, tile);
+    int head, s, u;                       // KV head, sequence, unit of the sequence
+    int at = 0, begin = 0, stop = 0, total = 0, n_wgs = 0, wg = 0;  // CUT: the range, and whose it is
+    if constexpr (CUT) {
+        total = pu.total * c.kv_heads;
+        n_wgs = min((int)gridDim.x, total);
+        // (each XCD takes a contiguous part of the list: a KV head's keys stay in one L2)
+        wg = n_wgs % 8 == 0 && (int)blockIdx.x < n_wgs ? ((int)blockIdx.x & 7) * (n_wgs >> 3) + ((int)blockIdx.x >> 3)
+                                                       : (int)blockIdx.x;
+        if (wg >= n_wgs) {
+            if (threadIdx.x == 0) joins[wg].rows = 0;
+            return;
+        }
+        at = begin = pg_start(wg, total, n_wgs);
+        stop = pg_start(wg + 1, total, n_wgs);
+        head = (unsigned)begin / (unsigned)pu.total;
+        s = pu.find(begin - head * pu.total, u);
+    } else {
+        // the last tiles of the sequences, which walk the most keys, first (sorted
+        // over all sequences 3 % more: neighbours share a sequence's keys)
+        head = blockIdx.x % c.kv_heads;
+        const int unit = pu.total - 1 - (int)(blockIdx.x / c.kv_heads);
+        if (unit < 0) return;
+        s = pu.find(unit, u);
+    }
+    for (;;) {
     const PgSeq sq = pu.get(s);
+    if constexpr (CUT) {
+        if (sq.n == 0) {
+            if (++s == b.n_seqs) {
+                s = 0;
+                head++;
+            }
+            continue;
+        }
+    }
+    const int nk = CUT ? key_tiles(sq) : 1, tile = CUT ? (unsigned)u / (unsigned)nk : u;
+    const int t0 = CUT ? u - tile * nk : 0, m_units = CUT ? min(nk - t0, stop - at) : 1;
+    const bool whole = m_units == nk;
     const int rows = sq.n * grp, i0 = tile * X::ROWS;
     const int mine = min(i0 + 32 * w + n, rows - 1);
     const int row = sq.row0 + mine / grp, qh = head * grp + mine % grp;
@@ -116,7 +160,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
     const int wg_first = pos0 + i0 / grp, wg_last = pos0 + min(i0 + X::ROWS - 1, rows - 1) / grp;
     const int first = pos0 + min(i0 + 32 * w, rows - 1) / grp;
     const int last = i0 + 32 * w < rows ? pos0 + min(i0 + 32 * w + 31, rows - 1) / grp : -1;
-    const int tiles = wg_last >= 0 ? wg_last / PF_KEYS + 1 : 0;
+    int tiles = wg_last >= 0 ? wg_last / PF_KEYS + 1 : 0;
+    if constexpr (CUT) tiles = min(tiles, t0 + m_units);
 
     // Q^T, the B operand: dims 16 t + 8 h + e of row n
     v8 qf[X::NP][X::KS];
@@ -193,11 +238,11 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
     const int vr = (lane >> 2) & 3;
     const uint32_t vbase = (4 * h + vr) * X::ROW + 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ X::vswz(vr)) + 8 * (lane & 1);
 
-    if (tiles) {
-        fetch_ids(0);
-        issue(0);
+    if (t0 < tiles) {
+        fetch_ids(t0 * PF_KEYS);
+        issue(t0);
     }
-    for (int t = 0; t < tiles; t++) {
+    for (int t = t0; t < tiles; t++) {
         const int j0 = t * PF_KEYS;
         // tile t landed, in every wavefront, and tile t - 1 is read
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -341,21 +386,62 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         }
     }
     l += pf_other_half(l);
-    if (i0 + 32 * w + n >= rows) return;
-    const float inv = 1.0f / l;
-    T* dst = out + (size_t)row * ldo + (size_t)qh * HD + 4 * h;
+    if (i0 + 32 * w + n < rows) {
+        if (!CUT || whole) {
+            const float inv = 1.0f / l;
+            T* dst = out + (size_t)row * ldo + (size_t)qh * HD + 4 * h;
 #pragma unroll
-    for (int d = 0; d < X::DT; d++)
+            for (int d = 0; d < X::DT; d++)
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
-            T y[4];
+                for (int g = 0; g < 4; g++) {
+                    T y[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float x = o[d][4 * g + i] * inv;
-                y[i] = (T)(sq.bad ? pg_nan() : limit < 0 ? 0.0f : x);
+                    for (int i = 0; i < 4; i++) {
+                        const float x = o[d][4 * g + i] * inv;
+                        y[i] = (T)(sq.bad ? pg_nan() : limit < 0 ? 0.0f : x);
+                    }
+                    __builtin_memcpy(__builtin_assume_aligned(dst + 32 * d + 8 * g, 8), y, sizeof y);
+                }
+        } else {
+            float* slot = part + ((size_t)2 * wg + (at != begin)) * pg_slot(X::ROWS, HD);
+            float* dst = slot + (32 * w + n) * HD + 4 * h;
+#pragma unroll
+            for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    *reinterpret_cast<pg_f4*>(dst + 32 * d + 8 * g) =
+                        pg_f4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+            if (h == 0) {
+                slot[X::ROWS * HD + 32 * w + n] = m;
+                slot[X::ROWS * HD + X::ROWS + 32 * w + n] = l;
             }
-            __builtin_memcpy(__builtin_assume_aligned(dst + 32 * d + 8 * g, 8), y, sizeof y);
         }
+    }
+    if constexpr (!CUT) return;
+    if (at + m_units == stop) {
+        if (threadIdx.x == 0)
+            joins[wg] = pg_join(t0 == 0 && !whole, min(X::ROWS, rows - i0), sq, head, i0, at + nk - 1, total, n_wgs,
+                                2 * wg + (at != begin));
+        return;
+    }
+    at += m_units;
+    u += m_units;
+    if (u == (int)(((long)rows + X::ROWS - 1) / X::ROWS) * nk) {
+        u = 0;
+        if (++s == b.n_seqs) {
+            s = 0;
+            head++;
+        }
+    }
+    __syncthreads();  // the last key tile is read
+    }
+}
+
+// Whether a call's tiles are cut: see paged_prefill_kernel.
+constexpr int PF_CUT_TILES = PF_WGS, PF_CUT_KEYS = 2048;
+bool prefill_cut(const PagedKv& kv, const PagedRows& r, int grp) {
+    return pg_tiles_bound(r, grp, 32 * PF_WAVES) * kv.kv_heads <= PF_CUT_TILES && r.cap >= PF_CUT_KEYS &&
+           r.cap <= 1 << 27;  // (the units are an int)
 }
 
 struct PrefillCall {
@@ -363,17 +449,36 @@ struct PrefillCall {
     hipStream_t s;
     template <class E, class T, int HD>
     hipError_t run() const {
+        constexpr int ROWS = PrefillTile<E, T, HD>::ROWS;
         const int grp = p.n_heads / p.kv.kv_heads;
-        // a bound on the tiles: each sequence's last may be partly empty
-        const long tiles = (long)p.rows.rows * grp / PrefillTile<E, T, HD>::ROWS + p.rows.n_seqs;
-        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD>), dim3((unsigned)(tiles * p.kv.kv_heads)),
-                           dim3(64 * PF_WAVES), 0, s, p.kv, p.rows, grp, static_cast<const T*>(p.q), p.ldq, p.scale,
-                           static_cast<T*>(p.out), p.ldo);
-        return hipGetLastError();
+        const T* q = static_cast<const T*>(p.q);
+        T* out = static_cast<T*>(p.out);
+        if (!prefill_cut(p.kv, p.rows, grp)) {
+            hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, false>),
+                               dim3((unsigned)(pg_tiles_bound(p.rows, grp, ROWS) * p.kv.kv_heads)), dim3(64 * PF_WAVES), 0,
+                               s, p.kv, p.rows, grp, q, p.ldq, p.scale, out, p.ldo, nullptr, nullptr);
+            return hipGetLastError();
+        }
+        float* part = static_cast<float*>(p.work);
+        PgJoin* joins = reinterpret_cast<PgJoin*>(part + (size_t)2 * PF_WGS * pg_slot(ROWS, HD));
+        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, true>), dim3(PF_WGS), dim3(64 * PF_WAVES), 0, s, p.kv, p.rows,
+                           grp, q, p.ldq, p.scale, out, p.ldo, part, joins);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        return launch_paged_join(dtype_of<T>(), HD, joins, part, PF_WGS, ROWS, ROWS, grp, p.out, p.ldo, s);
+    }
+    template <class T>
+    static int dtype_of() {
+        return std::is_same<T, float>::value ? GGML_F32 : std::is_same<T, _Float16>::value ? GGML_F16 : GGML_BF16;
     }
 };
 
 }  // namespace
+
+size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    if (!prefill_cut(kv, r, n_heads / kv.kv_heads)) return 0;
+    return PF_WGS * (2 * pg_slot(32 * PF_WAVES, hd) * sizeof(float) + sizeof(PgJoin));
+}
 
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;

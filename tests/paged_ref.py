@@ -85,20 +85,21 @@ def attend(q, k, v, pos, scale):
     """q [m, H, D] over k, v [n, hk, D], row i sees keys 0 .. pos[i]: (out, A, B,
     max |v|) in 64 bits, out zeros where pos < 0."""
     m, H, D = q.shape
-    hk = k.shape[1]
+    hk, pos = k.shape[1], np.asarray(pos)
     out, A, B = np.zeros((m, H, D)), np.zeros((m, H, 1)), np.zeros((m, H, D))
     q, k, v = (a.astype(np.float64) for a in (q, k, v))
-    for i in range(m):
-        n = int(pos[i]) + 1
-        if n <= 0:
-            continue
-        for h in range(H):
-            kk, vv = k[:n, h * hk // H], v[:n, h * hk // H]
-            s = kk @ q[i, h] * scale
-            A[i, h] = (np.abs(kk) @ np.abs(q[i, h])).max() * abs(scale)
-            p = np.exp(s - s.max())
-            out[i, h] = p @ vv / p.sum()
-            B[i, h] = p @ np.abs(vv) / p.sum()
+    n = int(pos.max(initial=-1)) + 1
+    if n <= 0:
+        return out, A, B, 0.0
+    seen = np.arange(n)[None] <= pos[:, None]
+    some = seen.any(1)
+    for h in range(H):
+        kk, vv = k[:n, h * hk // H], v[:n, h * hk // H]
+        s = np.where(seen, q[:, h] @ kk.T * scale, -np.inf)
+        A[:, h, 0] = np.where(seen, np.abs(q[:, h]) @ np.abs(kk).T * abs(scale), 0).max(1)
+        p = np.exp(s - np.where(some, s.max(1), 0.0)[:, None])
+        p /= np.where(some, p.sum(1), 1.0)[:, None]
+        out[:, h], B[:, h] = p @ vv, p @ np.abs(vv)
     return out, A, B, np.abs(v).max(initial=0.0)
 
 

@@ -309,14 +309,72 @@ def test_prefill_long(dev, act, cache, H, hk, D, past, new):
     c.check(scale=-0.2)
 
 
+# batches that take the tiles of 128 rows: many rows times heads; with more than
+# 2048 keys and few tiles these are cut
 @pytest.mark.parametrize("act,cache", TYPES)
-@pytest.mark.parametrize("D", [64, 128])
-def test_prefill_keys_a_row_does_not_see_may_hold_anything(dev, act, cache, D):
+@pytest.mark.parametrize("H,hk,D,ps,past,new", [
+    (32, 4, 128, 16, [0, 0, 5, 100, 0, 33, -4], [150, 0, 64, 3, 65, 31, 9]),
+    (35, 5, 64, 64, [0, 700, 0, 1], [128, 100, 1, 63]),
+    (64, 64, 64, 32, [0, 0], [129, 64]),
+    (32, 2, 128, 16, [2100, 0, 2500, 0, -30], [140, 5, 100, 33, 40]),
+    (40, 1, 64, 256, [5000], [230])])
+def test_prefill_tiles(dev, act, cache, H, hk, D, ps, past, new):
+    say("prefill tiles", act, cache, H, hk, D, past, new)
+    c = Case(dev, seed(15, act, cache, H), act, cache, H, hk, D, ps, past, new, row0=3, tail=5, pad=8)
+    c.upload()
+    c.run()
+    a = c.check()
+    c.run()
+    np.testing.assert_array_equal(c.got(), a)
+    c.run(-0.2)
+    c.check(scale=-0.2)
+    c.run(0.0)
+    c.check(scale=0.0)
+
+
+def test_prefill_tiles_of_more_sequences_than_lanes(dev):
+    say("prefill tiles, many sequences")
+    for past, new in ((0, 5), (2100, 3)):
+        n = 150
+        c = Case(dev, seed(16, past), BF16, BF16, 64, 1, 64, 16, [past] * n, [new + i % 3 for i in range(n)])
+        if past:
+            c.kv[:-2] = [new + i % 3 for i in range(n - 2)]  # (most of them short)
+        c.upload()
+        c.run()
+        c.check()
+
+
+def test_prefill_tiles_malformed(dev):
+    """As test_malformed_batches_stay_in_bounds, for the tiles of 128 rows."""
+    for past in (0, 2300):
+        say("malformed tiles", past)
+        c = Case(dev, seed(17, past), F16, F16, 40, 2, 64, 16, [past, past, 3, 0, 10], [120, 140, 5, 33, 6])
+        c.pool.table[1, (past + 50) // 16] = -7
+        page = (past + 50) // 16 * 16 - past         # sequence 1's first row that sees it
+        c.kv[3] = -1 << 20
+        c.start[5] = c.rows + 1
+        c.upload()
+        c.run()
+        got, w = c.got(), 40 * 64
+        c.new[4] = 0
+        c.check(skip=(1, 3))
+        s1, s3 = c.start[1], c.start[3]
+        assert np.isnan(got[s1 + page:s1 + 140, :w]).all() and np.isfinite(got[s1:s1 + page, :w]).all()
+        assert np.isnan(got[s3:s3 + 33, :w]).all()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new,ats", [
+    (4, 2, 64, (0, 30), (170, 160), (1, 20, 63, 97, 150)), (4, 2, 128, (0, 30), (170, 160), (1, 20, 63, 97, 150)),
+    (32, 2, 128, (0, 30), (170, 160), (1, 20, 97)), (48, 4, 64, (0, 30), (100, 90), (5, 64)),
+    (32, 2, 128, (2200, 2000), (150, 140), (2250, 2100)), (40, 2, 64, (2200, 2000), (150, 140), (2230,))])
+def test_prefill_keys_a_row_does_not_see_may_hold_anything(dev, act, cache, H, hk, D, past, new, ats):
     """NaN and infinite keys and values from some position on: the rows before
     it as if they were not there, whatever tile they share with the others."""
-    say("prefill nan", act, cache, D)
-    for at in (1, 20, 63, 97, 150):
-        c = Case(dev, seed(11, act, at), act, cache, 4, 2, D, 16, [0, 30], [170, 160])
+    say("prefill nan", act, cache, H, D, past)
+    for at in ats:
+        c = Case(dev, seed(11, act, at), act, cache, H, hk, D, 16, past, new)
+        clean = [c.pool.get(s, min(at, int(c.kv[s]))) for s in range(2)]
         for s in range(2):
             n = int(c.kv[s])
             k, v = c.pool.get(s, n)
@@ -326,18 +384,16 @@ def test_prefill_keys_a_row_does_not_see_may_hold_anything(dev, act, cache, D):
             c.pool.put(s, np.arange(n), k, v)
         c.upload()
         c.run()
-        got, w = c.got(), 4 * D
-        clean = Case(dev, seed(11, act, at), act, cache, 4, 2, D, 16, [0, 30], [170, 160])
-        q = R.from_bits(R.to_bits(clean.q, act), act)
-        for s, p in enumerate((0, 30)):
-            m = max(0, at - p)
+        got, w = c.got(), H * D
+        q = R.from_bits(R.to_bits(c.q, act), act)
+        for s, p in enumerate(past):
+            m = max(0, min(at - p, c.new[s]))
             r0 = int(c.start[s])
             # the rows that see them are no numbers
             assert not np.isfinite(got[r0 + m:r0 + c.new[s], :w]).any()
             if not m:
                 continue
-            k, v = clean.pool.get(s, at)
-            want, A, B, V = R.attend(q[r0:r0 + m, :w].reshape(m, 4, D), k, v, p + np.arange(m), c.scale)
+            want, A, B, V = R.attend(q[r0:r0 + m, :w].reshape(m, H, D), *clean[s], p + np.arange(m), c.scale)
             tol = R.bound(want, A, B, V, at, D, act, cache, True)
             err = np.abs(got[r0:r0 + m, :w].reshape(want.shape) - want)
             assert (err <= tol).all(), (at, s, np.argwhere(~(err <= tol))[:3])
