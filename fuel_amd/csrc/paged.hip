@@ -473,11 +473,12 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
 // Joins the pieces of cut tiles: workgroup (w, y) takes rows PJ_ROWS y .. of the
 // one that workgroup w left to be joined, if it left one.  HD / 4 threads a row,
 // as many groups of such threads as there is room for with every so many-th
-// piece each, PJ_STEP pieces a step, whose loads are one memory round trip.
+// piece each, PJ_STEP pieces a step, whose loads are one memory round trip (8 of
+// the small pieces of 16 rows; a tile of 128 rows has two or three, and as many
+// workgroups hide that trip).
 constexpr int PJ_WG = 256;
 constexpr int PJ_ROWS = 4;
-constexpr int PJ_STEP = 8;
-template <class T, int HD>
+template <class T, int HD, int PJ_STEP>
 __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins,
                                                            const float* __restrict__ part, int tile_rows, int grp,
                                                            T* __restrict__ out, int ldo) {
@@ -686,9 +687,8 @@ struct AppendCall {
 
 // Sizes of a call of the 16-row kernel: keys a unit, and workgroups (a range
 // each, no more than the units that lengths up to cap can have).  Calls with
-// tiles for every CU and up to PD_WHOLE keys are not cut: a second launch costs
-// more than the longer walk.
-constexpr int PD_WHOLE = 512;
+// tiles for every CU and up to PG_WHOLE_KEYS keys are not cut: a second launch
+// costs more than the longer walk.
 struct Rows16Plan {
     int unit, wgs;
     bool cut;
@@ -697,7 +697,7 @@ Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads) {
     const int grp = n_heads / kv.kv_heads;
     const long tiles = pg_tiles_bound(r, grp, 16) * kv.kv_heads;
     Rows16Plan p;
-    p.unit = tiles >= 256 && r.cap <= PD_WHOLE ? PD_WHOLE : PD_UNIT;
+    p.unit = tiles >= 256 && r.cap <= PG_WHOLE_KEYS ? PG_WHOLE_KEYS : PD_UNIT;
     const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
     p.cut = r.cap > p.unit;
     p.wgs = (int)(units < PD_WGS || !p.cut ? units : PD_WGS);
@@ -707,7 +707,8 @@ Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads) {
 template <class T, int HD>
 hipError_t join(const PgJoin* joins, const float* part, int wgs, int tile_rows, int rows, int grp, void* out, int ldo,
                 hipStream_t s) {
-    hipLaunchKernelGGL((paged_join_kernel<T, HD>), dim3(wgs, (rows + PJ_ROWS - 1) / PJ_ROWS), dim3(PJ_WG), 0, s, joins, part,
+    const auto kernel = tile_rows == 16 ? paged_join_kernel<T, HD, 8> : paged_join_kernel<T, HD, 2>;
+    hipLaunchKernelGGL(kernel, dim3(wgs, (rows + PJ_ROWS - 1) / PJ_ROWS), dim3(PJ_WG), 0, s, joins, part,
                        tile_rows, grp, static_cast<T*>(out), ldo);
     return hipGetLastError();
 }

@@ -45,6 +45,34 @@ inline long pg_tiles_bound(const PagedRows& r, int grp, int tile_rows) {
     return r.row_start ? (long)r.rows * grp / tile_rows + r.n_seqs : (long)r.n_seqs * ((grp + tile_rows - 1) / tile_rows);
 }
 
+// Which kernel a call takes.  ROWS16: 16 query rows a tile, the keys of a call
+// over all workgroups (paged.hip).  TILES: 128 rows a tile, a workgroup each;
+// CUT: the same, the keys over all workgroups (paged_prefill.hip).  One row a
+// sequence: always ROWS16.  Otherwise by what they took, in us, over 1 or 4
+// sequences, 4 .. 1500 new rows after 0 .. 16000 cached, 2 .. 32 KV heads, f32
+// and bf16 (K: keys of the longest sequence, n: tiles times KV heads; the
+// estimate is the same for all types, since the workspace's size is):
+//   ROWS16  12 + n16 K / 20000        (8 + .. where no tile is cut)
+//   TILES    9 + 0.024 K              (n128 <= 256: its longest walk)
+//            9 + 0.037 K max(1, n128 / 512)
+//   CUT     28 + n128 K / 13000       (the second launch and the pieces' bytes)
+// Of 32 heads over 8, bf16: 128 rows after 600: 22 / 25 / 30 (ROWS16 / TILES /
+// CUT), 300 after 600: 41 / 29 / 45, 300 after 4096: 159 / 103 / 64, 1500 after
+// 600: 248 / 63 / 86.
+enum PagedKind { PG_ROWS16, PG_TILES, PG_CUT };
+constexpr int PG_WHOLE_KEYS = 512;  // ROWS16 with a tile for every CU: cut only beyond
+inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads) {
+    if (!r.row_start) return PG_ROWS16;
+    const int grp = n_heads / kv.kv_heads;
+    const double k = r.cap, n16 = (double)pg_tiles_bound(r, grp, 16) * kv.kv_heads,
+                 n128 = (double)pg_tiles_bound(r, grp, 128) * kv.kv_heads;
+    const double rows16 = (r.cap <= 128 || (r.cap <= PG_WHOLE_KEYS && n16 >= 256) ? 8 : 12) + n16 * k / 20000;
+    const double tiles = 9 + (n128 <= 256 ? 0.024 * k : 0.037 * k * (n128 > 512 ? n128 / 512 : 1.0));
+    const double cut = r.cap <= 1 << 24 && n128 <= 4096 ? 28 + n128 * k / 13000 : 1e30;  // (its units are an int)
+    if (rows16 <= tiles && rows16 <= cut) return PG_ROWS16;
+    return tiles <= cut ? PG_TILES : PG_CUT;
+}
+
 // Cut tiles.  Workgroups that share the keys of a tile of `rows` query rows
 // leave slots of floats in the workspace, two a workgroup: o [rows][hd]
 // (unnormalized), m [rows], l [rows]; and each a record of what is to be joined.

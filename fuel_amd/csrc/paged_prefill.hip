@@ -437,13 +437,6 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
     }
 }
 
-// Whether a call's tiles are cut: see paged_prefill_kernel.
-constexpr int PF_CUT_TILES = PF_WGS, PF_CUT_KEYS = 2048;
-bool prefill_cut(const PagedKv& kv, const PagedRows& r, int grp) {
-    return pg_tiles_bound(r, grp, 32 * PF_WAVES) * kv.kv_heads <= PF_CUT_TILES && r.cap >= PF_CUT_KEYS &&
-           r.cap <= 1 << 27;  // (the units are an int)
-}
-
 struct PrefillCall {
     const PagedAttendArgs& p;
     hipStream_t s;
@@ -453,7 +446,7 @@ struct PrefillCall {
         const int grp = p.n_heads / p.kv.kv_heads;
         const T* q = static_cast<const T*>(p.q);
         T* out = static_cast<T*>(p.out);
-        if (!prefill_cut(p.kv, p.rows, grp)) {
+        if (pg_kind(p.kv, p.rows, p.n_heads) != PG_CUT) {
             hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, false>),
                                dim3((unsigned)(pg_tiles_bound(p.rows, grp, ROWS) * p.kv.kv_heads)), dim3(64 * PF_WAVES), 0,
                                s, p.kv, p.rows, grp, q, p.ldq, p.scale, out, p.ldo, nullptr, nullptr);
@@ -476,7 +469,7 @@ struct PrefillCall {
 }  // namespace
 
 size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
-    if (!prefill_cut(kv, r, n_heads / kv.kv_heads)) return 0;
+    if (pg_kind(kv, r, n_heads) != PG_CUT) return 0;
     return PF_WGS * (2 * pg_slot(32 * PF_WAVES, hd) * sizeof(float) + sizeof(PgJoin));
 }
 

@@ -344,6 +344,16 @@ def test_prefill_tiles_of_more_sequences_than_lanes(dev):
         c.check()
 
 
+def test_prefill_cut_tiles_of_more_sequences_than_lanes(dev):
+    say("cut tiles, many sequences")
+    past = [0] * 70
+    past[3], past[66] = 5900, 3100
+    c = Case(dev, seed(18), F16, F16, 16, 1, 64, 16, past, [40 - i % 5 for i in range(70)])
+    c.upload()
+    c.run()
+    c.check()
+
+
 def test_prefill_tiles_malformed(dev):
     """As test_malformed_batches_stay_in_bounds, for the tiles of 128 rows."""
     for past in (0, 2300):
@@ -367,6 +377,7 @@ def test_prefill_tiles_malformed(dev):
 @pytest.mark.parametrize("H,hk,D,past,new,ats", [
     (4, 2, 64, (0, 30), (170, 160), (1, 20, 63, 97, 150)), (4, 2, 128, (0, 30), (170, 160), (1, 20, 63, 97, 150)),
     (32, 2, 128, (0, 30), (170, 160), (1, 20, 97)), (48, 4, 64, (0, 30), (100, 90), (5, 64)),
+    (64, 4, 64, (0, 30), (170, 160), (5, 97)),
     (32, 2, 128, (2200, 2000), (150, 140), (2250, 2100)), (40, 2, 64, (2200, 2000), (150, 140), (2230,))])
 def test_prefill_keys_a_row_does_not_see_may_hold_anything(dev, act, cache, H, hk, D, past, new, ats):
     """NaN and infinite keys and values from some position on: the rows before
