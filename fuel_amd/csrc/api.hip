@@ -1486,7 +1486,7 @@ int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, co
     if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
     if (!paged_types(kv->dtype, dtype))
         return fail(FRQ_UNSUPPORTED, "%s: dtype %d over a cache of dtype %d", who, dtype, kv->dtype);
-    const bool rows16 = pg_kind(a.kv, a.rows, (int)n_heads) == PG_ROWS16;
+    const bool rows16 = pg_kind(a.kv, a.rows, (int)n_heads, (int)kv->head_dim) == PG_ROWS16;
     if (rows16 && !paged_rows16_fits(a.kv, a.rows, (int)n_heads))
         return fail(FRQ_UNSUPPORTED, "%s: n_seqs=%zu of up to %d tokens", who, b->n_seqs, a.rows.cap);
     const bool none = b->n_seqs == 0 || b->rows == 0;
@@ -1557,7 +1557,7 @@ size_t frq_paged_attention_workspace(const frq_paged_kv* kv, const frq_paged_bat
     PagedKv k;
     PagedRows r;
     if (paged_args("paged_attention_workspace", kv, b, n_heads, &k, &r)) return 0;
-    return (pg_kind(k, r, (int)n_heads) == PG_ROWS16 ? paged_rows16_work_bytes : paged_prefill_work_bytes)(
+    return (pg_kind(k, r, (int)n_heads, (int)kv->head_dim) == PG_ROWS16 ? paged_rows16_work_bytes : paged_prefill_work_bytes)(
         k, r, (int)n_heads, (int)kv->head_dim);
 }
 

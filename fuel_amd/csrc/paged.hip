@@ -686,18 +686,16 @@ struct AppendCall {
 };
 
 // Sizes of a call of the 16-row kernel: keys a unit, and workgroups (a range
-// each, no more than the units that lengths up to cap can have).  Calls with
-// tiles for every CU and up to PG_WHOLE_KEYS keys are not cut: a second launch
-// costs more than the longer walk.
+// each, no more than the units that lengths up to cap can have).
 struct Rows16Plan {
     int unit, wgs;
     bool cut;
 };
-Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads) {
+Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     const int grp = n_heads / kv.kv_heads;
     const long tiles = pg_tiles_bound(r, grp, 16) * kv.kv_heads;
     Rows16Plan p;
-    p.unit = tiles >= 256 && r.cap <= PG_WHOLE_KEYS ? PG_WHOLE_KEYS : PD_UNIT;
+    p.unit = pg_whole(kv, r, n_heads, hd) ? PG_WHOLE_KEYS : PD_UNIT;
     const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
     p.cut = r.cap > p.unit;
     p.wgs = (int)(units < PD_WGS || !p.cut ? units : PD_WGS);
@@ -719,7 +717,7 @@ struct Rows16Call {
     template <class E, class T, int HD>
     hipError_t run() const {
         const int grp = p.n_heads / p.kv.kv_heads;
-        const Rows16Plan pl = rows16_plan(p.kv, p.rows, p.n_heads);
+        const Rows16Plan pl = rows16_plan(p.kv, p.rows, p.n_heads, HD);
         float* part = static_cast<float*>(p.work);
         PgJoin* joins = pl.cut ? reinterpret_cast<PgJoin*>(part + (size_t)2 * pl.wgs * pg_slot(16, HD)) : nullptr;
         // Past the caches where one tile reads its keys alone and the batch's may
@@ -739,7 +737,7 @@ struct Rows16Call {
 }  // namespace
 
 size_t paged_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
-    const Rows16Plan p = rows16_plan(kv, r, n_heads);
+    const Rows16Plan p = rows16_plan(kv, r, n_heads, hd);
     return p.cut ? p.wgs * (2 * pg_slot(16, hd) * sizeof(float) + sizeof(PgJoin)) : 0;
 }
 

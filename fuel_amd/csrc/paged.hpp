@@ -52,7 +52,7 @@ inline long pg_tiles_bound(const PagedRows& r, int grp, int tile_rows) {
 // sequences, 4 .. 1500 new rows after 0 .. 16000 cached, 2 .. 32 KV heads, f32
 // and bf16 (K: keys of the longest sequence, n: tiles times KV heads; the
 // estimate is the same for all types, since the workspace's size is):
-//   ROWS16  12 + n16 K / 20000        (8 + .. where no tile is cut)
+//   ROWS16  12 + n16 K / 20000        (8 + .. where its tiles stay whole)
 //   TILES    9 + 0.024 K              (n128 <= 256: its longest walk)
 //            9 + 0.037 K max(1, n128 / 512)
 //   CUT     28 + n128 K / 13000       (the second launch and the pieces' bytes)
@@ -60,13 +60,23 @@ inline long pg_tiles_bound(const PagedRows& r, int grp, int tile_rows) {
 // CUT), 300 after 600: 41 / 29 / 45, 300 after 4096: 159 / 103 / 64, 1500 after
 // 600: 248 / 63 / 86.
 enum PagedKind { PG_ROWS16, PG_TILES, PG_CUT };
-constexpr int PG_WHOLE_KEYS = 512;  // ROWS16 with a tile for every CU: cut only beyond
-inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads) {
+// Whether ROWS16 leaves its tiles whole: short walks, which a second launch
+// would cost more than they take.  One token a sequence, cut / whole, us: 8
+// tiles of 200 keys of 128 10.6 / 8.2, of 400 10.3 / 10.6, 128 tiles of 400
+// 13.2 / 11.4, of 1000 19.6 / 19.9; 8 tiles of 400 keys of 64 9.9 / 7.8.  (Of
+// longer ones whole tiles gain up to 10 % where all are as long as the longest
+// and there is one for every CU, and lose more where they are not.)
+constexpr int PG_WHOLE_KEYS = 1024;
+inline bool pg_whole(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    const long tiles = pg_tiles_bound(r, n_heads / kv.kv_heads, 16) * kv.kv_heads;
+    return (long)r.cap * hd <= (tiles >= 128 ? 65536 : 32768);
+}
+inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     if (!r.row_start) return PG_ROWS16;
     const int grp = n_heads / kv.kv_heads;
     const double k = r.cap, n16 = (double)pg_tiles_bound(r, grp, 16) * kv.kv_heads,
                  n128 = (double)pg_tiles_bound(r, grp, 128) * kv.kv_heads;
-    const double rows16 = (r.cap <= 128 || (r.cap <= PG_WHOLE_KEYS && n16 >= 256) ? 8 : 12) + n16 * k / 20000;
+    const double rows16 = (pg_whole(kv, r, n_heads, hd) ? 8 : 12) + n16 * k / 20000;
     const double tiles = 9 + (n128 <= 256 ? 0.024 * k : 0.037 * k * (n128 > 512 ? n128 / 512 : 1.0));
     const double cut = r.cap <= 1 << 24 && n128 <= 4096 ? 28 + n128 * k / 13000 : 1e30;  // (its units are an int)
     if (rows16 <= tiles && rows16 <= cut) return PG_ROWS16;

@@ -446,7 +446,7 @@ struct PrefillCall {
         const int grp = p.n_heads / p.kv.kv_heads;
         const T* q = static_cast<const T*>(p.q);
         T* out = static_cast<T*>(p.out);
-        if (pg_kind(p.kv, p.rows, p.n_heads) != PG_CUT) {
+        if (pg_kind(p.kv, p.rows, p.n_heads, HD) != PG_CUT) {
             hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, false>),
                                dim3((unsigned)(pg_tiles_bound(p.rows, grp, ROWS) * p.kv.kv_heads)), dim3(64 * PF_WAVES), 0,
                                s, p.kv, p.rows, grp, q, p.ldq, p.scale, out, p.ldo, nullptr, nullptr);
@@ -469,7 +469,7 @@ struct PrefillCall {
 }  // namespace
 
 size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
-    if (pg_kind(kv, r, n_heads) != PG_CUT) return 0;
+    if (pg_kind(kv, r, n_heads, hd) != PG_CUT) return 0;
     return PF_WGS * (2 * pg_slot(32 * PF_WAVES, hd) * sizeof(float) + sizeof(PgJoin));
 }
 
