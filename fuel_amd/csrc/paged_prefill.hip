@@ -49,11 +49,11 @@ __device__ __forceinline__ pf_f16 pf_mfma(PgElem<__bf16>::v8 a, PgElem<__bf16>::
 // 64 lanes' 16 bytes from base + voff to LDS address lds + 16 * lane.  Written
 // in assembly so that the compiler does not wait for it before every LDS read
 // (it cannot tell the tile being filled from the one being read): the kernel
-// waits itself.  The wait states cover M0 and a base that a lane read made.
+// waits itself.  One wait state between the M0 write and its use.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void pf_dma(const void* base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds)
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base), "s"(lds)
                  : "memory", "m0");
 }
 #pragma clang diagnostic pop
@@ -205,31 +205,39 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
     float m = -1e30f, l = 0.0f;
 
-    // DMA source offsets
+    // DMA: instruction i of this wavefront takes rows ((i PF_WAVES + w) RPI) .. of
+    // a tile, all in one group of 16 keys.  Source offsets of the lane within it:
     constexpr int CPR = HD / 8;
     const int dr = w * X::RPI + lane / CPR, pc = lane % CPR;
-    const uint32_t koff = (lane / CPR) * X::ROW + 16 * (pc ^ X::kswz(dr));
-    const uint32_t voff = (lane / CPR) * X::ROW + 16 * (pc ^ X::vswz(dr));
+    const uint32_t koff = (dr & 15) * X::ROW + 16 * (pc ^ X::kswz(dr));
+    const uint32_t voff = (dr & 15) * X::ROW + 16 * (pc ^ X::vswz(dr));
     const int* table = b.table + (size_t)s * b.max_pages;
-    // page ids of 64 groups of 16 keys, lane i that of group i from key id0 on
-    int id0 = 0, id = 0;
+    // Byte offsets in the pools of 64 groups of 16 keys, lane i that of group i from
+    // key id0 on, and which groups' page is none (theirs lead to page 0).
+    int id0 = 0;
+    uint32_t off_lo = 0, off_hi = 0;
+    uint64_t none = 0;
     auto fetch_ids = [&](int j0) {
         id0 = j0;
-        const int j = j0 + 16 * lane;
-        id = j < sq.kv ? table[j >> c.log_ps] : 0;
+        const int j = j0 + 16 * lane, id = j < sq.kv ? table[j >> c.log_ps] : 0;
+        const bool off = (unsigned)id >= (unsigned)c.n_pages;
+        none = __ballot(off);
+        const size_t at = ((((size_t)(off ? 0 : id) * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * X::ROW;
+        off_lo = (uint32_t)at;
+        off_hi = (uint32_t)(at >> 32);
     };
     auto issue = [&](int t) {
         const int j0 = t * PF_KEYS;
         if (j0 - id0 >= 1024) fetch_ids(j0);
+        const int g0 = (j0 - id0) >> 4;
+        const uint32_t kto = pf_lds(s_k[t & 1]) + w * 1024, vto = pf_lds(s_v[t & 1]) + w * 1024;
 #pragma unroll
         for (int i = 0; i < X::NI; i++) {
-            const int r0 = (i * PF_WAVES + w) * X::RPI;
-            int page = __builtin_amdgcn_readlane(id, (j0 - id0 + r0) >> 4);
-            if ((unsigned)page >= (unsigned)c.n_pages) page = 0;
-            const size_t at = ((((size_t)page * c.kv_heads + head) << c.log_ps) + ((j0 + r0) & ((1 << c.log_ps) - 1))) * X::ROW;
-            const uint32_t to = (i * PF_WAVES + w) * 1024;
-            pf_dma(static_cast<const uint8_t*>(c.k) + at, koff, pf_lds(s_k[t & 1]) + to);
-            pf_dma(static_cast<const uint8_t*>(c.v) + at, voff, pf_lds(s_v[t & 1]) + to);
+            const int g = g0 + ((i * PF_WAVES + w) * X::RPI >> 4);
+            const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, g) << 32 |
+                                  (uint32_t)__builtin_amdgcn_readlane(off_lo, g);
+            pf_dma(static_cast<const uint8_t*>(c.k) + from, koff, kto + i * PF_WAVES * 1024);
+            pf_dma(static_cast<const uint8_t*>(c.v) + from, voff, vto + i * PF_WAVES * 1024);
         }
     };
     // LDS read offsets of this lane: K row n (+ 32), chunks 2 t + h; V rows
@@ -248,11 +256,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        // pages that are none, one bit a group of 16 keys
-        uint32_t bad = 0;
-#pragma unroll
-        for (int i = 0; i < PF_KEYS / 16; i++)
-            bad |= (uint32_t)((unsigned)__builtin_amdgcn_readlane(id, ((j0 - id0) >> 4) + i) >= (unsigned)c.n_pages) << i;
+        const uint32_t bad = (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
         const bool masked = j0 + PF_KEYS - 1 > wg_first || bad;
         uint64_t odd = 0;
         if (masked) {
@@ -281,7 +285,6 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
             __syncthreads();
             odd = (uint64_t)s_odd[1] << 32 | s_odd[0];
         }
-        const int id_now = id, id0_now = id0;
         if (t + 1 < tiles) issue(t + 1);
         if (j0 > last) continue;
 
@@ -371,7 +374,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                         if (32 * a + (i & 3) + 8 * (i >> 2) == (r & ~4)) p = st[a][i];
                 const float q2 = pf_other_half(p);
                 p = ((r >> 2) & 1) == h ? p : q2;
-                const int page = __builtin_amdgcn_readlane(id_now, (j0 - id0_now + r) >> 4);
+                const int page = table[(j0 + r) >> c.log_ps];
                 const E* src = static_cast<const E*>(c.v) +
                                ((((size_t)page * c.kv_heads + head) << c.log_ps) + ((j0 + r) & ((1 << c.log_ps) - 1))) * HD;
                 if (j0 + r > limit) continue;
