@@ -470,23 +470,22 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
     }
 }
 
-// Joins the pieces of cut tiles: workgroup (w, y) takes rows PJ_ROWS y .. of the
+// Joins the pieces of cut tiles: workgroup (w, y) takes rows wg_rows y .. of the
 // one that workgroup w left to be joined, if it left one.  HD / 4 threads a row,
 // as many groups of such threads as there is room for with every so many-th
 // piece each, PJ_STEP pieces a step, whose loads are one memory round trip (8 of
 // the small pieces of 16 rows; a tile of 128 rows has two or three, and as many
 // workgroups hide that trip).
 constexpr int PJ_WG = 256;
-constexpr int PJ_ROWS = 4;
 template <class T, int HD, int PJ_STEP>
 __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins,
-                                                           const float* __restrict__ part, int tile_rows, int grp,
-                                                           T* __restrict__ out, int ldo) {
+                                                           const float* __restrict__ part, int tile_rows, int wg_rows,
+                                                           int grp, T* __restrict__ out, int ldo) {
     constexpr int TH = HD / 4;
     __shared__ pg_f4 s_o[PJ_WG];
     __shared__ float s_l[PJ_WG / TH], s_m[PJ_WG / TH];
     const PgJoin j = joins[blockIdx.x];
-    const int r0 = PJ_ROWS * blockIdx.y, rows = min(PJ_ROWS, j.rows - r0);
+    const int r0 = wg_rows * blockIdx.y, rows = min(wg_rows, j.rows - r0);
     if (rows <= 0) return;
     const int groups = (unsigned)(PJ_WG / TH) / (unsigned)rows, w0 = blockIdx.x;
     const int d = threadIdx.x % TH, x = threadIdx.x / TH, p = (unsigned)x / (unsigned)rows, r = r0 + x - p * rows;
@@ -702,12 +701,16 @@ Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int h
     return p;
 }
 
+// wg_rows: rows a joining workgroup.  4, or 1 where few tiles are cut into many
+// pieces each (a whole call with 4 / 1: 2 sequences of 29561, 128 pieces, 28.9 /
+// 22.7 us; 5 of up to 60888, 100 pieces, 36.3 / 32.8; one of 131071, 8 KV heads,
+// 64 pieces, 92.6 / 91.2).
 template <class T, int HD>
-hipError_t join(const PgJoin* joins, const float* part, int wgs, int tile_rows, int rows, int grp, void* out, int ldo,
-                hipStream_t s) {
+hipError_t join(const PgJoin* joins, const float* part, int wgs, int tile_rows, int rows, int wg_rows, int grp, void* out,
+                int ldo, hipStream_t s) {
     const auto kernel = tile_rows == 16 ? paged_join_kernel<T, HD, 8> : paged_join_kernel<T, HD, 2>;
-    hipLaunchKernelGGL(kernel, dim3(wgs, (rows + PJ_ROWS - 1) / PJ_ROWS), dim3(PJ_WG), 0, s, joins, part,
-                       tile_rows, grp, static_cast<T*>(out), ldo);
+    hipLaunchKernelGGL(kernel, dim3(wgs, (rows + wg_rows - 1) / wg_rows), dim3(PJ_WG), 0, s, joins, part, tile_rows, wg_rows,
+                       grp, static_cast<T*>(out), ldo);
     return hipGetLastError();
 }
 
@@ -730,7 +733,9 @@ struct Rows16Call {
                            static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !pl.cut) return e;
-        return join<T, HD>(joins, part, pl.wgs, 16, p.rows.row_start || grp > 16 ? 16 : grp, grp, p.out, p.ldo, s);
+        const bool many = pl.wgs >= 32 * pg_tiles_bound(p.rows, grp, 16) * p.kv.kv_heads;
+        return join<T, HD>(joins, part, pl.wgs, 16, p.rows.row_start || grp > 16 ? 16 : grp, many ? 1 : 4, grp, p.out, p.ldo,
+                           s);
     }
 };
 
@@ -760,7 +765,7 @@ hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float
     const auto run = dtype == GGML_F32   ? (hd == 64 ? join<float, 64> : join<float, 128>)
                      : dtype == GGML_F16 ? (hd == 64 ? join<_Float16, 64> : join<_Float16, 128>)
                                          : (hd == 64 ? join<__bf16, 64> : join<__bf16, 128>);
-    return run(joins, part, wgs, tile_rows, rows, grp, out, ldo, s);
+    return run(joins, part, wgs, tile_rows, rows, 4, grp, out, ldo, s);
 }
 
 hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
