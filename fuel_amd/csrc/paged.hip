@@ -470,6 +470,50 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
     }
 }
 
+// Whole tiles of short walks, a wavefront each: where a tile is a few blocks of
+// 32 keys, waiting for memory in turn is all that it does, and eight or more of
+// them, not two or three, wait on a CU at a time; nor is there a merge.  One
+// token a sequence, 128 dims, us, four wavefronts a tile / one:
+//   keys          20          60         120         250          500
+//    512 tiles  7.7/6.6     8.2/7.6   10.0/12.0   16.1/19.8   25.5/33.7
+//    768       11.2/6.2    12.6/8.1   15.9/13.2   22.3/21.9   35.3/38.5
+//   4096       46.9/17.2   49.3/25.3  65.6/44.1   98.4/87.9  169.7/169.1
+// and up to half as long again where a batch's lengths differ much.
+template <class E, class T, int HD, bool ONCE>
+__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(PagedKv c, PagedRows b, int grp, int each,
+                                                                              const T* __restrict__ q, int ldq,
+                                                                              float scale, T* __restrict__ out, int ldo) {
+    using A = Rows16<E, T, HD>;
+    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+    const int at = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * PA_WAVES + (threadIdx.x >> 6)));
+    const auto tiles_of = [&](const PgSeq& x) { return pd_tiles(x, grp); };
+    PgUnits<decltype(tiles_of)> pu(b, tiles_of, each);
+    if (at >= pu.total * c.kv_heads) return;
+    const int head = (unsigned)at / (unsigned)pu.total;
+    int tile;
+    const int s = pu.find(at - head * pu.total, tile);
+    const PgSeq sq = pu.get(s);
+    const int all = sq.n * grp, i0 = 16 * tile, i = min(i0 + r, all - 1), pos0 = sq.kv - sq.n;
+    const int row = sq.row0 + i / grp, h = head * grp + i % grp;
+    A a;
+    a.load_q(q + (size_t)row * ldq + (size_t)h * HD, scale);
+    a.limit = pos0 + i / grp;
+    a.start();
+    pd_walk<E, T, HD, ONCE>(a, c, b.table + (size_t)s * b.max_pages, head, 0, pos0 + min(i0 + 15, all - 1) / grp + 1,
+                            sq.kv, pos0 + i0 / grp);
+    a.finish();
+    if (i0 + r >= all) return;
+    const float inv = 1.0f / a.l;
+    T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        T y[A::VW];
+#pragma unroll
+        for (int t = 0; t < A::VW; t++) y[t] = (T)(sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : a.o[t][k] * inv);
+        __builtin_memcpy(__builtin_assume_aligned(dst + A::VW * k, 8), y, sizeof y);
+    }
+}
+
 // Joins the pieces of cut tiles: workgroup (w, y) takes rows wg_rows y .. of the
 // one that workgroup w left to be joined, if it left one.  HD / 4 threads a row,
 // as many groups of such threads as there is room for with every so many-th
@@ -684,11 +728,12 @@ struct AppendCall {
     }
 };
 
-// Sizes of a call of the 16-row kernel: keys a unit, and workgroups (a range
-// each, no more than the units that lengths up to cap can have).
+// Sizes of a call of the 16-row kernels: keys a unit, and workgroups (a range
+// each, no more than the units that lengths up to cap can have) or, alone, the
+// wavefronts of a tile each.
 struct Rows16Plan {
     int unit, wgs;
-    bool cut;
+    bool cut, alone;
 };
 Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     const int grp = n_heads / kv.kv_heads;
@@ -698,6 +743,7 @@ Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int h
     const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
     p.cut = r.cap > p.unit;
     p.wgs = (int)(units < PD_WGS || !p.cut ? units : PD_WGS);
+    p.alone = r.cap <= 32 || (r.cap <= 256 && tiles > PD_WGS);
     return p;
 }
 
@@ -727,8 +773,15 @@ struct Rows16Call {
         // exceed the 256 MB last-level cache (537 MB 103.9 -> 92.8 us, 201 MB 55.6
         // -> 50.5; what the cache still holds of 82 MB it would lose, 26.8 -> 29.1)
         const double bytes = (double)p.rows.n_seqs * p.rows.cap * p.kv.kv_heads * HD * 4;
-        const auto kernel = !p.rows.row_start && grp <= 16 && bytes > 256e6 ? paged_rows16_kernel<E, T, HD, true>
-                                                           : paged_rows16_kernel<E, T, HD, false>;
+        const bool once = !p.rows.row_start && grp <= 16 && bytes > 256e6;
+        if (pl.alone) {
+            const auto kernel = once ? paged_rows16_alone_kernel<E, T, HD, true> : paged_rows16_alone_kernel<E, T, HD, false>;
+            hipLaunchKernelGGL(kernel, dim3((pl.wgs + PA_WAVES - 1) / PA_WAVES), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp,
+                               p.rows.row_start ? 0 : (grp + 15) >> 4, static_cast<const T*>(p.q), p.ldq, p.scale,
+                               static_cast<T*>(p.out), p.ldo);
+            return hipGetLastError();
+        }
+        const auto kernel = once ? paged_rows16_kernel<E, T, HD, true> : paged_rows16_kernel<E, T, HD, false>;
         hipLaunchKernelGGL(kernel, dim3(pl.wgs), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp, pl.unit,
                            static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part, joins);
         const hipError_t e = hipGetLastError();

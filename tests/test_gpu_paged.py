@@ -279,6 +279,32 @@ def test_malformed_batches_stay_in_bounds(dev):
     assert np.isnan(got[s3:s3 + 33, :w]).all()
 
 
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("decode", [True, False])
+@pytest.mark.parametrize("H,hk,D,top", [(20, 20, 128, 100), (40, 20, 64, 250), (3, 3, 128, 31), (70, 2, 64, 30)])
+def test_many_short_sequences(dev, act, cache, decode, H, hk, D, top):
+    """A wavefront a tile: lengths of none, one and up to `top`, a length that is
+    none, a page that is none, sequences of no rows, keys behind a row that are
+    no numbers."""
+    say("many short", act, cache, decode, H, D, top)
+    rng = seed(18, act, cache, H, decode)
+    kv = np.concatenate([[0, 1, 2, 16, 17, top, top, 25, 25], rng.integers(1, top + 1, 24)])
+    new = [1] * len(kv) if decode else [0, 1, 2, 3, 17, 4, 0, 3, 9] + [int(n) for n in rng.integers(0, 4, 24)]
+    c = Case(dev, rng, act, cache, H, hk, D, 16, [int(n) - m for n, m in zip(kv, new)], new, row0=0 if decode else 2,
+             tail=0 if decode else 3, pad=8, decode=decode, max_kv_len=top)
+    c.kv[7] = top + 1
+    c.pool.table[8, 1] = -1  # (positions 16 ..: all rows of sequence 8)
+    page, slot = c.pool.table[5, (top - 1) // 16], (top - 1) % 16
+    c.pool.k[page, :, slot + 1:], c.pool.v[page, :, slot + 1:] = R.NAN[cache], R.NAN[cache]
+    c.upload()
+    c.run()
+    got = c.check(skip=(7, 8))
+    for s in (7, 8):
+        assert np.isnan(got[c.start[s]:c.start[s] + new[s], :H * D]).all()
+    c.run()
+    np.testing.assert_array_equal(c.got(), got)
+
+
 # ---- prefill ----
 
 @pytest.mark.parametrize("act,cache", TYPES)
