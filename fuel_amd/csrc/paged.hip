@@ -282,7 +282,6 @@ struct Rows16 {
 // written out, the cut pieces (at most two a workgroup) leave their sums in
 // the workspace for paged_join_kernel.
 constexpr int PD_UNIT = 32 * PA_WAVES;
-constexpr int PD_WGS = 512;  // two a CU, all resident at once
 
 // Tiles of a sequence, and units of each; one without keys has one unit, which
 // writes its rows.
@@ -514,24 +513,38 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(Pa
     }
 }
 
-// Joins the pieces of cut tiles: workgroup (w, y) takes rows wg_rows y .. of the
-// one that workgroup w left to be joined, if it left one.  HD / 4 threads a row,
-// as many groups of such threads as there is room for with every so many-th
-// piece each, PJ_STEP pieces a step, whose loads are one memory round trip (8 of
-// the small pieces of 16 rows; a tile of 128 rows has two or three, and as many
-// workgroups hide that trip).
+// Joins the pieces of cut tiles: workgroups (x, y) take rows wg_rows y .. of the
+// one that workgroup x left to be joined, if it left one, or with fewer x than
+// records of the x-th that is left at all.  HD / 4 threads a row, as many groups
+// of such threads as there is room for with every so many-th piece each, PJ_STEP
+// pieces a step, whose loads are one memory round trip.
 constexpr int PJ_WG = 256;
 template <class T, int HD, int PJ_STEP>
-__global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins,
+__global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins, int records,
                                                            const float* __restrict__ part, int tile_rows, int wg_rows,
                                                            int grp, T* __restrict__ out, int ldo) {
     constexpr int TH = HD / 4;
     __shared__ pg_f4 s_o[PJ_WG];
     __shared__ float s_l[PJ_WG / TH], s_m[PJ_WG / TH];
-    const PgJoin j = joins[blockIdx.x];
+    __shared__ uint64_t s_some[PG_WGS / 64];
+    int w0 = blockIdx.x;
+    if ((int)gridDim.x < records) {
+        for (int i = threadIdx.x; i < PG_WGS; i += PJ_WG) {
+            const uint64_t some = __ballot(i < records && joins[i].rows > 0);
+            if ((threadIdx.x & 63) == 0) s_some[i >> 6] = some;
+        }
+        __syncthreads();
+        int skip = blockIdx.x, k = 0;
+        for (; k < PG_WGS / 64 && skip >= __popcll(s_some[k]); k++) skip -= __popcll(s_some[k]);
+        if (k == PG_WGS / 64) return;
+        uint64_t some = s_some[k];
+        for (; skip; skip--) some &= some - 1;
+        w0 = __builtin_amdgcn_readfirstlane(64 * k + __builtin_ctzll(some));
+    }
+    const PgJoin j = joins[w0];
     const int r0 = wg_rows * blockIdx.y, rows = min(wg_rows, j.rows - r0);
     if (rows <= 0) return;
-    const int groups = (unsigned)(PJ_WG / TH) / (unsigned)rows, w0 = blockIdx.x;
+    const int groups = (unsigned)(PJ_WG / TH) / (unsigned)rows;
     const int d = threadIdx.x % TH, x = threadIdx.x / TH, p = (unsigned)x / (unsigned)rows, r = r0 + x - p * rows;
     const float* row = part + r * HD + 4 * d;
     const float* stat = part + tile_rows * HD + r;
@@ -742,21 +755,28 @@ Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int h
     p.unit = pg_whole(kv, r, n_heads, hd) ? PG_WHOLE_KEYS : PD_UNIT;
     const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
     p.cut = r.cap > p.unit;
-    p.wgs = (int)(units < PD_WGS || !p.cut ? units : PD_WGS);
-    p.alone = r.cap <= 32 || (r.cap <= 256 && tiles > PD_WGS);
+    p.wgs = (int)(units < PG_WGS || !p.cut ? units : PG_WGS);
+    p.alone = r.cap <= 32 || (r.cap <= 256 && tiles > PG_WGS);
     return p;
 }
 
-// wg_rows: rows a joining workgroup.  4, or 1 where few tiles are cut into many
-// pieces each (a whole call with 4 / 1: 2 sequences of 29561, 128 pieces, 28.9 /
-// 22.7 us; 5 of up to 60888, 100 pieces, 36.3 / 32.8; one of 131071, 8 KV heads,
-// 64 pieces, 92.6 / 91.2).
+// wgs: workgroups that may have left pieces, of at most `tiles` tiles with
+// `rows` rows.  Tiles of 128 rows, few (in four pieces or more each): 8 pieces a
+// step, and only as many workgroups as there are tiles, since empty ones of more
+// than the chip holds at a time take their turn as well: 16 tiles in 32 pieces
+// 54.5 -> 8.3 us, 64 in 8 22.4 -> 10.7 (of 256 in 2 or 3, where most workgroups
+// have one, finding it costs more: 18.2 -> 23.5).  Tiles of 16 rows in many pieces
+// each, a row a workgroup: 2 sequences of 29561, 128 pieces, 28.9 -> 22.7 us a whole
+// call; one of 131071, 8 KV heads, 64 pieces, 92.6 -> 91.2.
 template <class T, int HD>
-hipError_t join(const PgJoin* joins, const float* part, int wgs, int tile_rows, int rows, int wg_rows, int grp, void* out,
+hipError_t join(const PgJoin* joins, const float* part, int wgs, long tiles, int tile_rows, int rows, int grp, void* out,
                 int ldo, hipStream_t s) {
-    const auto kernel = tile_rows == 16 ? paged_join_kernel<T, HD, 8> : paged_join_kernel<T, HD, 2>;
-    hipLaunchKernelGGL(kernel, dim3(wgs, (rows + wg_rows - 1) / wg_rows), dim3(PJ_WG), 0, s, joins, part, tile_rows, wg_rows,
-                       grp, static_cast<T*>(out), ldo);
+    const bool few = tiles <= wgs / 4;
+    const auto kernel = tile_rows == 16 || few ? paged_join_kernel<T, HD, 8> : paged_join_kernel<T, HD, 2>;
+    const int wg_rows = tile_rows == 16 && tiles <= wgs / 32 ? 1 : 4, y = (rows + wg_rows - 1) / wg_rows;
+    const int x = few && wgs * y > 2048 ? (int)tiles : wgs;
+    hipLaunchKernelGGL(kernel, dim3(x, y), dim3(PJ_WG), 0, s, joins, wgs, part, tile_rows, wg_rows, grp,
+                       static_cast<T*>(out), ldo);
     return hipGetLastError();
 }
 
@@ -786,9 +806,8 @@ struct Rows16Call {
                            static_cast<const T*>(p.q), p.ldq, p.scale, static_cast<T*>(p.out), p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess || !pl.cut) return e;
-        const bool many = pl.wgs >= 32 * pg_tiles_bound(p.rows, grp, 16) * p.kv.kv_heads;
-        return join<T, HD>(joins, part, pl.wgs, 16, p.rows.row_start || grp > 16 ? 16 : grp, many ? 1 : 4, grp, p.out, p.ldo,
-                           s);
+        return join<T, HD>(joins, part, pl.wgs, pg_tiles_bound(p.rows, grp, 16) * p.kv.kv_heads, 16,
+                           p.rows.row_start || grp > 16 ? 16 : grp, grp, p.out, p.ldo, s);
     }
 };
 
@@ -813,12 +832,12 @@ hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppen
     return paged_with_types(kv_dtype, dtype, hd, AppendCall{p, s});
 }
 
-hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, int tile_rows, int rows,
-                             int grp, void* out, int ldo, hipStream_t s) {
+hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, long tiles, int tile_rows,
+                             int rows, int grp, void* out, int ldo, hipStream_t s) {
     const auto run = dtype == GGML_F32   ? (hd == 64 ? join<float, 64> : join<float, 128>)
                      : dtype == GGML_F16 ? (hd == 64 ? join<_Float16, 64> : join<_Float16, 128>)
                                          : (hd == 64 ? join<__bf16, 64> : join<__bf16, 128>);
-    return run(joins, part, wgs, tile_rows, rows, 4, grp, out, ldo, s);
+    return run(joins, part, wgs, tiles, tile_rows, rows, grp, out, ldo, s);
 }
 
 hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {

@@ -83,6 +83,10 @@ inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int
     return tiles <= cut ? PG_TILES : PG_CUT;
 }
 
+// Workgroups of a call whose keys are cut into equal ranges: two a CU, all
+// resident at once.
+constexpr int PG_WGS = 512;
+
 // Cut tiles.  Workgroups that share the keys of a tile of `rows` query rows
 // leave slots of floats in the workspace, two a workgroup: o [rows][hd]
 // (unnormalized), m [rows], l [rows]; and each a record of what is to be joined.

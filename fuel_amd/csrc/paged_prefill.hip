@@ -92,7 +92,6 @@ struct PrefillTile {
 // tile), as the 16-row kernel does: where a batch has fewer tiles than fill the
 // chip and many keys each.  Tiles that a range cuts leave their sums in the
 // workspace.
-constexpr int PF_WGS = 512;  // two a CU
 
 template <class E, class T, int HD, bool CUT>
 __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv c, PagedRows b, int grp,
@@ -456,12 +455,13 @@ struct PrefillCall {
             return hipGetLastError();
         }
         float* part = static_cast<float*>(p.work);
-        PgJoin* joins = reinterpret_cast<PgJoin*>(part + (size_t)2 * PF_WGS * pg_slot(ROWS, HD));
-        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, true>), dim3(PF_WGS), dim3(64 * PF_WAVES), 0, s, p.kv, p.rows,
+        PgJoin* joins = reinterpret_cast<PgJoin*>(part + (size_t)2 * PG_WGS * pg_slot(ROWS, HD));
+        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, true>), dim3(PG_WGS), dim3(64 * PF_WAVES), 0, s, p.kv, p.rows,
                            grp, q, p.ldq, p.scale, out, p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        return launch_paged_join(dtype_of<T>(), HD, joins, part, PF_WGS, ROWS, ROWS, grp, p.out, p.ldo, s);
+        return launch_paged_join(dtype_of<T>(), HD, joins, part, PG_WGS,
+                                 pg_tiles_bound(p.rows, grp, ROWS) * p.kv.kv_heads, ROWS, ROWS, grp, p.out, p.ldo, s);
     }
     template <class T>
     static int dtype_of() {
@@ -473,7 +473,7 @@ struct PrefillCall {
 
 size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     if (pg_kind(kv, r, n_heads, hd) != PG_CUT) return 0;
-    return PF_WGS * (2 * pg_slot(32 * PF_WAVES, hd) * sizeof(float) + sizeof(PgJoin));
+    return PG_WGS * (2 * pg_slot(32 * PF_WAVES, hd) * sizeof(float) + sizeof(PgJoin));
 }
 
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
