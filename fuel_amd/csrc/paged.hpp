@@ -48,17 +48,18 @@ inline long pg_tiles_bound(const PagedRows& r, int grp, int tile_rows) {
 // Which kernel a call takes.  ROWS16: 16 query rows a tile, the keys of a call
 // over all workgroups (paged.hip).  TILES: 128 rows a tile, a workgroup each;
 // CUT: the same, the keys over all workgroups (paged_prefill.hip).  One row a
-// sequence: always ROWS16.  Otherwise by what they took, in us, over 1 or 4
-// sequences, 4 .. 1500 new rows after 0 .. 16000 cached, 2 .. 32 KV heads, f32
-// and bf16 (K: keys of the longest sequence, n: tiles times KV heads; the
-// estimate is the same for all types, since the workspace's size is):
+// sequence: always ROWS16.  Otherwise by what they took, in us, over 1 .. 48
+// sequences, 2 .. 3000 new rows after 0 .. 32000 cached, 1 .. 32 KV heads, all
+// types (K: keys of the longest sequence, n: tiles times KV heads; the estimate is
+// the same for all types, since the workspace's size is):
 //   ROWS16  12 + n16 K / 20000        (8 + .. where its tiles stay whole)
-//   TILES    9 + 0.024 K              (n128 <= 256: its longest walk)
-//            9 + 0.037 K max(1, n128 / 512)
-//   CUT     28 + n128 K / 13000       (the second launch and the pieces' bytes)
-// Of 32 heads over 8, bf16: 128 rows after 600: 22 / 25 / 30 (ROWS16 / TILES /
-// CUT), 300 after 600: 41 / 29 / 45, 300 after 4096: 159 / 103 / 64, 1500 after
-// 600: 248 / 63 / 86.
+//   TILES   10 + 0.034 K max(1/2, n128 / 512)
+//   CUT     26 + n128 K / 15000       (the second launch and the pieces' bytes)
+// Over 420 such batches the choice is 1.6 % slower than the fastest of the three in
+// the mean, at worst by half (the host knows the rows of a batch and its longest
+// sequence, not how they go together).  Of 32 heads over 8, bf16: 128 rows after
+// 600: 22 / 18 / 27 (ROWS16 / TILES / CUT), 300 after 600: 41 / 20 / 35, 300 after
+// 4096: 155 / 64 / 52, 1500 after 600: 248 / 55 / 79.
 enum PagedKind { PG_ROWS16, PG_TILES, PG_CUT };
 // Whether ROWS16 leaves its tiles whole: short walks, which a second launch
 // would cost more than they take.  One token a sequence, cut / whole, us: 8
@@ -77,8 +78,8 @@ inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int
     const double k = r.cap, n16 = (double)pg_tiles_bound(r, grp, 16) * kv.kv_heads,
                  n128 = (double)pg_tiles_bound(r, grp, 128) * kv.kv_heads;
     const double rows16 = (pg_whole(kv, r, n_heads, hd) ? 8 : 12) + n16 * k / 20000;
-    const double tiles = 9 + (n128 <= 256 ? 0.024 * k : 0.037 * k * (n128 > 512 ? n128 / 512 : 1.0));
-    const double cut = r.cap <= 1 << 24 && n128 <= 4096 ? 28 + n128 * k / 13000 : 1e30;  // (its units are an int)
+    const double tiles = 10 + 0.034 * k * (n128 > 256 ? n128 / 512 : 0.5);
+    const double cut = r.cap <= 1 << 24 && n128 <= 4096 ? 26 + n128 * k / 15000 : 1e30;  // (its units are an int)
     if (rows16 <= tiles && rows16 <= cut) return PG_ROWS16;
     return tiles <= cut ? PG_TILES : PG_CUT;
 }

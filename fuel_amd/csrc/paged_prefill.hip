@@ -1,10 +1,10 @@
 // Causal attention of packed prompt rows over a paged KV cache (paged.hpp).
 //
 // A sequence's rows and the G = n_heads / kv_heads query heads of a KV head are
-// one list of n * G query rows, as in paged.hip; a workgroup takes PF_ROWS of
-// them, 32 a wavefront, and walks the keys in tiles of 64 that it stages in LDS,
-// shared by its four wavefronts: the next tile's LDS DMA runs while a tile is
-// worked, one barrier a tile.
+// one list of n * G query rows, as in paged.hip; a workgroup of four wavefronts
+// takes 128 of them, 32 a wavefront, or 64, two wavefronts with half the keys each
+// to 32 rows, and walks the keys in tiles of 64 that it stages in LDS: the next
+// tile's LDS DMA runs while a tile is worked, one barrier a tile.
 //   S^T (keys x rows) = K . Q^T on v_mfma_f32_32x32x16: the C layout leaves lane
 //     32 h + n keys 8 i + 4 h + (0..3) of row n, which is what the second
 //     product takes as its B operand, in a key order that V's reads follow: P
@@ -33,6 +33,7 @@ namespace frq {
 namespace {
 
 constexpr int PF_WAVES = 4;
+constexpr int PF_ROWS = 32 * PF_WAVES;
 constexpr int PF_KEYS = 64;
 constexpr float PF_SHIFT = 8.0f, PF_LAZY = 7.0f;
 
@@ -78,8 +79,7 @@ struct PrefillTile {
     static constexpr int NP = WIDE ? P::SPLIT : 1;
     static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
-    static constexpr int RPI = 512 / HD, NI = HD / 32;  // rows a DMA instruction, instructions a wavefront and tile
-    static constexpr int ROWS = 32 * PF_WAVES;
+    static constexpr int RPI = 512 / HD, NI = TILE / 1024;  // rows a DMA instruction, instructions a tile
     // LDS chunk pc of row r holds the row's chunk pc ^ kswz(r) of K, pc ^ vswz(r)
     // of V: the 16 rows by 16 bytes, and the 4 rows by 64, that a read touches at
     // once lie in different ones of the 64 banks.
@@ -92,8 +92,16 @@ struct PrefillTile {
 // tile), as the 16-row kernel does: where a batch has fewer tiles than fill the
 // chip and many keys each.  Tiles that a range cuts leave their sums in the
 // workspace.
+// KW wavefronts share 32 rows, with 64 / KW keys of a tile each.  KW = 2 is for
+// batches of so few tiles that the one with the most keys lasts as long as the call:
+// two of its workgroups, of 64 rows, work on a CU as one of 128 does, and end sooner
+// where they are alone.  32 heads over 8, new rows 300 / 700 / 1000 (80 .. 256
+// tiles), us: bf16 14.3 / 22.2 / 28.9 with KW = 1, 12.1 / 19.4 / 25.0 with 2, f32
+// 18.0 / 29.1 / 39.2 and 14.4 / 24.2 / 32.5; beyond that not all of them start at
+// once (1500 rows after 600, 384 tiles: 55 and 62).
+constexpr int PF_FEW = 256;
 
-template <class E, class T, int HD, bool CUT>
+template <class E, class T, int HD, int KW, bool CUT>
 __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv c, PagedRows b, int grp,
                                                                          const T* __restrict__ q, int ldq, float scale,
                                                                          T* __restrict__ out, int ldo,
@@ -101,14 +109,18 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                                                                          PgJoin* __restrict__ joins) {
     using X = PrefillTile<E, T, HD>;
     using v8 = typename X::v8;
+    constexpr int RW = PF_WAVES / KW, ROWS = 32 * RW;
+    constexpr int NA = 2 / KW;  // groups of 32 keys of a tile a wavefront
     __shared__ __align__(1024) uint8_t s_k[2][X::TILE], s_v[2][X::TILE];
+    __shared__ float s_m[ROWS], s_l[ROWS];
     __shared__ uint32_t s_odd[2];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), w = KW == 1 ? wave : wave % RW;
+    const int key0 = KW == 1 ? 0 : 32 * (wave / RW);  // first of its keys in a tile
     // key tiles of a sequence's tiles of rows (one where it has no keys)
     const auto key_tiles = [&](const PgSeq& x) { return x.kv <= PF_KEYS ? 1 : (x.kv + PF_KEYS - 1) / PF_KEYS; };
     const auto units = [&](const PgSeq& x) {
-        const int row_tiles = (int)(((long)x.n * grp + X::ROWS - 1) / X::ROWS);
+        const int row_tiles = (int)(((long)x.n * grp + ROWS - 1) / ROWS);
         return CUT ? row_tiles * key_tiles(x) : row_tiles;
     };
     PgUnits<decltype(units)> pu(b, units);
@@ -137,305 +149,333 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         s = pu.find(unit, u);
     }
     for (;;) {
-    const PgSeq sq = pu.get(s);
-    if constexpr (CUT) {
-        if (sq.n == 0) {
+        const PgSeq sq = pu.get(s);
+        if constexpr (CUT) {
+            if (sq.n == 0) {
+                if (++s == b.n_seqs) {
+                    s = 0;
+                    head++;
+                }
+                continue;
+            }
+        }
+        const int nk = CUT ? key_tiles(sq) : 1, tile = CUT ? (unsigned)u / (unsigned)nk : u;
+        const int t0 = CUT ? u - tile * nk : 0, m_units = CUT ? min(nk - t0, stop - at) : 1;
+        const bool whole = m_units == nk;
+        const int rows = sq.n * grp, i0 = tile * ROWS;
+        const int mine = min(i0 + 32 * w + n, rows - 1);
+        const int row = sq.row0 + mine / grp, qh = head * grp + mine % grp;
+        const int pos0 = sq.kv - sq.n;
+        const int limit = pos0 + mine / grp;
+        // first and last position of the workgroup's and of this wavefront's rows
+        const int wg_first = pos0 + i0 / grp, wg_last = pos0 + min(i0 + ROWS - 1, rows - 1) / grp;
+        const int first = pos0 + min(i0 + 32 * w, rows - 1) / grp;
+        const int last = i0 + 32 * w < rows ? pos0 + min(i0 + 32 * w + 31, rows - 1) / grp : -1;
+        int tiles = wg_last >= 0 ? wg_last / PF_KEYS + 1 : 0;
+        if constexpr (CUT) tiles = min(tiles, t0 + m_units);
+
+        // Q^T, the B operand: dims 16 t + 8 h + e of row n
+        v8 qf[X::NP][X::KS];
+        float factor = fabsf(scale) * 1.4426950408889634f;
+        {
+            const T* x = q + (size_t)row * ldq + (size_t)qh * HD;
+            float f[X::KS][8], a = 0.0f;
+#pragma unroll
+            for (int t = 0; t < X::KS; t++) {
+                T raw[8];
+                __builtin_memcpy(raw, __builtin_assume_aligned(x + 16 * t + 8 * h, 16), sizeof raw);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    f[t][e] = scale < 0.0f ? -(float)raw[e] : (float)raw[e];
+                    a = fmaxf(a, fabsf(f[t][e]));
+                }
+            }
+            int ex = 0;
+            if constexpr (X::WIDE && std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
+                a = fmaxf(a, pf_other_half(a));
+                if (a > 0.0f && a < __builtin_inff()) ex = min(120, max(-120, __builtin_amdgcn_frexp_expf(a)));
+                factor = __builtin_amdgcn_ldexpf(factor, ex);
+            }
+#pragma unroll
+            for (int t = 0; t < X::KS; t++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float rest = __builtin_amdgcn_ldexpf(f[t][e], -ex);
+#pragma unroll
+                    for (int p = 0; p < X::NP; p++) {
+                        qf[p][t][e] = (E)rest;
+                        rest -= (float)qf[p][t][e];
+                    }
+                }
+        }
+
+        pf_f16 o[X::DT];
+#pragma unroll
+        for (int d = 0; d < X::DT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+        float m = -1e30f, l = 0.0f;
+
+        // DMA: instruction i of this wavefront takes rows ((i PF_WAVES + wave) RPI) .. of
+        // a tile, all in one group of 16 keys.  Source offsets of the lane within it:
+        constexpr int CPR = HD / 8;
+        const int dr = wave * X::RPI + lane / CPR, pc = lane % CPR;
+        const uint32_t koff = (dr & 15) * X::ROW + 16 * (pc ^ X::kswz(dr));
+        const uint32_t voff = (dr & 15) * X::ROW + 16 * (pc ^ X::vswz(dr));
+        const int* table = b.table + (size_t)s * b.max_pages;
+        // Byte offsets in the pools of 64 groups of 16 keys, lane i that of group i from
+        // key id0 on, and which groups' page is none (theirs lead to page 0).
+        int id0 = 0;
+        uint32_t off_lo = 0, off_hi = 0;
+        uint64_t none = 0;
+        auto fetch_ids = [&](int j0) {
+            id0 = j0;
+            const int j = j0 + 16 * lane, id = j < sq.kv ? table[j >> c.log_ps] : 0;
+            const bool off = (unsigned)id >= (unsigned)c.n_pages;
+            none = __ballot(off);
+            const size_t at = ((((size_t)(off ? 0 : id) * c.kv_heads + head) << c.log_ps) +
+                               (j & ((1 << c.log_ps) - 1))) * X::ROW;
+            off_lo = (uint32_t)at;
+            off_hi = (uint32_t)(at >> 32);
+        };
+        auto issue = [&](int t) {
+            const int j0 = t * PF_KEYS;
+            if (j0 - id0 >= 1024) fetch_ids(j0);
+            const int g0 = (j0 - id0) >> 4;
+            const uint32_t kto = pf_lds(s_k[t & 1]) + wave * 1024, vto = pf_lds(s_v[t & 1]) + wave * 1024;
+#pragma unroll
+            for (int i = 0; i < X::NI / PF_WAVES; i++) {
+                const int g = g0 + ((i * PF_WAVES + wave) * X::RPI >> 4);
+                const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, g) << 32 |
+                                      (uint32_t)__builtin_amdgcn_readlane(off_lo, g);
+                pf_dma(static_cast<const uint8_t*>(c.k) + from, koff, kto + i * PF_WAVES * 1024);
+                pf_dma(static_cast<const uint8_t*>(c.v) + from, voff, vto + i * PF_WAVES * 1024);
+            }
+        };
+        // LDS read offsets of this lane: K row n (+ 32), chunks 2 t + h; V rows
+        // 4 h + (lane / 4) % 4 (+ 16 k + 8 j), dims 16 ((lane / 16) % 2) + 4 (lane % 4) (+ 32 d)
+        const uint32_t kbase = n * X::ROW + 16 * (h ^ X::kswz(n));
+        const int vr = (lane >> 2) & 3;
+        const uint32_t vbase = (4 * h + vr) * X::ROW +
+                               16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ X::vswz(vr)) + 8 * (lane & 1);
+
+        if (t0 < tiles) {
+            fetch_ids(t0 * PF_KEYS);
+            issue(t0);
+        }
+        for (int t = t0; t < tiles; t++) {
+            const int j0 = t * PF_KEYS;
+            // tile t landed, in every wavefront, and tile t - 1 is read
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            const uint32_t bad = (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
+            const bool masked = j0 + PF_KEYS - 1 > wg_first || bad;
+            uint64_t odd = 0;
+            if (masked) {
+                // rows of V that are no keys are cleared, so are infinite and NaN
+                // values, whose keys are noted: 0 * inf must not reach the rows
+                // that do not see them
+                if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
+                __syncthreads();
+                for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
+                    const int r = ch / CPR;
+                    uint4* at = reinterpret_cast<uint4*>(s_v[t & 1]) + ch;
+                    const uint4 u = *at;
+                    uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                    const bool none = j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1);
+                    bool hit = false;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        if (pg_word_inf<E>(x[k])) {
+                            hit = true;
+                            x[k] = 0;
+                        }
+                    }
+                    if (none || hit) *at = none ? make_uint4(0, 0, 0, 0) : make_uint4(x[0], x[1], x[2], x[3]);
+                    if (hit && !none) atomicOr(&s_odd[r >> 5], 1u << (r & 31));
+                }
+                __syncthreads();
+                odd = KW == 2 ? s_odd[wave / RW] : (uint64_t)s_odd[1] << 32 | s_odd[0];
+            }
+            if (t + 1 < tiles) issue(t + 1);
+            const int jw = j0 + key0;  // this wavefront's first key
+            if (jw > last) continue;
+
+            const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
+            const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
+            pf_f16 st[NA];
+#pragma unroll
+            for (int a = 0; a < NA; a++) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) st[a][i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < X::KS; k++) {
+                    const v8 kf = *reinterpret_cast<const v8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
+#pragma unroll
+                    for (int p = X::NP - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
+                }
+            }
+            const bool mask = jw + 32 * NA - 1 > first || bad;
+            if (mask) {
+#pragma unroll
+                for (int a = 0; a < NA; a++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int r = 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h;
+                        if ((bad >> ((key0 + r) >> 4)) & 1) st[a][i] = pg_nan();
+                        if (jw + r > limit) st[a][i] = -__builtin_inff();
+                    }
+            }
+            float top = st[0][0];
+#pragma unroll
+            for (int a = 0; a < NA; a++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
+            top = fmaxf(top, pf_other_half(top)) * factor;
+            if (__any(top > m + PF_LAZY)) {
+                const float mn = fmaxf(m, top);
+                const float f = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before)
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < X::DT; d++) o[d] *= f;
+            }
+            const float ms = m - PF_SHIFT;
+#pragma unroll
+            for (int a = 0; a < NA; a++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) st[a][i] = fmaf(st[a][i], factor, -ms);
+            if (mask) {  // (again: a factor of 0 would make NaN of -inf)
+#pragma unroll
+                for (int a = 0; a < NA; a++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (jw + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h > limit) st[a][i] = -__builtin_inff();
+            }
+            v8 pp[X::NP][2 * NA];
+#pragma unroll
+            for (int a = 0; a < NA; a++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    st[a][i] = __builtin_amdgcn_exp2f(st[a][i]);
+                    l += st[a][i];
+                    float rest = st[a][i];
+#pragma unroll
+                    for (int p = 0; p < X::NP; p++) {
+                        pp[p][2 * a + (i >> 3)][i & 7] = (E)rest;
+                        rest -= (float)pp[p][2 * a + (i >> 3)][i & 7];
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < 2 * NA; k++)
+#pragma unroll
+                for (int d = 0; d < X::DT; d++) {
+                    const uint8_t* at = vt + 16 * k * X::ROW + (vbase ^ (64 * d));
+                    const pf_s4 lo = pf_read_tr(at), hi = pf_read_tr(at + 8 * X::ROW);
+                    const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                    for (int p = X::NP - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
+                }
+            if (masked) {
+                for (; odd; odd &= odd - 1) {  // the cleared values, for the rows that see them
+                    const int r = __builtin_ctzll(odd);
+                    float p = 0.0f;
+#pragma unroll
+                    for (int a = 0; a < NA; a++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (32 * a + (i & 3) + 8 * (i >> 2) == (r & ~4)) p = st[a][i];
+                    const float q2 = pf_other_half(p);
+                    p = ((r >> 2) & 1) == h ? p : q2;
+                    const int page = table[(jw + r) >> c.log_ps];
+                    const E* src = static_cast<const E*>(c.v) +
+                                   ((((size_t)page * c.kv_heads + head) << c.log_ps) +
+                                    ((jw + r) & ((1 << c.log_ps) - 1))) * HD;
+                    if (jw + r > limit) continue;
+#pragma unroll
+                    for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float v = (float)src[32 * d + (i & 3) + 8 * (i >> 2) + 4 * h];
+                            if (!(fabsf(v) < __builtin_inff())) o[d][i] = fmaf(p, v, o[d][i]);
+                        }
+                }
+            }
+        }
+        l += pf_other_half(l);
+        if constexpr (KW == 2) {  // the two that share rows
+            static_assert(16 * X::DT * 64 * 4 * RW <= sizeof s_k, "the sums of half the wavefronts");
+            __syncthreads();
+            float* s_o = reinterpret_cast<float*>(s_k) + 16 * X::DT * 64 * w + lane;
+            if (key0) {
+#pragma unroll
+                for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s_o[64 * (16 * d + i)] = o[d][i];
+                s_m[32 * w + n] = m;
+                s_l[32 * w + n] = l;
+            }
+            __syncthreads();
+            if (!key0) {
+                const float m2 = s_m[32 * w + n], mn = fmaxf(m, m2);
+                const float f = __builtin_amdgcn_exp2f(m - mn), f2 = __builtin_amdgcn_exp2f(m2 - mn);
+                m = mn;
+                l = l * f + s_l[32 * w + n] * f2;
+#pragma unroll
+                for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[d][i] = fmaf(s_o[64 * (16 * d + i)], f2, o[d][i] * f);
+            }
+        }
+        if (key0 == 0 && i0 + 32 * w + n < rows) {
+            if (!CUT || whole) {
+                const float inv = 1.0f / l;
+                T* dst = out + (size_t)row * ldo + (size_t)qh * HD + 4 * h;
+#pragma unroll
+                for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++) {
+                        T y[4];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float x = o[d][4 * g + i] * inv;
+                            y[i] = (T)(sq.bad ? pg_nan() : limit < 0 ? 0.0f : x);
+                        }
+                        __builtin_memcpy(__builtin_assume_aligned(dst + 32 * d + 8 * g, 8), y, sizeof y);
+                    }
+            } else {
+                float* slot = part + ((size_t)2 * wg + (at != begin)) * pg_slot(ROWS, HD);
+                float* dst = slot + (32 * w + n) * HD + 4 * h;
+#pragma unroll
+                for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                    for (int g = 0; g < 4; g++)
+                        *reinterpret_cast<pg_f4*>(dst + 32 * d + 8 * g) =
+                            pg_f4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+                if (h == 0) {
+                    slot[ROWS * HD + 32 * w + n] = m;
+                    slot[ROWS * HD + ROWS + 32 * w + n] = l;
+                }
+            }
+        }
+        if constexpr (!CUT) return;
+        if (at + m_units == stop) {
+            if (threadIdx.x == 0)
+                joins[wg] = pg_join(t0 == 0 && !whole, min(ROWS, rows - i0), sq, head, i0, at + nk - 1, total, n_wgs,
+                                    2 * wg + (at != begin));
+            return;
+        }
+        at += m_units;
+        u += m_units;
+        if (u == (int)(((long)rows + ROWS - 1) / ROWS) * nk) {
+            u = 0;
             if (++s == b.n_seqs) {
                 s = 0;
                 head++;
             }
-            continue;
         }
-    }
-    const int nk = CUT ? key_tiles(sq) : 1, tile = CUT ? (unsigned)u / (unsigned)nk : u;
-    const int t0 = CUT ? u - tile * nk : 0, m_units = CUT ? min(nk - t0, stop - at) : 1;
-    const bool whole = m_units == nk;
-    const int rows = sq.n * grp, i0 = tile * X::ROWS;
-    const int mine = min(i0 + 32 * w + n, rows - 1);
-    const int row = sq.row0 + mine / grp, qh = head * grp + mine % grp;
-    const int pos0 = sq.kv - sq.n;
-    const int limit = pos0 + mine / grp;
-    // first and last position of the workgroup's and of this wavefront's rows
-    const int wg_first = pos0 + i0 / grp, wg_last = pos0 + min(i0 + X::ROWS - 1, rows - 1) / grp;
-    const int first = pos0 + min(i0 + 32 * w, rows - 1) / grp;
-    const int last = i0 + 32 * w < rows ? pos0 + min(i0 + 32 * w + 31, rows - 1) / grp : -1;
-    int tiles = wg_last >= 0 ? wg_last / PF_KEYS + 1 : 0;
-    if constexpr (CUT) tiles = min(tiles, t0 + m_units);
-
-    // Q^T, the B operand: dims 16 t + 8 h + e of row n
-    v8 qf[X::NP][X::KS];
-    float factor = fabsf(scale) * 1.4426950408889634f;
-    {
-        const T* x = q + (size_t)row * ldq + (size_t)qh * HD;
-        float f[X::KS][8], a = 0.0f;
-#pragma unroll
-        for (int t = 0; t < X::KS; t++) {
-            T raw[8];
-            __builtin_memcpy(raw, __builtin_assume_aligned(x + 16 * t + 8 * h, 16), sizeof raw);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                f[t][e] = scale < 0.0f ? -(float)raw[e] : (float)raw[e];
-                a = fmaxf(a, fabsf(f[t][e]));
-            }
-        }
-        int ex = 0;
-        if constexpr (X::WIDE && std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
-            a = fmaxf(a, pf_other_half(a));
-            if (a > 0.0f && a < __builtin_inff()) ex = min(120, max(-120, __builtin_amdgcn_frexp_expf(a)));
-            factor = __builtin_amdgcn_ldexpf(factor, ex);
-        }
-#pragma unroll
-        for (int t = 0; t < X::KS; t++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                float rest = __builtin_amdgcn_ldexpf(f[t][e], -ex);
-#pragma unroll
-                for (int p = 0; p < X::NP; p++) {
-                    qf[p][t][e] = (E)rest;
-                    rest -= (float)qf[p][t][e];
-                }
-            }
-    }
-
-    pf_f16 o[X::DT];
-#pragma unroll
-    for (int d = 0; d < X::DT; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-    float m = -1e30f, l = 0.0f;
-
-    // DMA: instruction i of this wavefront takes rows ((i PF_WAVES + w) RPI) .. of
-    // a tile, all in one group of 16 keys.  Source offsets of the lane within it:
-    constexpr int CPR = HD / 8;
-    const int dr = w * X::RPI + lane / CPR, pc = lane % CPR;
-    const uint32_t koff = (dr & 15) * X::ROW + 16 * (pc ^ X::kswz(dr));
-    const uint32_t voff = (dr & 15) * X::ROW + 16 * (pc ^ X::vswz(dr));
-    const int* table = b.table + (size_t)s * b.max_pages;
-    // Byte offsets in the pools of 64 groups of 16 keys, lane i that of group i from
-    // key id0 on, and which groups' page is none (theirs lead to page 0).
-    int id0 = 0;
-    uint32_t off_lo = 0, off_hi = 0;
-    uint64_t none = 0;
-    auto fetch_ids = [&](int j0) {
-        id0 = j0;
-        const int j = j0 + 16 * lane, id = j < sq.kv ? table[j >> c.log_ps] : 0;
-        const bool off = (unsigned)id >= (unsigned)c.n_pages;
-        none = __ballot(off);
-        const size_t at = ((((size_t)(off ? 0 : id) * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * X::ROW;
-        off_lo = (uint32_t)at;
-        off_hi = (uint32_t)(at >> 32);
-    };
-    auto issue = [&](int t) {
-        const int j0 = t * PF_KEYS;
-        if (j0 - id0 >= 1024) fetch_ids(j0);
-        const int g0 = (j0 - id0) >> 4;
-        const uint32_t kto = pf_lds(s_k[t & 1]) + w * 1024, vto = pf_lds(s_v[t & 1]) + w * 1024;
-#pragma unroll
-        for (int i = 0; i < X::NI; i++) {
-            const int g = g0 + ((i * PF_WAVES + w) * X::RPI >> 4);
-            const uint64_t from = (uint64_t)(uint32_t)__builtin_amdgcn_readlane(off_hi, g) << 32 |
-                                  (uint32_t)__builtin_amdgcn_readlane(off_lo, g);
-            pf_dma(static_cast<const uint8_t*>(c.k) + from, koff, kto + i * PF_WAVES * 1024);
-            pf_dma(static_cast<const uint8_t*>(c.v) + from, voff, vto + i * PF_WAVES * 1024);
-        }
-    };
-    // LDS read offsets of this lane: K row n (+ 32), chunks 2 t + h; V rows
-    // 4 h + (lane / 4) % 4 (+ 16 k + 8 j), dims 16 ((lane / 16) % 2) + 4 (lane % 4) (+ 32 d)
-    const uint32_t kbase = n * X::ROW + 16 * (h ^ X::kswz(n));
-    const int vr = (lane >> 2) & 3;
-    const uint32_t vbase = (4 * h + vr) * X::ROW + 16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ X::vswz(vr)) + 8 * (lane & 1);
-
-    if (t0 < tiles) {
-        fetch_ids(t0 * PF_KEYS);
-        issue(t0);
-    }
-    for (int t = t0; t < tiles; t++) {
-        const int j0 = t * PF_KEYS;
-        // tile t landed, in every wavefront, and tile t - 1 is read
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        const uint32_t bad = (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
-        const bool masked = j0 + PF_KEYS - 1 > wg_first || bad;
-        uint64_t odd = 0;
-        if (masked) {
-            // rows of V that are no keys are cleared, so are infinite and NaN
-            // values, whose keys are noted: 0 * inf must not reach the rows
-            // that do not see them
-            if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
-            __syncthreads();
-            for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
-                const int r = ch / CPR;
-                uint4* at = reinterpret_cast<uint4*>(s_v[t & 1]) + ch;
-                const uint4 u = *at;
-                uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                const bool none = j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1);
-                bool hit = false;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    if (pg_word_inf<E>(x[k])) {
-                        hit = true;
-                        x[k] = 0;
-                    }
-                }
-                if (none || hit) *at = none ? make_uint4(0, 0, 0, 0) : make_uint4(x[0], x[1], x[2], x[3]);
-                if (hit && !none) atomicOr(&s_odd[r >> 5], 1u << (r & 31));
-            }
-            __syncthreads();
-            odd = (uint64_t)s_odd[1] << 32 | s_odd[0];
-        }
-        if (t + 1 < tiles) issue(t + 1);
-        if (j0 > last) continue;
-
-        const uint8_t* kt = s_k[t & 1];
-        const uint8_t* vt = s_v[t & 1];
-        pf_f16 st[2];
-#pragma unroll
-        for (int a = 0; a < 2; a++) {
-#pragma unroll
-            for (int i = 0; i < 16; i++) st[a][i] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < X::KS; k++) {
-                const v8 kf = *reinterpret_cast<const v8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
-#pragma unroll
-                for (int p = X::NP - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
-            }
-        }
-        const bool mask = j0 + PF_KEYS - 1 > first || bad;
-        if (mask) {
-#pragma unroll
-            for (int a = 0; a < 2; a++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int r = 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h;
-                    if ((bad >> (r >> 4)) & 1) st[a][i] = pg_nan();
-                    if (j0 + r > limit) st[a][i] = -__builtin_inff();
-                }
-        }
-        float top = st[0][0];
-#pragma unroll
-        for (int a = 0; a < 2; a++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
-        top = fmaxf(top, pf_other_half(top)) * factor;
-        if (__any(top > m + PF_LAZY)) {
-            const float mn = fmaxf(m, top);
-            const float f = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before)
-            m = mn;
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < X::DT; d++) o[d] *= f;
-        }
-        const float ms = m - PF_SHIFT;
-#pragma unroll
-        for (int a = 0; a < 2; a++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) st[a][i] = fmaf(st[a][i], factor, -ms);
-        if (mask) {  // (again: a factor of 0 would make NaN of -inf)
-#pragma unroll
-            for (int a = 0; a < 2; a++)
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (j0 + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h > limit) st[a][i] = -__builtin_inff();
-        }
-        v8 pp[X::NP][4];
-#pragma unroll
-        for (int a = 0; a < 2; a++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                st[a][i] = __builtin_amdgcn_exp2f(st[a][i]);
-                l += st[a][i];
-                float rest = st[a][i];
-#pragma unroll
-                for (int p = 0; p < X::NP; p++) {
-                    pp[p][2 * a + (i >> 3)][i & 7] = (E)rest;
-                    rest -= (float)pp[p][2 * a + (i >> 3)][i & 7];
-                }
-            }
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-            for (int d = 0; d < X::DT; d++) {
-                const uint8_t* at = vt + 16 * k * X::ROW + (vbase ^ (64 * d));
-                const pf_s4 lo = pf_read_tr(at), hi = pf_read_tr(at + 8 * X::ROW);
-                const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int p = X::NP - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
-            }
-        if (masked) {
-            for (; odd; odd &= odd - 1) {  // the cleared values, for the rows that see them
-                const int r = __builtin_ctzll(odd);
-                float p = 0.0f;
-#pragma unroll
-                for (int a = 0; a < 2; a++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (32 * a + (i & 3) + 8 * (i >> 2) == (r & ~4)) p = st[a][i];
-                const float q2 = pf_other_half(p);
-                p = ((r >> 2) & 1) == h ? p : q2;
-                const int page = table[(j0 + r) >> c.log_ps];
-                const E* src = static_cast<const E*>(c.v) +
-                               ((((size_t)page * c.kv_heads + head) << c.log_ps) + ((j0 + r) & ((1 << c.log_ps) - 1))) * HD;
-                if (j0 + r > limit) continue;
-#pragma unroll
-                for (int d = 0; d < X::DT; d++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float v = (float)src[32 * d + (i & 3) + 8 * (i >> 2) + 4 * h];
-                        if (!(fabsf(v) < __builtin_inff())) o[d][i] = fmaf(p, v, o[d][i]);
-                    }
-            }
-        }
-    }
-    l += pf_other_half(l);
-    if (i0 + 32 * w + n < rows) {
-        if (!CUT || whole) {
-            const float inv = 1.0f / l;
-            T* dst = out + (size_t)row * ldo + (size_t)qh * HD + 4 * h;
-#pragma unroll
-            for (int d = 0; d < X::DT; d++)
-#pragma unroll
-                for (int g = 0; g < 4; g++) {
-                    T y[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float x = o[d][4 * g + i] * inv;
-                        y[i] = (T)(sq.bad ? pg_nan() : limit < 0 ? 0.0f : x);
-                    }
-                    __builtin_memcpy(__builtin_assume_aligned(dst + 32 * d + 8 * g, 8), y, sizeof y);
-                }
-        } else {
-            float* slot = part + ((size_t)2 * wg + (at != begin)) * pg_slot(X::ROWS, HD);
-            float* dst = slot + (32 * w + n) * HD + 4 * h;
-#pragma unroll
-            for (int d = 0; d < X::DT; d++)
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-                    *reinterpret_cast<pg_f4*>(dst + 32 * d + 8 * g) =
-                        pg_f4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-            if (h == 0) {
-                slot[X::ROWS * HD + 32 * w + n] = m;
-                slot[X::ROWS * HD + X::ROWS + 32 * w + n] = l;
-            }
-        }
-    }
-    if constexpr (!CUT) return;
-    if (at + m_units == stop) {
-        if (threadIdx.x == 0)
-            joins[wg] = pg_join(t0 == 0 && !whole, min(X::ROWS, rows - i0), sq, head, i0, at + nk - 1, total, n_wgs,
-                                2 * wg + (at != begin));
-        return;
-    }
-    at += m_units;
-    u += m_units;
-    if (u == (int)(((long)rows + X::ROWS - 1) / X::ROWS) * nk) {
-        u = 0;
-        if (++s == b.n_seqs) {
-            s = 0;
-            head++;
-        }
-    }
-    __syncthreads();  // the last key tile is read
+        __syncthreads();  // the last key tile is read
     }
 }
 
@@ -444,24 +484,26 @@ struct PrefillCall {
     hipStream_t s;
     template <class E, class T, int HD>
     hipError_t run() const {
-        constexpr int ROWS = PrefillTile<E, T, HD>::ROWS;
         const int grp = p.n_heads / p.kv.kv_heads;
         const T* q = static_cast<const T*>(p.q);
         T* out = static_cast<T*>(p.out);
+        const long tiles = pg_tiles_bound(p.rows, grp, PF_ROWS) * p.kv.kv_heads;
         if (pg_kind(p.kv, p.rows, p.n_heads, HD) != PG_CUT) {
-            hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, false>),
-                               dim3((unsigned)(pg_tiles_bound(p.rows, grp, ROWS) * p.kv.kv_heads)), dim3(64 * PF_WAVES), 0,
-                               s, p.kv, p.rows, grp, q, p.ldq, p.scale, out, p.ldo, nullptr, nullptr);
+            const bool few = tiles <= PF_FEW;
+            const auto kernel =
+                few ? paged_prefill_kernel<E, T, HD, 2, false> : paged_prefill_kernel<E, T, HD, 1, false>;
+            const long wgs = few ? pg_tiles_bound(p.rows, grp, PF_ROWS / 2) * p.kv.kv_heads : tiles;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * PF_WAVES), 0, s, p.kv, p.rows, grp, q, p.ldq,
+                               p.scale, out, p.ldo, nullptr, nullptr);
             return hipGetLastError();
         }
         float* part = static_cast<float*>(p.work);
-        PgJoin* joins = reinterpret_cast<PgJoin*>(part + (size_t)2 * PG_WGS * pg_slot(ROWS, HD));
-        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, true>), dim3(PG_WGS), dim3(64 * PF_WAVES), 0, s, p.kv, p.rows,
-                           grp, q, p.ldq, p.scale, out, p.ldo, part, joins);
+        PgJoin* joins = reinterpret_cast<PgJoin*>(part + (size_t)2 * PG_WGS * pg_slot(PF_ROWS, HD));
+        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, 1, true>), dim3(PG_WGS), dim3(64 * PF_WAVES), 0, s, p.kv,
+                           p.rows, grp, q, p.ldq, p.scale, out, p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        return launch_paged_join(dtype_of<T>(), HD, joins, part, PG_WGS,
-                                 pg_tiles_bound(p.rows, grp, ROWS) * p.kv.kv_heads, ROWS, ROWS, grp, p.out, p.ldo, s);
+        return launch_paged_join(dtype_of<T>(), HD, joins, part, PG_WGS, tiles, PF_ROWS, PF_ROWS, grp, p.out, p.ldo, s);
     }
     template <class T>
     static int dtype_of() {
@@ -473,7 +515,7 @@ struct PrefillCall {
 
 size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     if (pg_kind(kv, r, n_heads, hd) != PG_CUT) return 0;
-    return PG_WGS * (2 * pg_slot(32 * PF_WAVES, hd) * sizeof(float) + sizeof(PgJoin));
+    return PG_WGS * (2 * pg_slot(PF_ROWS, hd) * sizeof(float) + sizeof(PgJoin));
 }
 
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
