@@ -400,6 +400,35 @@ def test_prefill_tiles_malformed(dev):
 
 
 @pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D", [(20, 20, 128), (40, 20, 64)])
+def test_prefill_more_tiles_than_cus(dev, act, cache, H, hk, D):
+    """Whole tiles of 128 rows: prompts and a chunk, a page that is none, a length
+    that is none, keys and values that are no numbers from position 150 on."""
+    say("prefill many tiles", act, cache, H, D)
+    past, new = [0, 0, 70, 0, 3, 0, 5], [200, 1, 130, 60, 250, 0, 190]
+    c = Case(dev, seed(19, act, cache, H), act, cache, H, hk, D, 16, past, new, row0=1, tail=4, pad=8)
+    c.kv[3] = -5
+    c.pool.table[4, 100 // 16] = c.pool.n_pages          # positions 96 ..
+    at = 150
+    k, v = c.pool.get(0, 200)
+    k, v = k.copy(), v.copy()
+    k[at::3], v[at::3], v[at + 1::3], k[at + 2::3] = np.nan, np.inf, np.nan, -np.inf
+    clean = c.pool.get(0, at)
+    c.pool.put(0, np.arange(200), k, v)
+    c.upload()
+    c.run()
+    got, w = c.check(skip=(0, 3, 4)), H * D
+    s0, s3, s4 = (int(c.start[s]) for s in (0, 3, 4))
+    assert np.isnan(got[s3:s3 + 60, :w]).all()
+    assert np.isnan(got[s4 + 93:s4 + 250, :w]).all() and np.isfinite(got[s4:s4 + 93, :w]).all()
+    assert not np.isfinite(got[s0 + at:s0 + 200, :w]).any()
+    q = R.from_bits(R.to_bits(c.q, act), act)[s0:s0 + at, :w].reshape(at, H, D)
+    want, A, B, V = R.attend(q, *clean, np.arange(at), c.scale)
+    tol = R.bound(want, A, B, V, at, D, act, cache, True)
+    assert (np.abs(got[s0:s0 + at, :w].reshape(want.shape) - want) <= tol).all()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
 @pytest.mark.parametrize("H,hk,D,past,new,ats", [
     (4, 2, 64, (0, 30), (170, 160), (1, 20, 63, 97, 150)), (4, 2, 128, (0, 30), (170, 160), (1, 20, 63, 97, 150)),
     (32, 2, 128, (0, 30), (170, 160), (1, 20, 97)), (48, 4, 64, (0, 30), (100, 90), (5, 64)),
