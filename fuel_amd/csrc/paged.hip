@@ -302,10 +302,9 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
     while (j0 < j1) {
         const int end = min(j1, j0 + 1024);
         const int jl = j0 + 16 * lane;
-        const int id = jl < kv ? table[jl >> c.log_ps] : 0;
-        const bool off = (unsigned)id >= (unsigned)c.n_pages;
+        bool off;
+        const int page = pg_page(c, table, jl, kv, off);
         const uint64_t none = __ballot(off && jl < end);  // groups whose page is none
-        const int page = off ? 0 : id;
         auto rows = [&](const void* pool, int blk, const E* (&at)[2]) {
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -371,7 +370,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const auto units_of = [&](const PgSeq& x) { return pd_tiles(x, grp) * pd_units(x, unit); };
-    PgUnits<decltype(units_of)> pu(b, units_of, !b.row_start && b.cap <= unit ? (grp + 15) >> 4 : 0);
+    PgUnits<decltype(units_of)> pu(b, units_of, c.kv_heads, !b.row_start && b.cap <= unit ? (grp + 15) >> 4 : 0);
     const int units = pu.total, total = units * c.kv_heads, n_wgs = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= n_wgs) {
         if (joins && threadIdx.x == 0) joins[blockIdx.x].rows = 0;
@@ -486,7 +485,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(Pa
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int at = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * PA_WAVES + (threadIdx.x >> 6)));
     const auto tiles_of = [&](const PgSeq& x) { return pd_tiles(x, grp); };
-    PgUnits<decltype(tiles_of)> pu(b, tiles_of, each);
+    PgUnits<decltype(tiles_of)> pu(b, tiles_of, c.kv_heads, each);
     if (at >= pu.total * c.kv_heads) return;
     const int head = (unsigned)at / (unsigned)pu.total;
     int tile;

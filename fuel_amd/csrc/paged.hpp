@@ -140,7 +140,7 @@ struct PgSeq {
     int row0, n, kv;
     bool bad;
 };
-__device__ __forceinline__ PgSeq pg_seq(const PagedRows& b, int s) {
+__host__ __device__ __forceinline__ PgSeq pg_seq(const PagedRows& b, int s) {
     PgSeq q;
     q.row0 = s;
     q.n = 1;
@@ -155,10 +155,19 @@ __device__ __forceinline__ PgSeq pg_seq(const PagedRows& b, int s) {
     return q;
 }
 
-// Sums of v over lanes 0 .. the own one, by DPP (a chain of lane shuffles takes
-// ten times as long).
+// The page of position j of a sequence of kv (0 behind its end), and whether it
+// is none of the pool's: then its keys are read from page 0 and count as NaN.
+__host__ __device__ __forceinline__ int pg_page(const PagedKv& c, const int* table, int j, int kv, bool& none) {
+    const int id = j < kv ? table[j >> c.log_ps] : 0;
+    none = (unsigned)id >= (unsigned)c.n_pages;
+    return none ? 0 : id;
+}
+
+// Sums of v >= 0 over lanes 0 .. the own one, at most 0x7fffffff, by DPP (a chain
+// of lane shuffles takes ten times as long).
+__device__ __forceinline__ int pg_add(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
 __device__ __forceinline__ int pg_scan(int v) {
-#define FRQ_DPP_ADD(ctrl, rmask) v += __builtin_amdgcn_update_dpp(0, v, ctrl, rmask, 0xF, false)
+#define FRQ_DPP_ADD(ctrl, rmask) v = pg_add(v, __builtin_amdgcn_update_dpp(0, v, ctrl, rmask, 0xF, false))
     FRQ_DPP_ADD(0x111, 0xF);  // row_shr 1, 2, 4, 8: sums within each 16-lane row
     FRQ_DPP_ADD(0x112, 0xF);
     FRQ_DPP_ADD(0x114, 0xF);
@@ -175,7 +184,9 @@ __device__ __forceinline__ int pg_scan(int v) {
 // sequences [l share, (l + 1) share), whose loads do not wait for each other;
 // a lookup then loads one share: two memory round trips for any n_seqs <= 4096.
 // each: every sequence has so many units (0: not known), and none is loaded
-// before the lookup.
+// before the lookup.  A batch has no units if those of all heads are more than
+// 0x7fffffff, which the host refuses for rows that lie in one sequence each:
+// row_start lists rows over and over.
 template <class F>
 struct PgUnits {
     const PagedRows& b;
@@ -190,7 +201,8 @@ struct PgUnits {
         if (s < b.n_seqs) own = pg_seq(b, s);
     }
     __device__ __forceinline__ int mine() const { return s0 + (int)(threadIdx.x & 63) < b.n_seqs ? units(own) : 0; }
-    __device__ __forceinline__ PgUnits(const PagedRows& rows, F f, int each_ = 0) : b(rows), units(f), each(each_) {
+    __device__ __forceinline__ PgUnits(const PagedRows& rows, F f, int heads, int each_ = 0)
+        : b(rows), units(f), each(each_) {
         share = (b.n_seqs + 63) >> 6;
         if (each) {
             s0 = -64;
@@ -205,10 +217,11 @@ struct PgUnits {
             s0 = -64;
             const int from = share * (int)(threadIdx.x & 63), to = min(b.n_seqs, from + share);
 #pragma unroll 4
-            for (int s = from; s < to; s++) v += units(pg_seq(b, s));
+            for (int s = from; s < to; s++) v = pg_add(v, units(pg_seq(b, s)));
         }
         sum = pg_scan(v);
         total = __builtin_amdgcn_readlane(sum, 63);
+        if (total == 0x7fffffff || (long)total * heads > 0x7fffffff) total = 0;
     }
     // The sequence that holds unit at < total, and the unit's number in it.
     __device__ __forceinline__ int find(int at, int& in_seq) {
@@ -246,13 +259,13 @@ struct PgUnits {
 
 // Equal contiguous ranges of `total` units over n_wgs <= total workgroups: w's
 // starts at unit w * total / n_wgs, none is empty; and the one that holds unit u.
-__device__ __forceinline__ int pg_start(int w, int total, int n_wgs) {
+__host__ __device__ __forceinline__ int pg_start(int w, int total, int n_wgs) {
     if (n_wgs == total) return w;
     // (in 32 bits: n_wgs is below 2^16 here)
     const unsigned q = (unsigned)total / (unsigned)n_wgs, rest = (unsigned)total % (unsigned)n_wgs;
     return w * (int)q + (int)((unsigned)w * rest / (unsigned)n_wgs);
 }
-__device__ __forceinline__ int pg_owner(int u, int total, int n_wgs) {
+__host__ __device__ __forceinline__ int pg_owner(int u, int total, int n_wgs) {
     return (int)((((long)u + 1) * n_wgs - 1) / total);
 }
 __device__ __forceinline__ PgJoin pg_join(bool cut, int rows, const PgSeq& q, int head, int i0, int last_unit, int total,

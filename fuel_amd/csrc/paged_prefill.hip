@@ -123,7 +123,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         const int row_tiles = (int)(((long)x.n * grp + ROWS - 1) / ROWS);
         return CUT ? row_tiles * key_tiles(x) : row_tiles;
     };
-    PgUnits<decltype(units)> pu(b, units);
+    PgUnits<decltype(units)> pu(b, units, c.kv_heads);
     int head, s, u;                       // KV head, sequence, unit of the sequence
     int at = 0, begin = 0, stop = 0, total = 0, n_wgs = 0, wg = 0;  // CUT: the range, and whose it is
     if constexpr (CUT) {
@@ -230,11 +230,11 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         uint64_t none = 0;
         auto fetch_ids = [&](int j0) {
             id0 = j0;
-            const int j = j0 + 16 * lane, id = j < sq.kv ? table[j >> c.log_ps] : 0;
-            const bool off = (unsigned)id >= (unsigned)c.n_pages;
+            const int j = j0 + 16 * lane;
+            bool off;
+            const size_t page = pg_page(c, table, j, sq.kv, off);
             none = __ballot(off);
-            const size_t at = ((((size_t)(off ? 0 : id) * c.kv_heads + head) << c.log_ps) +
-                               (j & ((1 << c.log_ps) - 1))) * X::ROW;
+            const size_t at = (((page * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * X::ROW;
             off_lo = (uint32_t)at;
             off_hi = (uint32_t)(at >> 32);
         };

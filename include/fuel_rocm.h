@@ -364,6 +364,8 @@ typedef struct frq_paged_kv {
  *     an append the row is not stored
  *   row_start[s] .. row_start[s + 1] no range within [0, rows]: the sequence
  *     has no rows
+ *   row_start that decreases, so that rows are in several sequences: such rows
+ *     hold the result of one of them, or what they held
  *   rows before row_start[0] or from row_start[n_seqs] on: left as they were
  * Cache rows beyond a sequence's length, and keys a row does not see, may hold
  * anything (NaN included) without effect on it. */

@@ -305,6 +305,21 @@ def test_many_short_sequences(dev, act, cache, decode, H, hk, D, top):
     np.testing.assert_array_equal(c.got(), got)
 
 
+def test_ranges_over_and_over(dev):
+    """Ranges of rows that overlap so often that their work cannot be counted:
+    the call ends, and leaves rows outside of them alone."""
+    say("overlapping ranges")
+    for n, H, D, new, cap in ((6, 8, 64, 100, 4096), (5000, 64, 64, 475, 1 << 20)):
+        c = Case(dev, seed(20, n), F16, F16, H, 1, D, 1024, [0], [new], tail=2)
+        c.pool.table = np.zeros((n, cap // 1024), np.int32)
+        c.kv = np.full(n, cap, np.int32)
+        c.start = np.array([0, new] * (n // 2) + [0], np.int32)
+        c.upload()
+        c.run()
+        got = c.got()
+        assert (got[new:] == 7.0).all() and (got[:, H * D:] == 7.0).all()
+
+
 # ---- prefill ----
 
 @pytest.mark.parametrize("act,cache", TYPES)

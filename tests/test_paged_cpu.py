@@ -1,6 +1,9 @@
 """What the paged KV cache entry points refuse, before they touch a device: the
 calls name no device handle, so the arguments that pass end in that refusal."""
 import ctypes as C
+import os
+import shutil
+import subprocess
 
 import pytest
 
@@ -112,3 +115,18 @@ def test_null_structs_and_workspace():
 def test_python_wrappers_raise():
     with pytest.raises(F.FuelRocmError):
         F.PagedKvCache(None, 4, 16, 1, 64, k=P)
+
+
+HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+
+
+@pytest.mark.skipif(not os.path.exists(HIPCC), reason="needs hipcc")
+def test_index_arithmetic_of_malformed_batches(tmp_path):
+    """Pages, lengths and row ranges that are none lead no kernel out of the
+    table, the pool or the rows (paged_index.cpp, the header's own functions)."""
+    src = os.path.join(os.path.dirname(os.path.abspath(__file__)), "paged_index.cpp")
+    exe = str(tmp_path / "paged_index")
+    subprocess.run([HIPCC, "-O1", "-std=c++17", "-x", "hip", "--offload-host-only", src, "-o", exe], check=True,
+                   capture_output=True, timeout=300)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
