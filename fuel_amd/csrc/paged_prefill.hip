@@ -174,41 +174,6 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         int tiles = wg_last >= 0 ? wg_last / PF_KEYS + 1 : 0;
         if constexpr (CUT) tiles = min(tiles, t0 + m_units);
 
-        // Q^T, the B operand: dims 16 t + 8 h + e of row n
-        v8 qf[X::NP][X::KS];
-        float factor = fabsf(scale) * 1.4426950408889634f;
-        {
-            const T* x = q + (size_t)row * ldq + (size_t)qh * HD;
-            float f[X::KS][8], a = 0.0f;
-#pragma unroll
-            for (int t = 0; t < X::KS; t++) {
-                T raw[8];
-                __builtin_memcpy(raw, __builtin_assume_aligned(x + 16 * t + 8 * h, 16), sizeof raw);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    f[t][e] = scale < 0.0f ? -(float)raw[e] : (float)raw[e];
-                    a = fmaxf(a, fabsf(f[t][e]));
-                }
-            }
-            int ex = 0;
-            if constexpr (X::WIDE && std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
-                a = fmaxf(a, pf_other_half(a));
-                if (a > 0.0f && a < __builtin_inff()) ex = min(120, max(-120, __builtin_amdgcn_frexp_expf(a)));
-                factor = __builtin_amdgcn_ldexpf(factor, ex);
-            }
-#pragma unroll
-            for (int t = 0; t < X::KS; t++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    float rest = __builtin_amdgcn_ldexpf(f[t][e], -ex);
-#pragma unroll
-                    for (int p = 0; p < X::NP; p++) {
-                        qf[p][t][e] = (E)rest;
-                        rest -= (float)qf[p][t][e];
-                    }
-                }
-        }
-
         pf_f16 o[X::DT];
 #pragma unroll
         for (int d = 0; d < X::DT; d++)
@@ -263,6 +228,42 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
             fetch_ids(t0 * PF_KEYS);
             issue(t0);
         }
+
+        // Q^T, the B operand: dims 16 t + 8 h + e of row n
+        v8 qf[X::NP][X::KS];
+        float factor = fabsf(scale) * 1.4426950408889634f;
+        {
+            const T* x = q + (size_t)row * ldq + (size_t)qh * HD;
+            float f[X::KS][8], a = 0.0f;
+#pragma unroll
+            for (int t = 0; t < X::KS; t++) {
+                T raw[8];
+                __builtin_memcpy(raw, __builtin_assume_aligned(x + 16 * t + 8 * h, 16), sizeof raw);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    f[t][e] = scale < 0.0f ? -(float)raw[e] : (float)raw[e];
+                    a = fmaxf(a, fabsf(f[t][e]));
+                }
+            }
+            int ex = 0;
+            if constexpr (X::WIDE && std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
+                a = fmaxf(a, pf_other_half(a));
+                if (a > 0.0f && a < __builtin_inff()) ex = min(120, max(-120, __builtin_amdgcn_frexp_expf(a)));
+                factor = __builtin_amdgcn_ldexpf(factor, ex);
+            }
+#pragma unroll
+            for (int t = 0; t < X::KS; t++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float rest = __builtin_amdgcn_ldexpf(f[t][e], -ex);
+#pragma unroll
+                    for (int p = 0; p < X::NP; p++) {
+                        qf[p][t][e] = (E)rest;
+                        rest -= (float)qf[p][t][e];
+                    }
+                }
+        }
+
         for (int t = t0; t < tiles; t++) {
             const int j0 = t * PF_KEYS;
             // tile t landed, in every wavefront, and tile t - 1 is read
