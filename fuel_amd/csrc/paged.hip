@@ -74,31 +74,27 @@ struct Rows16 {
         ValueWord w[8];
     };
 
-    // Lane 16 g + r takes row r: dims 32 t + 8 g + e of x (null: a row of zeros).
+    // Lane 16 g + r takes row r: dims 32 t + 8 g + e of x.
     __device__ void load_q(const T* x, float scale) {
         const int g = (threadIdx.x & 63) >> 4;
-        float f[KS][8];
-#pragma unroll
-        for (int t = 0; t < KS; t++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) f[t][e] = 0.0f;
-        if (x) {
-#pragma unroll
-            for (int t = 0; t < KS; t++) {
-                T raw[8];
-                __builtin_memcpy(raw, __builtin_assume_aligned(x + 32 * t + 8 * g, 16), sizeof raw);
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[t][e] = (float)raw[e];
-            }
-        }
+        // (negated for a negative scale: the maximum is taken of scores with a positive factor)
         factor = fabsf(scale) * 1.4426950408889634f;
-        if (scale < 0.0f) {  // (the maximum is taken of scores with a positive factor)
+        if constexpr (!WIDE) {
+            const uint32_t flip = scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
             for (int t = 0; t < KS; t++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) f[t][e] = -f[t][e];
+                q[0][t] = __builtin_bit_cast(v8, *reinterpret_cast<const pg_u4*>(x + 32 * t + 8 * g) ^ flip);
+            return;
         }
-        if constexpr (WIDE && std::is_same<E, _Float16>::value) {
+        float f[KS][8];
+#pragma unroll
+        for (int t = 0; t < KS; t++) {
+            T raw[8];
+            __builtin_memcpy(raw, __builtin_assume_aligned(x + 32 * t + 8 * g, 16), sizeof raw);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[t][e] = scale < 0.0f ? -(float)raw[e] : (float)raw[e];
+        }
+        if constexpr (std::is_same<E, _Float16>::value) {
             float a = 0.0f;
 #pragma unroll
             for (int t = 0; t < KS; t++)
@@ -425,7 +421,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
                 l += s_l[v][r] * wt[v];
             }
             float* slot = part + ((size_t)2 * blockIdx.x + (at != begin)) * pg_slot(16, HD);
-            const float inv = whole ? 1.0f / l : 1.0f;
+            // (of a bad length, or before position 0, all sums are 0)
+            const float inv = !whole ? 1.0f : sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : 1.0f / l;
             T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -436,7 +433,6 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
 #pragma unroll
                     for (int v = 1; v < PA_WAVES; v++) x[t] = fmaf(s_o[v - 1][4 * t + k][lane], wt[v], x[t]);
                     x[t] *= inv;
-                    if (whole) x[t] = sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : x[t];
                 }
                 if (whole) {
                     T y[A::VW];
@@ -501,13 +497,13 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(Pa
                             sq.kv, pos0 + i0 / grp);
     a.finish();
     if (i0 + r >= all) return;
-    const float inv = 1.0f / a.l;
+    const float inv = sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : 1.0f / a.l;  // (o is 0 in the first two)
     T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
         T y[A::VW];
 #pragma unroll
-        for (int t = 0; t < A::VW; t++) y[t] = (T)(sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : a.o[t][k] * inv);
+        for (int t = 0; t < A::VW; t++) y[t] = (T)(a.o[t][k] * inv);
         __builtin_memcpy(__builtin_assume_aligned(dst + A::VW * k, 8), y, sizeof y);
     }
 }

@@ -229,33 +229,43 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
             issue(t0);
         }
 
-        // Q^T, the B operand: dims 16 t + 8 h + e of row n
+        // Q^T, the B operand: dims 16 t + 8 h + e of row n (negated for a negative
+        // scale: the maximum is taken of scores with a positive factor)
         v8 qf[X::NP][X::KS];
         float factor = fabsf(scale) * 1.4426950408889634f;
-        {
-            const T* x = q + (size_t)row * ldq + (size_t)qh * HD;
+        const T* x = q + (size_t)row * ldq + (size_t)qh * HD + 8 * h;
+        if constexpr (!X::WIDE) {
+            const uint32_t flip = scale < 0.0f ? 0x80008000u : 0;
+#pragma unroll
+            for (int t = 0; t < X::KS; t++)
+                qf[0][t] = __builtin_bit_cast(v8, *reinterpret_cast<const pg_u4*>(x + 16 * t) ^ flip);
+        } else {
             float f[X::KS][8], a = 0.0f;
 #pragma unroll
             for (int t = 0; t < X::KS; t++) {
                 T raw[8];
-                __builtin_memcpy(raw, __builtin_assume_aligned(x + 16 * t + 8 * h, 16), sizeof raw);
+                __builtin_memcpy(raw, __builtin_assume_aligned(x + 16 * t, 16), sizeof raw);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    f[t][e] = scale < 0.0f ? -(float)raw[e] : (float)raw[e];
-                    a = fmaxf(a, fabsf(f[t][e]));
-                }
+                for (int e = 0; e < 8; e++) f[t][e] = scale < 0.0f ? -raw[e] : raw[e];
             }
-            int ex = 0;
-            if constexpr (X::WIDE && std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
+            if constexpr (std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
+#pragma unroll
+                for (int t = 0; t < X::KS; t++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) a = fmaxf(a, fabsf(f[t][e]));
                 a = fmaxf(a, pf_other_half(a));
-                if (a > 0.0f && a < __builtin_inff()) ex = min(120, max(-120, __builtin_amdgcn_frexp_expf(a)));
+                const int ex = a > 0.0f && a < __builtin_inff() ? min(120, max(-120, __builtin_amdgcn_frexp_expf(a))) : 0;
+#pragma unroll
+                for (int t = 0; t < X::KS; t++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) f[t][e] = __builtin_amdgcn_ldexpf(f[t][e], -ex);
                 factor = __builtin_amdgcn_ldexpf(factor, ex);
             }
 #pragma unroll
             for (int t = 0; t < X::KS; t++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    float rest = __builtin_amdgcn_ldexpf(f[t][e], -ex);
+                    float rest = f[t][e];
 #pragma unroll
                     for (int p = 0; p < X::NP; p++) {
                         qf[p][t][e] = (E)rest;
@@ -431,7 +441,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         }
         if (key0 == 0 && i0 + 32 * w + n < rows) {
             if (!CUT || whole) {
-                const float inv = 1.0f / l;
+                const float inv = sq.bad ? pg_nan() : limit < 0 ? 0.0f : 1.0f / l;  // (o is 0 in the first two)
                 T* dst = out + (size_t)row * ldo + (size_t)qh * HD + 4 * h;
 #pragma unroll
                 for (int d = 0; d < X::DT; d++)
@@ -439,10 +449,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                     for (int g = 0; g < 4; g++) {
                         T y[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float x = o[d][4 * g + i] * inv;
-                            y[i] = (T)(sq.bad ? pg_nan() : limit < 0 ? 0.0f : x);
-                        }
+                        for (int i = 0; i < 4; i++) y[i] = (T)(o[d][4 * g + i] * inv);
                         __builtin_memcpy(__builtin_assume_aligned(dst + 32 * d + 8 * g, 8), y, sizeof y);
                     }
             } else {

@@ -415,6 +415,25 @@ def test_prefill_tiles_malformed(dev):
 
 
 @pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", [(4, 2, 64, [0, -3], [20, 9]), (32, 8, 128, [0, 30], [300, 70]),
+                                             (20, 20, 64, [0, 60], [200, 700])])
+def test_prefill_scales(dev, act, cache, H, hk, D, past, new):
+    """Scales of 0 (the mean of the values a row sees), below 0 and far from 1,
+    infinite and NaN keys and values behind the last row."""
+    say("prefill scales", act, cache, H, D)
+    c = Case(dev, seed(21, act, cache, H), act, cache, H, hk, D, 16, past, new)
+    for s, n in enumerate(c.kv):
+        if n % 16:
+            page = c.pool.table[s, n // 16]
+            c.pool.k[page, :, n % 16:] = c.pool.v[page, :, n % 16:] = R.to_bits(np.float32(np.inf), cache)
+            c.pool.k[page, :, n % 16 + 1:] = R.NAN[cache]
+    c.upload()
+    for scale in (0.0, -0.09, 0.5, -1e-30):
+        c.run(scale=scale)
+        c.check(scale=float(np.float32(scale)))
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
 @pytest.mark.parametrize("H,hk,D", [(20, 20, 128), (40, 20, 64)])
 def test_prefill_more_tiles_than_cus(dev, act, cache, H, hk, D):
     """Whole tiles of 128 rows: prompts and a chunk, a page that is none, a length
