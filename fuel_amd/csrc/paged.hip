@@ -277,12 +277,19 @@ struct Rows16 {
 // end of one tile, some whole ones and the start of another; whole ones are
 // written out, the cut pieces (at most two a workgroup) leave their sums in
 // the workspace for paged_join_kernel.
+// Bound by HBM, and by some 10 us before the first keys arrive and for the join.
+// bf16, 32 heads over 8 of 128: 64 sequences of up to 8191, 413 MB, 73 us and 4.6
+// for the join; one of 131071, 537 MB, 87 and 5.2 (6.2 TB/s while it walks; reads
+// alone reach 6.75 here).  Large tiles of wavefronts, more workgroups, or the next
+// piece's first keys loaded under this one's merge took as long or longer.
 constexpr int PD_UNIT = 32 * PA_WAVES;
 
 // Tiles of a sequence, and units of each; one without keys has one unit, which
 // writes its rows.
 __device__ __forceinline__ int pd_tiles(const PgSeq& q, int grp) { return (q.n * grp + 15) >> 4; }
-__device__ __forceinline__ int pd_units(const PgSeq& q, int unit) { return q.kv <= unit ? 1 : (q.kv + unit - 1) / unit; }
+__device__ __forceinline__ int pd_units(const PgSeq& q, int unit) {
+    return q.kv <= unit ? 1 : (q.kv + unit - 1) / unit;
+}
 
 // One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of 32).
 // The next block's keys are loaded as soon as this one's scores are formed, its
@@ -475,8 +482,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
 // and up to half as long again where a batch's lengths differ much.
 template <class E, class T, int HD, bool ONCE>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(PagedKv c, PagedRows b, int grp, int each,
-                                                                              const T* __restrict__ q, int ldq,
-                                                                              float scale, T* __restrict__ out, int ldo) {
+                                                                              const T* __restrict__ q, int ldq, float scale,
+                                                                              T* __restrict__ out, int ldo) {
     using A = Rows16<E, T, HD>;
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int at = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * PA_WAVES + (threadIdx.x >> 6)));
@@ -627,6 +634,9 @@ __device__ __forceinline__ int pg_row_seq(const PagedRows& b, int row) {
 // once.  A thread's chunks are the same part of different heads, so it reads
 // its part of the position's table rows once.  A chunk's loads need the row
 // alone and go out before the row's sequence and position are known.
+// Bound by HBM for many rows (12252 of f32, 32 heads over 8 of 128: 553 MB in
+// 102 us), by three memory round trips for few (row_start and kv_len, page and table
+// rows, the stores; 2.8 us for one, 4.0 for 256).
 constexpr int AP_WG = 256;
 constexpr int AP_FEW = 2048;
 template <class E, class T, int HD>
@@ -764,8 +774,8 @@ Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads, int h
 // each, a row a workgroup: 2 sequences of 29561, 128 pieces, 28.9 -> 22.7 us a whole
 // call; one of 131071, 8 KV heads, 64 pieces, 92.6 -> 91.2.
 template <class T, int HD>
-hipError_t join(const PgJoin* joins, const float* part, int wgs, long tiles, int tile_rows, int rows, int grp, void* out,
-                int ldo, hipStream_t s) {
+hipError_t join(const PgJoin* joins, const float* part, int wgs, long tiles, int tile_rows, int rows, int grp,
+                void* out, int ldo, hipStream_t s) {
     const bool few = tiles <= wgs / 4;
     const auto kernel = tile_rows == 16 || few ? paged_join_kernel<T, HD, 8> : paged_join_kernel<T, HD, 2>;
     const int wg_rows = tile_rows == 16 && tiles <= wgs / 32 ? 1 : 4, y = (rows + wg_rows - 1) / wg_rows;
@@ -790,9 +800,10 @@ struct Rows16Call {
         const double bytes = (double)p.rows.n_seqs * p.rows.cap * p.kv.kv_heads * HD * 4;
         const bool once = !p.rows.row_start && grp <= 16 && bytes > 256e6;
         if (pl.alone) {
-            const auto kernel = once ? paged_rows16_alone_kernel<E, T, HD, true> : paged_rows16_alone_kernel<E, T, HD, false>;
-            hipLaunchKernelGGL(kernel, dim3((pl.wgs + PA_WAVES - 1) / PA_WAVES), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows, grp,
-                               p.rows.row_start ? 0 : (grp + 15) >> 4, static_cast<const T*>(p.q), p.ldq, p.scale,
+            const auto kernel =
+                once ? paged_rows16_alone_kernel<E, T, HD, true> : paged_rows16_alone_kernel<E, T, HD, false>;
+            hipLaunchKernelGGL(kernel, dim3((pl.wgs + PA_WAVES - 1) / PA_WAVES), dim3(64 * PA_WAVES), 0, s, p.kv, p.rows,
+                               grp, p.rows.row_start ? 0 : (grp + 15) >> 4, static_cast<const T*>(p.q), p.ldq, p.scale,
                                static_cast<T*>(p.out), p.ldo);
             return hipGetLastError();
         }
@@ -827,8 +838,8 @@ hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppen
     return paged_with_types(kv_dtype, dtype, hd, AppendCall{p, s});
 }
 
-hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, long tiles, int tile_rows,
-                             int rows, int grp, void* out, int ldo, hipStream_t s) {
+hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, long tiles,
+                             int tile_rows, int rows, int grp, void* out, int ldo, hipStream_t s) {
     const auto run = dtype == GGML_F32   ? (hd == 64 ? join<float, 64> : join<float, 128>)
                      : dtype == GGML_F16 ? (hd == 64 ? join<_Float16, 64> : join<_Float16, 128>)
                                          : (hd == 64 ? join<__bf16, 64> : join<__bf16, 128>);

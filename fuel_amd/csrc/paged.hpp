@@ -42,7 +42,8 @@ struct PagedRows {
 // A bound on the tiles of tile_rows query rows that a batch's sequences have:
 // each one's last may be partly empty.
 inline long pg_tiles_bound(const PagedRows& r, int grp, int tile_rows) {
-    return r.row_start ? (long)r.rows * grp / tile_rows + r.n_seqs : (long)r.n_seqs * ((grp + tile_rows - 1) / tile_rows);
+    return r.row_start ? (long)r.rows * grp / tile_rows + r.n_seqs
+                       : (long)r.n_seqs * ((grp + tile_rows - 1) / tile_rows);
 }
 
 // Which kernel a call takes.  ROWS16: 16 query rows a tile, the keys of a call
@@ -114,7 +115,9 @@ struct PgElem<_Float16> {
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static constexpr uint32_t INF = 0x7c007c00u;  // exponent bits of both halves of a word
     static constexpr int SPLIT = 2;               // parts that hold an f32 to 2^-22
-    __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
 };
 template <>
 struct PgElem<__bf16> {
@@ -122,7 +125,9 @@ struct PgElem<__bf16> {
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static constexpr uint32_t INF = 0x7f807f80u;
     static constexpr int SPLIT = 3;  // 8 significant bits each: an f32 to 2^-24
-    __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
 };
 
 // Whether a word holds an infinite or NaN half.
@@ -268,8 +273,8 @@ __host__ __device__ __forceinline__ int pg_start(int w, int total, int n_wgs) {
 __host__ __device__ __forceinline__ int pg_owner(int u, int total, int n_wgs) {
     return (int)((((long)u + 1) * n_wgs - 1) / total);
 }
-__device__ __forceinline__ PgJoin pg_join(bool cut, int rows, const PgSeq& q, int head, int i0, int last_unit, int total,
-                                          int n_wgs, int slot) {
+__device__ __forceinline__ PgJoin pg_join(bool cut, int rows, const PgSeq& q, int head, int i0, int last_unit,
+                                          int total, int n_wgs, int slot) {
     if (!cut) return PgJoin{};
     return PgJoin{rows, pg_owner(last_unit, total, n_wgs), slot, q.row0, q.kv - q.n, head, i0, 0};
 }
