@@ -634,7 +634,7 @@ __device__ __forceinline__ int pg_row_seq(const PagedRows& b, int row) {
 // once.  A thread's chunks are the same part of different heads, so it reads
 // its part of the position's table rows once.  A chunk's loads need the row
 // alone and go out before the row's sequence and position are known.
-// Bound by HBM for many rows (12252 of f32, 32 heads over 8 of 128: 553 MB in
+// Bound by HBM for many rows (12254 of f32, 32 heads over 8 of 128: 554 MB in
 // 102 us), by three memory round trips for few (row_start and kv_len, page and table
 // rows, the stores; 2.8 us for one, 4.0 for 256).
 constexpr int AP_WG = 256;
