@@ -400,16 +400,17 @@ size_t frq_paged_attention_workspace(const frq_paged_kv *kv, const frq_paged_bat
  * key and value appended before (frq_paged_append).  q and out are of type
  * dtype (FRQ_F32, or the cache's type), rows ldq and ldo elements apart.
  * Scores, softmax and sums are f32, f32 operands keep f32's precision.
- * Alignment as frq_paged_append, work 16-byte aligned.  Asynchronous,
- * allocates nothing; the same call gives the same bits. */
+ * Alignment as frq_paged_append, work 16-byte aligned; out, q and work must
+ * not overlap.  Asynchronous, allocates nothing; the same call gives the same
+ * bits. */
 int frq_paged_attention_decode(frq_device *dev, const frq_paged_kv *kv, const frq_paged_batch *batch, int dtype,
                                size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
                                size_t work_bytes, void *out_dev, size_t ldo);
 /* Causal attention of packed rows (whole prompts, or chunks whose earlier part
  * is cached): each row over the cache rows 0 .. its position, arguments as
  * frq_paged_attention_decode; the batch's own keys and values are appended
- * before.  With 16-bit operands the softmax weights are rounded to that type
- * for the product with V (their sum is not). */
+ * before.  With 16-bit operands the softmax weights may be rounded to that
+ * type for the product with V (their sum is not). */
 int frq_paged_attention_prefill(frq_device *dev, const frq_paged_kv *kv, const frq_paged_batch *batch, int dtype,
                                 size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
                                 size_t work_bytes, void *out_dev, size_t ldo);
