@@ -1447,7 +1447,9 @@ int paged_args(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b
         return fail(FRQ_UNSUPPORTED, "%s: n_seqs=%zu rows=%zu n_heads=%zu", who, b->n_seqs, b->rows, n_heads);
     if (!b->row_start && b->rows != b->n_seqs)
         return fail(FRQ_INVALID, "%s: rows=%zu, n_seqs=%zu without row_start", who, b->rows, b->n_seqs);
-    if (b->max_pages > imax / ps) return fail(FRQ_UNSUPPORTED, "%s: max_pages=%zu page_size=%zu", who, b->max_pages, ps);
+    // (2^30 positions: the kernels look up to 1024 past a sequence's end, in an int)
+    if (b->max_pages > ((size_t)1 << 30) / ps)
+        return fail(FRQ_UNSUPPORTED, "%s: max_pages=%zu page_size=%zu", who, b->max_pages, ps);
     const size_t cap = b->max_pages * ps;
     if (b->max_kv_len > cap)
         return fail(FRQ_INVALID, "%s: max_kv_len=%zu > max_pages * page_size = %zu", who, b->max_kv_len, cap);

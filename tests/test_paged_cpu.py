@@ -117,6 +117,17 @@ def test_python_wrappers_raise():
         F.PagedKvCache(None, 4, 16, 1, 64, k=P)
 
 
+@pytest.mark.parametrize("ps", [16, 1024])
+def test_positions_end_at_2_30(ps):
+    most = (1 << 30) // ps
+    one = dict(rows=3, row_start=None)
+    for fn in ("decode", "prefill"):
+        assert passes(attend(fn, c=kv(page_size=ps), b=batch(max_pages=most, **one)))
+        assert attend(fn, c=kv(page_size=ps), b=batch(max_pages=most + 1, **one)) == UNSUPPORTED
+    assert passes(append(c=kv(page_size=ps), b=batch(max_pages=most)))
+    assert append(c=kv(page_size=ps), b=batch(max_pages=most + 1)) == UNSUPPORTED
+
+
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 
 
