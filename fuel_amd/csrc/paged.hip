@@ -557,7 +557,7 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
             pg_f4 o[PJ_STEP];
             float m[PJ_STEP], l[PJ_STEP], mn = M;
 #pragma unroll
-            for (int i = 0; i < PJ_STEP; i++) {  // (past the last: the last again, with weight 0)
+            for (int i = 0; i < PJ_STEP; i++) {  // (past the last: the last again, not added)
                 const int wi = min(w + i * groups, j.last);
                 const size_t slot = (size_t)(wi == w0 ? j.slot : 2 * wi) * pg_slot(tile_rows, HD);
                 o[i] = *reinterpret_cast<const pg_f4*>(row + slot);
@@ -572,10 +572,11 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
             O *= f;
 #pragma unroll
             for (int i = 0; i < PJ_STEP; i++) {
-                const float e = w + i * groups <= j.last ? __builtin_amdgcn_exp2f(m[i] - mn) : 0.0f;
-                L = fmaf(l[i], e, L);
+                const bool add = w + i * groups <= j.last;
+                const float e = __builtin_amdgcn_exp2f(m[i] - mn);
+                L = fmaf(l[i], add ? e : 0.0f, L);
 #pragma unroll
-                for (int k = 0; k < 4; k++) O[k] = fmaf(o[i][k], e, O[k]);
+                for (int k = 0; k < 4; k++) O[k] = add ? fmaf(o[i][k], e, O[k]) : O[k];  // (o may be infinite)
             }
         }
         s_o[threadIdx.x] = O;
