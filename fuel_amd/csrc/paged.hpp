@@ -168,6 +168,79 @@ __host__ __device__ __forceinline__ int pg_page(const PagedKv& c, const int* tab
     return none ? 0 : id;
 }
 
+// Whether an infinite or NaN value is among a lane's sums.
+template <int N, class V>
+__device__ __forceinline__ bool pg_odd(const V (&o)[N]) {
+    float t = 0.0f;
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(V) / sizeof(float)); i++) t = fmaf(o[n][i], 0.0f, t);
+    return t != t;
+}
+
+// A row's softmax and sums over keys j0 .. j1 - 1 (those that mine(j) takes) as
+// the definition has them: f32 dot products, whole weights, no key that the row
+// does not see.  The kernels' products form q and the weights in parts, and of a
+// tile's rows some see keys that others do not: 0 * inf, and inf in parts of both
+// signs, are NaN there where the definition has a number or an infinity.  Such
+// sums never become finite again, so a wavefront that ends with one takes its keys
+// here once more.  SHARE lanes, 64 / SHARE apart, hold a row of HD dims; a lane's
+// are RUNS runs of 4, run i from dim(i) on.  x: the row's q.
+template <class E, class T, int HD, int SHARE, int RUNS, class Mine, class Dim>
+__device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int head, const T* x, float scale,
+                                         int limit, int j0, int j1, float shift, float floor, Mine mine, Dim dim,
+                                         float& m, float& l, pg_f4 (&o)[RUNS]) {
+    const auto row = [&](const void* pool, int j, bool& none) {
+        const int page = pg_page(c, table, j, j + 1, none);
+        return static_cast<const E*>(pool) +
+               ((((size_t)page * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * HD;
+    };
+    const auto score = [&](int j) {
+        bool none;
+        const E* k = row(c.k, j, none);
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < RUNS; i++) {
+            E y[4];
+            T z[4];
+            __builtin_memcpy(y, __builtin_assume_aligned(k + dim(i), 8), sizeof y);
+            __builtin_memcpy(z, __builtin_assume_aligned(x + dim(i), 8), sizeof z);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s = fmaf((float)z[e], (float)y[e], s);
+        }
+#pragma unroll
+        for (int d = 64 / SHARE; d < 64; d *= 2) s += __shfl_xor(s, d);
+        return none ? pg_nan() : s * (scale * 1.4426950408889634f);
+    };
+    m = floor;
+#pragma unroll 1
+    for (int j = j0; j < j1; j++) {
+        if (!mine(j)) continue;
+        const float s = score(j);
+        if (j <= limit) m = fmaxf(m, s);
+    }
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < RUNS; i++) o[i] = pg_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+    for (int j = j0; j < j1; j++) {
+        if (!mine(j)) continue;
+        const float p = __builtin_amdgcn_exp2f(score(j) - m + shift);
+        if (j > limit) continue;
+        bool none;
+        const E* v = row(c.v, j, none);
+        l += p;
+#pragma unroll
+        for (int i = 0; i < RUNS; i++) {
+            E y[4];
+            __builtin_memcpy(y, __builtin_assume_aligned(v + dim(i), 8), sizeof y);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[i][e] = fmaf(p, (float)y[e], o[i][e]);
+        }
+    }
+}
+
 // Sums of v >= 0 over lanes 0 .. the own one, at most 0x7fffffff, by DPP (a chain
 // of lane shuffles takes ten times as long).
 __device__ __forceinline__ int pg_add(int a, int b) { return __builtin_elementwise_add_sat(a, b); }

@@ -121,7 +121,6 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
     constexpr int NA = 2 / KW;  // groups of 32 keys of a tile a wavefront
     __shared__ __align__(1024) uint8_t s_k[2][X::TILE], s_v[2][X::TILE];
     __shared__ float s_m[ROWS], s_l[ROWS];
-    __shared__ uint32_t s_odd[2];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), w = KW == 1 ? wave : wave % RW;
     const int key0 = KW == 1 ? 0 : 32 * (wave / RW);  // first of its keys in a tile
@@ -175,8 +174,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         const int row = sq.row0 + mine / grp, qh = head * grp + mine % grp;
         const int pos0 = sq.kv - sq.n;
         const int limit = pos0 + mine / grp;
-        // first and last position of the workgroup's and of this wavefront's rows
-        const int wg_first = pos0 + i0 / grp, wg_last = pos0 + min(i0 + ROWS - 1, rows - 1) / grp;
+        // last position of the workgroup's rows, first and last of this wavefront's
+        const int wg_last = pos0 + min(i0 + ROWS - 1, rows - 1) / grp;
         const int first = pos0 + min(i0 + 32 * w, rows - 1) / grp;
         const int last = i0 + 32 * w < rows ? pos0 + min(i0 + 32 * w + 31, rows - 1) / grp : -1;
         int tiles = wg_last >= 0 ? wg_last / PF_KEYS + 1 : 0;
@@ -289,33 +288,13 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
             const uint32_t bad = (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
-            const bool masked = j0 + PF_KEYS - 1 > wg_first || bad;
-            uint64_t odd = 0;
-            if (masked) {
-                // rows of V that are no keys are cleared, so are infinite and NaN
-                // values, whose keys are noted: 0 * inf must not reach the rows
-                // that do not see them
-                if (threadIdx.x < 2) s_odd[threadIdx.x] = 0;
-                __syncthreads();
+            if (j0 + PF_KEYS > sq.kv || bad) {  // rows of V that are no keys hold anything
                 for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
                     const int r = ch / CPR;
-                    uint4* at = reinterpret_cast<uint4*>(s_v[t & 1]) + ch;
-                    const uint4 u = *at;
-                    uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                    const bool none = j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1);
-                    bool hit = false;
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        if (pg_word_inf<E>(x[k])) {
-                            hit = true;
-                            x[k] = 0;
-                        }
-                    }
-                    if (none || hit) *at = none ? make_uint4(0, 0, 0, 0) : make_uint4(x[0], x[1], x[2], x[3]);
-                    if (hit && !none) atomicOr(&s_odd[r >> 5], 1u << (r & 31));
+                    if (j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1))
+                        reinterpret_cast<uint4*>(s_v[t & 1])[ch] = make_uint4(0, 0, 0, 0);
                 }
                 __syncthreads();
-                odd = KW == 2 ? s_odd[wave / RW] : (uint64_t)s_odd[1] << 32 | s_odd[0];
             }
             if (t + 1 < tiles) issue(t + 1);
             const int jw = j0 + key0;  // this wavefront's first key
@@ -396,33 +375,19 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
 #pragma unroll
                     for (int p = X::NP - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
                 }
-            if (masked) {
-                for (; odd; odd &= odd - 1) {  // the cleared values, for the rows that see them
-                    const int r = __builtin_ctzll(odd);
-                    float p = 0.0f;
-#pragma unroll
-                    for (int a = 0; a < NA; a++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++)
-                            if (32 * a + (i & 3) + 8 * (i >> 2) == (r & ~4)) p = st[a][i];
-                    const float q2 = pf_other_half(p);
-                    p = ((r >> 2) & 1) == h ? p : q2;
-                    const int page = table[(jw + r) >> c.log_ps];
-                    const E* src = static_cast<const E*>(c.v) +
-                                   ((((size_t)page * c.kv_heads + head) << c.log_ps) +
-                                    ((jw + r) & ((1 << c.log_ps) - 1))) * HD;
-                    if (jw + r > limit) continue;
-#pragma unroll
-                    for (int d = 0; d < X::DT; d++)
-#pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float v = (float)src[32 * d + (i & 3) + 8 * (i >> 2) + 4 * h];
-                            if (!(fabsf(v) < __builtin_inff())) o[d][i] = fmaf(p, v, o[d][i]);
-                        }
-                }
-            }
         }
         l += pf_other_half(l);
+        if (__any(pg_odd(o))) {
+            pg_f4 y[4 * X::DT];
+            pg_plain<E, T, HD, 2>(
+                c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, t0 * PF_KEYS,
+                min(tiles * PF_KEYS, last + 1), PF_SHIFT, -1e30f,
+                [&](int j) { return KW == 1 || (j & 32) == key0; }, [&](int i) { return 8 * i + 4 * h; }, m, l, y);
+#pragma unroll
+            for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = y[4 * d + i / 4][i % 4];
+        }
         if constexpr (KW == 2) {  // the two that share rows
             static_assert(16 * X::DT * 64 * 4 * RW <= sizeof s_k, "the sums of half the wavefronts");
             __syncthreads();

@@ -30,6 +30,12 @@ def got_of(c, s):
     return c.got()[int(c.start[s]):int(c.start[s + 1]), :c.H * c.D].reshape(c.new[s], c.H, c.D)
 
 
+# heads, KV heads, dims, cached, new: 64-row tiles, 128-row tiles, cut 128-row tiles
+PREFILL = [(32, 2, 128, [0, 30], [170, 160]), (64, 4, 64, [0, 30], [170, 160]), (20, 20, 128, [0, 0, 70, 0, 3], [200, 260, 130, 60, 200]),
+           (40, 20, 64, [0, 0, 70], [200, 260, 130]), (32, 2, 128, [2200, 2000], [150, 140]),
+           (40, 2, 64, [2200, 2000], [150, 140])]
+
+
 def put_values(c, s, odd):
     """odd: (key, KV head, dim, value) of sequence s's V; its keys, and V with zeros there."""
     k, v = c.pool.get(s, int(c.kv[s]))
@@ -65,3 +71,24 @@ def test_decode_joins_infinite_pieces(dev, act, cache, H, hk, D, lens):
     c.run()
     for s, odd in enumerate(odds):
         check_values(c, s, odd, *plain[s], False)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", PREFILL)
+def test_prefill_single_values_that_are_no_numbers(dev, act, cache, H, hk, D, past, new):
+    """Single infinite and NaN elements of V, in even and odd dims, in early keys
+    that all rows see, on the diagonal and behind it."""
+    say("prefill single values", act, cache, H, D, past)
+    c = Case(dev, seed(30, act, cache, H, D), act, cache, H, hk, D, 16, past, new, row0=1, tail=2, pad=8)
+    inf, nan, g = np.inf, np.nan, hk - 1
+    odds = []
+    for s, (p, n) in enumerate(zip(past, new)):
+        at = p + n // 2
+        odds.append([(0, 0, 0, inf), (p + 17, g, 3, -inf), (at, 0, 6, nan), (at + 1, 0, 7, inf), (at + 1, g, 10, -inf),
+                     (at + 2, 0, 7, -inf), (p + n - 1, g, D - 1, inf), (p + n - 20, 0, D - 2, nan)])
+    plain = [put_values(c, s, odd) for s, odd in enumerate(odds)]
+    c.upload()
+    for _ in range(2):
+        c.run()
+        for s, odd in enumerate(odds):
+            check_values(c, s, odd, *plain[s], True)
