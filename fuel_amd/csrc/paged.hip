@@ -224,40 +224,30 @@ struct Rows16 {
     }
 
     // Keys that no row of the sequence may see: their rows hold anything.
-    // Whether an infinite or NaN value is left.
-    __device__ static bool clear(ValueRegs& v, const Mask& mk) {
+    __device__ static void clear(ValueRegs& v, const Mask& mk) {
         const int g = (threadIdx.x & 63) >> 4;
-        bool odd = false;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const bool none = mk.bad[i >> 2] || mk.j0 + 16 * (i >> 2) + 4 * g + (i & 3) >= mk.kv;
 #pragma unroll
-            for (int w = 0; w < VW / 2; w++) {
+            for (int w = 0; w < VW / 2; w++)
                 if (none) v.w[i][w] = 0;
-                odd |= pg_word_inf<E>(v.w[i][w]);
-            }
         }
-        return odd;
     }
 
-    // The product with V where a value in a key that some rows do not see is
-    // infinite or NaN: 0 * inf must not reach those rows, so each row adds
-    // only its own keys.
-    __device__ void product_seen(const float (&w)[8], const Mask& mk, const E* const (&va)[2]) {
-        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-        for (int j = 0; j < 32; j++) {
-            float p = w[0];
+    // The row's sums over keys [j0, j1) once more, where one is infinite or NaN.
+    // x: its q.
+    __device__ void mend(const PagedKv& c, const int* table, int head, const T* x, float scale, int j0, int j1) {
+        if (!__any(pg_odd(o))) return;
+        pg_f4 y[VW];
+        const int d0 = 4 * VW * ((threadIdx.x & 63) >> 4);
+        pg_plain<E, T, HD, 4>(
+            c, table, head, x, scale, limit, j0, j1, PA_SHIFT, -1e30f, [](int) { return true; },
+            [&](int i) { return d0 + 4 * i; }, m, l, y);
 #pragma unroll
-            for (int i = 1; i < 8; i++) p = (j >> 4) * 4 + (j & 3) == i ? w[i] : p;
-            p = __shfl(p, r + 16 * ((j >> 2) & 3));
-            if (mk.j0 + j <= limit) {
-                const E* row = (j < 16 ? va[0] : va[1]) + (j & 15) * HD + 4 * VW * g;
+        for (int t = 0; t < VW; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int t = 0; t < VW; t++) o[t][i] = fmaf(p, (float)row[VW * i + t], o[t][i]);
-            }
-        }
+            for (int k = 0; k < 4; k++) o[t][k] = y[(VW * k + t) / 4][(VW * k + t) % 4];
     }
 
     // The row's sum over the four lanes that share it.
@@ -335,12 +325,8 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
                 if (mask) a.template scores<true>(kr, mk, s);
                 else a.template scores<false>(kr, mk, s);
                 a.weights(s, pp);
-                if (mask && __any(A::clear(vr, mk))) {
-                    rows(c.v, i, at);
-                    a.product_seen(s, mk, at);
-                } else {
-                    a.product(vr, pp);
-                }
+                if (mask) A::clear(vr, mk);
+                a.product(vr, pp);
                 if (i == last) break;
                 rows(c.k, i + 1, at);
                 A::template load_k<ONCE>(kr, at);
@@ -403,9 +389,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
         const int first = pos0 + i0 / grp, seen = pos0 + min(i0 + 15, all - 1) / grp + 1;  // keys that some row sees
         const int k0 = u0 * unit, k1 = max(k0, min(seen, (u0 + m) * unit));
         const int per = ((k1 - k0 + 31) / 32 + PA_WAVES - 1) / PA_WAVES;
-        pd_walk<E, T, HD, ONCE>(a, c, b.table + (size_t)s * b.max_pages, head, k0 + 32 * w * per,
-                          min(k1, k0 + 32 * (w + 1) * per), sq.kv, first);
+        const int* table = b.table + (size_t)s * b.max_pages;
+        const int j0 = k0 + 32 * w * per, j1 = min(k1, j0 + 32 * per);
+        pd_walk<E, T, HD, ONCE>(a, c, table, head, j0, j1, sq.kv, first);
         a.finish();
+        a.mend(c, table, head, q + (size_t)row * ldq + (size_t)h * HD, scale, j0, j1);
         if (w > 0) {
 #pragma unroll
             for (int t = 0; t < A::VW; t++)
@@ -500,9 +488,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(Pa
     a.load_q(q + (size_t)row * ldq + (size_t)h * HD, scale);
     a.limit = pos0 + i / grp;
     a.start();
-    pd_walk<E, T, HD, ONCE>(a, c, b.table + (size_t)s * b.max_pages, head, 0, pos0 + min(i0 + 15, all - 1) / grp + 1,
-                            sq.kv, pos0 + i0 / grp);
+    const int* table = b.table + (size_t)s * b.max_pages;
+    const int seen = pos0 + min(i0 + 15, all - 1) / grp + 1;  // keys that some row sees
+    pd_walk<E, T, HD, ONCE>(a, c, table, head, 0, seen, sq.kv, pos0 + i0 / grp);
     a.finish();
+    a.mend(c, table, head, q + (size_t)row * ldq + (size_t)h * HD, scale, 0, seen);
     if (i0 + r >= all) return;
     const float inv = sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : 1.0f / a.l;  // (o is 0 in the first two)
     T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;

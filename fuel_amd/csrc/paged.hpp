@@ -113,7 +113,6 @@ template <>
 struct PgElem<_Float16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-    static constexpr uint32_t INF = 0x7c007c00u;  // exponent bits of both halves of a word
     static constexpr int SPLIT = 2;               // parts that hold an f32 to 2^-22
     __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -123,19 +122,11 @@ template <>
 struct PgElem<__bf16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
-    static constexpr uint32_t INF = 0x7f807f80u;
     static constexpr int SPLIT = 3;  // 8 significant bits each: an f32 to 2^-24
     __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
 };
-
-// Whether a word holds an infinite or NaN half.
-template <class E>
-__device__ __forceinline__ bool pg_word_inf(uint32_t w) {
-    const uint32_t t = ~w & PgElem<E>::INF;
-    return (t & 0xffffu) == 0 || (t >> 16) == 0;
-}
 
 __device__ __forceinline__ float pg_nan() { return __builtin_nanf(""); }
 

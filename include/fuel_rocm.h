@@ -369,7 +369,8 @@ typedef struct frq_paged_kv {
  *     hold the result of one of them, or what they held
  *   rows before row_start[0] or from row_start[n_seqs] on: left as they were
  * Cache rows beyond a sequence's length, and keys a row does not see, may hold
- * anything (NaN included) without effect on it. */
+ * anything (NaN included) without effect on it; infinite and NaN values that it
+ * sees give what f32 arithmetic makes of them, in their dims alone. */
 typedef struct frq_paged_batch {
     size_t n_seqs, max_pages, rows, max_kv_len;
     const int32_t *page_table, *kv_len, *row_start;

@@ -30,14 +30,17 @@ def got_of(c, s):
     return c.got()[int(c.start[s]):int(c.start[s + 1]), :c.H * c.D].reshape(c.new[s], c.H, c.D)
 
 
-# heads, KV heads, dims, cached, new: 64-row tiles, 128-row tiles, cut 128-row tiles
-PREFILL = [(32, 2, 128, [0, 30], [170, 160]), (64, 4, 64, [0, 30], [170, 160]), (20, 20, 128, [0, 0, 70, 0, 3], [200, 260, 130, 60, 200]),
+# heads, KV heads, dims, cached, new: 16-row tiles, 64-row tiles, 128-row tiles, cut 128-row tiles
+PREFILL = [(4, 2, 64, [0, 30], [170, 160]), (4, 2, 128, [0, 30], [170, 160]), (20, 20, 128, [40] * 30, [9] * 30),
+           (32, 2, 128, [0, 30], [170, 160]), (64, 4, 64, [0, 30], [170, 160]),
+           (20, 20, 128, [0, 0, 70, 0, 3], [200, 260, 130, 60, 200]),
            (40, 20, 64, [0, 0, 70], [200, 260, 130]), (32, 2, 128, [2200, 2000], [150, 140]),
            (40, 2, 64, [2200, 2000], [150, 140])]
 
 
 def put_values(c, s, odd):
-    """odd: (key, KV head, dim, value) of sequence s's V; its keys, and V with zeros there."""
+    """odd: (key, KV head, dim, value) of sequence s's V, the last where several name
+    one element; its keys, and V with zeros there."""
     k, v = c.pool.get(s, int(c.kv[s]))
     v, zeroed = v.copy(), v.copy()
     for j, g, d, x in odd:
@@ -52,7 +55,7 @@ def check_values(c, s, odd, k, zeroed, prefill):
     tol = R.bound(want, A, B, V, len(k), c.D, c.act, c.cache, prefill)
     grp = c.H // c.hk
     with np.errstate(invalid="ignore"):
-        for j, g, d, x in odd:  # (weights are above 0 in 64 bits, and in f32 for rows like these)
+        for (j, g, d), x in {o[:3]: o[3] for o in odd}.items():  # (weights are above 0 in 64 bits, and in f32 for rows like these)
             want[pos >= j, g * grp:(g + 1) * grp, d] += x
     compare(got_of(c, s), want, tol)
 
@@ -84,11 +87,63 @@ def test_prefill_single_values_that_are_no_numbers(dev, act, cache, H, hk, D, pa
     odds = []
     for s, (p, n) in enumerate(zip(past, new)):
         at = p + n // 2
-        odds.append([(0, 0, 0, inf), (p + 17, g, 3, -inf), (at, 0, 6, nan), (at + 1, 0, 7, inf), (at + 1, g, 10, -inf),
-                     (at + 2, 0, 7, -inf), (p + n - 1, g, D - 1, inf), (p + n - 20, 0, D - 2, nan)])
+        odds.append([(0, 0, 0, inf), (p + min(17, n - 1), g, 3, -inf), (at, 0, 6, nan), (at + 1, 0, 7, inf), (at + 1, g, 10, -inf),
+                     (at + 2, 0, 7, -inf), (p + n - 1, g, D - 1, inf), (p + max(0, n - 20), 0, D - 2, nan)])
     plain = [put_values(c, s, odd) for s, odd in enumerate(odds)]
     c.upload()
     for _ in range(2):
         c.run()
         for s, odd in enumerate(odds):
             check_values(c, s, odd, *plain[s], True)
+
+
+# 16-row tiles: cut over the workgroups, whole, a wavefront each
+DECODE = [(8, 2, 128, [1500, 1235, 0, 40]), (4, 1, 64, [9001]), (8, 8, 128, [300, 1, 77, 130]), (6, 2, 64, [1] * 3 + [500]),
+          (40, 20, 128, [20, 31, 2]), (64, 32, 64, [100] * 9 + [250] * 8)]
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,lens", DECODE)
+def test_decode_single_values_that_are_no_numbers(dev, act, cache, H, hk, D, lens):
+    """Single infinite and NaN elements of V early and late in a sequence: infinite
+    where the definition is, whichever block of keys holds them."""
+    say("decode single values", act, cache, H, D, lens[:4])
+    c = Case(dev, seed(32, act, cache, H, D), act, cache, H, hk, D, 16, [n - 1 for n in lens], [1] * len(lens), pad=8,
+             decode=True)
+    inf, nan = np.inf, np.nan
+    odds = [[(j, g % hk, d, x) for j, g, d, x in [(0, 0, 0, inf), (n // 3, 1, 3, -inf), (n // 2, 0, 8, nan), (n // 2, 0, 9, inf),
+                                                  (n // 3, 0, 9, -inf), (n - 1, 1, D - 1, inf)]] if n else [] for n in lens]
+    plain = [put_values(c, s, odd) for s, odd in enumerate(odds)]
+    c.upload()
+    for _ in range(2):
+        c.run()
+        for s, odd in enumerate(odds):
+            check_values(c, s, odd, *plain[s], False)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new,decode", [(*x, False) for x in PREFILL] +
+                         [(H, hk, D, [n - 1 for n in lens if n > 3], [1] * sum(n > 3 for n in lens), True)
+                          for H, hk, D, lens in DECODE])
+def test_keys_of_infinite_dims(dev, act, cache, H, hk, D, past, new, decode):
+    """A key of -inf in one dim: a weight of 0 for the rows whose q is above 0
+    there, no number for those below."""
+    say("infinite keys", act, cache, H, D, past[:3])
+    c = Case(dev, seed(33, act, cache, H, D), act, cache, H, hk, D, 16, past, new, decode=decode)
+    keys = [min(2 + p + n // 2, p + n - 1) for p, n in zip(past, new)]
+    plain = []
+    for s, j in enumerate(keys):
+        k, v = c.pool.get(s, int(c.kv[s]))
+        plain.append((np.delete(k, j, 0), np.delete(v, j, 0)))
+        k = k.copy()
+        k[j, :, 5] = -np.inf
+        c.pool.put(s, np.arange(len(k)), k, v)
+    c.upload()
+    c.run()
+    for s, j in enumerate(keys):
+        q, pos = rows_of(c, s)
+        assert (q[..., 5] != 0).all() and j > 0
+        want, A, B, V = R.attend(q, *plain[s], pos - (pos >= j), c.scale)
+        tol = R.bound(want, A, B, V, int(c.kv[s]), D, act, cache, not decode)
+        want[(pos >= j)[:, None] & (q[..., 5] < 0)] = np.nan
+        compare(got_of(c, s), want, tol)
