@@ -15,7 +15,8 @@
 //     The C layout leaves lane 16 g + r keys 4g + i (i < 4) of each group for
 //     row r: with both groups its 8 values of the PV product's k index, in an
 //     order that V's loads follow.  P never moves between lanes.
-//   p = e^(s - m), running maximum m and sum l per row (l per lane until the end)
+//   p = e^(s - m) and their sum l per row (l per lane until the end); m is the
+//     running maximum, of f16 parts a bound of the block's own (PG_DROP)
 //   O^T (dims x rows) += V^T . P^T: tile t takes the dims VW * r + t, so that
 //     lane 16 g + r's loads of its 8 keys, VW dims from VW * r, hold the A
 //     operand of all VW tiles, put together by byte permutes.
@@ -25,9 +26,8 @@
 // range.  16-bit activations: q as it is, p in two parts; their products cost
 // nothing here, where K and V bytes are the bound, and one part would add a
 // rounding as large as the output's own.
-// p carries a factor 2^PA_SHIFT, which l carries too: f16 parts of the many
-// small p of a long context keep steps of 2^-24 / 2^15 of the largest p
-// (2^15 < f16's largest, 65504).
+// p carries a factor 2^PA_SHIFT, which l carries too: f16 parts of small p keep
+// steps of 2^-24 / 2^15 of the largest p of 32 keys (2^15 < f16's largest, 65504).
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
@@ -64,7 +64,7 @@ struct Rows16 {
     float factor;  // score = S^T * factor, in units of log2
     int limit;     // the row's position; -1: it sees nothing
     pg_f4 o[VW];
-    float m, l;
+    float m, l, peak;  // peak: the largest score so far
 
     struct KeyRegs {
         pg_u4 w[2][KS];
@@ -127,7 +127,7 @@ struct Rows16 {
 #pragma unroll
         for (int t = 0; t < VW; t++) o[t] = pg_f4{0.f, 0.f, 0.f, 0.f};
         // (a finite floor: a row that has seen nothing yet keeps m = -1e30, l = 0, o = 0)
-        m = -1e30f;
+        m = peak = -1e30f;
         l = 0.0f;
     }
 
@@ -190,7 +190,10 @@ struct Rows16 {
         float top = s[0];
 #pragma unroll
         for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
-        const float mn = fmaxf(m, pg_row_max(top));
+        top = pg_row_max(top);
+        peak = fmaxf(peak, top);
+        // (whole steps: c is exact)
+        const float mn = std::is_same<E, _Float16>::value ? __builtin_ceilf(fmaxf(top, peak - PG_DROP)) : peak;
         const float c = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before: l = o = 0)
         m = mn;
         l *= c;

@@ -113,7 +113,7 @@ template <>
 struct PgElem<_Float16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
-    static constexpr int SPLIT = 2;               // parts that hold an f32 to 2^-22
+    static constexpr int SPLIT = 2;  // parts that hold an f32 to 2^-22
     __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -158,6 +158,13 @@ __host__ __device__ __forceinline__ int pg_page(const PagedKv& c, const int* tab
     none = (unsigned)id >= (unsigned)c.n_pages;
     return none ? 0 : id;
 }
+
+// f16 parts hold weights in steps of 2^-24.  Where keys have weights far below the
+// largest so far, the score that stands for the weight 1 follows theirs down, so
+// that those weights keep their digits too, by up to 2^PG_DROP: the sums stay in
+// f32's range (2^15 a weight, 2^16 a value, 2^30 keys), and what is lost is below
+// 2^-PG_DROP of what f32 sums keep.
+constexpr float PG_DROP = 40.0f;
 
 // Whether an infinite or NaN value is among a lane's sums.
 template <int N, class V>

@@ -14,9 +14,11 @@
 // LDS rows are kept unpadded (the DMA writes them in lane order); the DMA's
 // source addresses permute the 16-byte chunks of a row instead, so that the
 // rows one read touches fall in different banks.
-// The running maximum is renewed only when a row's scores pass it by 2^PF_LAZY:
-// the weights stay below 2^(PF_SHIFT + PF_LAZY) = 2^15, in f16's range, and the
-// sums and the output share the factor whatever it is.
+// The running maximum is renewed only when a row's scores pass it by LAZY: the
+// weights stay below 2^(SHIFT + LAZY) = 2^15, in f16's range, and the sums and the
+// output share the factor whatever it is.  Of f16 parts it is also lowered where a
+// tile's scores stay below it by PF_LOW (PG_DROP); tiles of 64 such rows of q and
+// keys, N(0, 1), differ by less.
 // 16-bit activations: p is rounded to the cache's type for the second product
 // (a relative 2^-11 or 2^-8 of each weight at most, the output's own rounding;
 // the sum l takes p as it is).  A second part, as the decode keeps, would cost
@@ -43,7 +45,7 @@ namespace {
 constexpr int PF_WAVES = 4;
 constexpr int PF_ROWS = 32 * PF_WAVES;
 constexpr int PF_KEYS = 64;
-constexpr float PF_SHIFT = 8.0f, PF_LAZY = 7.0f;
+constexpr float PF_LOW = 8.0f;
 
 typedef float pf_f16 __attribute__((ext_vector_type(16)));
 typedef short pf_s4 __attribute__((ext_vector_type(4)));
@@ -85,6 +87,9 @@ struct PrefillTile {
     using v8 = typename P::v8;
     static constexpr bool WIDE = std::is_same<T, float>::value;
     static constexpr int NP = WIDE ? P::SPLIT : 1;
+    static constexpr bool F16 = std::is_same<E, _Float16>::value;
+    // (f16 parts of an f32 weight: as many of its digits as f16's range holds)
+    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = 15.0f - LAZY;
     static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
     static constexpr int RPI = 512 / HD, NI = TILE / 1024;  // rows a DMA instruction, instructions a tile
@@ -186,7 +191,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         for (int d = 0; d < X::DT; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-        float m = -1e30f, l = 0.0f;
+        float m = -1e30f, l = 0.0f, peak = m;  // peak: the largest score so far
 
         // DMA: instruction i of this wavefront takes rows ((i PF_WAVES + wave) RPI) .. of
         // a tile, all in one group of 16 keys.  Source offsets of the lane within it:
@@ -331,15 +336,17 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
 #pragma unroll
                 for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
             top = fmaxf(top, pf_other_half(top)) * factor;
-            if (__any(top > m + PF_LAZY)) {
-                const float mn = fmaxf(m, top);
+            peak = fmaxf(peak, top);
+            const float low = X::F16 ? fmaxf(top, peak - PG_DROP) : m;
+            if (__any(top > m + X::LAZY || low < m - PF_LOW)) {
+                const float mn = fmaxf(top, low < m - PF_LOW ? low : m);
                 const float f = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before)
                 m = mn;
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < X::DT; d++) o[d] *= f;
             }
-            const float ms = m - PF_SHIFT;
+            const float ms = m - X::SHIFT;
 #pragma unroll
             for (int a = 0; a < NA; a++)
 #pragma unroll
@@ -381,7 +388,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
             pg_f4 y[4 * X::DT];
             pg_plain<E, T, HD, 2>(
                 c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, t0 * PF_KEYS,
-                min(tiles * PF_KEYS, last + 1), PF_SHIFT, -1e30f,
+                min(tiles * PF_KEYS, last + 1), X::SHIFT, -1e30f,
                 [&](int j) { return KW == 1 || (j & 32) == key0; }, [&](int i) { return 8 * i + 4 * h; }, m, l, y);
 #pragma unroll
             for (int d = 0; d < X::DT; d++)

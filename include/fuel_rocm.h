@@ -401,7 +401,10 @@ size_t frq_paged_attention_workspace(const frq_paged_kv *kv, const frq_paged_bat
  * - 1, out = softmax((q . k_j) * scale) . v_j per head, the new token's own
  * key and value appended before (frq_paged_append).  q and out are of type
  * dtype (FRQ_F32, or the cache's type), rows ldq and ldo elements apart.
- * Scores, softmax and sums are f32, f32 operands keep f32's precision.
+ * Scores, softmax and sums are f32.  f32 operands are multiplied in parts that
+ * hold them to 2^-22; over f16 pages a softmax weight is held to 2^-22 or to
+ * 2^-40 of the row's largest, and to 2^-32 of the largest of the 64 keys beside
+ * it, if that is less.
  * Alignment as frq_paged_append, work 16-byte aligned; out, q and work must
  * not overlap.  Asynchronous, allocates nothing; the same call gives the same
  * bits. */

@@ -147,3 +147,58 @@ def test_keys_of_infinite_dims(dev, act, cache, H, hk, D, past, new, decode):
         tol = R.bound(want, A, B, V, int(c.kv[s]), D, act, cache, not decode)
         want[(pos >= j)[:, None] & (q[..., 5] < 0)] = np.nan
         compare(got_of(c, s), want, tol)
+
+
+@pytest.mark.parametrize("decode", [False, True])
+@pytest.mark.parametrize("weight", [2.0 ** -30, 1e-9, 1e-10, 1e-8])
+@pytest.mark.parametrize("H,rows", [(1, 1), (32, 2), (64, 20), (128, 300)])
+def test_f32_rows_keep_small_weights(dev, H, rows, weight, decode):
+    """A key far above all others, late or early: the weights of the others, 1e-10
+    .. 1e-8 of its own, are all of dim 0 of the output.  f32 sums keep them to some
+    n steps of f32; over f16 pages they are held to the parts' 2^-22, but those in
+    a block or tile with the large one (64 keys), to 2^-40 of that one."""
+    rows = 1 if decode else rows
+    for n in (600, 9000 if H * rows > 10000 else 30001):
+        say("f32 small weights", H, rows, weight, decode, n)
+        D, at = 128, 17 if n == 600 else n - 2 * rows - 100
+        c = Case(dev, seed(34), F32, F16, H, 1, D, 16, [n - rows], [rows], decode=decode)
+        k, v = np.zeros((n, 1, D), np.float32), np.zeros((n, 1, D), np.float32)
+        k[at, 0, 0] = 32.0
+        v[:, 0, 0] = 1.0
+        v[at, 0, 0], v[at, 0, 1] = 0.0, 1.0
+        c.pool.put(0, np.arange(n), k, v)
+        c.q[:] = 0
+        c.q[:, ::D] = -np.log(weight) / 32 / 0.25
+        c.upload()
+        c.run(0.25)
+        q, pos = rows_of(c, 0)
+        want = R.attend(q, k, v, pos, 0.25)[0]
+        got = got_of(c, 0)
+        # the score 32 q 0.25 is rounded at most four times, where the weight's logarithm is some 23
+        near = 64 * 2.0 ** -41 / weight / n
+        tol = want[..., 0] * ((4 * 23 + 2 * n + 16) * R.U + 2.0 ** -22 + near)
+        err = np.abs(got[..., 0] - want[..., 0])
+        assert (err <= tol).all(), (err / want[..., 0]).max()
+        assert np.abs(got[..., 1] - 1).max() < 1e-3 and (got[..., 2:] == 0).all()
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,past,new", [(4, 900, 1), (4, 700, 30), (64, 300, 60), (32, 4000, 150), (32, 0, 700)])
+def test_scores_that_rise_and_fall(dev, act, cache, H, past, new):
+    """Scores that rise and fall by far more than the weights' types hold, in runs
+    of some tiles and of single keys, with a dim for each run's values."""
+    say("rise and fall", act, cache, H, past, new)
+    D, n = 128, past + new
+    rng = seed(35, act, cache, H)
+    c = Case(dev, rng, act, cache, H, 2, D, 16, [past], [new], decode=new == 1)
+    k, v = (a.copy() for a in c.pool.get(0, n))
+    run = np.arange(n) // 90
+    k[:, :, 0] = np.array([0, 60, -10, 150, 40, 149, -30, 100])[run % 8][:, None]
+    k[::37, :, 0] += 7
+    c.q[:, ::D] = 1.0
+    v[np.arange(n), :, run % 8] += 2.0
+    c.pool.put(0, np.arange(n), k, v)
+    for scale in (1.0, 0.125):
+        c.upload()
+        c.run(scale)
+        c.check(scale=scale)
