@@ -22,8 +22,8 @@
 //     operand of all VW tiles, put together by byte permutes.
 // f32 activations: q and p are split into parts of the cache's type (2 of f16,
 // 3 of bf16), which keeps products and sums at f32's precision.  f16 parts
-// take q scaled by a power of two per row (exact) so that no part leaves f16's
-// range.  16-bit activations: q as it is, p in two parts; their products cost
+// take q scaled by a power of two per row (exact), its largest to 2^14 .. 2^15:
+// no part leaves f16's range, and a small dim keeps steps of 2^-39 of the largest.  16-bit activations: q as it is, p in two parts; their products cost
 // nothing here, where K and V bytes are the bound, and one part would add a
 // rounding as large as the output's own.
 // p carries a factor 2^PA_SHIFT, which l carries too: f16 parts of small p keep
@@ -103,7 +103,7 @@ struct Rows16 {
             a = fmaxf(a, __shfl_xor(a, 16));
             a = fmaxf(a, __shfl_xor(a, 32));
             // (a row with an infinite value keeps it; its scores are no numbers anyway)
-            const int ex = a > 0.0f && a < __builtin_inff() ? min(120, max(-120, __builtin_amdgcn_frexp_expf(a))) : 0;
+            const int ex = a > 0.0f && a < __builtin_inff() ? max(-100, __builtin_amdgcn_frexp_expf(a) - 15) : 0;
 #pragma unroll
             for (int t = 0; t < KS; t++)
 #pragma unroll

@@ -260,13 +260,13 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
 #pragma unroll
                 for (int e = 0; e < 8; e++) f[t][e] = scale < 0.0f ? -raw[e] : raw[e];
             }
-            if constexpr (std::is_same<E, _Float16>::value) {  // (parts of f16: scaled into its range)
+            if constexpr (std::is_same<E, _Float16>::value) {  // (parts of f16: scaled to the top of its range)
 #pragma unroll
                 for (int t = 0; t < X::KS; t++)
 #pragma unroll
                     for (int e = 0; e < 8; e++) a = fmaxf(a, fabsf(f[t][e]));
                 a = fmaxf(a, pf_other_half(a));
-                const int ex = a > 0.0f && a < __builtin_inff() ? min(120, max(-120, __builtin_amdgcn_frexp_expf(a))) : 0;
+                const int ex = a > 0.0f && a < __builtin_inff() ? max(-100, __builtin_amdgcn_frexp_expf(a) - 15) : 0;
 #pragma unroll
                 for (int t = 0; t < X::KS; t++)
 #pragma unroll

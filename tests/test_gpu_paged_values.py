@@ -202,3 +202,21 @@ def test_scores_that_rise_and_fall(dev, act, cache, H, past, new):
         c.upload()
         c.run(scale)
         c.check(scale=scale)
+
+
+@pytest.mark.parametrize("cache", [F16, BF16])
+@pytest.mark.parametrize("H,past,new", [(4, 900, 1), (4, 700, 30), (64, 300, 60), (20, 0, 700), (32, 4000, 150)])
+def test_f32_rows_keep_small_dims(dev, cache, H, past, new):
+    """A dim of q of 2^20 that no key has: the scores are those of the other dims.
+    The parts of these, in steps of 2^-40 of 2^20 .. 2^21, add 2^-20 |k| a dim at
+    most, some 2^-17 in all: less than the bound's (D + 9) A u, A near 9 here."""
+    say("f32 small dims", cache, H, past, new)
+    D = 128
+    c = Case(dev, seed(36, cache, H), F32, cache, H, 4, D, 16, [past], [new], decode=new == 1)
+    k, v = (a.copy() for a in c.pool.get(0, past + new))
+    k[:, :, 3] = 0
+    c.pool.put(0, np.arange(past + new), k, v)
+    c.q[:, 3::D] = 2.0 ** 20 * 1.375
+    c.upload()
+    c.run()
+    c.check()
