@@ -126,8 +126,7 @@ struct Rows16 {
     __device__ void start() {
 #pragma unroll
         for (int t = 0; t < VW; t++) o[t] = pg_f4{0.f, 0.f, 0.f, 0.f};
-        // (a finite floor: a row that has seen nothing yet keeps m = -1e30, l = 0, o = 0)
-        m = peak = -1e30f;
+        m = peak = PG_LEAST;
         l = 0.0f;
     }
 
@@ -245,7 +244,7 @@ struct Rows16 {
         pg_f4 y[VW];
         const int d0 = 4 * VW * ((threadIdx.x & 63) >> 4);
         pg_plain<E, T, HD, 4>(
-            c, table, head, x, scale, limit, j0, j1, PA_SHIFT, -1e30f, [](int) { return true; },
+            c, table, head, x, scale, limit, j0, j1, PA_SHIFT, [](int) { return true; },
             [&](int i) { return d0 + 4 * i; }, m, l, y);
 #pragma unroll
         for (int t = 0; t < VW; t++)
@@ -543,7 +542,7 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
     const int d = threadIdx.x % TH, x = threadIdx.x / TH, p = (unsigned)x / (unsigned)rows, r = r0 + x - p * rows;
     const float* row = part + r * HD + 4 * d;
     const float* stat = part + tile_rows * HD + r;
-    float M = -1e30f, L = 0.0f;
+    float M = PG_LEAST, L = 0.0f;
     pg_f4 O = pg_f4{0.f, 0.f, 0.f, 0.f};
     if (p < groups) {
         for (int w = w0 + p; w <= j.last; w += groups * PJ_STEP) {
@@ -580,7 +579,7 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
     }
     __syncthreads();
     if (p) return;
-    float mx = -1e30f;
+    float mx = PG_LEAST;
     for (int i = 0; i < groups; i++) mx = fmaxf(mx, s_m[i * rows + x]);
     L = 0.0f;
     O = pg_f4{0.f, 0.f, 0.f, 0.f};

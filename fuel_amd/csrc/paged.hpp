@@ -159,6 +159,10 @@ __host__ __device__ __forceinline__ int pg_page(const PagedKv& c, const int* tab
     return none ? 0 : id;
 }
 
+// Maximum of no scores: below every finite one, and finite itself, so that a row
+// that has seen nothing keeps weights, sums and factors that are numbers.
+constexpr float PG_LEAST = -__FLT_MAX__;
+
 // f16 parts hold weights in steps of 2^-24.  Where keys have weights far below the
 // largest so far, the score that stands for the weight 1 follows theirs down, so
 // that those weights keep their digits too, by up to 2^PG_DROP: the sums stay in
@@ -187,8 +191,8 @@ __device__ __forceinline__ bool pg_odd(const V (&o)[N]) {
 // are RUNS runs of 4, run i from dim(i) on.  x: the row's q.
 template <class E, class T, int HD, int SHARE, int RUNS, class Mine, class Dim>
 __device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int head, const T* x, float scale,
-                                         int limit, int j0, int j1, float shift, float floor, Mine mine, Dim dim,
-                                         float& m, float& l, pg_f4 (&o)[RUNS]) {
+                                         int limit, int j0, int j1, float shift, Mine mine, Dim dim, float& m,
+                                         float& l, pg_f4 (&o)[RUNS]) {
     const auto row = [&](const void* pool, int j, bool& none) {
         const int page = pg_page(c, table, j, j + 1, none);
         return static_cast<const E*>(pool) +
@@ -211,7 +215,7 @@ __device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int
         for (int d = 64 / SHARE; d < 64; d *= 2) s += __shfl_xor(s, d);
         return none ? pg_nan() : s * (scale * 1.4426950408889634f);
     };
-    m = floor;
+    m = PG_LEAST;
 #pragma unroll 1
     for (int j = j0; j < j1; j++) {
         if (!mine(j)) continue;

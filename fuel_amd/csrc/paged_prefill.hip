@@ -191,7 +191,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         for (int d = 0; d < X::DT; d++)
 #pragma unroll
             for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-        float m = -1e30f, l = 0.0f, peak = m;  // peak: the largest score so far
+        float m = PG_LEAST, l = 0.0f, peak = m;  // peak: the largest score so far
 
         // DMA: instruction i of this wavefront takes rows ((i PF_WAVES + wave) RPI) .. of
         // a tile, all in one group of 16 keys.  Source offsets of the lane within it:
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
             pg_f4 y[4 * X::DT];
             pg_plain<E, T, HD, 2>(
                 c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, t0 * PF_KEYS,
-                min(tiles * PF_KEYS, last + 1), X::SHIFT, -1e30f,
+                min(tiles * PF_KEYS, last + 1), X::SHIFT,
                 [&](int j) { return KW == 1 || (j & 32) == key0; }, [&](int i) { return 8 * i + 4 * h; }, m, l, y);
 #pragma unroll
             for (int d = 0; d < X::DT; d++)

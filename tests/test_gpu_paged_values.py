@@ -220,3 +220,38 @@ def test_f32_rows_keep_small_dims(dev, cache, H, past, new):
     c.upload()
     c.run()
     c.check()
+
+
+@pytest.mark.parametrize("act,cache", [(F32, F16), (F32, BF16), (BF16, BF16)])
+@pytest.mark.parametrize("H,hk,D,past,new", [(4, 2, 128, [0, 4, 39, 1300], [1] * 4), (8, 2, 64, [0, 12], [7, 3]),
+                                             (64, 4, 128, [0, 3], [60, 70]), (64, 2, 64, [0, 0], [150, 290]),
+                                             (32, 2, 128, [3000], [140])])
+def test_scores_far_below_zero(dev, act, cache, H, hk, D, past, new):
+    """Scores of some -1e32 and lower: a row's weights are 1 for its largest and 0
+    for the others, whose distances are far above 1.  f32 scores err by (D + 9) u A
+    at most (paged_ref.py), A the largest of the row's, so that where its two largest
+    are within twice that they may come out in either order: a few rows, of which one
+    was seen (two scores 2.9e-8 A apart, u is 6e-8).  These only have to be finite."""
+    say("far below zero", act, cache, H, D, past)
+    rng = seed(37, act, cache, H)
+    c = Case(dev, rng, act, cache, H, hk, D, 16, past, new, decode=new[0] == 1)
+    for s, n in enumerate(c.kv):
+        k, v = c.pool.get(s, int(n))
+        c.pool.put(s, np.arange(n), np.abs(k) + 0.25, v)
+    c.q = -(np.abs(c.q) + 0.25) * np.float32(1e32)
+    c.upload()
+    c.run()
+    for s, n in enumerate(c.kv):
+        q, pos = rows_of(c, s)
+        k, v = c.pool.get(s, int(n))
+        want, A = R.attend(q, k, v, pos, c.scale)[:2]
+        tol = np.abs(want) * (16 * R.U + (0 if act == F32 else R.HALF[act]))
+        undecided = 0
+        for h in range(H):
+            x = np.where(np.arange(n)[None] <= pos[:, None], q[:, h].astype(float) @ k[:, h * hk // H].T.astype(float), -np.inf)
+            x = np.sort(x * c.scale, 1)
+            near = x[:, -1] - (x[:, -2] if n > 1 else -np.inf) < 2 * (D + 9) * R.U * A[:, h, 0]
+            undecided += int(near.sum())
+            tol[near, h] = 2 * np.abs(v).max()
+        assert undecided <= max(1, q.shape[0] * H // 500)
+        compare(got_of(c, s), want, tol)
