@@ -26,8 +26,8 @@
 // no part leaves f16's range, and a small dim keeps steps of 2^-39 of the largest.  16-bit activations: q as it is, p in two parts; their products cost
 // nothing here, where K and V bytes are the bound, and one part would add a
 // rounding as large as the output's own.
-// p carries a factor 2^PA_SHIFT, which l carries too: f16 parts of small p keep
-// steps of 2^-24 / 2^15 of the largest p of 32 keys (2^15 < f16's largest, 65504).
+// p carries a factor 2^TOP, which l carries too: f16 parts of small p keep steps
+// of 2^-24 / 2^15 of the largest p of 32 keys.
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
@@ -39,7 +39,6 @@ namespace frq {
 namespace {
 
 constexpr int PA_WAVES = 4;
-constexpr float PA_SHIFT = 15.0f;
 
 // The largest of the four lanes 16 g + r of a row, in all four.
 __device__ __forceinline__ float pg_row_max(float v) {
@@ -198,7 +197,7 @@ struct Rows16 {
         l *= c;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - mn + PA_SHIFT);
+            s[i] = __builtin_amdgcn_exp2f(s[i] - mn + P::TOP);
             l += s[i];
             float rest = s[i];
 #pragma unroll
@@ -244,7 +243,7 @@ struct Rows16 {
         pg_f4 y[VW];
         const int d0 = 4 * VW * ((threadIdx.x & 63) >> 4);
         pg_plain<E, T, HD, 4>(
-            c, table, head, x, scale, limit, j0, j1, PA_SHIFT, [](int) { return true; },
+            c, table, head, x, scale, limit, j0, j1, P::TOP, [](int) { return true; },
             [&](int i) { return d0 + 4 * i; }, m, l, y);
 #pragma unroll
         for (int t = 0; t < VW; t++)

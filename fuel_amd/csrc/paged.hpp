@@ -114,6 +114,9 @@ struct PgElem<_Float16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int SPLIT = 2;  // parts that hold an f32 to 2^-22
+    // Weights are 2^TOP at most: here as many of their digits as f16's range holds
+    // (its largest is 65504).
+    static constexpr float TOP = 15.0f;
     __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -123,6 +126,8 @@ struct PgElem<__bf16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int SPLIT = 3;  // 8 significant bits each: an f32 to 2^-24
+    // 2^30 keys' weights times values up to f32's largest sum within f32's range.
+    static constexpr float TOP = -31.0f;
     __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }

@@ -15,8 +15,8 @@
 // source addresses permute the 16-byte chunks of a row instead, so that the
 // rows one read touches fall in different banks.
 // The running maximum is renewed only when a row's scores pass it by LAZY: the
-// weights stay below 2^(SHIFT + LAZY) = 2^15, in f16's range, and the sums and the
-// output share the factor whatever it is.  Of f16 parts it is also lowered where a
+// weights stay below 2^(SHIFT + LAZY) = 2^TOP, and the sums and the output share
+// the factor whatever it is.  Of f16 parts it is also lowered where a
 // tile's scores stay below it by PF_LOW (PG_DROP); tiles of 64 such rows of q and
 // keys, N(0, 1), differ by less.
 // 16-bit activations: p is rounded to the cache's type for the second product
@@ -89,7 +89,7 @@ struct PrefillTile {
     static constexpr int NP = WIDE ? P::SPLIT : 1;
     static constexpr bool F16 = std::is_same<E, _Float16>::value;
     // (f16 parts of an f32 weight: as many of its digits as f16's range holds)
-    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = 15.0f - LAZY;
+    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = P::TOP - LAZY;
     static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
     static constexpr int RPI = 512 / HD, NI = TILE / 1024;  // rows a DMA instruction, instructions a tile

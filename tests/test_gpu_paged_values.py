@@ -255,3 +255,22 @@ def test_scores_far_below_zero(dev, act, cache, H, hk, D, past, new):
             tol[near, h] = 2 * np.abs(v).max()
         assert undecided <= max(1, q.shape[0] * H // 500)
         compare(got_of(c, s), want, tol)
+
+
+@pytest.mark.parametrize("act", [F32, BF16])
+@pytest.mark.parametrize("H,hk,D,past,new", [(4, 2, 128, [0, 4, 39, 2300], [1] * 4), (8, 2, 64, [0, 12], [7, 3]),
+                                             (64, 4, 128, [0, 3], [60, 70]), (64, 2, 64, [0, 0], [150, 290]),
+                                             (20, 20, 128, [0, 0, 70], [200, 260, 130]), (32, 2, 128, [3000], [140])])
+def test_values_at_the_end_of_the_range(dev, act, H, hk, D, past, new):
+    """Values up to bf16's largest: their weighted mean is a number."""
+    say("large values", act, H, D, past)
+    rng = seed(38, act, H)
+    c = Case(dev, rng, act, BF16, H, hk, D, 16, past, new, decode=new[0] == 1)
+    for s, n in enumerate(c.kv):
+        k, v = c.pool.get(s, int(n))
+        c.pool.put(s, np.arange(n), k, rng.uniform(-3.3e38, 3.3e38, v.shape) * (np.arange(D) % 2 == 0) + v)
+    c.upload()
+    c.run()
+    for scale in (c.scale, 0.0):
+        c.run(scale)
+        c.check(scale=scale)
