@@ -360,7 +360,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const auto units_of = [&](const PgSeq& x) { return pd_tiles(x, grp) * pd_units(x, unit); };
-    PgUnits<decltype(units_of)> pu(b, units_of, c.kv_heads, !b.row_start && b.cap <= unit ? (grp + 15) >> 4 : 0);
+    PgUnits<decltype(units_of)> pu(b, units_of, !b.row_start && b.cap <= unit ? (grp + 15) >> 4 : 0);
     const int units = pu.total, total = units * c.kv_heads, n_wgs = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= n_wgs) {
         if (joins && threadIdx.x == 0) joins[blockIdx.x].rows = 0;
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(Pa
     const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
     const int at = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * PA_WAVES + (threadIdx.x >> 6)));
     const auto tiles_of = [&](const PgSeq& x) { return pd_tiles(x, grp); };
-    PgUnits<decltype(tiles_of)> pu(b, tiles_of, c.kv_heads, each);
+    PgUnits<decltype(tiles_of)> pu(b, tiles_of, each);
     if (at >= pu.total * c.kv_heads) return;
     const int head = (unsigned)at / (unsigned)pu.total;
     int tile;

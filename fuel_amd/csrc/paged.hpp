@@ -269,9 +269,9 @@ __device__ __forceinline__ int pg_scan(int v) {
 // sequences [l share, (l + 1) share), whose loads do not wait for each other;
 // a lookup then loads one share: two memory round trips for any n_seqs <= 4096.
 // each: every sequence has so many units (0: not known), and none is loaded
-// before the lookup.  A batch has no units if those of all heads are more than
-// 0x7fffffff, which the host refuses for rows that lie in one sequence each:
-// row_start lists rows over and over.
+// before the lookup.  A batch whose sequences have more rows together than it has
+// (row_start lists rows over and over) has no units: its tiles can be more than
+// pg_tiles_bound(), and a grid of that would drop some, of any sequence.
 template <class F>
 struct PgUnits {
     const PagedRows& b;
@@ -286,7 +286,7 @@ struct PgUnits {
         if (s < b.n_seqs) own = pg_seq(b, s);
     }
     __device__ __forceinline__ int mine() const { return s0 + (int)(threadIdx.x & 63) < b.n_seqs ? units(own) : 0; }
-    __device__ __forceinline__ PgUnits(const PagedRows& rows, F f, int heads, int each_ = 0)
+    __device__ __forceinline__ PgUnits(const PagedRows& rows, F f, int each_ = 0)
         : b(rows), units(f), each(each_) {
         share = (b.n_seqs + 63) >> 6;
         if (each) {
@@ -294,19 +294,24 @@ struct PgUnits {
             total = b.n_seqs * each;
             return;
         }
-        int v = 0;
+        int v = 0, n = 0;
         if (share == 1) {
             load(0);
             v = mine();
+            n = own.n;
         } else {
             s0 = -64;
             const int from = share * (int)(threadIdx.x & 63), to = min(b.n_seqs, from + share);
 #pragma unroll 4
-            for (int s = from; s < to; s++) v = pg_add(v, units(pg_seq(b, s)));
+            for (int s = from; s < to; s++) {
+                const PgSeq q = pg_seq(b, s);
+                v = pg_add(v, units(q));
+                n = pg_add(n, q.n);
+            }
         }
         sum = pg_scan(v);
         total = __builtin_amdgcn_readlane(sum, 63);
-        if (total == 0x7fffffff || (long)total * heads > 0x7fffffff) total = 0;
+        if (b.row_start && __builtin_amdgcn_readlane(pg_scan(n), 63) > b.rows) total = 0;
     }
     // The sequence that holds unit at < total, and the unit's number in it.
     __device__ __forceinline__ int find(int at, int& in_seq) {
@@ -346,7 +351,7 @@ struct PgUnits {
 // starts at unit w * total / n_wgs, none is empty; and the one that holds unit u.
 __host__ __device__ __forceinline__ int pg_start(int w, int total, int n_wgs) {
     if (n_wgs == total) return w;
-    // (in 32 bits: n_wgs is below 2^16 here)
+    // (in 32 bits: n_wgs is at most PG_WGS here)
     const unsigned q = (unsigned)total / (unsigned)n_wgs, rest = (unsigned)total % (unsigned)n_wgs;
     return w * (int)q + (int)((unsigned)w * rest / (unsigned)n_wgs);
 }

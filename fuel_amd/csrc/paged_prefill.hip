@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         const int row_tiles = (int)(((long)x.n * grp + ROWS - 1) / ROWS);
         return CUT ? row_tiles * key_tiles(x) : row_tiles;
     };
-    PgUnits<decltype(units)> pu(b, units, c.kv_heads);
+    PgUnits<decltype(units)> pu(b, units);
     int head, s, u;                       // KV head, sequence, unit of the sequence
     int at = 0, begin = 0, stop = 0, total = 0, n_wgs = 0, wg = 0;  // CUT: the range, and whose it is
     if constexpr (CUT) {

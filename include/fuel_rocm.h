@@ -366,7 +366,8 @@ typedef struct frq_paged_kv {
  *   row_start[s] .. row_start[s + 1] no range within [0, rows]: the sequence
  *     has no rows
  *   row_start that decreases, so that rows are in several sequences: such rows
- *     hold the result of one of them, or what they held
+ *     hold the result of one of them, or what they held; where the sequences
+ *     have more than `rows` rows together, an attention call writes no row at all
  *   rows before row_start[0] or from row_start[n_seqs] on: left as they were
  * Cache rows beyond a sequence's length, and keys a row does not see, may hold
  * anything (NaN included) without effect on it; infinite and NaN values that it
