@@ -143,6 +143,8 @@ def work(case):
 # ---- inputs ----
 
 def prepare(case, seed):
+    if own:
+        _one_stream()
     g = torch.Generator("cuda").manual_seed(seed)
     rng = random.Random(seed)
     rows, kv = _lengths(case)
@@ -188,16 +190,28 @@ def prepare(case, seed):
 
 # ---- the package's operators ----
 
-_device = None
+_device = _stream = None
+
+
+def _one_stream():
+    """torch's work and the package's on one stream, so that each waits for what
+    the other did before: the device adopts a stream of torch's, which becomes the
+    current one (torch's default stream has no handle to adopt)."""
+    import fuel_amd as F
+
+    global _device, _stream
+    if _device is None:
+        _device, _stream = F.RocmDevice(0), torch.cuda.Stream()
+        _device.set_stream(_stream.cuda_stream)
+    if torch.cuda.current_stream() != _stream:
+        _stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(_stream)
 
 
 def _handle(state):
     """The cache, the batch and the workspace a serving program keeps."""
     import fuel_amd as F
 
-    global _device
-    if _device is None:
-        _device = F.RocmDevice(0)
     case = state["case"]
     code = {"f32": F.F32, "f16": F.F16, "bf16": F.BF16}
     n_pages = state["k_pages"].shape[0]
@@ -207,8 +221,6 @@ def _handle(state):
                          state["table"].shape[1], state["q"].shape[0],
                          row_start=None if case["kind"] == "decode" else state["start"].data_ptr(),
                          max_kv_len=state["max_kv_len"])
-    # the rows of the pages that prepare() filled are there before the device's own stream reads them
-    torch.cuda.synchronize()
     work = None
     if case["kind"] != "append":
         work = _device.alloc((max(1, F.paged_attention_workspace(cache, batch, case["heads"])),), "uint8")
