@@ -291,7 +291,14 @@ def _ptr(x) -> int:
     """Device address of a RocmStorage, or the address itself (None: null)."""
     if type(x) is int:
         return x
-    return x.ptr if isinstance(x, RocmStorage) else int(x or 0)
+    if isinstance(x, RocmStorage):
+        return x.ptr
+    if x is None:
+        return 0
+    if isinstance(x, np.integer):
+        return int(x)
+    # (a tensor or an array would pass its value, not its address)
+    raise FuelRocmError(N.FRQ_INVALID, f"expected a RocmStorage or a device address, got {type(x).__name__}")
 
 
 class PagedKvCache:
