@@ -356,24 +356,29 @@ def paged_attention_workspace(cache: PagedKvCache, batch: PagedBatch, n_heads: i
     return int(lib().frq_paged_attention_workspace(cache.ref, batch.ref, n_heads))
 
 
-def _paged_attention(fn, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo) -> None:
+def _paged_attention(fn, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo, work_bytes) -> None:
     wide = n_heads * cache.head_dim
-    check(fn(cache.dev.handle, cache.ref, batch.ref, dtype, n_heads, _ptr(q), ldq or wide, scale,
-             work.ptr if work is not None else None, work.nbytes if work is not None else 0, _ptr(out), ldo or wide))
+    if isinstance(work, RocmStorage):
+        work_bytes = work.nbytes
+    check(fn(cache.dev.handle, cache.ref, batch.ref, dtype, n_heads, _ptr(q), ldq or wide, scale, _ptr(work),
+             work_bytes, _ptr(out), ldo or wide))
 
 
 def paged_attention_decode(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
-                           work: RocmStorage | None = None, ldq: int = 0, ldo: int = 0) -> None:
+                           work=None, ldq: int = 0, ldo: int = 0, work_bytes: int = 0) -> None:
     """Attention of one new token per sequence over its cached rows
-    (frq_paged_attention_decode); work: paged_attention_workspace() bytes."""
-    _paged_attention(lib().frq_paged_attention_decode, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo)
+    (frq_paged_attention_decode); work: paged_attention_workspace() bytes, a
+    storage, or an address of work_bytes bytes."""
+    _paged_attention(lib().frq_paged_attention_decode, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo,
+                     work_bytes)
 
 
 def paged_attention_prefill(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
-                            work: RocmStorage | None = None, ldq: int = 0, ldo: int = 0) -> None:
+                            work=None, ldq: int = 0, ldo: int = 0, work_bytes: int = 0) -> None:
     """Causal attention of packed prompt rows over the cache
-    (frq_paged_attention_prefill); work: paged_attention_workspace() bytes."""
-    _paged_attention(lib().frq_paged_attention_prefill, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo)
+    (frq_paged_attention_prefill); work as paged_attention_decode()'s."""
+    _paged_attention(lib().frq_paged_attention_prefill, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo,
+                     work_bytes)
 
 
 # ---- synthetic inputs ----

@@ -58,3 +58,17 @@ def test_addresses_reach_the_library():
     cache, one = F.PagedKvCache(DEV, 9, 16, 2, 128, F.F16, np.int64(P), P), F.PagedBatch(P, np.uint64(P), 3, 4)
     assert cache.struct.k == P and one.struct.kv_len == P and one.struct.row_start is None
     assert "null device handle" in refused(F.paged_append, cache, one, F.F16, 4, P, P, P, P)
+
+
+def test_workspace_is_a_storage_or_an_address_of_so_many_bytes():
+    cache, one = F.PagedKvCache(DEV, 9, 16, 2, 128, F.F16, P, P), F.PagedBatch(P, P, 3, 1 << 16)
+    need = F.paged_attention_workspace(cache, one, 4)
+    assert need > 0
+    for fn in (F.paged_attention_decode, F.paged_attention_prefill):
+        args = (cache, one, F.F16, 4, P, P, 0.1)
+        for work in (None, P, storage(need - 1, np.uint8)):
+            assert "workspace" in refused(fn, *args, work)
+        assert "workspace" in refused(fn, *args, P, work_bytes=need - 1)
+        refused(fn, *args, np.zeros(need, np.uint8), work_bytes=need)
+        assert "null device handle" in refused(fn, *args, P, work_bytes=need)
+        assert "null device handle" in refused(fn, *args, storage(need, np.uint8))
