@@ -301,6 +301,21 @@ def _ptr(x) -> int:
     raise FuelRocmError(N.FRQ_INVALID, f"expected a RocmStorage or a device address, got {type(x).__name__}")
 
 
+def _paged_operand(name: str, x, dev, nbytes: int, dtype=None) -> int:
+    """Address of an operand.  A storage knows more than its address: it has to be
+    on the call's device, hold nbytes and, where one is given, be of that dtype."""
+    if type(x) is int:
+        return x
+    if isinstance(x, RocmStorage):
+        if dev is not None and x.dev is not dev and x.dev.ordinal != dev.ordinal:
+            raise FuelRocmError(N.FRQ_INVALID, f"{name}: on device {x.dev.ordinal}, the others on {dev.ordinal}")
+        if x.nbytes < nbytes:
+            raise FuelRocmError(N.FRQ_INVALID, f"{name}: {x.nbytes} bytes, the call reaches {nbytes}")
+        if dtype is not None and x.dtype != dtype:
+            raise FuelRocmError(N.FRQ_INVALID, f"{name}: {x.dtype}, expected {np.dtype(dtype)}")
+    return _ptr(x)
+
+
 class PagedKvCache:
     """Pools of KV pages [n_pages, n_kv_heads, page_size, head_dim] that a batch
     of sequences shares (frq_paged_kv).  dtype: F16 or BF16.  k, v: device
@@ -320,7 +335,9 @@ class PagedKvCache:
             for s in (k, v):
                 check(lib().frq_memset(dev.handle, C.c_void_p(s.ptr), 0, s.nbytes))
         self.k, self.v = k, v
-        self.struct = N.PagedKv(dtype, n_pages, page_size, n_kv_heads, head_dim, _ptr(k), _ptr(v))
+        pool = n_pages * n_kv_heads * page_size * head_dim * 2
+        self.struct = N.PagedKv(dtype, n_pages, page_size, n_kv_heads, head_dim, _paged_operand("k", k, dev, pool),
+                                _paged_operand("v", v, dev, pool))
         self.ref = C.byref(self.struct)
 
 
@@ -334,9 +351,27 @@ class PagedBatch:
         self.n_seqs, self.max_pages, self.max_kv_len = n_seqs, max_pages, max_kv_len
         self.rows = n_seqs if rows is None else rows
         self.page_table, self.kv_len, self.row_start = page_table, kv_len, row_start
-        self.struct = N.PagedBatch(n_seqs, max_pages, self.rows, max_kv_len, _ptr(page_table), _ptr(kv_len),
-                                   _ptr(row_start))
+        # the storages' device (None: addresses only)
+        self.dev = next((x.dev for x in (page_table, kv_len, row_start) if isinstance(x, RocmStorage)), None)
+        self.struct = N.PagedBatch(n_seqs, max_pages, self.rows, max_kv_len,
+                                   _paged_operand("page_table", page_table, self.dev, 4 * n_seqs * max_pages, np.int32),
+                                   _paged_operand("kv_len", kv_len, self.dev, 4 * n_seqs, np.int32),
+                                   _paged_operand("row_start", row_start, self.dev, 4 * (n_seqs + 1), np.int32))
         self.ref = C.byref(self.struct)
+
+
+def _paged_handle(cache: PagedKvCache, batch: PagedBatch):
+    """The handle of the device that a call runs on."""
+    dev = cache.dev
+    if batch.dev is not None and batch.dev is not dev and batch.dev.ordinal != dev.ordinal:
+        raise FuelRocmError(N.FRQ_INVALID, f"batch on device {batch.dev.ordinal}, the cache on {dev.ordinal}")
+    return dev.handle
+
+
+def _paged_rows(name: str, x, cache: PagedKvCache, batch: PagedBatch, dtype: int, width: int, ld: int) -> int:
+    """Address of `batch.rows` rows of `width` elements, ld apart."""
+    size = 4 if dtype == N.F32 else 2
+    return _paged_operand(name, x, cache.dev, ((batch.rows - 1) * ld + width) * size if batch.rows else 0)
 
 
 def paged_append(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, k, v, q_out, ldq: int = 0,
@@ -346,9 +381,17 @@ def paged_append(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: in
     storages or device addresses; a leading dimension of 0 stands for packed
     rows; rope_cos / rope_sin are [rope_rows, head_dim] f32 tables."""
     wide, narrow = n_heads * cache.head_dim, cache.n_kv_heads * cache.head_dim
-    check(lib().frq_paged_append(cache.dev.handle, cache.ref, batch.ref, dtype, n_heads, _ptr(q), ldq or wide, _ptr(k),
-                                 ldk or narrow, _ptr(v), ldv or narrow, _ptr(rope_cos), _ptr(rope_sin), rope_rows,
-                                 _ptr(q_out), ldqo or wide))
+    ldq, ldk, ldv, ldqo = ldq or wide, ldk or narrow, ldv or narrow, ldqo or wide
+    table = 4 * rope_rows * cache.head_dim
+    handle = _paged_handle(cache, batch)
+    check(lib().frq_paged_append(
+        handle, cache.ref, batch.ref, dtype, n_heads,
+        q if type(q) is int else _paged_rows("q", q, cache, batch, dtype, wide, ldq), ldq,
+        k if type(k) is int else _paged_rows("k", k, cache, batch, dtype, narrow, ldk), ldk,
+        v if type(v) is int else _paged_rows("v", v, cache, batch, dtype, narrow, ldv), ldv,
+        rope_cos if type(rope_cos) is int else _paged_operand("rope_cos", rope_cos, cache.dev, table, np.float32),
+        rope_sin if type(rope_sin) is int else _paged_operand("rope_sin", rope_sin, cache.dev, table, np.float32),
+        rope_rows, q_out if type(q_out) is int else _paged_rows("q_out", q_out, cache, batch, dtype, wide, ldqo), ldqo))
 
 
 def paged_attention_workspace(cache: PagedKvCache, batch: PagedBatch, n_heads: int) -> int:
@@ -358,10 +401,14 @@ def paged_attention_workspace(cache: PagedKvCache, batch: PagedBatch, n_heads: i
 
 def _paged_attention(fn, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo, work_bytes) -> None:
     wide = n_heads * cache.head_dim
+    ldq, ldo = ldq or wide, ldo or wide
     if isinstance(work, RocmStorage):
         work_bytes = work.nbytes
-    check(fn(cache.dev.handle, cache.ref, batch.ref, dtype, n_heads, _ptr(q), ldq or wide, scale, _ptr(work),
-             work_bytes, _ptr(out), ldo or wide))
+    handle = _paged_handle(cache, batch)
+    check(fn(handle, cache.ref, batch.ref, dtype, n_heads,
+             q if type(q) is int else _paged_rows("q", q, cache, batch, dtype, wide, ldq), ldq, scale,
+             _paged_operand("work", work, cache.dev, 0), work_bytes,
+             out if type(out) is int else _paged_rows("out", out, cache, batch, dtype, wide, ldo), ldo))
 
 
 def paged_attention_decode(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
