@@ -1527,6 +1527,8 @@ int frq_paged_append(frq_device* dev, const frq_paged_kv* kv, const frq_paged_ba
     const bool none = b->n_seqs == 0 || b->rows == 0;
     if (!none && (rc = paged_buffers(who, kv, b))) return rc;
     if (!q != !q_out) return fail(FRQ_INVALID, "%s: q and q_out go together", who);
+    if (q && q == q_out && ldq != ldqo)  // (rows would be written over before they are read)
+        return fail(FRQ_INVALID, "%s: in place with rows %zu and %zu apart", who, ldq, ldqo);
     if (!rope_cos != !rope_sin) return fail(FRQ_INVALID, "%s: rope_cos and rope_sin go together", who);
     if (rope_cos && (rope_rows == 0 || rope_rows > 0x7fffffff))
         return fail(FRQ_INVALID, "%s: rope_rows=%zu", who, rope_rows);

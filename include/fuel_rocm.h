@@ -381,13 +381,13 @@ typedef struct frq_paged_batch {
  * head_dim] of type dtype, rows ldq, ldk, ldv elements apart (the three may be
  * parts of one projection's output).  q and k are rotated (rope_f32
  * rotate-half, byte_kernels.rs:1885-1964) by the rows `position` of the
- * [rope_rows, head_dim] tables; rotated q goes to q_out (which may be q), k and
- * v to their page.  f32 arithmetic, one rounding to q_out's or the cache's
- * type.  A position >= rope_rows: NaN in q_out, nothing appended.  rope_cos
- * and rope_sin NULL: no rotation.  q and q_out NULL: k and v only.  Two rows
- * must not name the same page and position.  dtype: FRQ_F32 or the cache's
- * type.  Pointers 16-byte aligned, rows a multiple of 16 bytes apart.
- * Asynchronous, allocates nothing. */
+ * [rope_rows, head_dim] tables; rotated q goes to q_out (q itself with ldqo =
+ * ldq, or memory apart from q, k and v), k and v to their page.  f32 arithmetic,
+ * one rounding to q_out's or the cache's type.  A position >= rope_rows: NaN in
+ * q_out, nothing appended.  rope_cos and rope_sin NULL: no rotation.  q and q_out
+ * NULL: k and v only.  Two rows must not name the same page and position.  dtype:
+ * FRQ_F32 or the cache's type.  Pointers 16-byte aligned, rows a multiple of 16
+ * bytes apart.  Asynchronous, allocates nothing. */
 int frq_paged_append(frq_device *dev, const frq_paged_kv *kv, const frq_paged_batch *batch, int dtype, size_t n_heads,
                      const void *q_dev, size_t ldq, const void *k_dev, size_t ldk, const void *v_dev, size_t ldv,
                      const float *rope_cos_dev, const float *rope_sin_dev, size_t rope_rows, void *q_out_dev,
