@@ -1489,8 +1489,9 @@ int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, co
     if (!paged_types(kv->dtype, dtype))
         return fail(FRQ_UNSUPPORTED, "%s: dtype %d over a cache of dtype %d", who, dtype, kv->dtype);
     const bool rows16 = pg_kind(a.kv, a.rows, (int)n_heads, (int)kv->head_dim) == PG_ROWS16;
-    if (rows16 && !paged_rows16_fits(a.kv, a.rows, (int)n_heads))
-        return fail(FRQ_UNSUPPORTED, "%s: n_seqs=%zu of up to %d tokens", who, b->n_seqs, a.rows.cap);
+    if (rows16 ? !paged_rows16_fits(a.kv, a.rows, (int)n_heads, (int)kv->head_dim)
+               : !paged_prefill_fits(a.kv, a.rows, (int)n_heads))
+        return fail(FRQ_UNSUPPORTED, "%s: rows=%zu n_seqs=%zu of up to %d tokens", who, b->rows, b->n_seqs, a.rows.cap);
     const bool none = b->n_seqs == 0 || b->rows == 0;
     const size_t need = frq_paged_attention_workspace(kv, b, n_heads);
     if (!none && work_bytes < need)
@@ -1524,6 +1525,7 @@ int frq_paged_append(frq_device* dev, const frq_paged_kv* kv, const frq_paged_ba
     if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
     if (!paged_types(kv->dtype, dtype))
         return fail(FRQ_UNSUPPORTED, "%s: dtype %d into a cache of dtype %d", who, dtype, kv->dtype);
+    if (b->rows > (size_t)PG_GRID) return fail(FRQ_UNSUPPORTED, "%s: rows=%zu (up to %ld)", who, b->rows, PG_GRID);
     const bool none = b->n_seqs == 0 || b->rows == 0;
     if (!none && (rc = paged_buffers(who, kv, b))) return rc;
     if (!q != !q_out) return fail(FRQ_INVALID, "%s: q and q_out go together", who);

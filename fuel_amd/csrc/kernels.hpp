@@ -291,8 +291,9 @@ struct PagedAttendArgs {
     void* work;
 };
 // Few rows a sequence: 16-row tiles, the keys over all workgroups, cut tiles
-// joined (work of paged_rows16_work_bytes()); fits: the units are an int.
-bool paged_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
+// joined (work of paged_rows16_work_bytes()); fits: the units are an int, the
+// workgroups a grid.
+bool paged_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
 size_t paged_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
 hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 // The pieces of cut tiles that wgs workgroups left (paged.hpp), up to `rows` rows
@@ -300,7 +301,8 @@ hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAtten
 hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, long tiles,
                              int tile_rows, int rows, int grp, void* out, int ldo, hipStream_t s);
 // paged_prefill.hip: many rows a sequence, 128-row tiles (work of
-// paged_prefill_work_bytes()).
+// paged_prefill_work_bytes()); fits: the workgroups are a grid.
+bool paged_prefill_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
 size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 

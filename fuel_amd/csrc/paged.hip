@@ -816,8 +816,10 @@ size_t paged_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_head
     return p.cut ? p.wgs * (2 * pg_slot(16, hd) * sizeof(float) + sizeof(PgJoin)) : 0;
 }
 
-bool paged_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {
-    return pg_tiles_bound(r, n_heads / kv.kv_heads, 16) * kv.kv_heads <= 0x7fffffff / (r.cap / PD_UNIT + 1);
+bool paged_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    if (pg_tiles_bound(r, n_heads / kv.kv_heads, 16) * kv.kv_heads > 0x7fffffff / (r.cap / PD_UNIT + 1)) return false;
+    const Rows16Plan p = rows16_plan(kv, r, n_heads, hd);
+    return p.wgs <= (p.alone ? PA_WAVES * PG_GRID : PG_GRID);
 }
 
 bool paged_types(int kv_dtype, int dtype) {

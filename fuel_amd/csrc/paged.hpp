@@ -89,6 +89,10 @@ inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int
 // resident at once.
 constexpr int PG_WGS = 512;
 
+// Workgroups of 256 threads that one launch can have: HIP's grids end below 2^32
+// threads.
+constexpr long PG_GRID = (1L << 24) - 1;
+
 // Cut tiles.  Workgroups that share the keys of a tile of `rows` query rows
 // leave slots of floats in the workspace, two a workgroup: o [rows][hd]
 // (unnormalized), m [rows], l [rows]; and each a record of what is to be joined.

@@ -501,6 +501,10 @@ struct PrefillCall {
 
 }  // namespace
 
+bool paged_prefill_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {
+    return pg_tiles_bound(r, n_heads / kv.kv_heads, PF_ROWS) * kv.kv_heads <= PG_GRID;
+}
+
 size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     if (pg_kind(kv, r, n_heads, hd) != PG_CUT) return 0;
     return PG_WGS * (2 * pg_slot(PF_ROWS, hd) * sizeof(float) + sizeof(PgJoin));
