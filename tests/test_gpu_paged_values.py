@@ -274,3 +274,21 @@ def test_values_at_the_end_of_the_range(dev, act, H, hk, D, past, new):
     for scale in (c.scale, 0.0):
         c.run(scale)
         c.check(scale=scale)
+
+
+# past the caches: one tile reads its keys alone, and they may be more than 256 MB
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,n,cap", [(4, 2, 128, 4, 65536), (4, 2, 64, 4, 131072),   # 16-row tiles, cut
+                                          (16, 8, 128, 256, 256), (8, 8, 64, 500, 256)])  # a wavefront each
+def test_decode_past_the_caches(dev, act, cache, H, hk, D, n, cap):
+    say("past the caches", act, cache, H, D, n, cap)
+    assert n * cap * hk * D * 4 > 256e6
+    rng = seed(39, act, cache, D, n)
+    kv = np.concatenate([[0, 1, 256, 17], rng.integers(1, 90, n - 4)]) if cap == 256 else np.array([3000, 0, 1234, 31])
+    c = Case(dev, rng, act, cache, H, hk, D, 16, [int(x) - 1 for x in kv], [1] * n, pad=8, decode=True, width=cap // 16,
+             max_kv_len=cap)
+    c.upload()
+    c.run()
+    got = c.check()
+    c.run()
+    np.testing.assert_array_equal(c.got(), got)
