@@ -236,19 +236,33 @@ struct Rows16 {
         }
     }
 
-    // The row's sums over keys [j0, j1) once more, where one is infinite or NaN.
-    // x: its q.
-    __device__ void mend(const PagedKv& c, const int* table, int head, const T* x, float scale, int j0, int j1) {
-        if (!__any(pg_odd(o))) return;
-        pg_f4 y[VW];
-        const int d0 = 4 * VW * ((threadIdx.x & 63) >> 4);
+    // Whether the block holds an infinite or NaN value, in any lane.
+    __device__ static bool odd(const KeyRegs& k, const ValueRegs& v) {
+        bool any = false;
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) any |= pg_word_odd<E>(k.w[a][t][w]);
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int w = 0; w < VW / 2; w++) any |= pg_word_odd<E>(v.w[i][w]);
+        return __any(any);
+    }
+
+    // Keys [j0, j1) by pg_plain(); x: the row's q.
+    __device__ void plain(const PagedKv& c, const int* table, int head, const T* x, float scale, int j0, int j1) {
+        const int g = (threadIdx.x & 63) >> 4;
         pg_plain<E, T, HD, 4>(
-            c, table, head, x, scale, limit, j0, j1, P::TOP, [](int) { return true; },
-            [&](int i) { return d0 + 4 * i; }, m, l, y);
-#pragma unroll
-        for (int t = 0; t < VW; t++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) o[t][k] = y[(VW * k + t) / 4][(VW * k + t) % 4];
+            c, table, head, x, scale, limit, j0, j1, P::TOP, g == 0, [&](int i) { return 4 * (VW * g + i); },
+            [&](int i, int e, float f, float p, float v) {
+                const int t = (4 * i + e) % VW, k = (4 * i + e) / VW;
+                o[t][k] = fmaf(p, v, o[t][k] * f);
+            },
+            m, l);
+        peak = fmaxf(peak, m);
     }
 
     // The row's sum over the four lanes that share it.
@@ -347,6 +361,45 @@ __device__ __forceinline__ void pd_walk(Rows16<E, T, HD>& a, const PagedKv& c, c
     }
 }
 
+// The same keys once more, if their sums hold an infinite or NaN value: blocks of
+// such values or of pages that are none one key after another.  64 sequences of up to
+// 8191, a call waited for: 85 us, with one infinite value 128, with one in every 16
+// keys 750, all NaN 280.
+template <class E, class T, int HD>
+__device__ __forceinline__ void pd_walk_odd(Rows16<E, T, HD>& a, const PagedKv& c, const int* table, int head, int j0,
+                                            int j1, int kv, const T* x, float scale) {
+    using A = Rows16<E, T, HD>;
+    if (!__any(pg_odd(a.o))) return;
+    a.start();
+#pragma unroll 1
+    for (int j = j0; j < j1; j += 32) {
+        typename A::Mask mk{j, kv, {}};
+        const E *ka[2], *va[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const size_t page = pg_page(c, table, j + 16 * i, kv, mk.bad[i]);
+            const size_t at = (((page * c.kv_heads + head) << c.log_ps) + ((j + 16 * i) & ((1 << c.log_ps) - 1))) * HD;
+            ka[i] = static_cast<const E*>(c.k) + at;
+            va[i] = static_cast<const E*>(c.v) + at;
+        }
+        typename A::KeyRegs kr;
+        typename A::ValueRegs vr;
+        A::template load_k<false>(kr, ka);
+        A::template load_v<false>(vr, va);
+        A::clear(vr, mk);
+        if (mk.bad[0] || mk.bad[1] || A::odd(kr, vr)) {
+            a.plain(c, table, head, x, scale, j, min(j + 32, j1));
+            if (__all(pg_all_nan(a.o))) return;
+            continue;
+        }
+        float s[8];
+        typename A::v8 pp[A::NP];
+        a.template scores<true>(kr, mk, s);
+        a.weights(s, pp);
+        a.product(vr, pp);
+    }
+}
+
 template <class E, class T, int HD, bool ONCE>
 __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv c, PagedRows b, int grp, int unit,
                                                                         const T* __restrict__ q, int ldq, float scale,
@@ -393,8 +446,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(PagedKv 
         const int* table = b.table + (size_t)s * b.max_pages;
         const int j0 = k0 + 32 * w * per, j1 = min(k1, j0 + 32 * per);
         pd_walk<E, T, HD, ONCE>(a, c, table, head, j0, j1, sq.kv, first);
+        pd_walk_odd(a, c, table, head, j0, j1, sq.kv, q + (size_t)row * ldq + (size_t)h * HD, scale);
         a.finish();
-        a.mend(c, table, head, q + (size_t)row * ldq + (size_t)h * HD, scale, j0, j1);
         if (w > 0) {
 #pragma unroll
             for (int t = 0; t < A::VW; t++)
@@ -492,8 +545,8 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(Pa
     const int* table = b.table + (size_t)s * b.max_pages;
     const int seen = pos0 + min(i0 + 15, all - 1) / grp + 1;  // keys that some row sees
     pd_walk<E, T, HD, ONCE>(a, c, table, head, 0, seen, sq.kv, pos0 + i0 / grp);
+    pd_walk_odd(a, c, table, head, 0, seen, sq.kv, q + (size_t)row * ldq + (size_t)h * HD, scale);
     a.finish();
-    a.mend(c, table, head, q + (size_t)row * ldq + (size_t)h * HD, scale, 0, seen);
     if (i0 + r >= all) return;
     const float inv = sq.bad ? pg_nan() : a.limit < 0 ? 0.0f : 1.0f / a.l;  // (o is 0 in the first two)
     T* dst = out + (size_t)row * ldo + (size_t)h * HD + 4 * A::VW * g;

@@ -118,6 +118,7 @@ struct PgElem<_Float16> {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int SPLIT = 2;  // parts that hold an f32 to 2^-22
+    static constexpr uint32_t INF = 0x7c007c00u;  // exponent bits of both halves of a word
     // Weights are 2^TOP at most: here as many of their digits as f16's range holds
     // (its largest is 65504).
     static constexpr float TOP = 15.0f;
@@ -130,6 +131,7 @@ struct PgElem<__bf16> {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     static constexpr int SPLIT = 3;  // 8 significant bits each: an f32 to 2^-24
+    static constexpr uint32_t INF = 0x7f807f80u;
     // 2^30 keys' weights times values up to f32's largest sum within f32's range.
     static constexpr float TOP = -31.0f;
     __device__ static pg_f4 mfma16(v8 a, v8 b, pg_f4 c) {
@@ -190,64 +192,71 @@ __device__ __forceinline__ bool pg_odd(const V (&o)[N]) {
     return t != t;
 }
 
-// A row's softmax and sums over keys j0 .. j1 - 1 (those that mine(j) takes) as
-// the definition has them: f32 dot products, whole weights, no key that the row
-// does not see.  The kernels' products form q and the weights in parts, and of a
-// tile's rows some see keys that others do not: 0 * inf, and inf in parts of both
-// signs, are NaN there where the definition has a number or an infinity.  Such
-// sums never become finite again, so a wavefront that ends with one takes its keys
-// here once more.  SHARE lanes, 64 / SHARE apart, hold a row of HD dims; a lane's
-// are RUNS runs of 4, run i from dim(i) on.  x: the row's q.
-template <class E, class T, int HD, int SHARE, int RUNS, class Mine, class Dim>
-__device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int head, const T* x, float scale,
-                                         int limit, int j0, int j1, float shift, Mine mine, Dim dim, float& m,
-                                         float& l, pg_f4 (&o)[RUNS]) {
-    const auto row = [&](const void* pool, int j, bool& none) {
-        const int page = pg_page(c, table, j, j + 1, none);
-        return static_cast<const E*>(pool) +
-               ((((size_t)page * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * HD;
-    };
-    const auto score = [&](int j) {
-        bool none;
-        const E* k = row(c.k, j, none);
-        float s = 0.0f;
+// Whether all of them are NaN: nothing more changes them.
+template <int N, class V>
+__device__ __forceinline__ bool pg_all_nan(const V (&o)[N]) {
+    bool all = true;
 #pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(V) / sizeof(float)); i++) all &= o[n][i] != o[n][i];
+    return all;
+}
+
+// Whether a word holds an infinite or NaN half.
+template <class E>
+__device__ __forceinline__ bool pg_word_odd(uint32_t w) {
+    const uint32_t t = ~w & PgElem<E>::INF;
+    return (t & 0xffffu) == 0 || (t >> 16) == 0;
+}
+
+// Adds keys j0 .. j1 - 1 to a row's maximum and sums as the definition has them:
+// f32 dot products, whole weights, no key that the row does not see.  The kernels'
+// products form q and the weights in parts, and of a tile's rows some see keys that
+// others do not: 0 * inf, and inf in parts of both signs, are NaN there where the
+// definition has a number or an infinity.  Such sums never become finite again, so
+// keys that end with one are walked a second time, and the blocks of them that hold
+// an infinite or NaN value come here.  SHARE lanes, 64 / SHARE apart, hold a row of
+// HD dims; a lane's are RUNS runs of 4, run i from dim(i) on.  x: the row's q (from
+// memory: in the registers there is room for the kernels' own loops only); own_l:
+// whether l is the lane's; a weight is 2^shift at most; add(i, e, f, p, v): sum e of
+// run i becomes f times itself and p v.
+template <class E, class T, int HD, int SHARE, class Dim, class Add>
+__device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int head, const T* x, float scale,
+                                         int limit, int j0, int j1, float shift, bool own_l, Dim dim, Add add,
+                                         float& m, float& l) {
+    constexpr int RUNS = HD / SHARE / 4;
+    const float factor = scale * 1.4426950408889634f;
+#pragma unroll 1
+    for (int j = j0; j < j1; j++) {
+        bool none;
+        const int page = pg_page(c, table, j, j + 1, none);
+        const size_t row = ((((size_t)page * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * HD;
+        const E *k = static_cast<const E*>(c.k) + row, *v = static_cast<const E*>(c.v) + row;
+        float s = 0.0f;
+#pragma unroll 4
         for (int i = 0; i < RUNS; i++) {
             E y[4];
             T z[4];
             __builtin_memcpy(y, __builtin_assume_aligned(k + dim(i), 8), sizeof y);
             __builtin_memcpy(z, __builtin_assume_aligned(x + dim(i), 8), sizeof z);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s = fmaf((float)z[e], (float)y[e], s);
+            for (int e = 0; e < 4; e++) s = fmaf((float)z[e] * factor, (float)y[e], s);
         }
 #pragma unroll
         for (int d = 64 / SHARE; d < 64; d *= 2) s += __shfl_xor(s, d);
-        return none ? pg_nan() : s * (scale * 1.4426950408889634f);
-    };
-    m = PG_LEAST;
-#pragma unroll 1
-    for (int j = j0; j < j1; j++) {
-        if (!mine(j)) continue;
-        const float s = score(j);
-        if (j <= limit) m = fmaxf(m, s);
-    }
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < RUNS; i++) o[i] = pg_f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-    for (int j = j0; j < j1; j++) {
-        if (!mine(j)) continue;
-        const float p = __builtin_amdgcn_exp2f(score(j) - m + shift);
         if (j > limit) continue;
-        bool none;
-        const E* v = row(c.v, j, none);
-        l += p;
+        if (none) s = pg_nan();
+        const float mn = fmaxf(m, s), f = __builtin_amdgcn_exp2f(m - mn), p = __builtin_amdgcn_exp2f(s - mn + shift);
+        m = mn;
+        l = l * f + (own_l ? p : 0.0f);
 #pragma unroll
         for (int i = 0; i < RUNS; i++) {
             E y[4];
             __builtin_memcpy(y, __builtin_assume_aligned(v + dim(i), 8), sizeof y);
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[i][e] = fmaf(p, (float)y[e], o[i][e]);
+            for (int e = 0; e < 4; e++) add(i, e, f, p, (float)y[e]);
+            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few loads at once: the sums fill the registers)
         }
     }
 }

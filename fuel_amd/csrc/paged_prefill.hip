@@ -100,6 +100,19 @@ struct PrefillTile {
     __device__ static __forceinline__ int vswz(int r) { return HD == 128 ? 4 * (r & 3) : 4 * ((r >> 1) & 1); }
 };
 
+// Whether KEYS rows of K and V from kt and vt on hold an infinite or NaN value, or
+// a page of them is none.  Wave-uniform.
+template <class X, class E, int KEYS>
+__device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uint32_t bad) {
+    bool any = bad & ((1u << KEYS / 16) - 1);
+    for (int i = 16 * (threadIdx.x & 63); i < KEYS * X::ROW; i += 1024) {
+        const pg_u4 k = *reinterpret_cast<const pg_u4*>(kt + i), v = *reinterpret_cast<const pg_u4*>(vt + i);
+#pragma unroll
+        for (int w = 0; w < 4; w++) any |= pg_word_odd<E>(k[w]) || pg_word_odd<E>(v[w]);
+    }
+    return __any(any);
+}
+
 // A workgroup takes one tile of query rows, or with CUT an equal contiguous
 // range of all tiles' key tiles (head by head, sequence by sequence, tile by
 // tile), as the 16-row kernel does: where a batch has fewer tiles than fill the
@@ -187,11 +200,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         if constexpr (CUT) tiles = min(tiles, t0 + m_units);
 
         pf_f16 o[X::DT];
-#pragma unroll
-        for (int d = 0; d < X::DT; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-        float m = PG_LEAST, l = 0.0f, peak = m;  // peak: the largest score so far
+        float m, l, peak;  // peak: the largest score so far
 
         // DMA: instruction i of this wavefront takes rows ((i PF_WAVES + wave) RPI) .. of
         // a tile, all in one group of 16 keys.  Source offsets of the lane within it:
@@ -286,115 +295,136 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                 }
         }
 
-        for (int t = t0; t < tiles; t++) {
-            const int j0 = t * PF_KEYS;
-            // tile t landed, in every wavefront, and tile t - 1 is read
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
-            const uint32_t bad = (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
-            if (j0 + PF_KEYS > sq.kv || bad) {  // rows of V that are no keys hold anything
-                for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
-                    const int r = ch / CPR;
-                    if (j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1))
-                        reinterpret_cast<uint4*>(s_v[t & 1])[ch] = make_uint4(0, 0, 0, 0);
+        const auto walk = [&](auto again) {
+            constexpr bool AGAIN = decltype(again)::value;
+#pragma unroll
+            for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+            m = peak = PG_LEAST;
+            l = 0.0f;
+            for (int t = t0; t < tiles; t++) {
+                const int j0 = t * PF_KEYS;
+                // tile t landed, in every wavefront, and tile t - 1 is read
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                const uint32_t bad = (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
+                if (j0 + PF_KEYS > sq.kv || bad) {  // rows of V that are no keys hold anything
+                    for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
+                        const int r = ch / CPR;
+                        if (j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1))
+                            reinterpret_cast<uint4*>(s_v[t & 1])[ch] = make_uint4(0, 0, 0, 0);
+                    }
+                    __syncthreads();
                 }
-                __syncthreads();
-            }
-            if (t + 1 < tiles) issue(t + 1);
-            const int jw = j0 + key0;  // this wavefront's first key
-            if (jw > last) continue;
+                if (t + 1 < tiles) issue(t + 1);
+                const int jw = j0 + key0;  // this wavefront's first key
+                if (jw > last) continue;
 
-            const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
-            const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
-            pf_f16 st[NA];
-#pragma unroll
-            for (int a = 0; a < NA; a++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) st[a][i] = 0.0f;
-#pragma unroll
-                for (int k = 0; k < X::KS; k++) {
-                    const v8 kf = *reinterpret_cast<const v8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
-#pragma unroll
-                    for (int p = X::NP - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
+                const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
+                const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
+                if (AGAIN && pf_odd<X, E, 64 / KW>(kt, vt, bad >> (key0 >> 4))) {
+                    if (!__all(pg_all_nan(o)))
+                        pg_plain<E, T, HD, 2>(
+                            c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
+                            min(jw + 32 * NA, last + 1), X::SHIFT, h == 0, [&](int i) { return 8 * i + 4 * h; },
+                            [&](int i, int e, float f, float p, float v) {
+                                o[i / 4][4 * (i % 4) + e] = fmaf(p, v, o[i / 4][4 * (i % 4) + e] * f);
+                            },
+                            m, l);
+                    peak = fmaxf(peak, m);
+                    continue;
                 }
-            }
-            const bool mask = jw + 32 * NA - 1 > first || bad;
-            if (mask) {
+                pf_f16 st[NA];
+#pragma unroll
+                for (int a = 0; a < NA; a++) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) st[a][i] = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < X::KS; k++) {
+                        const v8 kf = *reinterpret_cast<const v8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
+#pragma unroll
+                        for (int p = X::NP - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
+                    }
+                }
+                const bool mask = jw + 32 * NA - 1 > first || bad;
+                if (mask) {
+#pragma unroll
+                    for (int a = 0; a < NA; a++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const int r = 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h;
+                            if ((bad >> ((key0 + r) >> 4)) & 1) st[a][i] = pg_nan();
+                            if (jw + r > limit) st[a][i] = -__builtin_inff();
+                        }
+                }
+                float top = st[0][0];
+#pragma unroll
+                for (int a = 0; a < NA; a++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
+                top = fmaxf(top, pf_other_half(top)) * factor;
+                peak = fmaxf(peak, top);
+                const float low = X::F16 ? fmaxf(top, peak - PG_DROP) : m;
+                if (__any(top > m + X::LAZY || low < m - PF_LOW)) {
+                    const float mn = fmaxf(top, low < m - PF_LOW ? low : m);
+                    const float f = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before)
+                    m = mn;
+                    l *= f;
+#pragma unroll
+                    for (int d = 0; d < X::DT; d++) o[d] *= f;
+                }
+                // (fmaf: one operation less a weight.  Of scores past 2^30 it leaves what the
+                // maximum was rounded by, which can be a weight that is infinite.)
+                const float ms = m - X::SHIFT;
+#pragma unroll
+                for (int a = 0; a < NA; a++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) st[a][i] = AGAIN ? st[a][i] * factor - ms : fmaf(st[a][i], factor, -ms);
+                if (mask) {  // (again: a factor of 0 would make NaN of -inf)
+#pragma unroll
+                    for (int a = 0; a < NA; a++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++)
+                            if (jw + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h > limit) st[a][i] = -__builtin_inff();
+                }
+                v8 pp[X::NP][2 * NA];
 #pragma unroll
                 for (int a = 0; a < NA; a++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
-                        const int r = 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h;
-                        if ((bad >> ((key0 + r) >> 4)) & 1) st[a][i] = pg_nan();
-                        if (jw + r > limit) st[a][i] = -__builtin_inff();
+                        st[a][i] = __builtin_amdgcn_exp2f(st[a][i]);
+                        l += st[a][i];
+                        float rest = st[a][i];
+#pragma unroll
+                        for (int p = 0; p < X::NP; p++) {
+                            pp[p][2 * a + (i >> 3)][i & 7] = (E)rest;
+                            rest -= (float)pp[p][2 * a + (i >> 3)][i & 7];
+                        }
+                    }
+#pragma unroll
+                for (int k = 0; k < 2 * NA; k++)
+#pragma unroll
+                    for (int d = 0; d < X::DT; d++) {
+                        const uint8_t* at = vt + 16 * k * X::ROW + (vbase ^ (64 * d));
+                        const pf_s4 lo = pf_read_tr(at), hi = pf_read_tr(at + 8 * X::ROW);
+                        const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int p = X::NP - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
                     }
             }
-            float top = st[0][0];
-#pragma unroll
-            for (int a = 0; a < NA; a++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
-            top = fmaxf(top, pf_other_half(top)) * factor;
-            peak = fmaxf(peak, top);
-            const float low = X::F16 ? fmaxf(top, peak - PG_DROP) : m;
-            if (__any(top > m + X::LAZY || low < m - PF_LOW)) {
-                const float mn = fmaxf(top, low < m - PF_LOW ? low : m);
-                const float f = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before)
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < X::DT; d++) o[d] *= f;
-            }
-            const float ms = m - X::SHIFT;
-#pragma unroll
-            for (int a = 0; a < NA; a++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) st[a][i] = fmaf(st[a][i], factor, -ms);
-            if (mask) {  // (again: a factor of 0 would make NaN of -inf)
-#pragma unroll
-                for (int a = 0; a < NA; a++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (jw + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h > limit) st[a][i] = -__builtin_inff();
-            }
-            v8 pp[X::NP][2 * NA];
-#pragma unroll
-            for (int a = 0; a < NA; a++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    st[a][i] = __builtin_amdgcn_exp2f(st[a][i]);
-                    l += st[a][i];
-                    float rest = st[a][i];
-#pragma unroll
-                    for (int p = 0; p < X::NP; p++) {
-                        pp[p][2 * a + (i >> 3)][i & 7] = (E)rest;
-                        rest -= (float)pp[p][2 * a + (i >> 3)][i & 7];
-                    }
-                }
-#pragma unroll
-            for (int k = 0; k < 2 * NA; k++)
-#pragma unroll
-                for (int d = 0; d < X::DT; d++) {
-                    const uint8_t* at = vt + 16 * k * X::ROW + (vbase ^ (64 * d));
-                    const pf_s4 lo = pf_read_tr(at), hi = pf_read_tr(at + 8 * X::ROW);
-                    const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                    for (int p = X::NP - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
-                }
+        };
+        walk(std::false_type{});
+        // Infinite or NaN sums: the same keys once more, tiles that hold such values
+        // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 8.2,
+        // all NaN 7.7, with one infinite value in every 16 keys, the worst there is, 350.
+        if (__builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)))) {
+            fetch_ids(t0 * PF_KEYS);
+            issue(t0);
+            walk(std::true_type{});
         }
         l += pf_other_half(l);
-        if (__any(pg_odd(o))) {
-            pg_f4 y[4 * X::DT];
-            pg_plain<E, T, HD, 2>(
-                c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, t0 * PF_KEYS,
-                min(tiles * PF_KEYS, last + 1), X::SHIFT,
-                [&](int j) { return KW == 1 || (j & 32) == key0; }, [&](int i) { return 8 * i + 4 * h; }, m, l, y);
-#pragma unroll
-            for (int d = 0; d < X::DT; d++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] = y[4 * d + i / 4][i % 4];
-        }
         if constexpr (KW == 2) {  // the two that share rows
             static_assert(16 * X::DT * 64 * 4 * RW <= sizeof s_k, "the sums of half the wavefronts");
             __syncthreads();
