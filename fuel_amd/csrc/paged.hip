@@ -23,9 +23,10 @@
 // f32 activations: q and p are split into parts of the cache's type (2 of f16,
 // 3 of bf16), which keeps products and sums at f32's precision.  f16 parts
 // take q scaled by a power of two per row (exact), its largest to 2^14 .. 2^15:
-// no part leaves f16's range, and a small dim keeps steps of 2^-39 of the largest.  16-bit activations: q as it is, p in two parts; their products cost
-// nothing here, where K and V bytes are the bound, and one part would add a
-// rounding as large as the output's own.
+// no part leaves f16's range, and a small dim keeps steps of 2^-39 of the largest.
+// 16-bit activations: q as it is, p in two parts; their products cost nothing
+// here, where K and V bytes are the bound, and one part would add a rounding as
+// large as the output's own.
 // p carries a factor 2^TOP, which l carries too: f16 parts of small p keep steps
 // of 2^-24 / 2^15 of the largest p of 32 keys.
 #include <hip/hip_runtime.h>
@@ -283,8 +284,8 @@ struct Rows16 {
 // written out, the cut pieces (at most two a workgroup) leave their sums in
 // the workspace for paged_join_kernel.
 // Bound by HBM, and by some 10 us before the first keys arrive and for the join.
-// bf16, 32 heads over 8 of 128: 64 sequences of up to 8191, 413 MB, 73 us and 4.6
-// for the join; one of 131071, 537 MB, 87 and 5.2 (6.2 TB/s while it walks; reads
+// bf16, 32 heads over 8 of 128: 64 sequences of up to 8191, 413 MB, 72 us and 4.6
+// for the join; one of 131071, 537 MB, 85 and 5.7 (6.3 TB/s while it walks; reads
 // alone reach 6.75 here).  Large tiles of wavefronts, more workgroups, or the next
 // piece's first keys loaded under this one's merge took as long or longer.
 constexpr int PD_UNIT = 32 * PA_WAVES;

@@ -21,17 +21,20 @@
 // keys, N(0, 1), differ by less.
 // 16-bit activations: p is rounded to the cache's type for the second product
 // (a relative 2^-11 or 2^-8 of each weight at most, the output's own rounding;
-// the sum l takes p as it is).  A second part, as the decode keeps, would cost
-// half as many matrix instructions again, which are the bound here.  f32
-// activations: q and p in parts that keep f32's precision.
-// One prompt of 16384, 32 heads over 8 of 128, bf16: 2.04 ms, 1.08 PFLOP/s, where a
-// large matrix product of the library makes 1.19: the matrix pipe 56 % busy, beside
+// the sum l takes p as it is).  A second part, as the 16-row kernel keeps, costs
+// half as many matrix instructions again, which are the bound here: a prompt of
+// 16384 2.78 ms instead of 2.04, 17 ragged ones 0.196 instead of 0.159, for an
+// output 0.0015 of it from 64 bits instead of 0.0020 (bf16; f16 0.0002, 0.0003).
+// f32 activations: q and p in parts that keep f32's precision.
+// One prompt of 16384, 32 heads over 8 of 128, bf16: 2.0 ms, 1.10 PFLOP/s, where a
+// large matrix product of the library makes 1.19: the matrix pipe 57 % busy, beside
 // 6.4 VALU instructions to an MFMA, at the 1.8 GHz that the chip's power leaves (the
-// softmax left out: 2.03 ms).  17 prompts of 67 .. 1683: 0.16 ms, 0.70 PFLOP/s: some
-// 9 key tiles to a tile of rows, whose start, masked last tile and end count, and
-// 6 rounds of unequal workgroups.  No faster: two groups of wavefronts in turn at
-// the matrix pipe, S^T of the next tile under this one's softmax, wave priorities,
-// eight wavefronts on 256 rows, three tiles in LDS, three wavefronts a SIMD (spills).
+// softmax left out: 2.03 of then 2.10 ms).  17 prompts of 67 .. 1683: 0.16 ms, 0.72
+// PFLOP/s: some 9 key tiles to a tile of rows, whose start, masked last tile and end
+// count, and 6 rounds of unequal workgroups.  No faster: two groups of wavefronts in
+// turn at the matrix pipe, S^T of the next tile under this one's softmax, wave
+// priorities, eight wavefronts on 256 rows, three tiles in LDS, three wavefronts a
+// SIMD (spills).
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
@@ -124,7 +127,8 @@ __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uin
 // where they are alone.  32 heads over 8, new rows 300 / 700 / 1000 (80 .. 256
 // tiles), us: bf16 14.3 / 22.2 / 28.9 with KW = 1, 12.1 / 19.4 / 25.0 with 2, f32
 // 18.0 / 29.1 / 39.2 and 14.4 / 24.2 / 32.5; beyond that not all of them start at
-// once (1500 rows after 600, 384 tiles: 55 and 62).
+// once (1500 rows after 600, 384 tiles: 55 and 62).  (f32 rows over f16 pages take 4 %
+// more on both sides since their maximum is renewed at every passing.)
 constexpr int PF_FEW = 256;
 
 template <class E, class T, int HD, int KW, bool CUT>
