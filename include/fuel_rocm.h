@@ -416,7 +416,8 @@ int frq_paged_attention_decode(frq_device *dev, const frq_paged_kv *kv, const fr
  * is cached): each row over the cache rows 0 .. its position, arguments as
  * frq_paged_attention_decode; the batch's own keys and values are appended
  * before.  With 16-bit operands the softmax weights may be rounded to that
- * type for the product with V (their sum is not). */
+ * type for the product with V (their sum is not): they are in batches of many
+ * rows, as the sizes of the structs have it, and not with f32 operands. */
 int frq_paged_attention_prefill(frq_device *dev, const frq_paged_kv *kv, const frq_paged_batch *batch, int dtype,
                                 size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
                                 size_t work_bytes, void *out_dev, size_t ldo);
