@@ -349,7 +349,8 @@ typedef struct frq_paged_kv {
  *   kv_len [n_seqs]: tokens of each sequence, this call's rows included
  *   row_start [n_seqs + 1], non-decreasing: sequence s has the rows
  *     row_start[s] .. row_start[s + 1] - 1; NULL: row s alone (rows = n_seqs)
- * max_pages * page_size is at most 2^30.
+ * max_pages * page_size is at most 2^30.  The arrays are read while a call runs
+ * and must not change until it has.
  * rows is the number of rows of the call's q, k, v and outputs.  max_kv_len
  * is the caller's bound on kv_len (at most max_pages * page_size; 0 stands
  * for that): work is divided by it, so a near bound helps short contexts, and

@@ -3,9 +3,10 @@ have their results, or the call writes nothing."""
 import numpy as np
 import pytest
 
+import fuel_amd as F
 import paged_ref as R
 from paged_ref import BF16, F16
-from test_gpu_paged import Case, say, seed
+from test_gpu_paged import Case, put, say, seed
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +51,27 @@ def test_more_rows_in_ranges_than_rows(dev, H, hk, D, past, f, n):
     for _ in range(2):
         c.run()
         assert (c.got() == 7.0).all()
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_batches_without_pages(dev, decode):
+    """max_pages 0 and no table: lengths of 0 give zeros, others are none."""
+    say("no pages", decode)
+    n, H, D = 5, 4, 128
+    c = Case(dev, seed(42), F16, F16, H, 2, D, 16, [0] * n, [1] * n, decode=decode)
+    c.kv = np.array([0, 0, 5, 0, -1], np.int32)
+    c.upload()
+    batch = F.PagedBatch(None, c.ints[1], n, 0, n, None if decode else c.ints[2])
+    assert F.paged_attention_workspace(c.kvc, batch, H) == 0
+    k, v = (put(dev, np.ones((n, 2 * D), np.float32), F16) for _ in range(2))
+    before = c.k_dev.numpy()
+    out = put(dev, np.full((n, H * D), 7.0, np.float32), F16)
+    F.paged_append(c.kvc, batch, F16, H, c.q_dev, k, v, out)
+    want = np.zeros((n, H * D), np.float32)
+    want[[2, 4]] = np.nan
+    np.testing.assert_array_equal(R.from_bits(out.numpy(), F16), want)
+    np.testing.assert_array_equal(c.k_dev.numpy(), before)
+    out.copy_from(R.to_bits(np.full((n, H * D), 7.0, np.float32), F16))
+    attend = F.paged_attention_decode if decode else F.paged_attention_prefill
+    attend(c.kvc, batch, F16, H, c.q_dev, out, c.scale)
+    np.testing.assert_array_equal(R.from_bits(out.numpy(), F16), want)
