@@ -225,38 +225,51 @@ template <class E, class T, int HD, int SHARE, class Dim, class Add>
 __device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int head, const T* x, float scale,
                                          int limit, int j0, int j1, float shift, bool own_l, Dim dim, Add add,
                                          float& m, float& l) {
-    constexpr int RUNS = HD / SHARE / 4;
+    constexpr int RUNS = HD / SHARE / 4, KEYS = 4;  // keys at a time: q is read once for them
     const float factor = scale * 1.4426950408889634f;
 #pragma unroll 1
-    for (int j = j0; j < j1; j++) {
+    for (int j = j0; j < j1; j += KEYS) {  // (of one page: j0 is a multiple of 16)
         bool none;
         const int page = pg_page(c, table, j, j + 1, none);
         const size_t row = ((((size_t)page * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * HD;
         const E *k = static_cast<const E*>(c.k) + row, *v = static_cast<const E*>(c.v) + row;
-        float s = 0.0f;
-#pragma unroll 4
+        float s[KEYS] = {}, mn = m;
+#pragma unroll 2
         for (int i = 0; i < RUNS; i++) {
-            E y[4];
             T z[4];
-            __builtin_memcpy(y, __builtin_assume_aligned(k + dim(i), 8), sizeof y);
             __builtin_memcpy(z, __builtin_assume_aligned(x + dim(i), 8), sizeof z);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s = fmaf((float)z[e] * factor, (float)y[e], s);
+            for (int u = 0; u < KEYS; u++) {
+                E y[4];
+                __builtin_memcpy(y, __builtin_assume_aligned(k + u * HD + dim(i), 8), sizeof y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[u] = fmaf((float)z[e] * factor, (float)y[e], s[u]);
+            }
         }
 #pragma unroll
-        for (int d = 64 / SHARE; d < 64; d *= 2) s += __shfl_xor(s, d);
+        for (int u = 0; u < KEYS; u++) {
+#pragma unroll
+            for (int d = 64 / SHARE; d < 64; d *= 2) s[u] += __shfl_xor(s[u], d);
+            if (none) s[u] = pg_nan();
+            if (j + u <= limit) mn = fmaxf(mn, s[u]);
+        }
         if (j > limit) continue;
-        if (none) s = pg_nan();
-        const float mn = fmaxf(m, s), f = __builtin_amdgcn_exp2f(m - mn), p = __builtin_amdgcn_exp2f(s - mn + shift);
+        const float f = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
-        l = l * f + (own_l ? p : 0.0f);
+        l *= f;
 #pragma unroll
-        for (int i = 0; i < RUNS; i++) {
-            E y[4];
-            __builtin_memcpy(y, __builtin_assume_aligned(v + dim(i), 8), sizeof y);
+        for (int u = 0; u < KEYS; u++) {
+            if (j + u > limit) break;
+            const float p = __builtin_amdgcn_exp2f(s[u] - mn + shift);
+            if (own_l) l += p;
 #pragma unroll
-            for (int e = 0; e < 4; e++) add(i, e, f, p, (float)y[e]);
-            if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few loads at once: the sums fill the registers)
+            for (int i = 0; i < RUNS; i++) {
+                E y[4];
+                __builtin_memcpy(y, __builtin_assume_aligned(v + u * HD + dim(i), 8), sizeof y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) add(i, e, u ? 1.0f : f, p, (float)y[e]);
+                if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few loads at once: the sums fill the registers)
+            }
         }
     }
 }

@@ -421,8 +421,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         };
         walk(std::false_type{});
         // Infinite or NaN sums: the same keys once more, tiles that hold such values
-        // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 8.2,
-        // all NaN 7.7, with one infinite value in every 16 keys, the worst there is, 350.
+        // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 7.7,
+        // all NaN 7.2, with one infinite value in every 16 keys, the worst there is, 205.
         if (__builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)))) {
             fetch_ids(t0 * PF_KEYS);
             issue(t0);
