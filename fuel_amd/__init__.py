@@ -8,6 +8,7 @@ from ._native import BF16, F16, F32, Q4K, Q6K, Q8K, Q8_0, FuelRocmError, LIB_PAT
 from .backend import (
     PagedBatch,
     PagedKvCache,
+    PagedKvCache8,
     QMatMulParams,
     RocmDevice,
     RocmQStorage,
@@ -23,6 +24,7 @@ from .backend import (
     paged_attention_decode,
     paged_attention_prefill,
     paged_attention_workspace,
+    paged_plan,
     qmatmul_f32_rocm_wrapper,
     qmatmul_plan,
     quantize_q8_0,
@@ -35,7 +37,7 @@ __all__ = [
     "BF16", "F16", "F32", "Q4K", "Q6K", "Q8K", "Q8_0", "FuelRocmError", "LIB_PATH", "SIGNATURES", "lib",
     "QMatMulParams", "RocmDevice", "RocmQStorage", "RocmStorage", "block_isums", "block_size",
     "device_count", "fill_normal", "fill_random_bits", "moe_ffn", "moe_route",
-    "PagedBatch", "PagedKvCache", "paged_append", "paged_attention_decode", "paged_attention_prefill",
-    "paged_attention_workspace",
+    "PagedBatch", "PagedKvCache", "PagedKvCache8", "paged_append", "paged_attention_decode", "paged_attention_prefill",
+    "paged_attention_workspace", "paged_plan",
     "qmatmul_f32_rocm_wrapper", "qmatmul_plan", "quantize_q8_0", "quantize_q8k", "type_size", "GgufFile",
 ]

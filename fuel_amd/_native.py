@@ -39,6 +39,13 @@ class PagedKv(C.Structure):
                 ("head_dim", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p)]
 
 
+class PagedKv8(C.Structure):
+    """frq_paged_kv8"""
+    _fields_ = [("n_pages", C.c_size_t), ("page_size", C.c_size_t), ("n_kv_heads", C.c_size_t),
+                ("head_dim", C.c_size_t), ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p)]
+
+
 class PagedBatch(C.Structure):
     """frq_paged_batch"""
     _fields_ = [("n_seqs", C.c_size_t), ("max_pages", C.c_size_t), ("rows", C.c_size_t), ("max_kv_len", C.c_size_t),
@@ -107,6 +114,11 @@ SIGNATURES = {
     "frq_paged_attention_workspace": (_sz, [_vp, _vp, _sz]),
     "frq_paged_attention_decode": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, C.c_float, _vp, _sz, _vp, _sz]),
     "frq_paged_attention_prefill": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, C.c_float, _vp, _sz, _vp, _sz]),
+    "frq_paged8_append": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _sz, _vp, _sz]),
+    "frq_paged8_attention_workspace": (_sz, [_vp, _vp, _sz]),
+    "frq_paged8_attention_decode": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, C.c_float, _vp, _sz, _vp, _sz]),
+    "frq_paged8_attention_prefill": (_i32, [_vp, _vp, _vp, _i32, _sz, _vp, _sz, C.c_float, _vp, _sz, _vp, _sz]),
+    "frq_paged_plan": (_i32, [_vp, _sz, _sz, _sz, _sz, _sz] + [_vp] * 10),
     "frq_block_isums": (_i32, [_vp, _i32, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
     "frq_fill_random_bits": (_i32, [_vp, _vp, _sz, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32]),
     "frq_fill_normal": (_i32, [_vp, _vp, _sz, C.c_uint64, C.c_uint32, C.c_float, C.c_float]),

@@ -341,6 +341,34 @@ class PagedKvCache:
         self.ref = C.byref(self.struct)
 
 
+class PagedKvCache8:
+    """The same with e4m3 codes [n_pages, n_kv_heads, page_size, head_dim] and an
+    e8m0 scale for every 16 positions of a head [n_pages, n_kv_heads, page_size / 16]
+    (frq_paged_kv8), bytes both; the paged calls below take either cache.  k, v,
+    k_scale, v_scale: device addresses or storages of the caller's own; otherwise
+    zeroed ones are allocated."""
+
+    def __init__(self, dev: RocmDevice, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, k=None, v=None,
+                 k_scale=None, v_scale=None):
+        own = [k, v, k_scale, v_scale]
+        if any(x is None for x in own) != all(x is None for x in own):
+            raise FuelRocmError(N.FRQ_INVALID, "PagedKvCache8: k, v and their scales go together")
+        self.dev = dev
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = n_pages, page_size, n_kv_heads, head_dim
+        shape, scales = (n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads, page_size // 16)
+        if k is None:
+            own = [dev.alloc(s, np.uint8) for s in (shape, shape, scales, scales)]
+            for s in own:
+                check(lib().frq_memset(dev.handle, C.c_void_p(s.ptr), 0, s.nbytes))
+        self.k, self.v, self.k_scale, self.v_scale = own
+        rows = n_pages * n_kv_heads * page_size
+        self.struct = N.PagedKv8(n_pages, page_size, n_kv_heads, head_dim,
+                                 *(_paged_operand(n, x, dev, size) for n, x, size in
+                                   zip(("k", "v", "k_scale", "v_scale"), own,
+                                       (rows * head_dim, rows * head_dim, rows // 16, rows // 16))))
+        self.ref = C.byref(self.struct)
+
+
 class PagedBatch:
     """The sequences of a call and its packed rows (frq_paged_batch): page_table
     [n_seqs, max_pages], kv_len [n_seqs] and row_start [n_seqs + 1] (None: one
@@ -360,7 +388,12 @@ class PagedBatch:
         self.ref = C.byref(self.struct)
 
 
-def _paged_handle(cache: PagedKvCache, batch: PagedBatch):
+def _paged_call(cache, name: str):
+    """frq_paged_{name}, or frq_paged8_{name} for an 8-bit cache."""
+    return getattr(lib(), ("frq_paged8_" if isinstance(cache, PagedKvCache8) else "frq_paged_") + name)
+
+
+def _paged_handle(cache: PagedKvCache | PagedKvCache8, batch: PagedBatch):
     """The handle of the device that a call runs on."""
     dev = cache.dev
     if batch.dev is not None and batch.dev is not dev and batch.dev.ordinal != dev.ordinal:
@@ -368,13 +401,13 @@ def _paged_handle(cache: PagedKvCache, batch: PagedBatch):
     return dev.handle
 
 
-def _paged_rows(name: str, x, cache: PagedKvCache, batch: PagedBatch, dtype: int, width: int, ld: int) -> int:
+def _paged_rows(name: str, x, cache: PagedKvCache | PagedKvCache8, batch: PagedBatch, dtype: int, width: int, ld: int) -> int:
     """Address of `batch.rows` rows of `width` elements, ld apart."""
     size = 4 if dtype == N.F32 else 2
     return _paged_operand(name, x, cache.dev, ((batch.rows - 1) * ld + width) * size if batch.rows else 0)
 
 
-def paged_append(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, k, v, q_out, ldq: int = 0,
+def paged_append(cache: PagedKvCache | PagedKvCache8, batch: PagedBatch, dtype: int, n_heads: int, q, k, v, q_out, ldq: int = 0,
                  ldk: int = 0, ldv: int = 0, ldqo: int = 0, rope_cos=None, rope_sin=None, rope_rows: int = 0) -> None:
     """RoPE of the packed q and k rows (type dtype), rotated q to q_out, k and v
     into the cache at each row's position (frq_paged_append).  Operands are
@@ -384,7 +417,7 @@ def paged_append(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: in
     ldq, ldk, ldv, ldqo = ldq or wide, ldk or narrow, ldv or narrow, ldqo or wide
     table = 4 * rope_rows * cache.head_dim
     handle = _paged_handle(cache, batch)
-    check(lib().frq_paged_append(
+    check(_paged_call(cache, "append")(
         handle, cache.ref, batch.ref, dtype, n_heads,
         q if type(q) is int else _paged_rows("q", q, cache, batch, dtype, wide, ldq), ldq,
         k if type(k) is int else _paged_rows("k", k, cache, batch, dtype, narrow, ldk), ldk,
@@ -394,9 +427,9 @@ def paged_append(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: in
         rope_rows, q_out if type(q_out) is int else _paged_rows("q_out", q_out, cache, batch, dtype, wide, ldqo), ldqo))
 
 
-def paged_attention_workspace(cache: PagedKvCache, batch: PagedBatch, n_heads: int) -> int:
+def paged_attention_workspace(cache: PagedKvCache | PagedKvCache8, batch: PagedBatch, n_heads: int) -> int:
     """Bytes of scratch the paged attention calls need for this batch."""
-    return int(lib().frq_paged_attention_workspace(cache.ref, batch.ref, n_heads))
+    return int(_paged_call(cache, "attention_workspace")(cache.ref, batch.ref, n_heads))
 
 
 def _paged_attention(fn, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo, work_bytes) -> None:
@@ -411,21 +444,42 @@ def _paged_attention(fn, cache, batch, dtype, n_heads, q, out, scale, work, ldq,
              out if type(out) is int else _paged_rows("out", out, cache, batch, dtype, wide, ldo), ldo))
 
 
-def paged_attention_decode(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
+def paged_attention_decode(cache: PagedKvCache | PagedKvCache8, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
                            work=None, ldq: int = 0, ldo: int = 0, work_bytes: int = 0) -> None:
     """Attention of one new token per sequence over its cached rows
     (frq_paged_attention_decode); work: paged_attention_workspace() bytes, a
     storage, or an address of work_bytes bytes."""
-    _paged_attention(lib().frq_paged_attention_decode, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo,
+    _paged_attention(_paged_call(cache, "attention_decode"), cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo,
                      work_bytes)
 
 
-def paged_attention_prefill(cache: PagedKvCache, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
+def paged_attention_prefill(cache: PagedKvCache | PagedKvCache8, batch: PagedBatch, dtype: int, n_heads: int, q, out, scale: float,
                             work=None, ldq: int = 0, ldo: int = 0, work_bytes: int = 0) -> None:
     """Causal attention of packed prompt rows over the cache
     (frq_paged_attention_prefill); work as paged_attention_decode()'s."""
-    _paged_attention(lib().frq_paged_attention_prefill, cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo,
+    _paged_attention(_paged_call(cache, "attention_prefill"), cache, batch, dtype, n_heads, q, out, scale, work, ldq, ldo,
                      work_bytes)
+
+
+def paged_plan(dev: RocmDevice, n_seqs: int, max_pages: int, page_size: int, n_pages: int, rows: int, tokens, kv_len,
+               page_table, free_pages, n_free, row_start, slots=None, positions=None, kv_len_out=None,
+               n_free_out=None) -> None:
+    """Pages of a pool for the tokens that each sequence of a batch asks for or
+    drops (frq_paged_plan): the page table, lengths and row ranges of a PagedBatch,
+    and the rows' slots and positions.  Operands are int32 (slots int64) in device
+    memory, storages or addresses; kv_len and n_free are renewed in place without
+    kv_len_out and n_free_out."""
+    kv_len_out = kv_len if kv_len_out is None else kv_len_out
+    n_free_out = n_free if n_free_out is None else n_free_out
+    check(lib().frq_paged_plan(
+        dev.handle, n_seqs, max_pages, page_size, n_pages, rows,
+        *(_paged_operand(name, x, dev, size * n, dtype) for name, x, n, size, dtype in (
+            ("tokens", tokens, n_seqs, 4, np.int32), ("kv_len", kv_len, n_seqs, 4, np.int32),
+            ("kv_len_out", kv_len_out, n_seqs, 4, np.int32),
+            ("page_table", page_table, n_seqs * max_pages, 4, np.int32),
+            ("free_pages", free_pages, n_pages, 4, np.int32), ("n_free", n_free, 1, 4, np.int32),
+            ("n_free_out", n_free_out, 1, 4, np.int32), ("row_start", row_start, n_seqs + 1, 4, np.int32),
+            ("slots", slots, rows, 8, np.int64), ("positions", positions, rows, 4, np.int32)))))
 
 
 # ---- synthetic inputs ----

@@ -14,6 +14,7 @@
 #include "common.hpp"
 #include "gguf.hpp"
 #include "kernels.hpp"
+#include "paged8.hpp"
 
 using namespace frq;
 
@@ -1426,12 +1427,9 @@ int frq_argmax_embed(frq_device* dev, const float* logits, size_t vocab, const f
 
 namespace {
 
-// The structs of a paged call as the kernels take them, or a refusal.
-int paged_args(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b, size_t n_heads, PagedKv* kvo,
-               PagedRows* ro) {
-    if (!kv || !b) return fail(FRQ_INVALID, "%s: null cache or batch", who);
-    if (kv->dtype != GGML_F16 && kv->dtype != GGML_BF16)
-        return fail(FRQ_UNSUPPORTED, "%s: cache dtype %d (supported: f16, bf16)", who, kv->dtype);
+// The sizes of a paged call as the kernels take them, or a refusal.
+int paged_sizes(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b, size_t n_heads, PagedKv* kvo,
+                PagedRows* ro) {
     if (kv->head_dim != 64 && kv->head_dim != 128)
         return fail(FRQ_UNSUPPORTED, "%s: head_dim=%zu (supported: 64, 128)", who, kv->head_dim);
     const size_t ps = kv->page_size;
@@ -1461,6 +1459,26 @@ int paged_args(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b
     return FRQ_OK;
 }
 
+int paged_args(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b, size_t n_heads, PagedKv* kvo,
+               PagedRows* ro) {
+    if (!kv || !b) return fail(FRQ_INVALID, "%s: null cache or batch", who);
+    if (kv->dtype != GGML_F16 && kv->dtype != GGML_BF16)
+        return fail(FRQ_UNSUPPORTED, "%s: cache dtype %d (supported: f16, bf16)", who, kv->dtype);
+    return paged_sizes(who, kv, b, n_heads, kvo, ro);
+}
+
+// The same of an 8-bit cache; `shape` is the cache as the other checks take it.
+int paged8_args(const char* who, const frq_paged_kv8* kv, const frq_paged_batch* b, size_t n_heads, int dtype,
+                frq_paged_kv* shape, PagedKv8* kvo, PagedRows* ro) {
+    if (!kv || !b) return fail(FRQ_INVALID, "%s: null cache or batch", who);
+    if (dtype != GGML_F32 && dtype != GGML_F16 && dtype != GGML_BF16)
+        return fail(FRQ_UNSUPPORTED, "%s: dtype %d (supported: f32, f16, bf16)", who, dtype);
+    *shape = frq_paged_kv{dtype, kv->n_pages, kv->page_size, kv->n_kv_heads, kv->head_dim, kv->k, kv->v};
+    kvo->k_scale = kv->k_scale;
+    kvo->v_scale = kv->v_scale;
+    return paged_sizes(who, shape, b, n_heads, kvo, ro);
+}
+
 int paged_buffers(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b) {
     if (!kv->k || !kv->v || !b->kv_len || (b->max_pages && !b->page_table))
         return fail(FRQ_INVALID, "%s: null cache, page_table or kv_len", who);
@@ -1480,20 +1498,12 @@ int paged_operand(const char* who, const char* name, int dtype, const void* p, s
     return FRQ_OK;
 }
 
-int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
-                    size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes, void* out,
-                    size_t ldo) {
+// The operands of an attention call that needs `need` bytes of workspace.
+int paged_attend_operands(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype, size_t n_heads,
+                          const void* q, size_t ldq, float scale, void* work, size_t work_bytes, size_t need, void* out,
+                          size_t ldo, PagedAttendArgs* a) {
     int rc;
-    PagedAttendArgs a{};
-    if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
-    if (!paged_types(kv->dtype, dtype))
-        return fail(FRQ_UNSUPPORTED, "%s: dtype %d over a cache of dtype %d", who, dtype, kv->dtype);
-    const bool rows16 = pg_kind(a.kv, a.rows, (int)n_heads, (int)kv->head_dim) == PG_ROWS16;
-    if (rows16 ? !paged_rows16_fits(a.kv, a.rows, (int)n_heads, (int)kv->head_dim)
-               : !paged_prefill_fits(a.kv, a.rows, (int)n_heads))
-        return fail(FRQ_UNSUPPORTED, "%s: rows=%zu n_seqs=%zu of up to %d tokens", who, b->rows, b->n_seqs, a.rows.cap);
     const bool none = b->n_seqs == 0 || b->rows == 0;
-    const size_t need = frq_paged_attention_workspace(kv, b, n_heads);
     if (!none && work_bytes < need)
         return fail(FRQ_WORKSPACE, "%s: workspace %zu < %zu bytes", who, work_bytes, need);
     if (!none && need && !work) return fail(FRQ_INVALID, "%s: null workspace", who);
@@ -1501,31 +1511,22 @@ int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, co
     if (!none && (rc = paged_buffers(who, kv, b))) return rc;
     if (!none && (rc = paged_operand(who, "q", dtype, q, n_heads * kv->head_dim, ldq))) return rc;
     if (!none && (rc = paged_operand(who, "out", dtype, out, n_heads * kv->head_dim, ldo))) return rc;
-    DevGuard guard(dev);
-    if ((rc = use_device(dev)) || none) return rc;
-    a.n_heads = (int)n_heads;
-    a.q = q;
-    a.ldq = (int)ldq;
-    a.scale = scale;
-    a.out = out;
-    a.ldo = (int)ldo;
-    a.work = work;
-    HIP_TRY((rows16 ? launch_paged_rows16 : launch_paged_prefill)(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
+    a->n_heads = (int)n_heads;
+    a->q = q;
+    a->ldq = (int)ldq;
+    a->scale = scale;
+    a->out = out;
+    a->ldo = (int)ldo;
+    a->work = work;
     return FRQ_OK;
 }
 
-}  // namespace
-
-int frq_paged_append(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype, size_t n_heads,
-                     const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv,
-                     const float* rope_cos, const float* rope_sin, size_t rope_rows, void* q_out, size_t ldqo) {
-    const char* who = "paged_append";
+// The operands of an append.
+int paged_append_operands(const char* who, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype, size_t n_heads,
+                          const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv,
+                          const float* rope_cos, const float* rope_sin, size_t rope_rows, void* q_out, size_t ldqo,
+                          PagedAppendArgs* a) {
     int rc;
-    PagedAppendArgs a{};
-    if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
-    if (!paged_types(kv->dtype, dtype))
-        return fail(FRQ_UNSUPPORTED, "%s: dtype %d into a cache of dtype %d", who, dtype, kv->dtype);
-    if (b->rows > (size_t)PG_GRID) return fail(FRQ_UNSUPPORTED, "%s: rows=%zu (up to %ld)", who, b->rows, PG_GRID);
     const bool none = b->n_seqs == 0 || b->rows == 0;
     if (!none && (rc = paged_buffers(who, kv, b))) return rc;
     if (!q != !q_out) return fail(FRQ_INVALID, "%s: q and q_out go together", who);
@@ -1541,21 +1542,138 @@ int frq_paged_append(frq_device* dev, const frq_paged_kv* kv, const frq_paged_ba
     if (!none && q && (rc = paged_operand(who, "q_out", dtype, q_out, n_heads * hd, ldqo))) return rc;
     if (!none && (rc = paged_operand(who, "k", dtype, k, kw, ldk))) return rc;
     if (!none && (rc = paged_operand(who, "v", dtype, v, kw, ldv))) return rc;
+    a->n_heads = (int)n_heads;
+    a->q = q;
+    a->ldq = (int)ldq;
+    a->k = k;
+    a->ldk = (int)ldk;
+    a->v = v;
+    a->ldv = (int)ldv;
+    a->cos = rope_cos;
+    a->sin = rope_sin;
+    a->rope_rows = (int)rope_rows;
+    a->q_out = q_out;
+    a->ldqo = (int)ldqo;
+    return FRQ_OK;
+}
+
+int paged_attention(const char* who, frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
+                    size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes, void* out,
+                    size_t ldo) {
+    int rc;
+    PagedAttendArgs a{};
+    if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
+    if (!paged_types(kv->dtype, dtype))
+        return fail(FRQ_UNSUPPORTED, "%s: dtype %d over a cache of dtype %d", who, dtype, kv->dtype);
+    const bool rows16 = pg_kind(a.kv, a.rows, (int)n_heads, (int)kv->head_dim) == PG_ROWS16;
+    if (rows16 ? !paged_rows16_fits(a.kv, a.rows, (int)n_heads, (int)kv->head_dim)
+               : !paged_prefill_fits(a.kv, a.rows, (int)n_heads))
+        return fail(FRQ_UNSUPPORTED, "%s: rows=%zu n_seqs=%zu of up to %d tokens", who, b->rows, b->n_seqs, a.rows.cap);
+    const size_t need = frq_paged_attention_workspace(kv, b, n_heads);
+    if ((rc = paged_attend_operands(who, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes, need, out, ldo, &a)))
+        return rc;
+    DevGuard guard(dev);
+    if ((rc = use_device(dev)) || b->n_seqs == 0 || b->rows == 0) return rc;
+    HIP_TRY((rows16 ? launch_paged_rows16 : launch_paged_prefill)(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
+    return FRQ_OK;
+}
+
+int paged8_attention(const char* who, frq_device* dev, const frq_paged_kv8* kv, const frq_paged_batch* b, int dtype,
+                     size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes, void* out,
+                     size_t ldo) {
+    int rc;
+    PagedAttendArgs a{};
+    PagedKv8 c{};
+    frq_paged_kv shape;
+    if ((rc = paged8_args(who, kv, b, n_heads, dtype, &shape, &c, &a.rows))) return rc;
+    if (!paged8_rows16_fits(c, a.rows, (int)n_heads, (int)kv->head_dim))
+        return fail(FRQ_UNSUPPORTED, "%s: rows=%zu n_seqs=%zu of up to %d tokens", who, b->rows, b->n_seqs, a.rows.cap);
+    const size_t need = frq_paged8_attention_workspace(kv, b, n_heads);
+    if ((rc = paged_attend_operands(who, &shape, b, dtype, n_heads, q, ldq, scale, work, work_bytes, need, out, ldo,
+                                    &a)))
+        return rc;
+    const bool none = b->n_seqs == 0 || b->rows == 0;
+    if (!none && (!c.k_scale || !c.v_scale)) return fail(FRQ_INVALID, "%s: null scales", who);
     DevGuard guard(dev);
     if ((rc = use_device(dev)) || none) return rc;
-    a.n_heads = (int)n_heads;
-    a.q = q;
-    a.ldq = (int)ldq;
-    a.k = k;
-    a.ldk = (int)ldk;
-    a.v = v;
-    a.ldv = (int)ldv;
-    a.cos = rope_cos;
-    a.sin = rope_sin;
-    a.rope_rows = (int)rope_rows;
-    a.q_out = q_out;
-    a.ldqo = (int)ldqo;
-    HIP_TRY(launch_paged_append(kv->dtype, dtype, (int)hd, a, dev->stream));
+    HIP_TRY(launch_paged8_rows16(dtype, (int)kv->head_dim, a, c, dev->stream));
+    return FRQ_OK;
+}
+
+}  // namespace
+
+int frq_paged_append(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype, size_t n_heads,
+                     const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv,
+                     const float* rope_cos, const float* rope_sin, size_t rope_rows, void* q_out, size_t ldqo) {
+    const char* who = "paged_append";
+    int rc;
+    PagedAppendArgs a{};
+    if ((rc = paged_args(who, kv, b, n_heads, &a.kv, &a.rows))) return rc;
+    if (!paged_types(kv->dtype, dtype))
+        return fail(FRQ_UNSUPPORTED, "%s: dtype %d into a cache of dtype %d", who, dtype, kv->dtype);
+    if (b->rows > (size_t)PG_GRID) return fail(FRQ_UNSUPPORTED, "%s: rows=%zu (up to %ld)", who, b->rows, PG_GRID);
+    if ((rc = paged_append_operands(who, kv, b, dtype, n_heads, q, ldq, k, ldk, v, ldv, rope_cos, rope_sin, rope_rows,
+                                    q_out, ldqo, &a)))
+        return rc;
+    DevGuard guard(dev);
+    if ((rc = use_device(dev)) || b->n_seqs == 0 || b->rows == 0) return rc;
+    HIP_TRY(launch_paged_append(kv->dtype, dtype, (int)kv->head_dim, a, dev->stream));
+    return FRQ_OK;
+}
+
+int frq_paged8_append(frq_device* dev, const frq_paged_kv8* kv, const frq_paged_batch* b, int dtype, size_t n_heads,
+                      const void* q, size_t ldq, const void* k, size_t ldk, const void* v, size_t ldv,
+                      const float* rope_cos, const float* rope_sin, size_t rope_rows, void* q_out, size_t ldqo) {
+    const char* who = "paged8_append";
+    int rc;
+    PagedAppendArgs a{};
+    PagedKv8 c{};
+    frq_paged_kv shape;
+    if ((rc = paged8_args(who, kv, b, n_heads, dtype, &shape, &c, &a.rows))) return rc;
+    const size_t parts = (n_heads * kv->head_dim / 16 + 255) / 256;  // workgroups of a row's q at most
+    if (b->rows > (size_t)PG_GRID / parts ||
+        (long)(b->rows * parts) + paged8_append_waves(c, a.rows) / 4 >= PG_GRID)
+        return fail(FRQ_UNSUPPORTED, "%s: rows=%zu n_seqs=%zu", who, b->rows, b->n_seqs);
+    if ((rc = paged_append_operands(who, &shape, b, dtype, n_heads, q, ldq, k, ldk, v, ldv, rope_cos, rope_sin,
+                                    rope_rows, q_out, ldqo, &a)))
+        return rc;
+    const bool none = b->n_seqs == 0 || b->rows == 0;
+    if (!none && (!c.k_scale || !c.v_scale)) return fail(FRQ_INVALID, "%s: null scales", who);
+    DevGuard guard(dev);
+    if ((rc = use_device(dev)) || none) return rc;
+    HIP_TRY(launch_paged8_append(dtype, (int)kv->head_dim, a, c, dev->stream));
+    return FRQ_OK;
+}
+
+int frq_paged_plan(frq_device* dev, size_t n_seqs, size_t max_pages, size_t page_size, size_t n_pages, size_t rows,
+                   const int32_t* tokens, const int32_t* kv_len, int32_t* kv_len_out, int32_t* page_table,
+                   int32_t* free_pages, const int32_t* n_free, int32_t* n_free_out, int32_t* row_start, int64_t* slots,
+                   int32_t* positions) {
+    const char* who = "paged_plan";
+    const size_t most = (size_t)1 << 30;
+    if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)))
+        return fail(FRQ_UNSUPPORTED, "%s: page_size=%zu (a power of two, 16 .. 1024)", who, page_size);
+    if (max_pages > most / page_size)
+        return fail(FRQ_UNSUPPORTED, "%s: max_pages=%zu page_size=%zu", who, max_pages, page_size);
+    if (n_seqs > most || n_pages > most || rows > most)
+        return fail(FRQ_UNSUPPORTED, "%s: n_seqs=%zu n_pages=%zu rows=%zu (up to 2^30)", who, n_seqs, n_pages, rows);
+    if (!n_free || !n_free_out || !row_start || (n_pages && !free_pages))
+        return fail(FRQ_INVALID, "%s: null free_pages, n_free or row_start", who);
+    if (n_seqs && (!tokens || !kv_len || !kv_len_out || (max_pages && !page_table)))
+        return fail(FRQ_INVALID, "%s: null tokens, kv_len or page_table", who);
+    for (const void* p : {(const void*)tokens, (const void*)kv_len, (const void*)kv_len_out, (const void*)page_table,
+                          (const void*)free_pages, (const void*)n_free, (const void*)n_free_out,
+                          (const void*)row_start, (const void*)positions})
+        if (!aligned4(p)) return fail(FRQ_MISALIGNED, "%s: an array not 4-byte aligned", who);
+    if ((uintptr_t)slots & 7) return fail(FRQ_MISALIGNED, "%s: slots not 8-byte aligned", who);
+    DevGuard guard(dev);
+    int rc = use_device(dev);
+    if (rc) return rc;
+    int log_ps = 4;
+    while (((size_t)1 << log_ps) < page_size) log_ps++;
+    const PagedPlanArgs a{(int)n_seqs, (int)max_pages, log_ps, (int)n_pages, (int)rows, tokens, kv_len, kv_len_out,
+                          page_table, free_pages, n_free, n_free_out, row_start, slots, positions};
+    HIP_TRY(launch_paged_plan(a, dev->stream));
     return FRQ_OK;
 }
 
@@ -1581,6 +1699,30 @@ int frq_paged_attention_prefill(frq_device* dev, const frq_paged_kv* kv, const f
                                 void* out, size_t ldo) {
     return paged_attention("paged_attention_prefill", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
                            out, ldo);
+}
+
+size_t frq_paged8_attention_workspace(const frq_paged_kv8* kv, const frq_paged_batch* b, size_t n_heads) {
+    frq_paged_kv shape;
+    PagedKv8 k;
+    PagedRows r;
+    if (paged8_args("paged8_attention_workspace", kv, b, n_heads, GGML_F32, &shape, &k, &r)) return 0;
+    return paged8_rows16_work_bytes(k, r, (int)n_heads, (int)kv->head_dim);
+}
+
+int frq_paged8_attention_decode(frq_device* dev, const frq_paged_kv8* kv, const frq_paged_batch* b, int dtype,
+                                size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes,
+                                void* out, size_t ldo) {
+    if (b && b->row_start)
+        return fail(FRQ_INVALID, "paged8_attention_decode: one row a sequence (row_start must be NULL)");
+    return paged8_attention("paged8_attention_decode", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes, out,
+                            ldo);
+}
+
+int frq_paged8_attention_prefill(frq_device* dev, const frq_paged_kv8* kv, const frq_paged_batch* b, int dtype,
+                                 size_t n_heads, const void* q, size_t ldq, float scale, void* work, size_t work_bytes,
+                                 void* out, size_t ldo) {
+    return paged8_attention("paged8_attention_prefill", dev, kv, b, dtype, n_heads, q, ldq, scale, work, work_bytes,
+                            out, ldo);
 }
 
 int frq_fill_random_bits(frq_device* dev, uint32_t* y, size_t n, uint64_t start, uint64_t seed, uint32_t base,

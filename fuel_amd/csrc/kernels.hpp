@@ -306,4 +306,28 @@ bool paged_prefill_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
 size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 
+// paged8.hip: the same over an 8-bit cache (paged8.hpp; `kv` of the arguments is not
+// read).  Wavefronts of an append beside those of q; the grid has to hold them.
+struct PagedKv8;
+long paged8_append_waves(const PagedKv& kv, const PagedRows& r);
+hipError_t launch_paged8_append(int dtype, int hd, const PagedAppendArgs& p, const PagedKv8& c, hipStream_t s);
+bool paged8_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
+size_t paged8_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
+hipError_t launch_paged8_rows16(int dtype, int hd, const PagedAttendArgs& p, const PagedKv8& c, hipStream_t s);
+// paged_plan.hip: pages for the tokens that sequences ask for or drop.
+struct PagedPlanArgs {
+    int n_seqs, max_pages, log_ps, n_pages, rows;
+    const int* tokens;
+    const int* kv_len;
+    int* kv_len_out;
+    int* table;
+    int* free_pages;
+    const int* n_free;
+    int* n_free_out;
+    int* row_start;
+    int64_t* slots;  // null: none
+    int* positions;
+};
+hipError_t launch_paged_plan(const PagedPlanArgs& p, hipStream_t s);
+
 }  // namespace frq

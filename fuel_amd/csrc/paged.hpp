@@ -69,16 +69,16 @@ enum PagedKind { PG_ROWS16, PG_TILES, PG_CUT };
 // longer ones whole tiles gain up to 10 % where all are as long as the longest
 // and there is one for every CU, and lose more where they are not.)
 constexpr int PG_WHOLE_KEYS = 1024;
-inline bool pg_whole(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+inline bool pg_whole(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size) {
     const long tiles = pg_tiles_bound(r, n_heads / kv.kv_heads, 16) * kv.kv_heads;
     return (long)r.cap * hd <= (tiles >= 128 ? 65536 : 32768);
 }
-inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size = 2) {
     if (!r.row_start) return PG_ROWS16;
     const int grp = n_heads / kv.kv_heads;
     const double k = r.cap, n16 = (double)pg_tiles_bound(r, grp, 16) * kv.kv_heads,
                  n128 = (double)pg_tiles_bound(r, grp, 128) * kv.kv_heads;
-    const double rows16 = (pg_whole(kv, r, n_heads, hd) ? 8 : 12) + n16 * k / 20000;
+    const double rows16 = (pg_whole(kv, r, n_heads, hd, size) ? 8 : 12) + n16 * k / 20000;
     const double tiles = 10 + 0.034 * k * (n128 > 256 ? n128 / 512 : 0.5);
     const double cut = r.cap <= 1 << 24 && n128 <= 4096 ? 26 + n128 * k / 15000 : 1e30;  // (its units are an int)
     if (rows16 <= tiles && rows16 <= cut) return PG_ROWS16;
@@ -210,6 +210,27 @@ __device__ __forceinline__ bool pg_word_odd(uint32_t w) {
     return (t & 0xffffu) == 0 || (t >> 16) == 0;
 }
 
+// The keys and values of four positions from j on (of one page), a multiple of 4,
+// as f32: what pg_plain() reads.
+template <class E, int HD>
+struct PgCells {
+    const E *k, *v;
+    __device__ __forceinline__ PgCells(const PagedKv& c, int page, int head, int j) {
+        const size_t row = ((((size_t)page * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * HD;
+        k = static_cast<const E*>(c.k) + row;
+        v = static_cast<const E*>(c.v) + row;
+    }
+    __device__ __forceinline__ static void read(const E* at, float (&x)[4]) {
+        E y[4];
+        __builtin_memcpy(y, __builtin_assume_aligned(at, 8), sizeof y);
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = (float)y[e];
+    }
+    // Dims d .. d + 3 of key or value u.
+    __device__ __forceinline__ void key(int u, int d, float (&x)[4]) const { read(k + u * HD + d, x); }
+    __device__ __forceinline__ void value(int u, int d, float (&x)[4]) const { read(v + u * HD + d, x); }
+};
+
 // Adds keys j0 .. j1 - 1 to a row's maximum and sums as the definition has them:
 // f32 dot products, whole weights, no key that the row does not see.  The kernels'
 // products form q and the weights in parts, and of a tile's rows some see keys that
@@ -221,8 +242,8 @@ __device__ __forceinline__ bool pg_word_odd(uint32_t w) {
 // memory: in the registers there is room for the kernels' own loops only); own_l:
 // whether l is the lane's; a weight is 2^shift at most; add(i, e, f, p, v): sum e of
 // run i becomes f times itself and p v.
-template <class E, class T, int HD, int SHARE, class Dim, class Add>
-__device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int head, const T* x, float scale,
+template <class Cells, class T, int HD, int SHARE, class Cache, class Dim, class Add>
+__device__ __forceinline__ void pg_plain(const Cache& c, const int* table, int head, const T* x, float scale,
                                          int limit, int j0, int j1, float shift, bool own_l, Dim dim, Add add,
                                          float& m, float& l) {
     constexpr int RUNS = HD / SHARE / 4, KEYS = 4;  // keys at a time: q is read once for them
@@ -231,8 +252,7 @@ __device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int
     for (int j = j0; j < j1; j += KEYS) {  // (of one page: j0 is a multiple of 16)
         bool none;
         const int page = pg_page(c, table, j, j + 1, none);
-        const size_t row = ((((size_t)page * c.kv_heads + head) << c.log_ps) + (j & ((1 << c.log_ps) - 1))) * HD;
-        const E *k = static_cast<const E*>(c.k) + row, *v = static_cast<const E*>(c.v) + row;
+        const Cells cells(c, page, head, j);
         float s[KEYS] = {}, mn = m;
 #pragma unroll 2
         for (int i = 0; i < RUNS; i++) {
@@ -240,10 +260,10 @@ __device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int
             __builtin_memcpy(z, __builtin_assume_aligned(x + dim(i), 8), sizeof z);
 #pragma unroll
             for (int u = 0; u < KEYS; u++) {
-                E y[4];
-                __builtin_memcpy(y, __builtin_assume_aligned(k + u * HD + dim(i), 8), sizeof y);
+                float y[4];
+                cells.key(u, dim(i), y);
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[u] = fmaf((float)z[e] * factor, (float)y[e], s[u]);
+                for (int e = 0; e < 4; e++) s[u] = fmaf((float)z[e] * factor, y[e], s[u]);
             }
         }
 #pragma unroll
@@ -264,10 +284,10 @@ __device__ __forceinline__ void pg_plain(const PagedKv& c, const int* table, int
             if (own_l) l += p;
 #pragma unroll
             for (int i = 0; i < RUNS; i++) {
-                E y[4];
-                __builtin_memcpy(y, __builtin_assume_aligned(v + u * HD + dim(i), 8), sizeof y);
+                float y[4];
+                cells.value(u, dim(i), y);
 #pragma unroll
-                for (int e = 0; e < 4; e++) add(i, e, u ? 1.0f : f, p, (float)y[e]);
+                for (int e = 0; e < 4; e++) add(i, e, u ? 1.0f : f, p, y[e]);
                 if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (few loads at once: the sums fill the registers)
             }
         }
@@ -373,6 +393,26 @@ struct PgUnits {
     }
 };
 
+// The last sequence that starts at or before packed row `row`, or -1 if none
+// does or the row lies behind them all: a search in steps of 64 (one load a
+// lane, one vote).  Wave-uniform.
+__device__ __forceinline__ int pg_row_seq(const PagedRows& b, int row) {
+    if (!b.row_start) return row;
+    const int lane = threadIdx.x & 63;
+    int lo = 0, n = b.n_seqs + 1;  // the answer is the last of lo .. lo + n - 1 that starts at or before row
+    for (;;) {
+        const int step = (n + 63) >> 6, at = lane * step;
+        const bool le = at < n && b.row_start[lo + at] <= row;
+        const uint64_t v = __ballot(le);
+        if (!v) return -1;
+        const int k = 63 - __builtin_clzll(v);
+        lo += k * step;
+        if (step == 1) break;
+        n = min(step, n - k * step);
+    }
+    return lo < b.n_seqs ? lo : -1;  // (row_start[n_seqs] <= row: behind the last)
+}
+
 // Equal contiguous ranges of `total` units over n_wgs <= total workgroups: w's
 // starts at unit w * total / n_wgs, none is empty; and the one that holds unit u.
 __host__ __device__ __forceinline__ int pg_start(int w, int total, int n_wgs) {
@@ -388,6 +428,11 @@ __device__ __forceinline__ PgJoin pg_join(bool cut, int rows, const PgSeq& q, in
                                           int total, int n_wgs, int slot) {
     if (!cut) return PgJoin{};
     return PgJoin{rows, pg_owner(last_unit, total, n_wgs), slot, q.row0, q.kv - q.n, head, i0, 0};
+}
+
+template <class T>
+constexpr int pg_dtype() {
+    return std::is_same<T, float>::value ? GGML_F32 : std::is_same<T, _Float16>::value ? GGML_F16 : GGML_BF16;
 }
 
 // Calls f.run<E, T, HD>() for the types of a call.

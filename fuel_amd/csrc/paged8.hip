@@ -1,0 +1,579 @@
+// Operators of a batch of sequences over an 8-bit paged KV cache (paged8.hpp):
+// append, and attention of few rows a sequence.
+//
+// Append.  e4m3 has a relative step of 2^-4 .. 2^-3 between its least normal number
+// and its largest, so a block of 16 positions of a head needs a power of two alone:
+//   2^e, the least for which its largest |value| is at most 448 * 2^e
+// (e from -127 to 120).  Rows that join older ones in their block take the block's
+// scale, or raise it: then the older codes are rounded once more, exactly but for
+// those that fall below the least normal number, 2^-14.8 of the block's largest.
+//
+// Attention: as paged.hip's 16-row tiles, 64 keys at a time.  K's codes go to the
+// matrix pipe as f16 (bf16 for bf16 rows) without their scale, exactly; a group of
+// 16 keys' scale is a factor of its scores, in f32.  V's go there as bf16 values,
+// exactly, so that no weight has to carry a scale.  f32 rows: q in two parts of f16,
+// weights in three of bf16.  16-bit rows: q as it is, weights in two parts of bf16.
+#include <hip/hip_runtime.h>
+
+#include "common.hpp"
+#include "kernels.hpp"
+#include "paged8.hpp"
+#include "paged_rows.hpp"
+
+namespace frq {
+
+namespace {
+
+template <class T, int HD>
+struct Rows8 {
+    using Cache = PagedKv8;
+    using Row = T;
+    static constexpr bool WIDE = std::is_same<T, float>::value;
+    using E = typename std::conditional<WIDE, _Float16, T>::type;  // of q and k in their products
+    using P = PgElem<__bf16>;                                      // of weights and v
+    using q8 = typename PgElem<E>::v8;
+    using v8 = P::v8;
+    static constexpr int NQ = WIDE ? 2 : 1, NP = WIDE ? 3 : 2;
+    static constexpr int DIM = HD, KS = HD / 32, VW = HD / 16;
+    static constexpr int STEP = 64, BYTES = HD;
+
+    q8 q[NQ][KS];
+    float factor;  // score = product * factor * the key's scale, in units of log2
+    int limit;     // the row's position; -1: it sees nothing
+    pg_f4 o[VW];
+    float m, l;
+
+    typedef uint32_t ValueWord __attribute__((ext_vector_type(VW / 4)));
+    struct KeyRegs {
+        pg_u4 w[4][HD / 64];
+    };
+    struct ValueRegs {
+        ValueWord w[16];
+    };
+
+    // Lane 16 g + r takes row r: in step t of the products dims 64 (t / 2) + 16 g +
+    // 8 (t % 2) + e, so that a lane's 16 codes of a key are one load.
+    __device__ void load_q(const T* x, float scale) {
+        const int g = (threadIdx.x & 63) >> 4;
+        pd_load_q<E>(q, factor, x, scale, [&](int t) { return 64 * (t >> 1) + 16 * g + 8 * (t & 1); });
+    }
+
+    __device__ void start() {
+#pragma unroll
+        for (int t = 0; t < VW; t++) o[t] = pg_f4{0.f, 0.f, 0.f, 0.f};
+        m = PG_LEAST;
+        l = 0.0f;
+    }
+
+    // The loads of 64 keys: group a's 16 rows start at ka[a] / va[a].  ONCE:
+    // nothing else of the call reads them, so they go past the caches.
+    template <bool ONCE, class W>
+    __device__ static W load(const uint8_t* p) {
+        return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const W*>(p)) : *reinterpret_cast<const W*>(p);
+    }
+    template <bool ONCE>
+    __device__ static void load_k(KeyRegs& k, const uint8_t* const (&ka)[4]) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int a = 0; a < 4; a++)
+#pragma unroll
+            for (int c = 0; c < HD / 64; c++) k.w[a][c] = load<ONCE, pg_u4>(ka[a] + r * HD + 64 * c + 16 * g);
+    }
+    template <bool ONCE>
+    __device__ static void load_v(ValueRegs& v, const uint8_t* const (&va)[4]) {
+        const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+#pragma unroll
+        for (int a = 0; a < 4; a++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v.w[4 * a + i] = load<ONCE, ValueWord>(va[a] + (4 * g + i) * HD + VW * r);
+    }
+
+    // What holds for the groups of a block of 64 keys from j0: their scales (2^0 for
+    // groups without keys, so that what is cleared stays 0), and which keys a row
+    // sees: none past its position, past the sequence's length kv or in a page that
+    // is none (bad: NaN).
+    struct Block {
+        int j0, kv, ks[4], vs[4];
+        uint32_t bad;
+    };
+
+    // The block's scores in log2 units: s[4 a + i] of key 16 a + 4 g + i.
+    template <bool MASK>
+    __device__ void scores(const KeyRegs& k, const Block& b, float (&s)[16]) const {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            pg_f4 st = pg_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int t = 0; t < KS; t++) {
+                const q8 x = p8_eight<E>(k.w[a][t >> 1][2 * (t & 1)], k.w[a][t >> 1][2 * (t & 1) + 1], 1.0f);
+#pragma unroll
+                for (int p = NQ - 1; p >= 0; p--) st = PgElem<E>::mfma16(x, q[p][t], st);
+            }
+            const float unit = p8_factor(b.ks[a]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float v = st[i] * factor * unit;
+                if constexpr (MASK) {
+                    if ((b.bad >> a) & 1) v = pg_nan();
+                    if (b.j0 + 16 * a + 4 * g + i > limit) v = -__builtin_inff();
+                }
+                s[4 * a + i] = v;
+            }
+        }
+    }
+
+    // Weights of the block's scores, maximum and sums renewed: pp[b] of groups 2 b
+    // and 2 b + 1.
+    __device__ void weights(const float (&s)[16], v8 (&pp)[2][NP]) {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        const float mn = fmaxf(m, pg_row_max(top));
+        const float c = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before: l = o = 0)
+        m = mn;
+        l *= c;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float rest = __builtin_amdgcn_exp2f(s[i] - mn + P::TOP);
+            l += rest;
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                pp[i >> 3][p][i & 7] = (__bf16)rest;
+                rest -= (float)pp[i >> 3][p][i & 7];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < VW; t++) o[t] *= c;
+    }
+
+    __device__ void product(const ValueRegs& v, const Block& b, const v8 (&pp)[2][NP]) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            uint32_t x[8][VW / 2];  // pairs of dims of 8 keys
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float operand = p8_operand(b.vs[2 * h + (i >> 2)]);
+#pragma unroll
+                for (int w = 0; w < VW / 4; w++) {
+                    x[i][2 * w] = p8_pair<false>(v.w[8 * h + i][w], operand, __bf16());
+                    x[i][2 * w + 1] = p8_pair<true>(v.w[8 * h + i][w], operand, __bf16());
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < VW; t++) {
+                const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;  // high or low halves of two words
+                pg_u4 a;
+#pragma unroll
+                for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(x[2 * i + 1][t >> 1], x[2 * i][t >> 1], sel);
+#pragma unroll
+                for (int p = NP - 1; p >= 0; p--) o[t] = P::mfma16(__builtin_bit_cast(v8, a), pp[h][p], o[t]);
+            }
+        }
+    }
+
+    // Keys that no row of the sequence may see: their rows hold anything.
+    __device__ static void clear(ValueRegs& v, const Block& b) {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const bool none = ((b.bad >> (i >> 2)) & 1) || b.j0 + 16 * (i >> 2) + 4 * g + (i & 3) >= b.kv;
+#pragma unroll
+            for (int w = 0; w < VW / 4; w++)
+                if (none) v.w[i][w] = 0;
+        }
+    }
+
+    // Whether the block holds a NaN, or values beyond f32's range, in any lane.
+    __device__ static bool odd(const KeyRegs& k, const ValueRegs& v, const Block& b) {
+        bool any = b.bad;
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            any |= b.ks[a] > P8_TOP || b.vs[a] > P8_TOP;
+#pragma unroll
+            for (int c = 0; c < HD / 64; c++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) any |= p8_word_nan(k.w[a][c][w]);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+#pragma unroll
+            for (int w = 0; w < VW / 4; w++) any |= p8_word_nan(v.w[i][w]);
+        return __any(any);
+    }
+
+    // Keys [j0, j1) by pg_plain(); x: the row's q.
+    __device__ void plain(const PagedKv8& c, const int* table, int head, const T* x, float scale, int j0, int j1) {
+        const int g = (threadIdx.x & 63) >> 4;
+        pg_plain<P8Cells<HD>, T, HD, 4>(
+            c, table, head, x, scale, limit, j0, j1, P::TOP, g == 0, [&](int i) { return 4 * (VW * g + i); },
+            [&](int i, int e, float f, float p, float v) {
+                const int t = (4 * i + e) % VW, k = (4 * i + e) / VW;
+                o[t][k] = fmaf(p, v, o[t][k] * f);
+            },
+            m, l);
+    }
+
+    // Block i of the groups from j0 on.
+    __device__ static Block block(const P8Groups& gr, int j0, int i, int kv) {
+        Block b{j0 + 64 * i, kv, {}, {}, (uint32_t)(gr.none >> (4 * i)) & 15};
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            const bool keys = b.j0 + 16 * a < kv && !((b.bad >> a) & 1);
+            b.ks[a] = keys ? __builtin_amdgcn_readlane(gr.k_scale, 4 * i + a) : P8_ONE;
+            b.vs[a] = keys ? __builtin_amdgcn_readlane(gr.v_scale, 4 * i + a) : P8_ONE;
+        }
+        return b;
+    }
+    __device__ static void rows(const P8Groups& gr, const void* pool, int i, const uint8_t* (&at)[4]) {
+#pragma unroll
+        for (int a = 0; a < 4; a++) at[a] = static_cast<const uint8_t*>(pool) + gr.at(4 * i + a);
+    }
+
+    // One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of 64).
+    // The next block's keys are loaded as soon as this one's scores are formed, its
+    // values as soon as this one's product is.  Every row sees the keys up to all_see.
+    template <bool ONCE>
+    __device__ __forceinline__ void walk(const PagedKv8& c, const int* table, int head, int j0, int j1, int kv,
+                                         int all_see) {
+        while (j0 < j1) {
+            const int end = min(j1, j0 + 1024);
+            P8Groups gr;
+            gr.load<HD>(c, table, head, j0, kv);
+            const int last = (end - j0 + 63) / 64 - 1;
+            const uint8_t* at[4];
+            KeyRegs kr;
+            ValueRegs vr;
+            float s[16];
+            v8 pp[2][NP];
+            rows(gr, c.k, 0, at);
+            load_k<ONCE>(kr, at);
+            rows(gr, c.v, 0, at);
+            load_v<ONCE>(vr, at);
+            for (int i = 0;; i++) {
+                const Block b = block(gr, j0, i, kv);
+                const bool mask = b.j0 + 63 > all_see || b.bad;
+                if (i == last || mask) {  // (apart from the loop's body, which keeps its loads in flight)
+                    if (mask) scores<true>(kr, b, s);
+                    else scores<false>(kr, b, s);
+                    weights(s, pp);
+                    if (mask) clear(vr, b);
+                    product(vr, b, pp);
+                    if (i == last) break;
+                    rows(gr, c.k, i + 1, at);
+                    load_k<ONCE>(kr, at);
+                    rows(gr, c.v, i + 1, at);
+                    load_v<ONCE>(vr, at);
+                    continue;
+                }
+                scores<false>(kr, b, s);
+                rows(gr, c.k, i + 1, at);
+                load_k<ONCE>(kr, at);
+                weights(s, pp);
+                product(vr, b, pp);
+                rows(gr, c.v, i + 1, at);
+                load_v<ONCE>(vr, at);
+            }
+            j0 = end;
+        }
+    }
+
+    // The same keys once more, if their sums hold an infinite or NaN value: blocks of
+    // such values or of pages that are none one key after another.
+    __device__ __forceinline__ void walk_odd(const PagedKv8& c, const int* table, int head, int j0, int j1, int kv,
+                                             const T* x, float scale) {
+        if (!__any(pg_odd(o))) return;
+        start();
+#pragma unroll 1
+        for (int j = j0; j < j1; j += 64) {
+            P8Groups gr;
+            gr.load<HD>(c, table, head, j, kv);
+            const Block b = block(gr, j, 0, kv);
+            const uint8_t *ka[4], *va[4];
+            rows(gr, c.k, 0, ka);
+            rows(gr, c.v, 0, va);
+            KeyRegs kr;
+            ValueRegs vr;
+            load_k<false>(kr, ka);
+            load_v<false>(vr, va);
+            clear(vr, b);
+            if (odd(kr, vr, b)) {
+                plain(c, table, head, x, scale, j, min(j + 64, j1));
+                if (__all(pg_all_nan(o))) return;
+                continue;
+            }
+            float s[16];
+            v8 pp[2][NP];
+            scores<true>(kr, b, s);
+            weights(s, pp);
+            product(vr, b, pp);
+        }
+    }
+
+    // The row's sum over the four lanes that share it.
+    __device__ void finish() {
+        l += __shfl_xor(l, 16);
+        l += __shfl_xor(l, 32);
+    }
+};
+
+struct Rows8Call {
+    const PagedAttendArgs& p;
+    const PagedKv8& c;
+    hipStream_t s;
+    template <class T, int HD>
+    hipError_t run() const {
+        return rows16_launch<Rows8<T, HD>>(p, c, s);
+    }
+};
+
+// ---- append ----
+
+// The scale byte of values of at most amax (finite).
+__device__ __forceinline__ int p8_scale_of(float amax) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, amax);
+    // 448 = 1.75 * 2^8: exponent - 8, one more where the mantissa is past 1.75
+    const int b = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u);
+    return max(b, 0);
+}
+
+// Four codes of x * 2^(127 - b).
+__device__ __forceinline__ uint32_t p8_codes(const float* x, int b) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        y[e] = __builtin_amdgcn_ldexpf(x[e], P8_ONE - b);
+        // (of the last scale, the codes that stand for numbers of f32)
+        if (b > P8_TOP && fabsf(y[e]) < __builtin_inff()) y[e] = fminf(fmaxf(y[e], -240.0f), 240.0f);
+    }
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+}
+
+// Four codes of scale byte `was` as codes of scale byte b >= was.
+__device__ __forceinline__ uint32_t p8_again(uint32_t w, int was, int b) {
+    const float x[4] = {__builtin_amdgcn_cvt_f32_fp8((int)w, 0), __builtin_amdgcn_cvt_f32_fp8((int)w, 1),
+                        __builtin_amdgcn_cvt_f32_fp8((int)w, 2), __builtin_amdgcn_cvt_f32_fp8((int)w, 3)};
+    return was == 255 ? 0x7f7f7f7fu : p8_codes(x, P8_ONE + b - was);
+}
+
+// Workgroups below q_wgs: `parts` to a packed row, chunks of its q as paged_append_kernel
+// takes them.  The others: a wavefront takes 16 rows of codes, four lanes a row, each
+// HD / 8 dims of its lower half and those HD / 2 further (a rotation's pairs):
+//   ONE (one row a sequence)   one position's rows of up to 16 heads of k and v
+//   otherwise                  the up to 16 rows of a block, of one head of k or v
+constexpr int A8_WG = 256;
+template <class T, int HD, bool ONE>
+__global__ __launch_bounds__(A8_WG) void paged8_append_kernel(PagedKv8 c, PagedRows b, int n_heads, int q_wgs, int parts,
+                                                              const T* q, int ldq, const T* __restrict__ k, int ldk,
+                                                              const T* __restrict__ v, int ldv,
+                                                              const float* __restrict__ cs,
+                                                              const float* __restrict__ sn, int rope_rows, T* q_out,
+                                                              int ldqo) {
+    constexpr int HALF = HD / 2;
+    if ((int)blockIdx.x < q_wgs) {
+        constexpr int CP = HALF / 8;
+        const int row = (unsigned)blockIdx.x / (unsigned)parts, part = blockIdx.x - row * parts;
+        const int s = pg_row_seq(b, row);
+        if (s < 0) return;
+        const PgSeq sq = pg_seq(b, s);
+        if (row < sq.row0 || row >= sq.row0 + sq.n) return;
+        const int pos = sq.kv - sq.n + (row - sq.row0);
+        const bool bad = sq.bad || (cs && pos >= rope_rows), seen = pos >= 0 && !bad;
+        for (int e = A8_WG * part + threadIdx.x; e < CP * n_heads; e += A8_WG * parts) {
+            const int h = e / CP, i = 8 * (e % CP);
+            const T* x = q + (size_t)row * ldq + h * HD + i;
+            T lo[8], hi[8];
+            float cl[8], ch[8], sl[8], sh[8];
+            __builtin_memcpy(lo, __builtin_assume_aligned(x, 16), sizeof lo);
+            __builtin_memcpy(hi, __builtin_assume_aligned(x + HALF, 16), sizeof hi);
+            if (cs && seen) {
+                const float *ct = cs + (size_t)pos * HD + i, *st = sn + (size_t)pos * HD + i;
+                __builtin_memcpy(cl, __builtin_assume_aligned(ct, 16), sizeof cl);
+                __builtin_memcpy(ch, __builtin_assume_aligned(ct + HALF, 16), sizeof ch);
+                __builtin_memcpy(sl, __builtin_assume_aligned(st, 16), sizeof sl);
+                __builtin_memcpy(sh, __builtin_assume_aligned(st + HALF, 16), sizeof sh);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float y = (float)lo[j], z = (float)hi[j];
+                if (cs && seen) {
+                    const float u = y, w = z;
+                    y = u * cl[j] - w * sl[j];
+                    z = w * ch[j] + u * sh[j];
+                }
+                lo[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : y);
+                hi[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : z);
+            }
+            T* to = q_out + (size_t)row * ldqo + h * HD + i;
+            __builtin_memcpy(__builtin_assume_aligned(to, 16), lo, sizeof lo);
+            __builtin_memcpy(__builtin_assume_aligned(to + HALF, 16), hi, sizeof hi);
+        }
+        return;
+    }
+    constexpr int N = HD / 8;  // dims of a half a lane takes
+    const int lane = threadIdx.x & 63, sub = lane >> 2, i = N * (lane & 3);
+    const int at = __builtin_amdgcn_readfirstlane((int)((blockIdx.x - q_wgs) * (A8_WG / 64) + (threadIdx.x >> 6)));
+    int s, head, lo, hi;  // sequence, head, and the block's positions [lo, hi) that are new
+    bool value;
+    PgSeq sq;
+    const auto ends = [&](const PgSeq& x, int& first) {  // the sequence's rows that are stored: positions [first, end)
+        first = max(x.kv - x.n, 0);
+        return x.n && !x.bad ? max(first, cs ? min(x.kv, rope_rows) : x.kv) : first;
+    };
+    if constexpr (ONE) {
+        const int waves = (2 * c.kv_heads + 15) >> 4;
+        s = (unsigned)at / (unsigned)waves;
+        if (s >= b.n_seqs) return;
+        const int unit = 16 * (at - s * waves) + sub;
+        value = unit >= c.kv_heads;
+        head = unit - (value ? c.kv_heads : 0);
+        sq = pg_seq(b, s);
+        hi = ends(sq, lo);
+        if (lo >= hi) return;
+        if (head >= c.kv_heads) {  // (these lanes take no part in their group's sums)
+            head = 0;
+            hi = lo;
+        }
+    } else {
+        const auto blocks = [&](const PgSeq& x) {
+            int first;
+            const int end = ends(x, first);
+            return end > first ? ((end - 1) >> 4) - (first >> 4) + 1 : 0;
+        };
+        PgUnits<decltype(blocks)> pu(b, blocks);
+        const int unit = (unsigned)at / (unsigned)(2 * c.kv_heads);
+        if (unit >= pu.total) return;
+        int u;
+        s = pu.find(unit, u);
+        sq = pu.get(s);
+        value = (at - unit * 2 * c.kv_heads) & 1;
+        head = (at - unit * 2 * c.kv_heads) >> 1;
+        int first;
+        const int end = ends(sq, first), j0 = ((first >> 4) + u) << 4;
+        lo = max(j0, first);
+        hi = min(j0 + 16, end);
+    }
+    const int j0 = lo & ~15, pos = ONE ? lo : j0 + sub;
+    bool none;
+    const int page = pg_page(c, b.table + (size_t)s * b.max_pages, j0, sq.kv, none);
+    if (none) return;
+    const size_t row = (((size_t)page * c.kv_heads + head) << c.log_ps) + (j0 & ((1 << c.log_ps) - 1));
+    uint8_t* codes = static_cast<uint8_t*>(value ? c.v : c.k) + row * HD + i;
+    uint8_t* scale = (value ? c.v_scale : c.k_scale) + (row >> 4);
+    const bool mine = pos >= lo && pos < hi;
+    float x[2][N];
+#pragma unroll
+    for (int e = 0; e < N; e++) x[0][e] = x[1][e] = 0.0f;
+    float amax = 0.0f;
+    if (mine) {
+        const T* from = (value ? v : k) + (size_t)(sq.row0 + pos - (sq.kv - sq.n)) * (value ? ldv : ldk) + head * HD + i;
+        T a[N], z[N];
+        __builtin_memcpy(a, __builtin_assume_aligned(from, 16), sizeof a);
+        __builtin_memcpy(z, __builtin_assume_aligned(from + HALF, 16), sizeof z);
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            x[0][e] = (float)a[e];
+            x[1][e] = (float)z[e];
+        }
+        if (cs && !value) {
+            const float *ct = cs + (size_t)pos * HD + i, *st = sn + (size_t)pos * HD + i;
+            float cl[N], ch[N], sl[N], sh[N];
+            __builtin_memcpy(cl, __builtin_assume_aligned(ct, 16), sizeof cl);
+            __builtin_memcpy(ch, __builtin_assume_aligned(ct + HALF, 16), sizeof ch);
+            __builtin_memcpy(sl, __builtin_assume_aligned(st, 16), sizeof sl);
+            __builtin_memcpy(sh, __builtin_assume_aligned(st + HALF, 16), sizeof sh);
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float y = x[0][e], w = x[1][e];
+                x[0][e] = y * cl[e] - w * sl[e];
+                x[1][e] = w * ch[e] + y * sh[e];
+            }
+        }
+#pragma unroll
+        for (int d = 0; d < 2; d++)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float y = fabsf(x[d][e]);
+                amax = y < __builtin_inff() ? fmaxf(amax, y) : amax;
+            }
+    }
+#pragma unroll
+    for (int d = 1; d < (ONE ? 4 : 64); d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+    if (ONE && hi <= lo) return;
+    int byte = p8_scale_of(amax);
+    if (lo > j0) {  // older rows
+        const int was = *scale, need = byte;
+        byte = was == 255 ? need : max(was, need);
+        if (byte != was) {
+            const auto again = [&](uint8_t* to) {
+                uint32_t w[N / 4];
+                __builtin_memcpy(w, __builtin_assume_aligned(to, 8), sizeof w);
+#pragma unroll
+                for (int e = 0; e < N / 4; e++) w[e] = p8_again(w[e], was, byte);
+                __builtin_memcpy(__builtin_assume_aligned(to, 8), w, sizeof w);
+            };
+            for (int r = ONE ? 0 : sub; r < lo - j0; r += ONE ? 1 : 16) {
+                again(codes + r * HD);
+                again(codes + r * HD + HALF);
+            }
+        }
+    }
+    if (mine) {
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            uint32_t w[N / 4];
+#pragma unroll
+            for (int e = 0; e < N / 4; e++) w[e] = p8_codes(x[d] + 4 * e, byte);
+            __builtin_memcpy(__builtin_assume_aligned(codes + (pos - j0) * HD + d * HALF, 8), w, sizeof w);
+        }
+    }
+    if (ONE ? (lane & 3) == 0 : lane == 0) *scale = (uint8_t)byte;
+}
+
+struct Append8Call {
+    const PagedAppendArgs& p;
+    const PagedKv8& c;
+    hipStream_t s;
+    template <class T, int HD>
+    hipError_t run() const {
+        const int chunks = HD / 16 * (p.q ? p.n_heads : 0);
+        const int parts = chunks ? (chunks + A8_WG - 1) / A8_WG : 0;
+        const long q_wgs = (long)p.rows.rows * parts, waves = paged8_append_waves(c, p.rows);
+        const long wgs = q_wgs + (waves + A8_WG / 64 - 1) / (A8_WG / 64);
+        const auto kernel = p.rows.row_start ? paged8_append_kernel<T, HD, false> : paged8_append_kernel<T, HD, true>;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(A8_WG), 0, s, c, p.rows, p.n_heads, (int)q_wgs, parts,
+                           static_cast<const T*>(p.q), p.ldq, static_cast<const T*>(p.k), p.ldk,
+                           static_cast<const T*>(p.v), p.ldv, p.cos, p.sin, p.rope_rows, static_cast<T*>(p.q_out),
+                           p.ldqo);
+        return hipGetLastError();
+    }
+};
+
+}  // namespace
+
+long paged8_append_waves(const PagedKv& kv, const PagedRows& r) {
+    // n rows lie in at most n / 16 + 2 blocks of 16 positions
+    return r.row_start ? ((long)r.rows / 16 + 2l * (r.n_seqs < r.rows ? r.n_seqs : r.rows)) * 2 * kv.kv_heads
+                       : (long)r.n_seqs * ((2 * kv.kv_heads + 15) / 16);
+}
+
+hipError_t launch_paged8_append(int dtype, int hd, const PagedAppendArgs& p, const PagedKv8& c, hipStream_t s) {
+    if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
+    return paged8_with_types(dtype, hd, Append8Call{p, c, s});
+}
+
+size_t paged8_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    return rows16_work_bytes(kv, r, n_heads, hd, 1);
+}
+
+bool paged8_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    return rows16_fits(kv, r, n_heads, hd, 1);
+}
+
+hipError_t launch_paged8_rows16(int dtype, int hd, const PagedAttendArgs& p, const PagedKv8& c, hipStream_t s) {
+    if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
+    return paged8_with_types(dtype, hd, Rows8Call{p, c, s});
+}
+
+}  // namespace frq

@@ -330,7 +330,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                 const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
                 if (AGAIN && pf_odd<X, E, 64 / KW>(kt, vt, bad >> (key0 >> 4))) {
                     if (!__all(pg_all_nan(o)))
-                        pg_plain<E, T, HD, 2>(
+                        pg_plain<PgCells<E, HD>, T, HD, 2>(
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
                             min(jw + 32 * NA, last + 1), X::SHIFT, h == 0, [&](int i) { return 8 * i + 4 * h; },
                             [&](int i, int e, float f, float p, float v) {
@@ -525,11 +525,7 @@ struct PrefillCall {
                            p.rows, grp, q, p.ldq, p.scale, out, p.ldo, part, joins);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        return launch_paged_join(dtype_of<T>(), HD, joins, part, PG_WGS, tiles, PF_ROWS, PF_ROWS, grp, p.out, p.ldo, s);
-    }
-    template <class T>
-    static int dtype_of() {
-        return std::is_same<T, float>::value ? GGML_F32 : std::is_same<T, _Float16>::value ? GGML_F16 : GGML_BF16;
+        return launch_paged_join(pg_dtype<T>(), HD, joins, part, PG_WGS, tiles, PF_ROWS, PF_ROWS, grp, p.out, p.ldo, s);
     }
 };
 

@@ -423,6 +423,78 @@ int frq_paged_attention_prefill(frq_device *dev, const frq_paged_kv *kv, const f
                                 size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
                                 size_t work_bytes, void *out_dev, size_t ldo);
 
+/* ---- the same over a cache of 8 bits a value ----
+ * k and v are pools of pages [n_pages, n_kv_heads, page_size, head_dim] of e4m3
+ * codes (OCP's: largest 448, no infinities, 0x7f and 0xff NaN), 16-byte aligned;
+ * k_scale and v_scale [n_pages, n_kv_heads, page_size / 16] bytes b (OCP's e8m0), a
+ * scale for every 16 positions of a head:
+ *   value = code * 2^(b - 127), b = 255: NaN
+ * Sizes as frq_paged_kv's.  No contents are wrong ones: a pool may start as zeros. */
+typedef struct frq_paged_kv8 {
+    size_t n_pages, page_size, n_kv_heads, head_dim;
+    uint8_t *k, *v, *k_scale, *v_scale;
+} frq_paged_kv8;
+/* frq_paged_append into such a cache (dtype FRQ_F32, FRQ_F16 or FRQ_BF16).  The
+ * rows of a head that lie in one block of 16 positions get the least scale, 2^-127 to
+ * 2^120, under which their largest finite magnitude is at most 448, or the block's
+ * present one, if older rows are in the block and theirs is larger; each value the
+ * nearest code (ties to even).  Where the scale grows the older rows' codes are
+ * rounded to it once more (exactly, but for values below 2^-14 of the block's
+ * largest).  Infinite and NaN values become NaN codes and take no part in the scale;
+ * older rows under a NaN scale become NaN.  Positions of the block behind the
+ * appended rows are no part of the cache any more: a sequence whose end was moved
+ * back may be appended to, its later rows are not kept.  Two rows must not lie in the
+ * same block of a page but those of one sequence; nothing of k and v is appended by
+ * a batch whose sequences have more than `rows` rows together. */
+int frq_paged8_append(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype, size_t n_heads,
+                      const void *q_dev, size_t ldq, const void *k_dev, size_t ldk, const void *v_dev, size_t ldv,
+                      const float *rope_cos_dev, const float *rope_sin_dev, size_t rope_rows, void *q_out_dev,
+                      size_t ldqo);
+/* frq_paged_attention_workspace, _decode and _prefill over such a cache, dtype
+ * FRQ_F32, FRQ_F16 or FRQ_BF16.  Codes and scales are taken as the values that they
+ * stand for, scores, softmax and sums are f32: f32 operands are multiplied in parts
+ * that hold them to 2^-22.  With 16-bit rows a softmax weight is held to 2^-16 for the
+ * product with V, in batches of many rows, as the sizes of the structs have it, to
+ * 2^-8 (their sum is not rounded).  A scale counts as 2^119 at most in a row's sums
+ * that are finite; NaN as frq_paged_batch has it. */
+size_t frq_paged8_attention_workspace(const frq_paged_kv8 *kv, const frq_paged_batch *batch, size_t n_heads);
+int frq_paged8_attention_decode(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype,
+                                size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
+                                size_t work_bytes, void *out_dev, size_t ldo);
+int frq_paged8_attention_prefill(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype,
+                                 size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
+                                 size_t work_bytes, void *out_dev, size_t ldo);
+
+/* ---- pages of a pool for the sequences of a batch ----
+ * A step's page table, lengths, row ranges and slots, on the device from what each
+ * sequence asks for, so that a captured step needs no host.  free_pages [n_pages] with
+ * *n_free entries is the stack of the pool's free pages, page_table [n_seqs,
+ * max_pages], kv_len [n_seqs] as a frq_paged_batch has them before the step; tokens
+ * [n_seqs]:
+ *   t < 0   the sequence's last -t tokens (all, if it has fewer) are dropped; the
+ *           pages past its new end go on the stack, sequence by sequence, page by page
+ *           (of those that the stack has no room for, none)
+ *   t > 0   t tokens are granted if the table holds them (kv_len + t <= max_pages *
+ *           page_size), the pages that sequences up to this one ask for fit the stack
+ *           or this one asks for none, and the tokens that sequences up to this one
+ *           ask for are at most `rows`; granted or not, those that the table holds
+ *           count in these sums.  Its new pages are the stack's topmost, in order.
+ * after all drops.  Written:
+ *   kv_len_out [n_seqs], *n_free_out: as after the step; they may be kv_len and n_free
+ *   page_table: the new pages' entries; free_pages: the dropped pages
+ *   row_start [n_seqs + 1]: the granted tokens as packed rows (an empty range: not
+ *     granted)
+ *   slots, positions [rows] (or NULL): page * page_size + offset and position of each
+ *     packed row, -1 for rows from row_start[n_seqs] on
+ * A kv_len that is none (negative, or more than the table holds) stays, its sequence
+ * gets and gives nothing; *n_free counts as 0 .. n_pages.  page_size is a power of two
+ * from 16 to 1024, max_pages * page_size, n_seqs, n_pages and rows at most 2^30.  The
+ * arrays are apart but for the two pairs.  Asynchronous, allocates nothing. */
+int frq_paged_plan(frq_device *dev, size_t n_seqs, size_t max_pages, size_t page_size, size_t n_pages, size_t rows,
+                   const int32_t *tokens_dev, const int32_t *kv_len_dev, int32_t *kv_len_out_dev,
+                   int32_t *page_table_dev, int32_t *free_pages_dev, const int32_t *n_free_dev, int32_t *n_free_out_dev,
+                   int32_t *row_start_dev, int64_t *slots_dev, int32_t *positions_dev);
+
 /* ---- integer taps (build-internal parity probes; no reference counterpart) ----
  * Quantize rows of f32 activations into fuel's activation blocks
  * (BlockQ8K::from_float k_quants.rs:2230-2267, BlockQ8_0::from_float
