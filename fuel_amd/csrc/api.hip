@@ -1586,7 +1586,9 @@ int paged8_attention(const char* who, frq_device* dev, const frq_paged_kv8* kv, 
     PagedKv8 c{};
     frq_paged_kv shape;
     if ((rc = paged8_args(who, kv, b, n_heads, dtype, &shape, &c, &a.rows))) return rc;
-    if (!paged8_rows16_fits(c, a.rows, (int)n_heads, (int)kv->head_dim))
+    const bool rows16 = pg_kind(c, a.rows, (int)n_heads, (int)kv->head_dim, 1) == PG_ROWS16;
+    if (rows16 ? !paged8_rows16_fits(c, a.rows, (int)n_heads, (int)kv->head_dim)
+               : !paged_prefill_fits(c, a.rows, (int)n_heads))
         return fail(FRQ_UNSUPPORTED, "%s: rows=%zu n_seqs=%zu of up to %d tokens", who, b->rows, b->n_seqs, a.rows.cap);
     const size_t need = frq_paged8_attention_workspace(kv, b, n_heads);
     if ((rc = paged_attend_operands(who, &shape, b, dtype, n_heads, q, ldq, scale, work, work_bytes, need, out, ldo,
@@ -1596,7 +1598,7 @@ int paged8_attention(const char* who, frq_device* dev, const frq_paged_kv8* kv, 
     if (!none && (!c.k_scale || !c.v_scale)) return fail(FRQ_INVALID, "%s: null scales", who);
     DevGuard guard(dev);
     if ((rc = use_device(dev)) || none) return rc;
-    HIP_TRY(launch_paged8_rows16(dtype, (int)kv->head_dim, a, c, dev->stream));
+    HIP_TRY((rows16 ? launch_paged8_rows16 : launch_paged8_prefill)(dtype, (int)kv->head_dim, a, c, dev->stream));
     return FRQ_OK;
 }
 
@@ -1681,8 +1683,9 @@ size_t frq_paged_attention_workspace(const frq_paged_kv* kv, const frq_paged_bat
     PagedKv k;
     PagedRows r;
     if (paged_args("paged_attention_workspace", kv, b, n_heads, &k, &r)) return 0;
-    return (pg_kind(k, r, (int)n_heads, (int)kv->head_dim) == PG_ROWS16 ? paged_rows16_work_bytes : paged_prefill_work_bytes)(
-        k, r, (int)n_heads, (int)kv->head_dim);
+    return pg_kind(k, r, (int)n_heads, (int)kv->head_dim) == PG_ROWS16
+               ? paged_rows16_work_bytes(k, r, (int)n_heads, (int)kv->head_dim)
+               : paged_prefill_work_bytes(k, r, (int)n_heads, (int)kv->head_dim);
 }
 
 int frq_paged_attention_decode(frq_device* dev, const frq_paged_kv* kv, const frq_paged_batch* b, int dtype,
@@ -1706,7 +1709,9 @@ size_t frq_paged8_attention_workspace(const frq_paged_kv8* kv, const frq_paged_b
     PagedKv8 k;
     PagedRows r;
     if (paged8_args("paged8_attention_workspace", kv, b, n_heads, GGML_F32, &shape, &k, &r)) return 0;
-    return paged8_rows16_work_bytes(k, r, (int)n_heads, (int)kv->head_dim);
+    const int heads = (int)n_heads, hd = (int)kv->head_dim;
+    return pg_kind(k, r, heads, hd, 1) == PG_ROWS16 ? paged8_rows16_work_bytes(k, r, heads, hd)
+                                                    : paged_prefill_work_bytes(k, r, heads, hd, 1);
 }
 
 int frq_paged8_attention_decode(frq_device* dev, const frq_paged_kv8* kv, const frq_paged_batch* b, int dtype,

@@ -39,7 +39,7 @@
 
 #include "common.hpp"
 #include "kernels.hpp"
-#include "paged.hpp"
+#include "paged8.hpp"
 
 namespace frq {
 
@@ -84,15 +84,23 @@ __device__ __forceinline__ float pf_other_half(float v) {
     return __builtin_bit_cast(float, (threadIdx.x & 32) ? (uint32_t)a[0] : (uint32_t)a[1]);
 }
 
-template <class E, class T, int HD>
+// EK, EV: the types of K and V in LDS, and so of q and of the weights in their
+// products, NQ and NP parts of each.
+template <class C, class EK_, class EV_, class T, int HD, int NQ_, int NP_>
 struct PrefillTile {
-    using P = PgElem<E>;
-    using v8 = typename P::v8;
+    using Cache = C;
+    using Row = T;
+    using EK = EK_;
+    using EV = EV_;
+    using k8 = typename PgElem<EK>::v8;
+    using v8 = typename PgElem<EV>::v8;
+    static constexpr bool BYTES = std::is_same<C, PagedKv8>::value;  // an 8-bit cache
+    using Cells = typename std::conditional<BYTES, P8Cells<HD>, PgCells<EV, HD>>::type;
     static constexpr bool WIDE = std::is_same<T, float>::value;
-    static constexpr int NP = WIDE ? P::SPLIT : 1;
-    static constexpr bool F16 = std::is_same<E, _Float16>::value;
+    static constexpr int DIM = HD, NQ = NQ_, NP = NP_;
+    static constexpr bool F16 = std::is_same<EV, _Float16>::value;
     // (f16 parts of an f32 weight: as many of its digits as f16's range holds)
-    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = P::TOP - LAZY;
+    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = PgElem<EV>::TOP - LAZY;
     static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
     static constexpr int RPI = 512 / HD, NI = TILE / 1024;  // rows a DMA instruction, instructions a tile
@@ -105,16 +113,41 @@ struct PrefillTile {
 
 // Whether KEYS rows of K and V from kt and vt on hold an infinite or NaN value, or
 // a page of them is none.  Wave-uniform.
-template <class X, class E, int KEYS>
+template <class X, int KEYS>
 __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uint32_t bad) {
     bool any = bad & ((1u << KEYS / 16) - 1);
     for (int i = 16 * (threadIdx.x & 63); i < KEYS * X::ROW; i += 1024) {
         const pg_u4 k = *reinterpret_cast<const pg_u4*>(kt + i), v = *reinterpret_cast<const pg_u4*>(vt + i);
 #pragma unroll
-        for (int w = 0; w < 4; w++) any |= pg_word_odd<E>(k[w]) || pg_word_odd<E>(v[w]);
+        for (int w = 0; w < 4; w++) any |= pg_word_odd<typename X::EK>(k[w]) || pg_word_odd<typename X::EV>(v[w]);
     }
     return __any(any);
 }
+
+// What holds for the four groups of 16 keys of a tile of an 8-bit cache: their scales,
+// a byte each (2^0 for groups without keys, so that what is cleared stays 0), and
+// which groups' page is none.
+struct Tile8 {
+    uint32_t ks, vs, bad;
+    __device__ __forceinline__ static Tile8 of(const P8Groups& gr, int g0, int j0, int kv) {
+        Tile8 t{0, 0, (uint32_t)(gr.none >> g0) & 15};
+#pragma unroll
+        for (int a = 0; a < 4; a++) {
+            const bool keys = j0 + 16 * a < kv && !((t.bad >> a) & 1);
+            t.ks |= (uint32_t)(keys ? __builtin_amdgcn_readlane(gr.k_scale, g0 + a) : P8_ONE) << (8 * a);
+            t.vs |= (uint32_t)(keys ? __builtin_amdgcn_readlane(gr.v_scale, g0 + a) : P8_ONE) << (8 * a);
+        }
+        return t;
+    }
+    // Groups of no page, or of a scale that is NaN or takes codes past f32's range.
+    __device__ __forceinline__ uint32_t odd() const {
+        uint32_t any = bad;
+#pragma unroll
+        for (int a = 0; a < 4; a++)
+            if (((ks >> (8 * a)) & 255) > P8_TOP || ((vs >> (8 * a)) & 255) > P8_TOP) any |= 1u << a;
+        return any;
+    }
+};
 
 // A workgroup takes one tile of query rows, or with CUT an equal contiguous
 // range of all tiles' key tiles (head by head, sequence by sequence, tile by
@@ -131,14 +164,18 @@ __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uin
 // more on both sides since their maximum is renewed at every passing.)
 constexpr int PF_FEW = 256;
 
-template <class E, class T, int HD, int KW, bool CUT>
-__global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv c, PagedRows b, int grp,
-                                                                         const T* __restrict__ q, int ldq, float scale,
-                                                                         T* __restrict__ out, int ldo,
-                                                                         float* __restrict__ part,
+template <class X, int KW, bool CUT>
+__global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typename X::Cache c, PagedRows b, int grp,
+                                                                         const typename X::Row* __restrict__ q, int ldq,
+                                                                         float scale, typename X::Row* __restrict__ out,
+                                                                         int ldo, float* __restrict__ part,
                                                                          PgJoin* __restrict__ joins) {
-    using X = PrefillTile<E, T, HD>;
+    using T = typename X::Row;
+    using EK = typename X::EK;
+    using EV = typename X::EV;
+    using k8 = typename X::k8;
     using v8 = typename X::v8;
+    constexpr int HD = X::DIM;
     constexpr int RW = PF_WAVES / KW, ROWS = 32 * RW;
     constexpr int NA = 2 / KW;  // groups of 32 keys of a tile a wavefront
     __shared__ __align__(1024) uint8_t s_k[2][X::TILE], s_v[2][X::TILE];
@@ -213,6 +250,13 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         const uint32_t koff = (dr & 15) * X::ROW + 16 * (pc ^ X::kswz(dr));
         const uint32_t voff = (dr & 15) * X::ROW + 16 * (pc ^ X::vswz(dr));
         const int* table = b.table + (size_t)s * b.max_pages;
+        // 8 bits: the tile after next is in registers, 16 codes of a row a lane, PASS
+        // rows a thread; it is decoded into LDS behind the barrier that frees it.
+        constexpr int PASS = HD / 64, PR = PF_KEYS / PASS;  // rows of a pass
+        pg_u4 rk[PASS], rv[PASS];
+        P8Groups gr;
+        Tile8 raw, cur;
+        const int br = (int)threadIdx.x / (HD / 16), bp = (int)threadIdx.x % (HD / 16);
         // Byte offsets in the pools of 64 groups of 16 keys, lane i that of group i from
         // key id0 on, and which groups' page is none (theirs lead to page 0).
         int id0 = 0;
@@ -220,6 +264,10 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         uint64_t none = 0;
         auto fetch_ids = [&](int j0) {
             id0 = j0;
+            if constexpr (X::BYTES) {
+                gr.template load<HD>(c, table, head, j0, sq.kv);
+                return;
+            }
             const int j = j0 + 16 * lane;
             bool off;
             const size_t page = pg_page(c, table, j, sq.kv, off);
@@ -242,6 +290,46 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                 pf_dma(static_cast<const uint8_t*>(c.v) + from, voff, vto + i * PF_WAVES * 1024);
             }
         };
+        auto fetch8 = [&](int t) {
+            const int j0 = t * PF_KEYS;
+            if (j0 - id0 >= 1024) fetch_ids(j0);
+            const int g0 = (j0 - id0) >> 4;
+            raw = Tile8::of(gr, g0, j0, sq.kv);
+#pragma unroll
+            for (int i = 0; i < PASS; i++) {
+                const uint64_t at = gr.at(g0 + ((i * PR + wave * (1024 / HD)) >> 4)) + 16 * (threadIdx.x & 63) +
+                                    (HD == 128 ? 1024 * (wave & 1) : 0);
+                rk[i] = *reinterpret_cast<const pg_u4*>(static_cast<const uint8_t*>(c.k) + at);
+                rv[i] = *reinterpret_cast<const pg_u4*>(static_cast<const uint8_t*>(c.v) + at);
+            }
+        };
+        auto decode8 = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < PASS; i++) {
+                const int r = i * PR + br, g = (i * PR + wave * (1024 / HD)) >> 4;
+                const float unit = p8_operand((raw.vs >> (8 * g)) & 255);
+                pg_u4 x = rv[i];
+                if (t * PF_KEYS + r >= sq.kv || ((raw.bad >> g) & 1)) x = pg_u4{0, 0, 0, 0};  // (no keys: they hold anything)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    *reinterpret_cast<k8*>(s_k[t & 1] + r * X::ROW + 16 * ((2 * bp + e) ^ X::kswz(r))) =
+                        p8_eight<EK>(rk[i][2 * e], rk[i][2 * e + 1], 1.0f);
+                    *reinterpret_cast<v8*>(s_v[t & 1] + r * X::ROW + 16 * ((2 * bp + e) ^ X::vswz(r))) =
+                        p8_eight<EV>(x[2 * e], x[2 * e + 1], unit);
+                }
+            }
+            cur = raw;
+        };
+        auto first_tile = [&] {
+            fetch_ids(t0 * PF_KEYS);
+            if constexpr (X::BYTES) {
+                fetch8(t0);
+                decode8(t0);
+                if (t0 + 1 < tiles) fetch8(t0 + 1);
+            } else {
+                issue(t0);
+            }
+        };
         // LDS read offsets of this lane: K row n (+ 32), chunks 2 t + h; V rows
         // 4 h + (lane / 4) % 4 (+ 16 k + 8 j), dims 16 ((lane / 16) % 2) + 4 (lane % 4) (+ 32 d)
         const uint32_t kbase = n * X::ROW + 16 * (h ^ X::kswz(n));
@@ -249,21 +337,18 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         const uint32_t vbase = (4 * h + vr) * X::ROW +
                                16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ X::vswz(vr)) + 8 * (lane & 1);
 
-        if (t0 < tiles) {
-            fetch_ids(t0 * PF_KEYS);
-            issue(t0);
-        }
+        if (t0 < tiles) first_tile();
 
         // Q^T, the B operand: dims 16 t + 8 h + e of row n (negated for a negative
         // scale: the maximum is taken of scores with a positive factor)
-        v8 qf[X::NP][X::KS];
+        k8 qf[X::NQ][X::KS];
         float factor = fabsf(scale) * 1.4426950408889634f;
         const T* x = q + (size_t)row * ldq + (size_t)qh * HD + 8 * h;
         if constexpr (!X::WIDE) {
             const uint32_t flip = scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
             for (int t = 0; t < X::KS; t++)
-                qf[0][t] = __builtin_bit_cast(v8, *reinterpret_cast<const pg_u4*>(x + 16 * t) ^ flip);
+                qf[0][t] = __builtin_bit_cast(k8, *reinterpret_cast<const pg_u4*>(x + 16 * t) ^ flip);
         } else {
             float f[X::KS][8], a = 0.0f;
 #pragma unroll
@@ -273,7 +358,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
 #pragma unroll
                 for (int e = 0; e < 8; e++) f[t][e] = scale < 0.0f ? -raw[e] : raw[e];
             }
-            if constexpr (std::is_same<E, _Float16>::value) {  // (parts of f16: scaled to the top of its range)
+            if constexpr (std::is_same<EK, _Float16>::value) {  // (parts of f16: scaled to the top of its range)
 #pragma unroll
                 for (int t = 0; t < X::KS; t++)
 #pragma unroll
@@ -292,8 +377,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                 for (int e = 0; e < 8; e++) {
                     float rest = f[t][e];
 #pragma unroll
-                    for (int p = 0; p < X::NP; p++) {
-                        qf[p][t][e] = (E)rest;
+                    for (int p = 0; p < X::NQ; p++) {
+                        qf[p][t][e] = (EK)rest;
                         rest -= (float)qf[p][t][e];
                     }
                 }
@@ -310,11 +395,19 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
             for (int t = t0; t < tiles; t++) {
                 const int j0 = t * PF_KEYS;
                 // tile t landed, in every wavefront, and tile t - 1 is read
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                if constexpr (X::BYTES) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                const uint32_t bad = (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
-                if (j0 + PF_KEYS > sq.kv || bad) {  // rows of V that are no keys hold anything
+                const Tile8 t8 = cur;
+                const uint32_t bad = X::BYTES ? t8.bad
+                                              : (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
+                if (X::BYTES) {
+                    if (t + 1 < tiles) {
+                        decode8(t + 1);
+                        if (t + 2 < tiles) fetch8(t + 2);
+                    }
+                } else if (j0 + PF_KEYS > sq.kv || bad) {  // rows of V that are no keys hold anything
                     for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
                         const int r = ch / CPR;
                         if (j0 + r >= sq.kv || ((bad >> (r >> 4)) & 1))
@@ -322,15 +415,15 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                     }
                     __syncthreads();
                 }
-                if (t + 1 < tiles) issue(t + 1);
+                if (!X::BYTES && t + 1 < tiles) issue(t + 1);
                 const int jw = j0 + key0;  // this wavefront's first key
                 if (jw > last) continue;
 
                 const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
                 const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
-                if (AGAIN && pf_odd<X, E, 64 / KW>(kt, vt, bad >> (key0 >> 4))) {
+                if (AGAIN && pf_odd<X, 64 / KW>(kt, vt, (X::BYTES ? t8.odd() : bad) >> (key0 >> 4))) {
                     if (!__all(pg_all_nan(o)))
-                        pg_plain<PgCells<E, HD>, T, HD, 2>(
+                        pg_plain<typename X::Cells, T, HD, 2>(
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
                             min(jw + 32 * NA, last + 1), X::SHIFT, h == 0, [&](int i) { return 8 * i + 4 * h; },
                             [&](int i, int e, float f, float p, float v) {
@@ -347,9 +440,9 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                     for (int i = 0; i < 16; i++) st[a][i] = 0.0f;
 #pragma unroll
                     for (int k = 0; k < X::KS; k++) {
-                        const v8 kf = *reinterpret_cast<const v8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
+                        const k8 kf = *reinterpret_cast<const k8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
 #pragma unroll
-                        for (int p = X::NP - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
+                        for (int p = X::NQ - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
                     }
                 }
                 const bool mask = jw + 32 * NA - 1 > first || bad;
@@ -363,12 +456,34 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                             if (jw + r > limit) st[a][i] = -__builtin_inff();
                         }
                 }
+                // the factors of the scores of groups of 16 keys
+                float fac[2 * NA];
+#pragma unroll
+                for (int g = 0; g < 2 * NA; g++) {
+                    fac[g] = factor;
+                    if constexpr (X::BYTES) {
+                        fac[g] *= p8_factor((t8.ks >> (8 * (g + (key0 >> 4)))) & 255);
+                        fac[g] = fac[g] > __FLT_MAX__ ? __FLT_MAX__ : fac[g];  // (of NaN: NaN)
+                    }
+                }
                 float top = st[0][0];
+                if constexpr (X::BYTES) {
+                    top = -__builtin_inff();
 #pragma unroll
-                for (int a = 0; a < NA; a++)
+                    for (int g = 0; g < 2 * NA; g++) {
+                        float most = st[g >> 1][8 * (g & 1)];
 #pragma unroll
-                    for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
-                top = fmaxf(top, pf_other_half(top)) * factor;
+                        for (int i = 1; i < 8; i++) most = fmaxf(most, st[g >> 1][8 * (g & 1) + i]);
+                        top = fmaxf(top, most * fac[g]);
+                    }
+                    top = fmaxf(top, pf_other_half(top));
+                } else {
+#pragma unroll
+                    for (int a = 0; a < NA; a++)
+#pragma unroll
+                        for (int i = 0; i < 16; i++) top = fmaxf(top, st[a][i]);
+                    top = fmaxf(top, pf_other_half(top)) * factor;
+                }
                 peak = fmaxf(peak, top);
                 const float low = X::F16 ? fmaxf(top, peak - PG_DROP) : m;
                 if (__any(top > m + X::LAZY || low < m - PF_LOW)) {
@@ -385,7 +500,9 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
 #pragma unroll
                 for (int a = 0; a < NA; a++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) st[a][i] = AGAIN ? st[a][i] * factor - ms : fmaf(st[a][i], factor, -ms);
+                    for (int i = 0; i < 16; i++)
+                        st[a][i] = AGAIN ? st[a][i] * fac[2 * a + (i >> 3)] - ms
+                                         : fmaf(st[a][i], fac[2 * a + (i >> 3)], -ms);
                 if (mask) {  // (again: a factor of 0 would make NaN of -inf)
 #pragma unroll
                     for (int a = 0; a < NA; a++)
@@ -403,7 +520,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
                         float rest = st[a][i];
 #pragma unroll
                         for (int p = 0; p < X::NP; p++) {
-                            pp[p][2 * a + (i >> 3)][i & 7] = (E)rest;
+                            pp[p][2 * a + (i >> 3)][i & 7] = (EV)rest;
                             rest -= (float)pp[p][2 * a + (i >> 3)][i & 7];
                         }
                     }
@@ -424,8 +541,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
         // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 7.7,
         // all NaN 7.2, with one infinite value in every 16 keys, the worst there is, 205.
         if (__builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)))) {
-            fetch_ids(t0 * PF_KEYS);
-            issue(t0);
+            first_tile();
             walk(std::true_type{});
         }
         l += pf_other_half(l);
@@ -501,31 +617,49 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(PagedKv
     }
 }
 
+template <class X>
+hipError_t prefill_launch(const PagedAttendArgs& p, const typename X::Cache& c, hipStream_t s) {
+    using T = typename X::Row;
+    const int grp = p.n_heads / c.kv_heads;
+    const T* q = static_cast<const T*>(p.q);
+    T* out = static_cast<T*>(p.out);
+    const long tiles = pg_tiles_bound(p.rows, grp, PF_ROWS) * c.kv_heads;
+    if (pg_kind(c, p.rows, p.n_heads, X::DIM, X::BYTES ? 1 : 2) != PG_CUT) {
+        const bool few = tiles <= PF_FEW;
+        const auto kernel = few ? paged_prefill_kernel<X, 2, false> : paged_prefill_kernel<X, 1, false>;
+        const long wgs = few ? pg_tiles_bound(p.rows, grp, PF_ROWS / 2) * c.kv_heads : tiles;
+        hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * PF_WAVES), 0, s, c, p.rows, grp, q, p.ldq, p.scale,
+                           out, p.ldo, nullptr, nullptr);
+        return hipGetLastError();
+    }
+    float* part = static_cast<float*>(p.work);
+    PgJoin* joins = reinterpret_cast<PgJoin*>(part + (size_t)2 * PG_WGS * pg_slot(PF_ROWS, X::DIM));
+    hipLaunchKernelGGL((paged_prefill_kernel<X, 1, true>), dim3(PG_WGS), dim3(64 * PF_WAVES), 0, s, c, p.rows, grp, q,
+                       p.ldq, p.scale, out, p.ldo, part, joins);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    return launch_paged_join(pg_dtype<T>(), X::DIM, joins, part, PG_WGS, tiles, PF_ROWS, PF_ROWS, grp, p.out, p.ldo, s);
+}
+
 struct PrefillCall {
     const PagedAttendArgs& p;
     hipStream_t s;
     template <class E, class T, int HD>
     hipError_t run() const {
-        const int grp = p.n_heads / p.kv.kv_heads;
-        const T* q = static_cast<const T*>(p.q);
-        T* out = static_cast<T*>(p.out);
-        const long tiles = pg_tiles_bound(p.rows, grp, PF_ROWS) * p.kv.kv_heads;
-        if (pg_kind(p.kv, p.rows, p.n_heads, HD) != PG_CUT) {
-            const bool few = tiles <= PF_FEW;
-            const auto kernel =
-                few ? paged_prefill_kernel<E, T, HD, 2, false> : paged_prefill_kernel<E, T, HD, 1, false>;
-            const long wgs = few ? pg_tiles_bound(p.rows, grp, PF_ROWS / 2) * p.kv.kv_heads : tiles;
-            hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(64 * PF_WAVES), 0, s, p.kv, p.rows, grp, q, p.ldq,
-                               p.scale, out, p.ldo, nullptr, nullptr);
-            return hipGetLastError();
-        }
-        float* part = static_cast<float*>(p.work);
-        PgJoin* joins = reinterpret_cast<PgJoin*>(part + (size_t)2 * PG_WGS * pg_slot(PF_ROWS, HD));
-        hipLaunchKernelGGL((paged_prefill_kernel<E, T, HD, 1, true>), dim3(PG_WGS), dim3(64 * PF_WAVES), 0, s, p.kv,
-                           p.rows, grp, q, p.ldq, p.scale, out, p.ldo, part, joins);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-        return launch_paged_join(pg_dtype<T>(), HD, joins, part, PG_WGS, tiles, PF_ROWS, PF_ROWS, grp, p.out, p.ldo, s);
+        constexpr int parts = std::is_same<T, float>::value ? PgElem<E>::SPLIT : 1;
+        return prefill_launch<PrefillTile<PagedKv, E, E, T, HD, parts, parts>>(p, p.kv, s);
+    }
+};
+
+struct Prefill8Call {
+    const PagedAttendArgs& p;
+    const PagedKv8& c;
+    hipStream_t s;
+    template <class T, int HD>
+    hipError_t run() const {
+        constexpr bool wide = std::is_same<T, float>::value;
+        using E = typename std::conditional<wide, _Float16, T>::type;
+        return prefill_launch<PrefillTile<PagedKv8, E, __bf16, T, HD, wide ? 2 : 1, wide ? 3 : 1>>(p, c, s);
     }
 };
 
@@ -535,14 +669,19 @@ bool paged_prefill_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {
     return pg_tiles_bound(r, n_heads / kv.kv_heads, PF_ROWS) * kv.kv_heads <= PG_GRID;
 }
 
-size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
-    if (pg_kind(kv, r, n_heads, hd) != PG_CUT) return 0;
+size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size) {
+    if (pg_kind(kv, r, n_heads, hd, size) != PG_CUT) return 0;
     return PG_WGS * (2 * pg_slot(PF_ROWS, hd) * sizeof(float) + sizeof(PgJoin));
 }
 
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s) {
     if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
     return paged_with_types(kv_dtype, dtype, hd, PrefillCall{p, s});
+}
+
+hipError_t launch_paged8_prefill(int dtype, int hd, const PagedAttendArgs& p, const PagedKv8& c, hipStream_t s) {
+    if (p.rows.rows <= 0 || p.rows.n_seqs <= 0) return hipSuccess;
+    return paged8_with_types(dtype, hd, Prefill8Call{p, c, s});
 }
 
 }  // namespace frq
