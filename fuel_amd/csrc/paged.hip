@@ -51,6 +51,7 @@ struct Rows16 {
     static constexpr int NP = WIDE ? P::SPLIT : 2;
     static constexpr int DIM = HD, KS = HD / 32, VW = HD / 16;
     static constexpr int STEP = 32, BYTES = 2 * HD;  // keys of a block; bytes of a key
+    static constexpr int RESIDENT = pg_resident(HD, 2);
 
     v8 q[NQ][KS];
     float factor;  // score = S^T * factor, in units of log2
@@ -335,17 +336,17 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
     constexpr int TH = HD / 4;
     __shared__ pg_f4 s_o[PJ_WG];
     __shared__ float s_l[PJ_WG / TH], s_m[PJ_WG / TH];
-    __shared__ uint64_t s_some[PG_WGS / 64];
+    __shared__ uint64_t s_some[PG_RECORDS / 64];
     int w0 = blockIdx.x;
     if ((int)gridDim.x < records) {
-        for (int i = threadIdx.x; i < PG_WGS; i += PJ_WG) {
+        for (int i = threadIdx.x; i < PG_RECORDS; i += PJ_WG) {
             const uint64_t some = __ballot(i < records && joins[i].rows > 0);
             if ((threadIdx.x & 63) == 0) s_some[i >> 6] = some;
         }
         __syncthreads();
         int skip = blockIdx.x, k = 0;
-        for (; k < PG_WGS / 64 && skip >= __popcll(s_some[k]); k++) skip -= __popcll(s_some[k]);
-        if (k == PG_WGS / 64) return;
+        for (; k < PG_RECORDS / 64 && skip >= __popcll(s_some[k]); k++) skip -= __popcll(s_some[k]);
+        if (k == PG_RECORDS / 64) return;
         uint64_t some = s_some[k];
         for (; skip; skip--) some &= some - 1;
         w0 = __builtin_amdgcn_readfirstlane(64 * k + __builtin_ctzll(some));

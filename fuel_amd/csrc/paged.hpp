@@ -85,9 +85,11 @@ inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int
     return tiles <= cut ? PG_TILES : PG_CUT;
 }
 
-// Workgroups of a call whose keys are cut into equal ranges: two a CU, all
-// resident at once.
+// Workgroups of a call whose keys are cut into equal ranges: two a CU (of 16-row
+// tiles of an 8-bit cache with dims of 64: three), all resident at once.
 constexpr int PG_WGS = 512;
+constexpr int pg_resident(int hd, int size) { return size == 1 && hd == 64 ? 3 : 2; }
+constexpr int PG_RECORDS = PG_WGS / 2 * 3;  // of such a call's workgroups, at most
 
 // Workgroups of 256 threads that one launch can have: HIP's grids end below 2^32
 // threads.
@@ -417,7 +419,7 @@ __device__ __forceinline__ int pg_row_seq(const PagedRows& b, int row) {
 // starts at unit w * total / n_wgs, none is empty; and the one that holds unit u.
 __host__ __device__ __forceinline__ int pg_start(int w, int total, int n_wgs) {
     if (n_wgs == total) return w;
-    // (in 32 bits: n_wgs is at most PG_WGS here)
+    // (in 32 bits: n_wgs is at most PG_RECORDS here)
     const unsigned q = (unsigned)total / (unsigned)n_wgs, rest = (unsigned)total % (unsigned)n_wgs;
     return w * (int)q + (int)((unsigned)w * rest / (unsigned)n_wgs);
 }

@@ -8,7 +8,7 @@
 // scale, or raise it: then the older codes are rounded once more, exactly but for
 // those that fall below the least normal number, 2^-14.8 of the block's largest.
 //
-// Attention: as paged.hip's 16-row tiles, 64 keys at a time.  K's codes go to the
+// Attention: as paged.hip's 16-row tiles, 32 keys at a time.  K's codes go to the
 // matrix pipe as f16 (bf16 for bf16 rows) without their scale, exactly; a group of
 // 16 keys' scale is a factor of its scores, in f32.  V's go there as bf16 values,
 // exactly, so that no weight has to carry a scale.  f32 rows: q in two parts of f16,
@@ -35,7 +35,16 @@ struct Rows8 {
     using v8 = P::v8;
     static constexpr int NQ = WIDE ? 2 : 1, NP = WIDE ? 3 : 2;
     static constexpr int DIM = HD, KS = HD / 32, VW = HD / 16;
-    static constexpr int STEP = 64, BYTES = HD;
+    // Groups of 16 keys of a block.  (Of four, where the 16 KB of two blocks of 32 go
+    // out at once: no faster, and 10.0 us for 7.6 where a wavefront has a few blocks.)
+    static constexpr int G = 2, STEP = 16 * G, BYTES = HD;
+    // Workgroups a CU.  Dims of 64: 512 workgroups of them 38.7 us, 768 31.8, 1024 35.7
+    // (128 sequences of 308 .. 2489, 8 KV heads); of 128: 83.8, 93.3, 131 (spills).
+    static constexpr int RESIDENT = pg_resident(HD, 1);
+    // Weights are 2^TOP at most; the maximum that they are of is renewed where scores
+    // pass it by LAZY: bf16 weights keep their digits whatever power of two they and
+    // the sums share.
+    static constexpr float LAZY = 7.0f, SHIFT = P::TOP - LAZY;
 
     q8 q[NQ][KS];
     float factor;  // score = product * factor * the key's scale, in units of log2
@@ -45,10 +54,10 @@ struct Rows8 {
 
     typedef uint32_t ValueWord __attribute__((ext_vector_type(VW / 4)));
     struct KeyRegs {
-        pg_u4 w[4][HD / 64];
+        pg_u4 w[G][HD / 64];
     };
     struct ValueRegs {
-        ValueWord w[16];
+        ValueWord w[4 * G];
     };
 
     // Lane 16 g + r takes row r: in step t of the products dims 64 (t / 2) + 16 g +
@@ -65,44 +74,43 @@ struct Rows8 {
         l = 0.0f;
     }
 
-    // The loads of 64 keys: group a's 16 rows start at ka[a] / va[a].  ONCE:
-    // nothing else of the call reads them, so they go past the caches.
+    // The loads of a block of keys: group a's 16 rows start at at[a], values' loads
+    // are those of groups 2 h and 2 h + 1.  ONCE: nothing else of the call reads them,
+    // so they go past the caches.
     template <bool ONCE, class W>
     __device__ static W load(const uint8_t* p) {
         return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const W*>(p)) : *reinterpret_cast<const W*>(p);
     }
     template <bool ONCE>
-    __device__ static void load_k(KeyRegs& k, const uint8_t* const (&ka)[4]) {
+    __device__ static void load_k(KeyRegs& k, const uint8_t* const (&at)[G]) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int a = 0; a < 4; a++)
+        for (int a = 0; a < G; a++)
 #pragma unroll
-            for (int c = 0; c < HD / 64; c++) k.w[a][c] = load<ONCE, pg_u4>(ka[a] + r * HD + 64 * c + 16 * g);
+            for (int c = 0; c < HD / 64; c++) k.w[a][c] = load<ONCE, pg_u4>(at[a] + r * HD + 64 * c + 16 * g);
     }
     template <bool ONCE>
-    __device__ static void load_v(ValueRegs& v, const uint8_t* const (&va)[4]) {
+    __device__ static void load_v(ValueRegs& v, const uint8_t* const (&at)[G], int h) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
-        for (int a = 0; a < 4; a++)
+        for (int a = 2 * h; a < 2 * h + 2; a++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) v.w[4 * a + i] = load<ONCE, ValueWord>(va[a] + (4 * g + i) * HD + VW * r);
+            for (int i = 0; i < 4; i++) v.w[4 * a + i] = load<ONCE, ValueWord>(at[a] + (4 * g + i) * HD + VW * r);
     }
 
-    // What holds for the groups of a block of 64 keys from j0: their scales (2^0 for
-    // groups without keys, so that what is cleared stays 0), and which keys a row
-    // sees: none past its position, past the sequence's length kv or in a page that
-    // is none (bad: NaN).
+    // What holds for the groups of a block from key j0: their scales (2^0 for groups
+    // without keys, so that what is cleared stays 0), and which keys a row sees: none
+    // past its position, past the sequence's length kv or in a page that is none (bad:
+    // NaN).
     struct Block {
-        int j0, kv, ks[4], vs[4];
+        int j0, kv, ks[G], vs[G];
         uint32_t bad;
     };
 
     // The block's scores in log2 units: s[4 a + i] of key 16 a + 4 g + i.
-    template <bool MASK>
-    __device__ void scores(const KeyRegs& k, const Block& b, float (&s)[16]) const {
-        const int g = (threadIdx.x & 63) >> 4;
+    __device__ void scores(const KeyRegs& k, const Block& b, float (&s)[4 * G]) const {
 #pragma unroll
-        for (int a = 0; a < 4; a++) {
+        for (int a = 0; a < G; a++) {
             pg_f4 st = pg_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < KS; t++) {
@@ -112,63 +120,67 @@ struct Rows8 {
             }
             const float unit = p8_factor(b.ks[a]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                float v = st[i] * factor * unit;
-                if constexpr (MASK) {
-                    if ((b.bad >> a) & 1) v = pg_nan();
-                    if (b.j0 + 16 * a + 4 * g + i > limit) v = -__builtin_inff();
-                }
-                s[4 * a + i] = v;
-            }
+            for (int i = 0; i < 4; i++) s[4 * a + i] = st[i] * factor * unit;
+            if (a & 1) __builtin_amdgcn_sched_barrier(0);  // (all of a block's at once spill)
+        }
+    }
+    // Those of keys that the row does not see.
+    __device__ void hide(const Block& b, float (&s)[4 * G]) const {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < 4 * G; i++) {
+            if ((b.bad >> (i >> 2)) & 1) s[i] = pg_nan();
+            if (b.j0 + 16 * (i >> 2) + 4 * g + (i & 3) > limit) s[i] = -__builtin_inff();
         }
     }
 
-    // Weights of the block's scores, maximum and sums renewed: pp[b] of groups 2 b
-    // and 2 b + 1.
-    __device__ void weights(const float (&s)[16], v8 (&pp)[2][NP]) {
+    __device__ void renew(const float (&s)[4 * G]) {
         float top = s[0];
 #pragma unroll
-        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-        const float mn = fmaxf(m, pg_row_max(top));
+        for (int i = 1; i < 4 * G; i++) top = fmaxf(top, s[i]);
+        top = pg_row_max(top);
+        if (!__any(top > m + LAZY)) return;
+        const float mn = fmaxf(m, top);
         const float c = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before: l = o = 0)
         m = mn;
         l *= c;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float rest = __builtin_amdgcn_exp2f(s[i] - mn + P::TOP);
-            l += rest;
-#pragma unroll
-            for (int p = 0; p < NP; p++) {
-                pp[i >> 3][p][i & 7] = (__bf16)rest;
-                rest -= (float)pp[i >> 3][p][i & 7];
-            }
-        }
-#pragma unroll
         for (int t = 0; t < VW; t++) o[t] *= c;
     }
 
-    __device__ void product(const ValueRegs& v, const Block& b, const v8 (&pp)[2][NP]) {
+    // Weights of groups 2 h and 2 h + 1 and their product with V.
+    __device__ void product(const float (&s)[4 * G], const ValueRegs& v, const Block& b, int h) {
+        v8 pp[NP];
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            uint32_t x[8][VW / 2];  // pairs of dims of 8 keys
+        for (int i = 0; i < 8; i++) {
+            float rest = __builtin_amdgcn_exp2f(s[8 * h + i] - m + SHIFT);
+            l += rest;
+#pragma unroll
+            for (int p = 0; p < NP; p++) {
+                pp[p][i] = (__bf16)rest;
+                rest -= (float)pp[p][i];
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < VW / 4; w++) {
+            uint32_t x[8][2];  // pairs of dims of 8 keys
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const float operand = p8_operand(b.vs[2 * h + (i >> 2)]);
-#pragma unroll
-                for (int w = 0; w < VW / 4; w++) {
-                    x[i][2 * w] = p8_pair<false>(v.w[8 * h + i][w], operand, __bf16());
-                    x[i][2 * w + 1] = p8_pair<true>(v.w[8 * h + i][w], operand, __bf16());
-                }
+                x[i][0] = p8_pair<false>(v.w[8 * h + i][w], operand, __bf16());
+                x[i][1] = p8_pair<true>(v.w[8 * h + i][w], operand, __bf16());
             }
 #pragma unroll
-            for (int t = 0; t < VW; t++) {
+            for (int t = 0; t < 4; t++) {
                 const uint32_t sel = (t & 1) ? 0x07060302u : 0x05040100u;  // high or low halves of two words
                 pg_u4 a;
 #pragma unroll
                 for (int i = 0; i < 4; i++) a[i] = __builtin_amdgcn_perm(x[2 * i + 1][t >> 1], x[2 * i][t >> 1], sel);
 #pragma unroll
-                for (int p = NP - 1; p >= 0; p--) o[t] = P::mfma16(__builtin_bit_cast(v8, a), pp[h][p], o[t]);
+                for (int p = NP - 1; p >= 0; p--)
+                    o[4 * w + t] = P::mfma16(__builtin_bit_cast(v8, a), pp[p], o[4 * w + t]);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
@@ -176,7 +188,7 @@ struct Rows8 {
     __device__ static void clear(ValueRegs& v, const Block& b) {
         const int g = (threadIdx.x & 63) >> 4;
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < 4 * G; i++) {
             const bool none = ((b.bad >> (i >> 2)) & 1) || b.j0 + 16 * (i >> 2) + 4 * g + (i & 3) >= b.kv;
 #pragma unroll
             for (int w = 0; w < VW / 4; w++)
@@ -188,7 +200,7 @@ struct Rows8 {
     __device__ static bool odd(const KeyRegs& k, const ValueRegs& v, const Block& b) {
         bool any = b.bad;
 #pragma unroll
-        for (int a = 0; a < 4; a++) {
+        for (int a = 0; a < G; a++) {
             any |= b.ks[a] > P8_TOP || b.vs[a] > P8_TOP;
 #pragma unroll
             for (int c = 0; c < HD / 64; c++)
@@ -196,41 +208,69 @@ struct Rows8 {
                 for (int w = 0; w < 4; w++) any |= p8_word_nan(k.w[a][c][w]);
         }
 #pragma unroll
-        for (int i = 0; i < 16; i++)
+        for (int i = 0; i < 4 * G; i++)
 #pragma unroll
             for (int w = 0; w < VW / 4; w++) any |= p8_word_nan(v.w[i][w]);
         return __any(any);
     }
 
-    // Keys [j0, j1) by pg_plain(); x: the row's q.
+    // Keys [j0, j1) as pg_plain() takes them, one at a time: the registers that four
+    // would take are those of a third workgroup on a CU.  x: the row's q.
     __device__ void plain(const PagedKv8& c, const int* table, int head, const T* x, float scale, int j0, int j1) {
         const int g = (threadIdx.x & 63) >> 4;
-        pg_plain<P8Cells<HD>, T, HD, 4>(
-            c, table, head, x, scale, limit, j0, j1, P::TOP, g == 0, [&](int i) { return 4 * (VW * g + i); },
-            [&](int i, int e, float f, float p, float v) {
-                const int t = (4 * i + e) % VW, k = (4 * i + e) / VW;
-                o[t][k] = fmaf(p, v, o[t][k] * f);
-            },
-            m, l);
+        const float unit = scale * 1.4426950408889634f;
+#pragma unroll 1
+        for (int j = j0; j < j1; j++) {
+            bool none;
+            const int page = pg_page(c, table, j, j + 1, none);
+            const P8Cells<HD> cell(c, page, head, j);
+            float s = 0.0f;
+#pragma unroll 1
+            for (int d = 4 * VW * g; d < 4 * VW * (g + 1); d += 4) {
+                float y[4];
+                cell.key(0, d, y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) s = fmaf((float)x[d + e] * unit, y[e], s);
+            }
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (none) s = pg_nan();
+            const bool sees = j <= limit;  // (no branch: the sums would be in registers twice)
+            const float mn = sees ? fmaxf(m, s) : m, f = __builtin_amdgcn_exp2f(m - mn);
+            const float p = __builtin_amdgcn_exp2f(s - mn + SHIFT);
+            m = mn;
+            l = l * f + (sees && g == 0 ? p : 0.0f);
+#pragma unroll
+            for (int i = 0; i < VW; i++) {
+                float y[4];
+                cell.value(0, 4 * (VW * g + i), y);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int t = (4 * i + e) % VW, k = (4 * i + e) / VW;
+                    o[t][k] = sees ? fmaf(p, y[e], o[t][k] * f) : o[t][k];
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
     }
 
     // Block i of the groups from j0 on.
     __device__ static Block block(const P8Groups& gr, int j0, int i, int kv) {
-        Block b{j0 + 64 * i, kv, {}, {}, (uint32_t)(gr.none >> (4 * i)) & 15};
+        Block b{j0 + STEP * i, kv, {}, {}, (uint32_t)(gr.none >> (G * i)) & ((1u << G) - 1)};
 #pragma unroll
-        for (int a = 0; a < 4; a++) {
+        for (int a = 0; a < G; a++) {
             const bool keys = b.j0 + 16 * a < kv && !((b.bad >> a) & 1);
-            b.ks[a] = keys ? __builtin_amdgcn_readlane(gr.k_scale, 4 * i + a) : P8_ONE;
-            b.vs[a] = keys ? __builtin_amdgcn_readlane(gr.v_scale, 4 * i + a) : P8_ONE;
+            b.ks[a] = keys ? __builtin_amdgcn_readlane(gr.k_scale, G * i + a) : P8_ONE;
+            b.vs[a] = keys ? __builtin_amdgcn_readlane(gr.v_scale, G * i + a) : P8_ONE;
         }
         return b;
     }
-    __device__ static void rows(const P8Groups& gr, const void* pool, int i, const uint8_t* (&at)[4]) {
+    __device__ static void rows(const P8Groups& gr, const void* pool, int i, const uint8_t* (&at)[G]) {
 #pragma unroll
-        for (int a = 0; a < 4; a++) at[a] = static_cast<const uint8_t*>(pool) + gr.at(4 * i + a);
+        for (int a = 0; a < G; a++) at[a] = static_cast<const uint8_t*>(pool) + gr.at(G * i + a);
     }
 
-    // One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of 64).
+    // One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of STEP).
     // The next block's keys are loaded as soon as this one's scores are formed, its
     // values as soon as this one's product is.  Every row sees the keys up to all_see.
     template <bool ONCE>
@@ -240,40 +280,39 @@ struct Rows8 {
             const int end = min(j1, j0 + 1024);
             P8Groups gr;
             gr.load<HD>(c, table, head, j0, kv);
-            const int last = (end - j0 + 63) / 64 - 1;
-            const uint8_t* at[4];
+            const int last = (end - j0 + STEP - 1) / STEP - 1;
+            const uint8_t* at[G];
             KeyRegs kr;
             ValueRegs vr;
-            float s[16];
-            v8 pp[2][NP];
             rows(gr, c.k, 0, at);
             load_k<ONCE>(kr, at);
             rows(gr, c.v, 0, at);
-            load_v<ONCE>(vr, at);
-            for (int i = 0;; i++) {
+#pragma unroll
+            for (int h = 0; h < G / 2; h++) load_v<ONCE>(vr, at, h);
+            const auto step = [&](int i, auto more) {
+                constexpr bool MORE = decltype(more)::value;
                 const Block b = block(gr, j0, i, kv);
-                const bool mask = b.j0 + 63 > all_see || b.bad;
-                if (i == last || mask) {  // (apart from the loop's body, which keeps its loads in flight)
-                    if (mask) scores<true>(kr, b, s);
-                    else scores<false>(kr, b, s);
-                    weights(s, pp);
-                    if (mask) clear(vr, b);
-                    product(vr, b, pp);
-                    if (i == last) break;
+                const bool mask = b.j0 + STEP - 1 > all_see || b.bad;
+                float s[4 * G];
+                scores(kr, b, s);
+                if constexpr (MORE) {
                     rows(gr, c.k, i + 1, at);
                     load_k<ONCE>(kr, at);
                     rows(gr, c.v, i + 1, at);
-                    load_v<ONCE>(vr, at);
-                    continue;
                 }
-                scores<false>(kr, b, s);
-                rows(gr, c.k, i + 1, at);
-                load_k<ONCE>(kr, at);
-                weights(s, pp);
-                product(vr, b, pp);
-                rows(gr, c.v, i + 1, at);
-                load_v<ONCE>(vr, at);
-            }
+                __builtin_amdgcn_sched_barrier(0);
+                if (__builtin_expect(mask, 0)) hide(b, s);
+                renew(s);
+                if (__builtin_expect(mask, 0)) clear(vr, b);
+#pragma unroll
+                for (int h = 0; h < G / 2; h++) {
+                    product(s, vr, b, h);
+                    if constexpr (MORE) load_v<ONCE>(vr, at, h);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            for (int i = 0; i < last; i++) step(i, std::true_type{});
+            step(last, std::false_type{});
             j0 = end;
         }
     }
@@ -282,31 +321,33 @@ struct Rows8 {
     // such values or of pages that are none one key after another.
     __device__ __forceinline__ void walk_odd(const PagedKv8& c, const int* table, int head, int j0, int j1, int kv,
                                              const T* x, float scale) {
-        if (!__any(pg_odd(o))) return;
+        if (__builtin_expect(!__any(pg_odd(o)), 1)) return;
         start();
 #pragma unroll 1
-        for (int j = j0; j < j1; j += 64) {
+        for (int j = j0; j < j1; j += STEP) {
             P8Groups gr;
             gr.load<HD>(c, table, head, j, kv);
             const Block b = block(gr, j, 0, kv);
-            const uint8_t *ka[4], *va[4];
+            const uint8_t *ka[G], *va[G];
             rows(gr, c.k, 0, ka);
             rows(gr, c.v, 0, va);
             KeyRegs kr;
             ValueRegs vr;
             load_k<false>(kr, ka);
-            load_v<false>(vr, va);
+#pragma unroll
+            for (int h = 0; h < G / 2; h++) load_v<false>(vr, va, h);
             clear(vr, b);
             if (odd(kr, vr, b)) {
-                plain(c, table, head, x, scale, j, min(j + 64, j1));
+                plain(c, table, head, x, scale, j, min(j + STEP, j1));
                 if (__all(pg_all_nan(o))) return;
                 continue;
             }
-            float s[16];
-            v8 pp[2][NP];
-            scores<true>(kr, b, s);
-            weights(s, pp);
-            product(vr, b, pp);
+            float s[4 * G];
+            scores(kr, b, s);
+            hide(b, s);
+            renew(s);
+#pragma unroll
+            for (int h = 0; h < G / 2; h++) product(s, vr, b, h);
         }
     }
 

@@ -5,6 +5,7 @@
 //   Cache, Row, DIM, VW   the cache's view, the rows' type, head_dim, DIM / 16
 //   STEP, BYTES           keys of a block, which a wavefront takes at a time; bytes
 //                         of a key or value row
+//   RESIDENT              workgroups a CU
 //   load_q, start, walk, walk_odd, finish;  o, m, l, limit
 // Lane 16 g + r holds of query row r the dims VW (4 g + k) + t as o[t][k], the
 // running maximum m, the sum l, and limit, the row's position.
@@ -99,8 +100,7 @@ __device__ __forceinline__ void pd_load_q(typename PgElem<E>::v8 (&q)[NQ][KS], f
 // alone reach 6.75 here).  Large tiles of wavefronts, more workgroups, or the next
 // piece's first keys loaded under this one's merge took as long or longer.
 
-// A block of keys for each wavefront (A::STEP), by the bytes of a cached value.
-inline int pd_unit(int size) { return 64 / size * PA_WAVES; }
+constexpr int PD_UNIT = 32 * PA_WAVES;
 
 // Tiles of a sequence, and units of each; one without keys has one unit, which
 // writes its rows.
@@ -110,7 +110,7 @@ __device__ __forceinline__ int pd_units(const PgSeq& q, int unit) {
 }
 
 template <class A, bool ONCE>
-__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(typename A::Cache c, PagedRows b, int grp, int unit,
+__global__ __launch_bounds__(64 * PA_WAVES, A::RESIDENT) void paged_rows16_kernel(typename A::Cache c, PagedRows b, int grp, int unit,
                                                                         const typename A::Row* __restrict__ q, int ldq, float scale,
                                                                         typename A::Row* __restrict__ out, int ldo,
                                                                         float* __restrict__ part,
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_kernel(typename
 //   4096       46.9/17.2   49.3/25.3  65.6/44.1   98.4/87.9  169.7/169.1
 // and up to half as long again where a batch's lengths differ much.
 template <class A, bool ONCE>
-__global__ __launch_bounds__(64 * PA_WAVES, 2) void paged_rows16_alone_kernel(typename A::Cache c, PagedRows b, int grp, int each,
+__global__ __launch_bounds__(64 * PA_WAVES, A::RESIDENT) void paged_rows16_alone_kernel(typename A::Cache c, PagedRows b, int grp, int each,
                                                                               const typename A::Row* __restrict__ q, int ldq, float scale,
                                                                               typename A::Row* __restrict__ out, int ldo) {
     using T = typename A::Row;
@@ -281,10 +281,11 @@ inline Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads
     const int grp = n_heads / kv.kv_heads;
     const long tiles = pg_tiles_bound(r, grp, 16) * kv.kv_heads;
     Rows16Plan p;
-    p.unit = pg_whole(kv, r, n_heads, hd, size) ? PG_WHOLE_KEYS : pd_unit(size);
+    p.unit = pg_whole(kv, r, n_heads, hd, size) ? PG_WHOLE_KEYS : PD_UNIT;
     const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
     p.cut = r.cap > p.unit;
-    p.wgs = (int)(units < PG_WGS || !p.cut ? units : PG_WGS);
+    const int most = PG_WGS / 2 * pg_resident(hd, size);
+    p.wgs = (int)(units < most || !p.cut ? units : most);
     p.alone = r.cap <= 32 || (r.cap <= 256 && tiles > PG_WGS);
     return p;
 }
@@ -296,7 +297,7 @@ inline size_t rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_hea
 
 inline bool rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size) {
     const long tiles = pg_tiles_bound(r, n_heads / kv.kv_heads, 16) * kv.kv_heads;
-    if (tiles > 0x7fffffff / (r.cap / pd_unit(size) + 1)) return false;
+    if (tiles > 0x7fffffff / (r.cap / PD_UNIT + 1)) return false;
     const Rows16Plan p = rows16_plan(kv, r, n_heads, hd, size);
     return p.wgs <= (p.alone ? PA_WAVES * PG_GRID : PG_GRID);
 }
