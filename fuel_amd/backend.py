@@ -471,15 +471,16 @@ def paged_plan(dev: RocmDevice, n_seqs: int, max_pages: int, page_size: int, n_p
     kv_len_out and n_free_out."""
     kv_len_out = kv_len if kv_len_out is None else kv_len_out
     n_free_out = n_free if n_free_out is None else n_free_out
+
+    def at(name, x, n, dtype=np.int32, size=4):
+        return x if type(x) is int else _paged_operand(name, x, dev, size * n, dtype)
+
     check(lib().frq_paged_plan(
-        dev.handle, n_seqs, max_pages, page_size, n_pages, rows,
-        *(_paged_operand(name, x, dev, size * n, dtype) for name, x, n, size, dtype in (
-            ("tokens", tokens, n_seqs, 4, np.int32), ("kv_len", kv_len, n_seqs, 4, np.int32),
-            ("kv_len_out", kv_len_out, n_seqs, 4, np.int32),
-            ("page_table", page_table, n_seqs * max_pages, 4, np.int32),
-            ("free_pages", free_pages, n_pages, 4, np.int32), ("n_free", n_free, 1, 4, np.int32),
-            ("n_free_out", n_free_out, 1, 4, np.int32), ("row_start", row_start, n_seqs + 1, 4, np.int32),
-            ("slots", slots, rows, 8, np.int64), ("positions", positions, rows, 4, np.int32)))))
+        dev.handle, n_seqs, max_pages, page_size, n_pages, rows, at("tokens", tokens, n_seqs),
+        at("kv_len", kv_len, n_seqs), at("kv_len_out", kv_len_out, n_seqs),
+        at("page_table", page_table, n_seqs * max_pages), at("free_pages", free_pages, n_pages),
+        at("n_free", n_free, 1), at("n_free_out", n_free_out, 1), at("row_start", row_start, n_seqs + 1),
+        at("slots", slots, rows, np.int64, 8), at("positions", positions, rows)))
 
 
 # ---- synthetic inputs ----

@@ -20,28 +20,65 @@ namespace frq {
 
 namespace {
 
-constexpr int PP_WG = 1024;
-constexpr int PP_WAVES = PP_WG / 64;
+// Rows a thread whose slots the one workgroup writes itself: a second launch costs
+// more than they do (256 sequences of one token each 7.4 us with it, 6.3 without).
+constexpr int PP_ROWS = 4;
 
-// Sums of v >= 0 over threads 0 .. the own one; their total in `all`.  `s` is free
-// again behind the next barrier but one.
-__device__ __forceinline__ int pp_scan(int v, int (&s)[PP_WAVES], int& all) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, sum = pg_scan(v);
+// Sums of N values >= 0 each over the threads before (in place), totals in `all`.
+// `s` is free again behind the next barrier but one.
+template <int N, int WAVES>
+__device__ __forceinline__ void pp_scan(int (&v)[N], int (&s)[2][WAVES], int (&all)[N]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int k = 0; k < N; k++) v[k] = pg_scan(v[k]);
     __syncthreads();
-    if (lane == 63) s[w] = sum;
+#pragma unroll
+    for (int k = 0; k < N; k++)
+        if (lane == 63) s[k][w] = v[k];
     __syncthreads();
-    const int part = pg_scan(lane < PP_WAVES ? s[lane] : 0);
-    all = __builtin_amdgcn_readlane(part, PP_WAVES - 1);
-    return pg_add(sum, w ? __builtin_amdgcn_readlane(part, w - 1) : 0);
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int part = pg_scan(lane < WAVES ? s[k][lane] : 0), before = __shfl_up(v[k], 1);
+        all[k] = __builtin_amdgcn_readlane(part, 63);
+        v[k] = pg_add(lane ? before : 0, w ? __builtin_amdgcn_readlane(part, w - 1) : 0);
+    }
 }
 
-// The first of n threads whose sum is past i.
-__device__ __forceinline__ int pp_find(const int (&sums)[PP_WG], int i) {
+// The first of N (a power of two) whose sum is past i, which the last one's is.
+template <int N>
+__device__ __forceinline__ int pp_find(const int (&sums)[N], int i) {
     int lo = 0;
 #pragma unroll
-    for (int step = PP_WG / 2; step; step /= 2)
+    for (int step = N / 2; step; step /= 2)
         if (sums[lo + step - 1] <= i) lo += step;
     return lo;
+}
+
+// store(t, i, load(t, i)) of each of `count` items i, t the one of N whose sum holds it.
+// Four items a thread at a time where there are that many: their searches and loads
+// do not wait for each other.
+template <int WG, int N, class Load, class Store>
+__device__ __forceinline__ void pp_each(const int (&sums)[N], int count, Load load, Store store) {
+    if (count <= WG) {
+        const int i = threadIdx.x;
+        if (i < count) {
+            const int t = pp_find(sums, i);
+            store(t, i, load(t, i));
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i < count; i += 4 * WG) {
+        int t[4], v[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int x = min(i + u * WG, count - 1);
+            t[u] = pp_find(sums, x);
+            v[u] = load(t[u], x);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (i + u * WG < count) store(t[u], i + u * WG, v[u]);
+    }
 }
 
 struct PpSeq {
@@ -59,95 +96,157 @@ __device__ __forceinline__ PpSeq pp_seq(const PagedPlanArgs& a, int s) {
     return q;
 }
 
-__global__ __launch_bounds__(PP_WG) void paged_plan_kernel(PagedPlanArgs a) {
-    __shared__ int s_wave[PP_WAVES], s_sum[PP_WG], s_first[PP_WG];
+// Slot and position of a row at position pos (-1: none) in a page.
+__device__ __forceinline__ void pp_slot(const PagedPlanArgs& a, int row, int pos, int page) {
+    if (a.slots) a.slots[row] = pos < 0 ? -1 : ((int64_t)page << a.log_ps) + (pos & ((1 << a.log_ps) - 1));
+    if (a.positions) a.positions[row] = pos;
+}
+
+// One workgroup of WG threads, a thread K sequences at a time.
+template <int K, int WG>
+__global__ __launch_bounds__(WG) void paged_plan_kernel(PagedPlanArgs a) {
+    constexpr int n = K * WG;
+    __shared__ int s_wave[2][WG / 64], s_sum[n], s_first[n];
     const int tid = threadIdx.x, ps1 = (1 << a.log_ps) - 1;
-    const auto pages = [&](int n) { return (int)(((unsigned)n + ps1) >> a.log_ps); };
+    const auto pages = [&](int x) { return (int)(((unsigned)x + ps1) >> a.log_ps); };
+    PpSeq q[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) q[k] = pp_seq(a, K * tid + k);
     int stack = min(max(*a.n_free, 0), a.n_pages);
     // drops
-    for (int base = 0; base < a.n_seqs; base += PP_WG) {
-        const PpSeq q = pp_seq(a, base + tid);
-        const int keep = q.tokens < 0 ? pages(max(q.kv + q.tokens, 0)) : 0, n = q.tokens < 0 ? pages(q.kv) - keep : 0;
-        int all;
-        const int sum = pp_scan(n, s_wave, all);
-        if (all == 0) continue;
-        s_sum[tid] = sum;
-        s_first[tid] = keep - (sum - n);
-        __syncthreads();
-        all = min(all, a.n_pages - stack);  // (lengths of more pages than there are)
-        for (int i = tid; i < all; i += PP_WG) {
-            const int t = pp_find(s_sum, i);
-            a.free_pages[stack + i] = a.table[(size_t)(base + t) * a.max_pages + s_first[t] + i];
+    for (int base = 0; base < a.n_seqs; base += n) {
+        int keep[K], gone[K], sum[1] = {0}, all[1];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (base) q[k] = pp_seq(a, base + K * tid + k);
+            keep[k] = pages(max(q[k].kv + min(q[k].tokens, 0), 0));
+            gone[k] = q[k].tokens < 0 ? pages(q[k].kv) - keep[k] : 0;
+            sum[0] = pg_add(sum[0], gone[k]);
         }
-        stack += all;
+        if (!__syncthreads_or(sum[0])) continue;
+        pp_scan(sum, s_wave, all);
+        int at = sum[0];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            s_first[K * tid + k] = keep[k] - at;
+            at = pg_add(at, gone[k]);
+            s_sum[K * tid + k] = at;
+        }
+        __syncthreads();
+        const int put = min(all[0], a.n_pages - stack);  // (lengths of more pages than there are)
+        pp_each<WG>(
+            s_sum, put, [&](int t, int i) { return a.table[(size_t)(base + t) * a.max_pages + s_first[t] + i]; },
+            [&](int, int i, int page) { a.free_pages[stack + i] = page; });
+        stack += put;
     }
     __syncthreads();
     // grants
+    const bool slots = a.rows <= PP_ROWS * WG && (a.slots || a.positions);
     int asked_pages = 0, asked_rows = 0, rows = 0, taken = 0;
-    for (int base = 0; base < a.n_seqs; base += PP_WG) {
-        const int s = base + tid;
-        const PpSeq q = pp_seq(a, s);
-        const int want = max(q.tokens, 0), have = q.tokens > 0 ? pages(q.kv) : 0;
-        const int need = q.tokens > 0 ? pages(q.kv + want) - have : 0;
-        int all_pages, all_rows, all_granted, all_taken;
-        const int sum_pages = pg_add(asked_pages, pp_scan(need, s_wave, all_pages));
-        const int sum_rows = pg_add(asked_rows, pp_scan(want, s_wave, all_rows));
-        const bool ok = want > 0 && (need == 0 || sum_pages <= stack) && sum_rows <= a.rows;
-        const int granted = ok ? want : 0, sum = pp_scan(granted, s_wave, all_granted);
-        const int mine = pp_scan(ok ? need : 0, s_wave, all_taken);
-        s_sum[tid] = mine;
-        s_first[tid] = have - (mine - (ok ? need : 0));
-        if (s < a.n_seqs) {
-            a.kv_len_out[s] = q.tokens < 0 ? max(q.kv + q.tokens, 0) : q.kv + granted;
-            a.row_start[s] = rows + sum - granted;
+    for (int base = 0; base < a.n_seqs; base += n) {
+        int want[K], have[K], need[K], sum[2] = {0, 0}, all[2];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (a.n_seqs > n) q[k] = pp_seq(a, base + K * tid + k);
+            want[k] = max(q[k].tokens, 0);
+            have[k] = pages(q[k].kv);
+            need[k] = want[k] ? pages(q[k].kv + want[k]) - have[k] : 0;
+            sum[0] = pg_add(sum[0], need[k]);
+            sum[1] = pg_add(sum[1], want[k]);
+        }
+        pp_scan(sum, s_wave, all);
+        const int end_pages = pg_add(asked_pages, all[0]), end_rows = pg_add(asked_rows, all[1]);
+        if (end_pages > stack || end_rows > a.rows) {  // not all: the sums of those that are
+            int at_pages = pg_add(asked_pages, sum[0]), at_rows = pg_add(asked_rows, sum[1]);
+            sum[0] = sum[1] = 0;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                at_pages = pg_add(at_pages, need[k]);
+                at_rows = pg_add(at_rows, want[k]);
+                if ((need[k] && at_pages > stack) || at_rows > a.rows) want[k] = need[k] = 0;
+                sum[0] += need[k];
+                sum[1] += want[k];
+            }
+            pp_scan(sum, s_wave, all);
+        }
+        asked_pages = end_pages;
+        asked_rows = end_rows;
+        int at = sum[0], row = sum[1];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int s = base + K * tid + k;
+            s_first[K * tid + k] = have[k] - at;
+            at += need[k];
+            s_sum[K * tid + k] = at;
+            if (s < a.n_seqs) {
+                a.kv_len_out[s] = q[k].tokens < 0 ? max(q[k].kv + q[k].tokens, 0) : q[k].kv + want[k];
+                a.row_start[s] = rows + row;
+            }
+            row += want[k];
         }
         __syncthreads();
-        for (int i = tid; i < all_taken; i += PP_WG) {
-            const int t = pp_find(s_sum, i);
-            a.table[(size_t)(base + t) * a.max_pages + s_first[t] + i] = a.free_pages[stack - 1 - taken - i];
+        pp_each<WG>(
+            s_sum, all[0], [&](int, int i) { return a.free_pages[stack - 1 - taken - i]; },
+            [&](int t, int i, int page) { a.table[(size_t)(base + t) * a.max_pages + s_first[t] + i] = page; });
+        if (slots) {
+            __syncthreads();
+            row = sum[1];
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                s_first[K * tid + k] = q[k].kv - row;  // position of the sequence's row i: that and i
+                row += want[k];
+                s_sum[K * tid + k] = row;
+            }
+            __syncthreads();
+            pp_each<WG>(
+                s_sum, all[1],
+                [&](int t, int i) {
+                    return a.table[(size_t)(base + t) * a.max_pages + ((s_first[t] + i) >> a.log_ps)];
+                },
+                [&](int t, int i, int page) { pp_slot(a, rows + i, s_first[t] + i, page); });
         }
-        asked_pages = pg_add(asked_pages, all_pages);
-        asked_rows = pg_add(asked_rows, all_rows);
-        rows += all_granted;
-        taken += all_taken;
+        rows += all[1];
+        taken += all[0];
     }
+    if (slots)
+        for (int row = rows + tid; row < a.rows; row += WG) pp_slot(a, row, -1, 0);
     if (tid == 0) {
         a.row_start[a.n_seqs] = rows;
         *a.n_free_out = stack - taken;
     }
 }
 
-// Slot and position of each packed row, -1 behind the last.
+// Slots of more rows, a thread each.
 __global__ __launch_bounds__(256) void paged_slots_kernel(PagedPlanArgs a) {
     const int row = blockIdx.x * 256 + threadIdx.x;
     if (row >= a.rows) return;
-    int64_t slot = -1;
-    int pos = -1;
-    if (row < a.row_start[a.n_seqs]) {
-        int lo = 0, n = a.n_seqs;  // the last of lo .. lo + n - 1 that starts at or before row
-        while (n > 1) {
-            const int half = n >> 1;
-            if (a.row_start[lo + half] <= row) {
-                lo += half;
-                n -= half;
-            } else {
-                n = half;
-            }
-        }
-        pos = a.kv_len_out[lo] - (a.row_start[lo + 1] - row);
-        const int page = a.table[(size_t)lo * a.max_pages + (pos >> a.log_ps)];
-        slot = ((int64_t)page << a.log_ps) + (pos & ((1 << a.log_ps) - 1));
+    if (row >= a.row_start[a.n_seqs]) {
+        pp_slot(a, row, -1, 0);
+        return;
     }
-    if (a.slots) a.slots[row] = slot;
-    if (a.positions) a.positions[row] = pos;
+    int s = 0, n = a.n_seqs;  // the last of s .. s + n - 1 that starts at or before row
+    while (n > 1) {
+        const int half = n >> 1;
+        const bool up = a.row_start[s + half] <= row;
+        s += up ? half : 0;
+        n = up ? n - half : half;
+    }
+    const int pos = a.kv_len_out[s] - (a.row_start[s + 1] - row);
+    pp_slot(a, row, pos, a.table[(size_t)s * a.max_pages + (pos >> a.log_ps)]);
 }
 
 }  // namespace
 
 hipError_t launch_paged_plan(const PagedPlanArgs& p, hipStream_t s) {
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(PP_WG), 0, s, p);
+    // (few wavefronts meet at a barrier sooner; many move more pages at a time)
+    const long most = p.n_seqs > p.rows >> p.log_ps ? p.n_seqs : p.rows >> p.log_ps;
+    const int wg = most <= 64 ? 64 : most <= 256 ? 256 : 1024;
+    const auto kernel = wg == 64    ? paged_plan_kernel<1, 64>
+                        : wg == 256 ? paged_plan_kernel<1, 256>
+                        : p.n_seqs <= 1024 ? paged_plan_kernel<1, 1024> : paged_plan_kernel<4, 1024>;
+    hipLaunchKernelGGL(kernel, dim3(1), dim3(wg), 0, s, p);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.rows == 0 || !(p.slots || p.positions)) return e;
+    if (e != hipSuccess || p.rows <= PP_ROWS * wg || !(p.slots || p.positions)) return e;
     hipLaunchKernelGGL(paged_slots_kernel, dim3((unsigned)((p.rows + 255l) / 256)), dim3(256), 0, s, p);
     return hipGetLastError();
 }

@@ -121,6 +121,22 @@ def test_plan_entries_that_are_none(dev):
     c.run()
 
 
+@pytest.mark.parametrize("n,ps,width", [(6, 1024, 1 << 20), (1100, 1024, 1 << 11), (1100, 16, 1 << 14)])
+def test_plan_sums_past_32_bits(dev, n, ps, width):
+    """More tokens and pages asked for than an int counts, small requests between."""
+    say("plan sums", n, ps, width)
+    rng = seed(63, n, ps)
+    cap = width * ps
+    for pages, rows in ((40, 2000), (3, 2000), (40, 7), (1000, 1 << 12)):
+        kv = rng.integers(0, 3, n)
+        table = np.full((n, width), -1, np.int32)
+        table[:, 0] = 1000 + np.arange(n)
+        tokens = rng.integers(0, 20, n)
+        tokens[rng.integers(0, n, n // 2)] = cap - 3
+        tokens[0], tokens[1], tokens[-1] = 2, 3, -1
+        Call(dev, tokens, kv, table, np.arange(pages), pages, ps, rows).run()
+
+
 def test_plan_of_nothing(dev):
     say("plan of nothing")
     i = lambda a, t=np.int32: dev.from_numpy(np.asarray(a, t))  # noqa: E731
