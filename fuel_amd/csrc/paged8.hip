@@ -398,13 +398,82 @@ __device__ __forceinline__ uint32_t p8_again(uint32_t w, int was, int b) {
     return was == 255 ? 0x7f7f7f7fu : p8_codes(x, P8_ONE + b - was);
 }
 
+// A lane's part of a row's head: N dims of its lower half and those HD / 2 further (a
+// rotation's pairs), of four lanes.
+template <class T, int HD>
+struct Append8Row {
+    static constexpr int N = HD / 8, HALF = HD / 2;
+    T lo[N], hi[N];
+    float x[2][N];
+
+    __device__ __forceinline__ void load(const T* from) {
+        __builtin_memcpy(lo, __builtin_assume_aligned(from, 16), sizeof lo);
+        __builtin_memcpy(hi, __builtin_assume_aligned(from + HALF, 16), sizeof hi);
+    }
+    // x, turned by the tables' rows from cs and sn on (null: as it is).
+    __device__ __forceinline__ void turn(const float* cs, const float* sn) {
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            x[0][e] = (float)lo[e];
+            x[1][e] = (float)hi[e];
+        }
+        if (!cs) return;
+        float cl[N], ch[N], sl[N], sh[N];
+        __builtin_memcpy(cl, __builtin_assume_aligned(cs, 16), sizeof cl);
+        __builtin_memcpy(ch, __builtin_assume_aligned(cs + HALF, 16), sizeof ch);
+        __builtin_memcpy(sl, __builtin_assume_aligned(sn, 16), sizeof sl);
+        __builtin_memcpy(sh, __builtin_assume_aligned(sn + HALF, 16), sizeof sh);
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const float y = x[0][e], w = x[1][e];
+            x[0][e] = y * cl[e] - w * sl[e];
+            x[1][e] = w * ch[e] + y * sh[e];
+        }
+    }
+    // The largest finite magnitude.
+    __device__ __forceinline__ float most() const {
+        float a = 0.0f;
+#pragma unroll
+        for (int d = 0; d < 2; d++)
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const float y = fabsf(x[d][e]);
+                a = y < __builtin_inff() ? fmaxf(a, y) : a;
+            }
+        return a;
+    }
+    __device__ __forceinline__ void put(uint8_t* to, int byte) const {
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            uint32_t w[N / 4];
+#pragma unroll
+            for (int e = 0; e < N / 4; e++) w[e] = p8_codes(x[d] + 4 * e, byte);
+            __builtin_memcpy(__builtin_assume_aligned(to + d * HALF, 8), w, sizeof w);
+        }
+    }
+    // Codes under byte `was` as codes under `byte`.
+    __device__ __forceinline__ static void again(uint8_t* at, int was, int byte) {
+#pragma unroll
+        for (int d = 0; d < 2; d++) {
+            uint32_t w[N / 4];
+            __builtin_memcpy(w, __builtin_assume_aligned(at + d * HALF, 8), sizeof w);
+#pragma unroll
+            for (int e = 0; e < N / 4; e++) w[e] = p8_again(w[e], was, byte);
+            __builtin_memcpy(__builtin_assume_aligned(at + d * HALF, 8), w, sizeof w);
+        }
+    }
+};
+
 // Workgroups below q_wgs: `parts` to a packed row, chunks of its q as paged_append_kernel
-// takes them.  The others: a wavefront takes 16 rows of codes, four lanes a row, each
-// HD / 8 dims of its lower half and those HD / 2 further (a rotation's pairs):
-//   ONE (one row a sequence)   one position's rows of up to 16 heads of k and v
-//   otherwise                  the up to 16 rows of a block, of one head of k or v
+// takes them.  The others: a wavefront takes 16 rows of codes, four lanes a row,
+//   NARROW      the same position of up to 16 heads of k and v: a row a wavefront, the
+//               first of a block's rows works all of them, one after another
+//   otherwise   the up to 16 rows of a block, of one head of k or v
+// Bound by HBM for many rows (11166 of f32, 32 heads over 8 of 128: 482 MB in 99 us,
+// 4.9 TB/s, as a copy), by four memory round trips for few: the row's sequence (two),
+// its page, its block's scale.
 constexpr int A8_WG = 256;
-template <class T, int HD, bool ONE>
+template <class T, int HD, bool NARROW>
 __global__ __launch_bounds__(A8_WG) void paged8_append_kernel(PagedKv8 c, PagedRows b, int n_heads, int q_wgs, int parts,
                                                               const T* q, int ldq, const T* __restrict__ k, int ldk,
                                                               const T* __restrict__ v, int ldv,
@@ -414,68 +483,81 @@ __global__ __launch_bounds__(A8_WG) void paged8_append_kernel(PagedKv8 c, PagedR
     constexpr int HALF = HD / 2;
     if ((int)blockIdx.x < q_wgs) {
         constexpr int CP = HALF / 8;
-        const int row = (unsigned)blockIdx.x / (unsigned)parts, part = blockIdx.x - row * parts;
+        const int row = (unsigned)blockIdx.x / (unsigned)parts, stride = A8_WG * parts;  // (a multiple of CP)
+        int e = A8_WG * (blockIdx.x - row * parts) + threadIdx.x;
+        const int i = 8 * (e % CP);
+        T lo[8], hi[8];
+        const auto fetch = [&] {  // (past the last head: the first one's again, not used)
+            const T* x = q + (size_t)row * ldq + (e < CP * n_heads ? e / CP * HD : 0) + i;
+            __builtin_memcpy(lo, __builtin_assume_aligned(x, 16), sizeof lo);
+            __builtin_memcpy(hi, __builtin_assume_aligned(x + HALF, 16), sizeof hi);
+        };
+        fetch();
         const int s = pg_row_seq(b, row);
         if (s < 0) return;
         const PgSeq sq = pg_seq(b, s);
         if (row < sq.row0 || row >= sq.row0 + sq.n) return;
         const int pos = sq.kv - sq.n + (row - sq.row0);
-        const bool bad = sq.bad || (cs && pos >= rope_rows), seen = pos >= 0 && !bad;
-        for (int e = A8_WG * part + threadIdx.x; e < CP * n_heads; e += A8_WG * parts) {
-            const int h = e / CP, i = 8 * (e % CP);
-            const T* x = q + (size_t)row * ldq + h * HD + i;
-            T lo[8], hi[8];
-            float cl[8], ch[8], sl[8], sh[8];
-            __builtin_memcpy(lo, __builtin_assume_aligned(x, 16), sizeof lo);
-            __builtin_memcpy(hi, __builtin_assume_aligned(x + HALF, 16), sizeof hi);
-            if (cs && seen) {
-                const float *ct = cs + (size_t)pos * HD + i, *st = sn + (size_t)pos * HD + i;
-                __builtin_memcpy(cl, __builtin_assume_aligned(ct, 16), sizeof cl);
-                __builtin_memcpy(ch, __builtin_assume_aligned(ct + HALF, 16), sizeof ch);
-                __builtin_memcpy(sl, __builtin_assume_aligned(st, 16), sizeof sl);
-                __builtin_memcpy(sh, __builtin_assume_aligned(st + HALF, 16), sizeof sh);
-            }
+        const bool bad = sq.bad || (cs && pos >= rope_rows), turned = cs && pos >= 0 && !bad;
+        float cl[8], ch[8], sl[8], sh[8];
+        if (turned) {
+            const float *ct = cs + (size_t)pos * HD + i, *st = sn + (size_t)pos * HD + i;
+            __builtin_memcpy(cl, __builtin_assume_aligned(ct, 16), sizeof cl);
+            __builtin_memcpy(ch, __builtin_assume_aligned(ct + HALF, 16), sizeof ch);
+            __builtin_memcpy(sl, __builtin_assume_aligned(st, 16), sizeof sl);
+            __builtin_memcpy(sh, __builtin_assume_aligned(st + HALF, 16), sizeof sh);
+        }
+        for (; e < CP * n_heads; e += stride, fetch()) {
+            T x[8], y[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                float y = (float)lo[j], z = (float)hi[j];
-                if (cs && seen) {
-                    const float u = y, w = z;
-                    y = u * cl[j] - w * sl[j];
-                    z = w * ch[j] + u * sh[j];
+                float u = (float)lo[j], w = (float)hi[j];
+                if (turned) {
+                    const float z = u;
+                    u = z * cl[j] - w * sl[j];
+                    w = w * ch[j] + z * sh[j];
                 }
-                lo[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : y);
-                hi[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : z);
+                x[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : u);
+                y[j] = (T)(bad ? pg_nan() : pos < 0 ? 0.0f : w);
             }
-            T* to = q_out + (size_t)row * ldqo + h * HD + i;
-            __builtin_memcpy(__builtin_assume_aligned(to, 16), lo, sizeof lo);
-            __builtin_memcpy(__builtin_assume_aligned(to + HALF, 16), hi, sizeof hi);
+            T* to = q_out + (size_t)row * ldqo + e / CP * HD + i;
+            __builtin_memcpy(__builtin_assume_aligned(to, 16), x, sizeof x);
+            __builtin_memcpy(__builtin_assume_aligned(to + HALF, 16), y, sizeof y);
         }
         return;
     }
-    constexpr int N = HD / 8;  // dims of a half a lane takes
-    const int lane = threadIdx.x & 63, sub = lane >> 2, i = N * (lane & 3);
+    using R = Append8Row<T, HD>;
+    const int lane = threadIdx.x & 63, sub = lane >> 2, i = R::N * (lane & 3);
     const int at = __builtin_amdgcn_readfirstlane((int)((blockIdx.x - q_wgs) * (A8_WG / 64) + (threadIdx.x >> 6)));
-    int s, head, lo, hi;  // sequence, head, and the block's positions [lo, hi) that are new
-    bool value;
-    PgSeq sq;
-    const auto ends = [&](const PgSeq& x, int& first) {  // the sequence's rows that are stored: positions [first, end)
+    // the positions of a sequence's rows that are stored
+    const auto ends = [&](const PgSeq& x, int& first) {
         first = max(x.kv - x.n, 0);
         return x.n && !x.bad ? max(first, cs ? min(x.kv, rope_rows) : x.kv) : first;
     };
-    if constexpr (ONE) {
-        const int waves = (2 * c.kv_heads + 15) >> 4;
-        s = (unsigned)at / (unsigned)waves;
-        if (s >= b.n_seqs) return;
-        const int unit = 16 * (at - s * waves) + sub;
+    int s, head, lo, hi;  // sequence, head, and the block's positions [lo, hi) that are new
+    bool value, mine;
+    PgSeq sq;
+    R x;
+    const auto row_of = [&](int pos) {
+        return (value ? v : k) + (size_t)(sq.row0 + pos - (sq.kv - sq.n)) * (value ? ldv : ldk) + head * HD + i;
+    };
+    if constexpr (NARROW) {
+        const int waves = (2 * c.kv_heads + 15) >> 4, row = (unsigned)at / (unsigned)waves;
+        if (row >= b.rows) return;
+        const int unit = 16 * (at - row * waves) + sub;
+        mine = unit < 2 * c.kv_heads;
         value = unit >= c.kv_heads;
-        head = unit - (value ? c.kv_heads : 0);
+        head = mine ? unit - (value ? c.kv_heads : 0) : 0;
+        x.load((value ? v : k) + (size_t)row * (value ? ldv : ldk) + head * HD + i);  // (most often the only row)
+        s = pg_row_seq(b, row);
+        if (s < 0) return;
         sq = pg_seq(b, s);
-        hi = ends(sq, lo);
-        if (lo >= hi) return;
-        if (head >= c.kv_heads) {  // (these lanes take no part in their group's sums)
-            head = 0;
-            hi = lo;
-        }
+        if (row < sq.row0 || row >= sq.row0 + sq.n) return;
+        lo = sq.kv - sq.n + (row - sq.row0);
+        int first;
+        const int end = ends(sq, first);
+        if (lo < first || lo >= end || (lo > first && (lo & 15))) return;
+        hi = min((lo | 15) + 1, end);
     } else {
         const auto blocks = [&](const PgSeq& x) {
             int first;
@@ -485,92 +567,67 @@ __global__ __launch_bounds__(A8_WG) void paged8_append_kernel(PagedKv8 c, PagedR
         PgUnits<decltype(blocks)> pu(b, blocks);
         const int unit = (unsigned)at / (unsigned)(2 * c.kv_heads);
         if (unit >= pu.total) return;
-        int u;
+        int u, first;
         s = pu.find(unit, u);
         sq = pu.get(s);
         value = (at - unit * 2 * c.kv_heads) & 1;
         head = (at - unit * 2 * c.kv_heads) >> 1;
-        int first;
-        const int end = ends(sq, first), j0 = ((first >> 4) + u) << 4;
-        lo = max(j0, first);
-        hi = min(j0 + 16, end);
+        const int end = ends(sq, first), j = ((first >> 4) + u) << 4;
+        lo = max(j, first);
+        hi = min(j + 16, end);
+        mine = j + sub >= lo && j + sub < hi;
+        x.load(row_of(mine ? j + sub : lo));
     }
-    const int j0 = lo & ~15, pos = ONE ? lo : j0 + sub;
+    const int j0 = lo & ~15;
     bool none;
     const int page = pg_page(c, b.table + (size_t)s * b.max_pages, j0, sq.kv, none);
     if (none) return;
     const size_t row = (((size_t)page * c.kv_heads + head) << c.log_ps) + (j0 & ((1 << c.log_ps) - 1));
     uint8_t* codes = static_cast<uint8_t*>(value ? c.v : c.k) + row * HD + i;
     uint8_t* scale = (value ? c.v_scale : c.k_scale) + (row >> 4);
-    const bool mine = pos >= lo && pos < hi;
-    float x[2][N];
-#pragma unroll
-    for (int e = 0; e < N; e++) x[0][e] = x[1][e] = 0.0f;
+    const int was = lo > j0 ? *scale : 0;
+    const auto turn = [&](int pos) {
+        const bool t = cs && !value;
+        x.turn(t ? cs + (size_t)pos * HD + i : nullptr, sn + (t ? (size_t)pos * HD + i : 0));
+    };
     float amax = 0.0f;
-    if (mine) {
-        const T* from = (value ? v : k) + (size_t)(sq.row0 + pos - (sq.kv - sq.n)) * (value ? ldv : ldk) + head * HD + i;
-        T a[N], z[N];
-        __builtin_memcpy(a, __builtin_assume_aligned(from, 16), sizeof a);
-        __builtin_memcpy(z, __builtin_assume_aligned(from + HALF, 16), sizeof z);
-#pragma unroll
-        for (int e = 0; e < N; e++) {
-            x[0][e] = (float)a[e];
-            x[1][e] = (float)z[e];
+    if constexpr (NARROW) {
+        turn(lo);
+        amax = x.most();
+        for (int pos = lo + 1; pos < hi; pos++) {
+            x.load(row_of(pos));
+            turn(pos);
+            amax = fmaxf(amax, x.most());
         }
-        if (cs && !value) {
-            const float *ct = cs + (size_t)pos * HD + i, *st = sn + (size_t)pos * HD + i;
-            float cl[N], ch[N], sl[N], sh[N];
-            __builtin_memcpy(cl, __builtin_assume_aligned(ct, 16), sizeof cl);
-            __builtin_memcpy(ch, __builtin_assume_aligned(ct + HALF, 16), sizeof ch);
-            __builtin_memcpy(sl, __builtin_assume_aligned(st, 16), sizeof sl);
-            __builtin_memcpy(sh, __builtin_assume_aligned(st + HALF, 16), sizeof sh);
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float y = x[0][e], w = x[1][e];
-                x[0][e] = y * cl[e] - w * sl[e];
-                x[1][e] = w * ch[e] + y * sh[e];
-            }
-        }
-#pragma unroll
-        for (int d = 0; d < 2; d++)
-#pragma unroll
-            for (int e = 0; e < N; e++) {
-                const float y = fabsf(x[d][e]);
-                amax = y < __builtin_inff() ? fmaxf(amax, y) : amax;
-            }
+    } else {
+        turn(mine ? j0 + sub : lo);
+        amax = x.most();  // (of the other lanes: lo's)
     }
 #pragma unroll
-    for (int d = 1; d < (ONE ? 4 : 64); d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-    if (ONE && hi <= lo) return;
+    for (int d = 1; d < (NARROW ? 4 : 64); d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+    if (NARROW && !mine) return;
     int byte = p8_scale_of(amax);
     if (lo > j0) {  // older rows
-        const int was = *scale, need = byte;
-        byte = was == 255 ? need : max(was, need);
-        if (byte != was) {
-            const auto again = [&](uint8_t* to) {
-                uint32_t w[N / 4];
-                __builtin_memcpy(w, __builtin_assume_aligned(to, 8), sizeof w);
-#pragma unroll
-                for (int e = 0; e < N / 4; e++) w[e] = p8_again(w[e], was, byte);
-                __builtin_memcpy(__builtin_assume_aligned(to, 8), w, sizeof w);
-            };
-            for (int r = ONE ? 0 : sub; r < lo - j0; r += ONE ? 1 : 16) {
-                again(codes + r * HD);
-                again(codes + r * HD + HALF);
-            }
-        }
+        byte = was == 255 ? byte : max(was, byte);
+        if (byte != was)
+            for (int r = NARROW ? 0 : sub; r < lo - j0; r += NARROW ? 1 : 16) R::again(codes + r * HD, was, byte);
     }
-    if (mine) {
-#pragma unroll
-        for (int d = 0; d < 2; d++) {
-            uint32_t w[N / 4];
-#pragma unroll
-            for (int e = 0; e < N / 4; e++) w[e] = p8_codes(x[d] + 4 * e, byte);
-            __builtin_memcpy(__builtin_assume_aligned(codes + (pos - j0) * HD + d * HALF, 8), w, sizeof w);
+    if constexpr (NARROW) {
+        for (int pos = hi - 1;; pos--) {  // (the last one's is at hand)
+            x.put(codes + (pos - j0) * HD, byte);
+            if (pos == lo) break;
+            x.load(row_of(pos - 1));
+            turn(pos - 1);
         }
+    } else if (mine) {
+        x.put(codes + sub * HD, byte);
     }
-    if (ONE ? (lane & 3) == 0 : lane == 0) *scale = (uint8_t)byte;
+    if (NARROW ? (lane & 3) == 0 : lane == 0) *scale = (uint8_t)byte;
 }
+
+// Few rows a sequence: NARROW (256 sequences of one row each, 8 KV heads: 5.7 us, 9.4
+// otherwise; a block's rows one after another, up to 16, take it longer then).
+inline bool append8_narrow(const PagedRows& r) { return !r.row_start || r.rows <= 2l * r.n_seqs; }
 
 struct Append8Call {
     const PagedAppendArgs& p;
@@ -582,7 +639,7 @@ struct Append8Call {
         const int parts = chunks ? (chunks + A8_WG - 1) / A8_WG : 0;
         const long q_wgs = (long)p.rows.rows * parts, waves = paged8_append_waves(c, p.rows);
         const long wgs = q_wgs + (waves + A8_WG / 64 - 1) / (A8_WG / 64);
-        const auto kernel = p.rows.row_start ? paged8_append_kernel<T, HD, false> : paged8_append_kernel<T, HD, true>;
+        const auto kernel = append8_narrow(p.rows) ? paged8_append_kernel<T, HD, true> : paged8_append_kernel<T, HD, false>;
         hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(A8_WG), 0, s, c, p.rows, p.n_heads, (int)q_wgs, parts,
                            static_cast<const T*>(p.q), p.ldq, static_cast<const T*>(p.k), p.ldk,
                            static_cast<const T*>(p.v), p.ldv, p.cos, p.sin, p.rope_rows, static_cast<T*>(p.q_out),
@@ -594,9 +651,9 @@ struct Append8Call {
 }  // namespace
 
 long paged8_append_waves(const PagedKv& kv, const PagedRows& r) {
+    if (append8_narrow(r)) return (long)r.rows * ((2 * kv.kv_heads + 15) / 16);
     // n rows lie in at most n / 16 + 2 blocks of 16 positions
-    return r.row_start ? ((long)r.rows / 16 + 2l * (r.n_seqs < r.rows ? r.n_seqs : r.rows)) * 2 * kv.kv_heads
-                       : (long)r.n_seqs * ((2 * kv.kv_heads + 15) / 16);
+    return ((long)r.rows / 16 + 2l * (r.n_seqs < r.rows ? r.n_seqs : r.rows)) * 2 * kv.kv_heads;
 }
 
 hipError_t launch_paged8_append(int dtype, int hd, const PagedAppendArgs& p, const PagedKv8& c, hipStream_t s) {

@@ -109,15 +109,20 @@ class Case:
 # ---- append ----
 
 @pytest.mark.parametrize("act", TYPES)
+@pytest.mark.parametrize("few", [False, True])
 @pytest.mark.parametrize("H,hk,D,ps", [(4, 2, 128, 16), (7, 1, 64, 32), (40, 20, 128, 64)])
-def test_append(dev, act, H, hk, D, ps):
+def test_append(dev, act, few, H, hk, D, ps):
     """Ragged sequences (one empty, one whose first rows stand before position 0, one
     with a length that is none, one with a page outside the pool), blocks that older
     rows are in, of a smaller and of a larger scale than the new, rows before and
     behind them, q, k and v as parts of one wide row."""
-    say("append", act, H, hk, D, ps)
-    rng = seed(1, act, H, D)
+    say("append", act, few, H, hk, D, ps)
+    rng = seed(1, act, H, D, few)
     past, new = [0, 5, 31, -3, 40, 0, 2, 20, 13, 47, 15], [1, 30, 0, 9, 3, 65, 4, 7, 1, 2, 50]
+    if few:  # two rows a sequence at most in the mean
+        past, new = past + [int(x) for x in rng.integers(0, 60, 109)], new + [int(x) for x in rng.integers(0, 2, 109)]
+        new[50:53] = 12, 3, 17
+        past[50:53] = 10, 30, 8
     c = Case(dev, rng, act, H, hk, D, ps, past, new, row0=2, tail=3, width=8 if ps < 64 else 0, fill=False)
     for s, p in enumerate(past):
         c.pool.fill(rng, s, p, std=[1.0, 0.01, 60.0][s % 3])
@@ -163,7 +168,8 @@ def test_append(dev, act, H, hk, D, ps):
     c.check_cells()
 
 
-@pytest.mark.parametrize("act,hk,D", [(F32, 3, 64), (BF16, 8, 128), (F16, 17, 64)])
+@pytest.mark.parametrize("act,hk,D", [(F32, 3, 64), (BF16, 8, 128), (F16, 17, 64), (F32, 9, 128), (F16, 2, 128),
+                                      (BF16, 1, 64)])
 def test_append_tokens_one_by_one(dev, act, hk, D):
     """One row a sequence, from each position of a block on, magnitudes that grow and
     shrink from token to token; without tables, without q, and in place."""
