@@ -12,7 +12,8 @@
 // matrix pipe as f16 (bf16 for bf16 rows) without their scale, exactly; a group of
 // 16 keys' scale is a factor of its scores, in f32.  V's go there as bf16 values,
 // exactly, so that no weight has to carry a scale.  f32 rows: q in two parts of f16,
-// weights in three of bf16.  16-bit rows: q as it is, weights in two parts of bf16.
+// 16-bit rows as they are; weights in two parts of bf16, to 2^-16 of each: V's codes
+// are 2^-4 of what was appended.
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
@@ -33,7 +34,7 @@ struct Rows8 {
     using P = PgElem<__bf16>;                                      // of weights and v
     using q8 = typename PgElem<E>::v8;
     using v8 = P::v8;
-    static constexpr int NQ = WIDE ? 2 : 1, NP = WIDE ? 3 : 2;
+    static constexpr int NQ = WIDE ? 2 : 1, NP = 2;
     static constexpr int DIM = HD, KS = HD / 32, VW = HD / 16;
     // Groups of 16 keys of a block.  (Of four, where the 16 KB of two blocks of 32 go
     // out at once: no faster, and 10.0 us for 7.6 where a wavefront has a few blocks.)

@@ -659,7 +659,7 @@ struct Prefill8Call {
     hipError_t run() const {
         constexpr bool wide = std::is_same<T, float>::value;
         using E = typename std::conditional<wide, _Float16, T>::type;
-        return prefill_launch<PrefillTile<PagedKv8, E, __bf16, T, HD, wide ? 2 : 1, wide ? 3 : 1>>(p, c, s);
+        return prefill_launch<PrefillTile<PagedKv8, E, __bf16, T, HD, wide ? 2 : 1, wide ? 2 : 1>>(p, c, s);
     }
 };
 

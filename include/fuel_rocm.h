@@ -452,11 +452,11 @@ int frq_paged8_append(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_
                       size_t ldqo);
 /* frq_paged_attention_workspace, _decode and _prefill over such a cache, dtype
  * FRQ_F32, FRQ_F16 or FRQ_BF16.  Codes and scales are taken as the values that they
- * stand for, scores, softmax and sums are f32: f32 operands are multiplied in parts
- * that hold them to 2^-22.  With 16-bit rows a softmax weight is held to 2^-16 for the
- * product with V, in batches of many rows, as the sizes of the structs have it, to
- * 2^-8 (their sum is not rounded).  A scale counts as 2^119 at most in a row's sums
- * that are finite; NaN as frq_paged_batch has it. */
+ * stand for; scores, softmax and sums are f32.  f32 rows of q are multiplied in parts
+ * that hold them to 2^-22.  A softmax weight is held to 2^-16 for the product with V,
+ * with 16-bit rows in batches of many rows, as the sizes of the structs have it, to 2^-8
+ * (their sum is not rounded).  NaN as frq_paged_batch has it; a code times its scale
+ * past f32's range is infinite. */
 size_t frq_paged8_attention_workspace(const frq_paged_kv8 *kv, const frq_paged_batch *batch, size_t n_heads);
 int frq_paged8_attention_decode(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype,
                                 size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,

@@ -6,9 +6,8 @@ Values.  code * 2^(b - 127): exact in 64 bits, and in the 32 that appended rows 
 Bounds: paged_ref.py's, with these terms in the place of its.
 score: a code is exact as an f16 or bf16 operand and a scale is a power of two, so
   the products err as those of a 16-bit cache do; one factor more, exactly.
-weights as factors of V: bf16 parts, half a step 2^-8 each.  f32 rows keep three
-  (2^-24; 2^-22 is allowed as there), 16-bit rows two (2^-16), in tiles of 128 rows one
-  (2^-8).  bf16 has f32's range: no absolute term but where a value leaves it.
+weights as factors of V: bf16 parts, half a step 2^-8 each.  Two are kept (2^-16),
+  of 16-bit rows in tiles of 128 rows one (2^-8).  bf16 has f32's range: no absolute term but where a value leaves it.
 """
 import numpy as np
 
@@ -121,6 +120,6 @@ class Pool:
 
 def bound(out, A, B, n, D, act, tiles):
     d = ((D + 10) * A + 4) * U
-    w = 2.0 ** -22 if act == F32 else 2.0 ** -8 if tiles else 2.0 ** -16
+    w = 2.0 ** -8 if tiles and act != F32 else 2.0 ** -16
     tol = (2 * (d + n * U) + 16 * U + w) * B + TINY[R.BF16]
     return tol + (0 if act == F32 else HALF[act] * (np.abs(out) + tol + TINY[act]))
