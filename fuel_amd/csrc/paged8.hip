@@ -78,12 +78,14 @@ struct Rows8 {
     // The loads of a block of keys: group a's 16 rows start at at[a], values' loads
     // are those of groups 2 h and 2 h + 1.  ONCE: nothing else of the call reads them,
     // so they go past the caches.
+    using Base = const P8Global<uint8_t>*;
     template <bool ONCE, class W>
-    __device__ static W load(const uint8_t* p) {
-        return ONCE ? __builtin_nontemporal_load(reinterpret_cast<const W*>(p)) : *reinterpret_cast<const W*>(p);
+    __device__ static W load(Base p) {
+        const auto* w = reinterpret_cast<const P8Global<W>*>(p);
+        return ONCE ? __builtin_nontemporal_load(w) : *w;
     }
     template <bool ONCE>
-    __device__ static void load_k(KeyRegs& k, const uint8_t* const (&at)[G]) {
+    __device__ static void load_k(KeyRegs& k, const Base (&at)[G]) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int a = 0; a < G; a++)
@@ -91,7 +93,7 @@ struct Rows8 {
             for (int c = 0; c < HD / 64; c++) k.w[a][c] = load<ONCE, pg_u4>(at[a] + r * HD + 64 * c + 16 * g);
     }
     template <bool ONCE>
-    __device__ static void load_v(ValueRegs& v, const uint8_t* const (&at)[G], int h) {
+    __device__ static void load_v(ValueRegs& v, const Base (&at)[G], int h) {
         const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int a = 2 * h; a < 2 * h + 2; a++)
@@ -266,9 +268,9 @@ struct Rows8 {
         }
         return b;
     }
-    __device__ static void rows(const P8Groups& gr, const void* pool, int i, const uint8_t* (&at)[G]) {
+    __device__ static void rows(const P8Groups& gr, const void* pool, int i, Base (&at)[G]) {
 #pragma unroll
-        for (int a = 0; a < G; a++) at[a] = static_cast<const uint8_t*>(pool) + gr.at(G * i + a);
+        for (int a = 0; a < G; a++) at[a] = p8_base(pool, gr.at(G * i + a));
     }
 
     // One wavefront over keys [j0, j1) of a sequence of kv (j0 a multiple of STEP).
@@ -282,7 +284,7 @@ struct Rows8 {
             P8Groups gr;
             gr.load<HD>(c, table, head, j0, kv);
             const int last = (end - j0 + STEP - 1) / STEP - 1;
-            const uint8_t* at[G];
+            Base at[G];
             KeyRegs kr;
             ValueRegs vr;
             rows(gr, c.k, 0, at);
@@ -329,7 +331,7 @@ struct Rows8 {
             P8Groups gr;
             gr.load<HD>(c, table, head, j, kv);
             const Block b = block(gr, j, 0, kv);
-            const uint8_t *ka[G], *va[G];
+            Base ka[G], va[G];
             rows(gr, c.k, 0, ka);
             rows(gr, c.v, 0, va);
             KeyRegs kr;

@@ -51,6 +51,16 @@ __device__ __forceinline__ typename PgElem<E>::v8 p8_eight(uint32_t a, uint32_t 
     return __builtin_bit_cast(typename PgElem<E>::v8, w);
 }
 
+// Byte `at` of a pool, in scalar registers: loads from there take 32-bit offsets of the
+// lanes.  (Left to itself the compiler adds pool, group and lane in vector registers.)
+template <class T>
+using P8Global = __attribute__((address_space(1))) T;
+__device__ __forceinline__ const P8Global<uint8_t>* p8_base(const void* pool, uint64_t at) {
+    uint64_t u = (uint64_t)pool + at;
+    asm("" : "+s"(u));
+    return (const P8Global<uint8_t>*)u;
+}
+
 // Whether a word holds a NaN code.
 __device__ __forceinline__ bool p8_word_nan(uint32_t w) {
     const uint32_t t = ~(w | 0x80808080u);  // a zero byte where there is one

@@ -124,28 +124,25 @@ __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uin
     return __any(any);
 }
 
-// What holds for the four groups of 16 keys of a tile of an 8-bit cache: their scales,
-// a byte each (2^0 for groups without keys, so that what is cleared stays 0), and
-// which groups' page is none.
+// What holds for the four groups of 16 keys of a tile of an 8-bit cache: the scale bytes
+// of k's NK groups from k0 on, KSTEP apart, and of v's NV groups from v0 on, VSTEP apart
+// (2^0 for groups without keys, so that what is cleared stays 0), which groups' page is none,
+// and which have a page that is none or a NaN scale of k (their keys are NaN).
+template <int NK, int KSTEP, int NV, int VSTEP>
 struct Tile8 {
-    uint32_t ks, vs, bad;
-    __device__ __forceinline__ static Tile8 of(const P8Groups& gr, int g0, int j0, int kv) {
-        Tile8 t{0, 0, (uint32_t)(gr.none >> g0) & 15};
+    int k[NK], v[NV];
+    uint32_t bad, nan;
+    __device__ __forceinline__ static Tile8 of(const P8Groups& gr, int g0, int j0, int kv, int k0, int v0) {
+        Tile8 t{{}, {}, (uint32_t)(gr.none >> g0) & 15, 0};
+        const int j = j0 + 16 * ((int)(threadIdx.x & 63) - g0);
+        const bool keys = j < kv && !((gr.none >> (threadIdx.x & 63)) & 1);
+        const int ks = keys ? gr.k_scale : P8_ONE, vs = keys ? gr.v_scale : P8_ONE;
+        t.nan = t.bad | ((uint32_t)(__ballot(ks == 255) >> g0) & 15);
 #pragma unroll
-        for (int a = 0; a < 4; a++) {
-            const bool keys = j0 + 16 * a < kv && !((t.bad >> a) & 1);
-            t.ks |= (uint32_t)(keys ? __builtin_amdgcn_readlane(gr.k_scale, g0 + a) : P8_ONE) << (8 * a);
-            t.vs |= (uint32_t)(keys ? __builtin_amdgcn_readlane(gr.v_scale, g0 + a) : P8_ONE) << (8 * a);
-        }
+        for (int a = 0; a < NK; a++) t.k[a] = __builtin_amdgcn_readlane(ks, g0 + k0 + KSTEP * a);
+#pragma unroll
+        for (int a = 0; a < NV; a++) t.v[a] = __builtin_amdgcn_readlane(vs, g0 + v0 + VSTEP * a);
         return t;
-    }
-    // Groups of no page, or of a scale that is NaN or takes codes past f32's range.
-    __device__ __forceinline__ uint32_t odd() const {
-        uint32_t any = bad;
-#pragma unroll
-        for (int a = 0; a < 4; a++)
-            if (((ks >> (8 * a)) & 255) > P8_TOP || ((vs >> (8 * a)) & 255) > P8_TOP) any |= 1u << a;
-        return any;
     }
 };
 
@@ -255,8 +252,14 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         constexpr int PASS = HD / 64, PR = PF_KEYS / PASS;  // rows of a pass
         pg_u4 rk[PASS], rv[PASS];
         P8Groups gr;
-        Tile8 raw, cur;
+        // (keys of bf16 carry their scale, so only keys of f16 need it at their scores)
+        constexpr bool SCALED = std::is_same<EK, __bf16>::value;
+        using T8 = Tile8<SCALED ? PASS : 2 * NA, SCALED ? PR / 16 : 1, PASS, PR / 16>;
+        T8 raw, cur;
+        const int group = wave * (1024 / HD) >> 4;  // of this wavefront's rows in a pass (PR / 16 a pass)
         const int br = (int)threadIdx.x / (HD / 16), bp = (int)threadIdx.x % (HD / 16);
+        const uint32_t boff = 16 * (threadIdx.x & 63) + (HD == 128 ? 1024 * (wave & 1) : 0);  // in its group
+        const uint32_t bk = br * X::ROW + 16 * ((2 * bp) ^ X::kswz(br)), bv = br * X::ROW + 16 * ((2 * bp) ^ X::vswz(br));
         // Byte offsets in the pools of 64 groups of 16 keys, lane i that of group i from
         // key id0 on, and which groups' page is none (theirs lead to page 0).
         int id0 = 0;
@@ -294,28 +297,32 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             const int j0 = t * PF_KEYS;
             if (j0 - id0 >= 1024) fetch_ids(j0);
             const int g0 = (j0 - id0) >> 4;
-            raw = Tile8::of(gr, g0, j0, sq.kv);
+            raw = T8::of(gr, g0, j0, sq.kv, SCALED ? group : key0 >> 4, group);
 #pragma unroll
             for (int i = 0; i < PASS; i++) {
-                const uint64_t at = gr.at(g0 + ((i * PR + wave * (1024 / HD)) >> 4)) + 16 * (threadIdx.x & 63) +
-                                    (HD == 128 ? 1024 * (wave & 1) : 0);
-                rk[i] = *reinterpret_cast<const pg_u4*>(static_cast<const uint8_t*>(c.k) + at);
-                rv[i] = *reinterpret_cast<const pg_u4*>(static_cast<const uint8_t*>(c.v) + at);
+                const uint64_t at = gr.at(g0 + group + PR / 16 * i);
+                rk[i] = *reinterpret_cast<const P8Global<pg_u4>*>(p8_base(c.k, at) + boff);
+                rv[i] = *reinterpret_cast<const P8Global<pg_u4>*>(p8_base(c.v, at) + boff);
             }
         };
         auto decode8 = [&](int t) {
+            if (t * PF_KEYS + PF_KEYS > sq.kv || raw.bad) {  // rows of V that are no keys hold anything
+#pragma unroll
+                for (int i = 0; i < PASS; i++) {
+                    const int r = i * PR + br;
+                    if (t * PF_KEYS + r >= sq.kv || ((raw.bad >> (r >> 4)) & 1)) rv[i] = pg_u4{0, 0, 0, 0};
+                }
+            }
+            uint8_t *k = s_k[t & 1], *v = s_v[t & 1];
 #pragma unroll
             for (int i = 0; i < PASS; i++) {
-                const int r = i * PR + br, g = (i * PR + wave * (1024 / HD)) >> 4;
-                const float unit = p8_operand((raw.vs >> (8 * g)) & 255);
-                pg_u4 x = rv[i];
-                if (t * PF_KEYS + r >= sq.kv || ((raw.bad >> g) & 1)) x = pg_u4{0, 0, 0, 0};  // (no keys: they hold anything)
+                const float ku = SCALED ? p8_operand(raw.k[i]) : 1.0f, vu = p8_operand(raw.v[i]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    *reinterpret_cast<k8*>(s_k[t & 1] + r * X::ROW + 16 * ((2 * bp + e) ^ X::kswz(r))) =
-                        p8_eight<EK>(rk[i][2 * e], rk[i][2 * e + 1], 1.0f);
-                    *reinterpret_cast<v8*>(s_v[t & 1] + r * X::ROW + 16 * ((2 * bp + e) ^ X::vswz(r))) =
-                        p8_eight<EV>(x[2 * e], x[2 * e + 1], unit);
+                    *reinterpret_cast<k8*>(k + i * PR * X::ROW + (bk ^ (16 * e))) =
+                        p8_eight<EK>(rk[i][2 * e], rk[i][2 * e + 1], ku);
+                    *reinterpret_cast<v8*>(v + i * PR * X::ROW + (bv ^ (16 * e))) =
+                        p8_eight<EV>(rv[i][2 * e], rv[i][2 * e + 1], vu);
                 }
             }
             cur = raw;
@@ -399,7 +406,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
-                const Tile8 t8 = cur;
+                const T8 t8 = cur;
                 const uint32_t bad = X::BYTES ? t8.bad
                                               : (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
                 if (X::BYTES) {
@@ -421,7 +428,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
 
                 const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
                 const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
-                if (AGAIN && pf_odd<X, 64 / KW>(kt, vt, (X::BYTES ? t8.odd() : bad) >> (key0 >> 4))) {
+                if (AGAIN && pf_odd<X, 64 / KW>(kt, vt, (X::BYTES ? t8.nan : bad) >> (key0 >> 4))) {
                     if (!__all(pg_all_nan(o)))
                         pg_plain<typename X::Cells, T, HD, 2>(
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
@@ -445,14 +452,15 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                         for (int p = X::NQ - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
                     }
                 }
-                const bool mask = jw + 32 * NA - 1 > first || bad;
+                const uint32_t gone = X::BYTES && !SCALED ? t8.nan : bad;  // groups whose keys are NaN
+                const bool mask = jw + 32 * NA - 1 > first || gone;
                 if (mask) {
 #pragma unroll
                     for (int a = 0; a < NA; a++)
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
                             const int r = 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h;
-                            if ((bad >> ((key0 + r) >> 4)) & 1) st[a][i] = pg_nan();
+                            if ((gone >> ((key0 + r) >> 4)) & 1) st[a][i] = pg_nan();
                             if (jw + r > limit) st[a][i] = -__builtin_inff();
                         }
                 }
@@ -461,13 +469,10 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
 #pragma unroll
                 for (int g = 0; g < 2 * NA; g++) {
                     fac[g] = factor;
-                    if constexpr (X::BYTES) {
-                        fac[g] *= p8_factor((t8.ks >> (8 * (g + (key0 >> 4)))) & 255);
-                        fac[g] = fac[g] > __FLT_MAX__ ? __FLT_MAX__ : fac[g];  // (of NaN: NaN)
-                    }
+                    if constexpr (X::BYTES && !SCALED) fac[g] = fminf(factor * p8_factor(t8.k[g]), __FLT_MAX__);  // (0 * inf)
                 }
                 float top = st[0][0];
-                if constexpr (X::BYTES) {
+                if constexpr (X::BYTES && !SCALED) {
                     top = -__builtin_inff();
 #pragma unroll
                     for (int g = 0; g < 2 * NA; g++) {
