@@ -410,9 +410,11 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 const uint32_t bad = X::BYTES ? t8.bad
                                               : (uint32_t)(none >> ((j0 - id0) >> 4)) & ((1u << PF_KEYS / 16) - 1);  // of its groups
                 if (X::BYTES) {
-                    if (t + 1 < tiles) {
+                    if (t + 1 < tiles) {  // (not among the products: the registers do not hold both)
+                        __builtin_amdgcn_sched_barrier(0);
                         decode8(t + 1);
                         if (t + 2 < tiles) fetch8(t + 2);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 } else if (j0 + PF_KEYS > sq.kv || bad) {  // rows of V that are no keys hold anything
                     for (int ch = threadIdx.x; ch < X::TILE / 16; ch += 64 * PF_WAVES) {
