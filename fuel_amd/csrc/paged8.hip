@@ -34,7 +34,7 @@ struct Rows8 {
     using P = PgElem<__bf16>;                                      // of weights and v
     using q8 = typename PgElem<E>::v8;
     using v8 = P::v8;
-    static constexpr int NQ = WIDE ? 2 : 1, NP = 2;
+    static constexpr int NQ = WIDE ? 2 : 1, NP = WIDE ? 3 : 2;
     static constexpr int DIM = HD, KS = HD / 32, VW = HD / 16;
     // Groups of 16 keys of a block.  (Of four, where the 16 KB of two blocks of 32 go
     // out at once: no faster, and 10.0 us for 7.6 where a wavefront has a few blocks.)

@@ -84,23 +84,21 @@ __device__ __forceinline__ float pf_other_half(float v) {
     return __builtin_bit_cast(float, (threadIdx.x & 32) ? (uint32_t)a[0] : (uint32_t)a[1]);
 }
 
-// EK, EV: the types of K and V in LDS, and so of q and of the weights in their
-// products, NQ and NP parts of each.
-template <class C, class EK_, class EV_, class T, int HD, int NQ_, int NP_>
+// E: the type of K and V in LDS, and so of q and of the weights in their products,
+// PARTS parts of each.
+template <class C, class E, class T, int HD, int PARTS>
 struct PrefillTile {
     using Cache = C;
     using Row = T;
-    using EK = EK_;
-    using EV = EV_;
-    using k8 = typename PgElem<EK>::v8;
-    using v8 = typename PgElem<EV>::v8;
+    using Elem = E;
+    using v8 = typename PgElem<E>::v8;
     static constexpr bool BYTES = std::is_same<C, PagedKv8>::value;  // an 8-bit cache
-    using Cells = typename std::conditional<BYTES, P8Cells<HD>, PgCells<EV, HD>>::type;
+    using Cells = typename std::conditional<BYTES, P8Cells<HD>, PgCells<E, HD>>::type;
     static constexpr bool WIDE = std::is_same<T, float>::value;
-    static constexpr int DIM = HD, NQ = NQ_, NP = NP_;
-    static constexpr bool F16 = std::is_same<EV, _Float16>::value;
+    static constexpr int DIM = HD, NP = PARTS;
+    static constexpr bool F16 = std::is_same<E, _Float16>::value;
     // (f16 parts of an f32 weight: as many of its digits as f16's range holds)
-    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = PgElem<EV>::TOP - LAZY;
+    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = PgElem<E>::TOP - LAZY;
     static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
     static constexpr int RPI = 512 / HD, NI = TILE / 1024;  // rows a DMA instruction, instructions a tile
@@ -119,7 +117,7 @@ __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uin
     for (int i = 16 * (threadIdx.x & 63); i < KEYS * X::ROW; i += 1024) {
         const pg_u4 k = *reinterpret_cast<const pg_u4*>(kt + i), v = *reinterpret_cast<const pg_u4*>(vt + i);
 #pragma unroll
-        for (int w = 0; w < 4; w++) any |= pg_word_odd<typename X::EK>(k[w]) || pg_word_odd<typename X::EV>(v[w]);
+        for (int w = 0; w < 4; w++) any |= pg_word_odd<typename X::Elem>(k[w]) || pg_word_odd<typename X::Elem>(v[w]);
     }
     return __any(any);
 }
@@ -127,13 +125,15 @@ __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uin
 // What holds for the four groups of 16 keys of a tile of an 8-bit cache: the scale bytes
 // of k's NK groups from k0 on, KSTEP apart, and of v's NV groups from v0 on, VSTEP apart
 // (2^0 for groups without keys, so that what is cleared stays 0), which groups' page is none,
-// and which have a page that is none or a NaN scale of k (their keys are NaN).
+// which have a page that is none or a NaN scale of k (their keys are NaN), and the
+// largest scale byte of v up to this tile.
 template <int NK, int KSTEP, int NV, int VSTEP>
 struct Tile8 {
     int k[NK], v[NV];
     uint32_t bad, nan;
-    __device__ __forceinline__ static Tile8 of(const P8Groups& gr, int g0, int j0, int kv, int k0, int v0) {
-        Tile8 t{{}, {}, (uint32_t)(gr.none >> g0) & 15, 0};
+    int top;
+    __device__ __forceinline__ static Tile8 of(const P8Groups& gr, int g0, int j0, int kv, int k0, int v0, int top) {
+        Tile8 t{{}, {}, (uint32_t)(gr.none >> g0) & 15, 0, top};
         const int j = j0 + 16 * ((int)(threadIdx.x & 63) - g0);
         const bool keys = j < kv && !((gr.none >> (threadIdx.x & 63)) & 1);
         const int ks = keys ? gr.k_scale : P8_ONE, vs = keys ? gr.v_scale : P8_ONE;
@@ -142,7 +142,14 @@ struct Tile8 {
         for (int a = 0; a < NK; a++) t.k[a] = __builtin_amdgcn_readlane(ks, g0 + k0 + KSTEP * a);
 #pragma unroll
         for (int a = 0; a < NV; a++) t.v[a] = __builtin_amdgcn_readlane(vs, g0 + v0 + VSTEP * a);
+        const int most = keys && vs < 255 ? vs : 0;
+#pragma unroll
+        for (int a = 0; a < 4; a++) t.top = max(t.top, __builtin_amdgcn_readlane(most, g0 + a));
         return t;
+    }
+    // The operand that makes values of group a's codes, in units of 2^(top - 127).
+    __device__ __forceinline__ float v_relative(int a) const {
+        return p8_operand(v[a] == 255 ? 255 : max(v[a] - top + 127, 0));
     }
 };
 
@@ -168,9 +175,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                                                                          int ldo, float* __restrict__ part,
                                                                          PgJoin* __restrict__ joins) {
     using T = typename X::Row;
-    using EK = typename X::EK;
-    using EV = typename X::EV;
-    using k8 = typename X::k8;
+    using E = typename X::Elem;
     using v8 = typename X::v8;
     constexpr int HD = X::DIM;
     constexpr int RW = PF_WAVES / KW, ROWS = 32 * RW;
@@ -253,9 +258,12 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         pg_u4 rk[PASS], rv[PASS];
         P8Groups gr;
         // (keys of bf16 carry their scale, so only keys of f16 need it at their scores)
-        constexpr bool SCALED = std::is_same<EK, __bf16>::value;
+        constexpr bool SCALED = std::is_same<E, __bf16>::value;
         using T8 = Tile8<SCALED ? PASS : 2 * NA, SCALED ? PR / 16 : 1, PASS, PR / 16>;
+        // (values of f16 are in units of the largest scale so far: within its range)
+        constexpr bool RELATIVE = X::BYTES && X::F16;
         T8 raw, cur;
+        int unit = 0;  // the byte of the scale that o is in units of
         const int group = wave * (1024 / HD) >> 4;  // of this wavefront's rows in a pass (PR / 16 a pass)
         const int br = (int)threadIdx.x / (HD / 16), bp = (int)threadIdx.x % (HD / 16);
         const uint32_t boff = 16 * (threadIdx.x & 63) + (HD == 128 ? 1024 * (wave & 1) : 0);  // in its group
@@ -297,7 +305,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             const int j0 = t * PF_KEYS;
             if (j0 - id0 >= 1024) fetch_ids(j0);
             const int g0 = (j0 - id0) >> 4;
-            raw = T8::of(gr, g0, j0, sq.kv, SCALED ? group : key0 >> 4, group);
+            raw = T8::of(gr, g0, j0, sq.kv, SCALED ? group : key0 >> 4, group, t == t0 ? 0 : raw.top);
 #pragma unroll
             for (int i = 0; i < PASS; i++) {
                 const uint64_t at = gr.at(g0 + group + PR / 16 * i);
@@ -316,13 +324,13 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             uint8_t *k = s_k[t & 1], *v = s_v[t & 1];
 #pragma unroll
             for (int i = 0; i < PASS; i++) {
-                const float ku = SCALED ? p8_operand(raw.k[i]) : 1.0f, vu = p8_operand(raw.v[i]);
+                const float ku = SCALED ? p8_operand(raw.k[i]) : 1.0f, vu = RELATIVE ? raw.v_relative(i) : p8_operand(raw.v[i]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    *reinterpret_cast<k8*>(k + i * PR * X::ROW + (bk ^ (16 * e))) =
-                        p8_eight<EK>(rk[i][2 * e], rk[i][2 * e + 1], ku);
+                    *reinterpret_cast<v8*>(k + i * PR * X::ROW + (bk ^ (16 * e))) =
+                        p8_eight<E>(rk[i][2 * e], rk[i][2 * e + 1], ku);
                     *reinterpret_cast<v8*>(v + i * PR * X::ROW + (bv ^ (16 * e))) =
-                        p8_eight<EV>(rv[i][2 * e], rv[i][2 * e + 1], vu);
+                        p8_eight<E>(rv[i][2 * e], rv[i][2 * e + 1], vu);
                 }
             }
             cur = raw;
@@ -348,14 +356,14 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
 
         // Q^T, the B operand: dims 16 t + 8 h + e of row n (negated for a negative
         // scale: the maximum is taken of scores with a positive factor)
-        k8 qf[X::NQ][X::KS];
+        v8 qf[X::NP][X::KS];
         float factor = fabsf(scale) * 1.4426950408889634f;
         const T* x = q + (size_t)row * ldq + (size_t)qh * HD + 8 * h;
         if constexpr (!X::WIDE) {
             const uint32_t flip = scale < 0.0f ? 0x80008000u : 0;
 #pragma unroll
             for (int t = 0; t < X::KS; t++)
-                qf[0][t] = __builtin_bit_cast(k8, *reinterpret_cast<const pg_u4*>(x + 16 * t) ^ flip);
+                qf[0][t] = __builtin_bit_cast(v8, *reinterpret_cast<const pg_u4*>(x + 16 * t) ^ flip);
         } else {
             float f[X::KS][8], a = 0.0f;
 #pragma unroll
@@ -365,7 +373,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
 #pragma unroll
                 for (int e = 0; e < 8; e++) f[t][e] = scale < 0.0f ? -raw[e] : raw[e];
             }
-            if constexpr (std::is_same<EK, _Float16>::value) {  // (parts of f16: scaled to the top of its range)
+            if constexpr (std::is_same<E, _Float16>::value) {  // (parts of f16: scaled to the top of its range)
 #pragma unroll
                 for (int t = 0; t < X::KS; t++)
 #pragma unroll
@@ -384,8 +392,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 for (int e = 0; e < 8; e++) {
                     float rest = f[t][e];
 #pragma unroll
-                    for (int p = 0; p < X::NQ; p++) {
-                        qf[p][t][e] = (EK)rest;
+                    for (int p = 0; p < X::NP; p++) {
+                        qf[p][t][e] = (E)rest;
                         rest -= (float)qf[p][t][e];
                     }
                 }
@@ -399,6 +407,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
             m = peak = PG_LEAST;
             l = 0.0f;
+            unit = 0;
             for (int t = t0; t < tiles; t++) {
                 const int j0 = t * PF_KEYS;
                 // tile t landed, in every wavefront, and tile t - 1 is read
@@ -428,6 +437,12 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 const int jw = j0 + key0;  // this wavefront's first key
                 if (jw > last) continue;
 
+                if (RELATIVE && t8.top != unit) {
+                    const float f = __builtin_amdgcn_ldexpf(1.0f, unit - t8.top);
+                    unit = t8.top;
+#pragma unroll
+                    for (int d = 0; d < X::DT; d++) o[d] *= f;
+                }
                 const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
                 const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
                 if (AGAIN && pf_odd<X, 64 / KW>(kt, vt, (X::BYTES ? t8.nan : bad) >> (key0 >> 4))) {
@@ -436,6 +451,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
                             min(jw + 32 * NA, last + 1), X::SHIFT, h == 0, [&](int i) { return 8 * i + 4 * h; },
                             [&](int i, int e, float f, float p, float v) {
+                                if (RELATIVE) v = __builtin_amdgcn_ldexpf(v, 127 - unit);
                                 o[i / 4][4 * (i % 4) + e] = fmaf(p, v, o[i / 4][4 * (i % 4) + e] * f);
                             },
                             m, l);
@@ -449,9 +465,9 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                     for (int i = 0; i < 16; i++) st[a][i] = 0.0f;
 #pragma unroll
                     for (int k = 0; k < X::KS; k++) {
-                        const k8 kf = *reinterpret_cast<const k8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
+                        const v8 kf = *reinterpret_cast<const v8*>(kt + 32 * a * X::ROW + (kbase ^ (32 * k)));
 #pragma unroll
-                        for (int p = X::NQ - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
+                        for (int p = X::NP - 1; p >= 0; p--) st[a] = pf_mfma(kf, qf[p][k], st[a]);
                     }
                 }
                 const uint32_t gone = X::BYTES && !SCALED ? t8.nan : bad;  // groups whose keys are NaN
@@ -521,14 +537,19 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
 #pragma unroll
                 for (int a = 0; a < NA; a++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        st[a][i] = __builtin_amdgcn_exp2f(st[a][i]);
-                        l += st[a][i];
-                        float rest = st[a][i];
+                    for (int i = 0; i < 16; i += 2) {
+                        typedef float f2 __attribute__((ext_vector_type(2)));
+                        using v2 = typename PgElem<E>::v2;
+                        f2 rest{__builtin_amdgcn_exp2f(st[a][i]), __builtin_amdgcn_exp2f(st[a][i + 1])};
+                        l += rest[0];
+                        l += rest[1];
 #pragma unroll
                         for (int p = 0; p < X::NP; p++) {
-                            pp[p][2 * a + (i >> 3)][i & 7] = (EV)rest;
-                            rest -= (float)pp[p][2 * a + (i >> 3)][i & 7];
+                            const v2 h = __builtin_convertvector(rest, v2);
+                            pp[p][2 * a + (i >> 3)][i & 7] = h[0];
+                            pp[p][2 * a + (i >> 3)][(i & 7) + 1] = h[1];
+                            rest[0] -= (float)h[0];
+                            rest[1] -= (float)h[1];
                         }
                     }
 #pragma unroll
@@ -552,6 +573,15 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             walk(std::true_type{});
         }
         l += pf_other_half(l);
+        if constexpr (RELATIVE) {  // as values; l of 0.5 .. 1, so that no o is past the values themselves
+            const int ex = l > 0.0f && l < __builtin_inff() ? __builtin_amdgcn_frexp_expf(l) : 0;
+            l = __builtin_amdgcn_ldexpf(l, -ex);
+            m += ex;
+#pragma unroll
+            for (int d = 0; d < X::DT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = __builtin_amdgcn_ldexpf(o[d][i], unit - 127 - ex);
+        }
         if constexpr (KW == 2) {  // the two that share rows
             static_assert(16 * X::DT * 64 * 4 * RW <= sizeof s_k, "the sums of half the wavefronts");
             __syncthreads();
@@ -654,7 +684,7 @@ struct PrefillCall {
     template <class E, class T, int HD>
     hipError_t run() const {
         constexpr int parts = std::is_same<T, float>::value ? PgElem<E>::SPLIT : 1;
-        return prefill_launch<PrefillTile<PagedKv, E, E, T, HD, parts, parts>>(p, p.kv, s);
+        return prefill_launch<PrefillTile<PagedKv, E, T, HD, parts>>(p, p.kv, s);
     }
 };
 
@@ -664,9 +694,9 @@ struct Prefill8Call {
     hipStream_t s;
     template <class T, int HD>
     hipError_t run() const {
-        constexpr bool wide = std::is_same<T, float>::value;
-        using E = typename std::conditional<wide, _Float16, T>::type;
-        return prefill_launch<PrefillTile<PagedKv8, E, __bf16, T, HD, wide ? 2 : 1, wide ? 2 : 1>>(p, c, s);
+        constexpr int parts = std::is_same<T, float>::value ? 2 : 1;
+        using E = typename std::conditional<std::is_same<T, float>::value, _Float16, T>::type;
+        return prefill_launch<PrefillTile<PagedKv8, E, T, HD, parts>>(p, c, s);
     }
 };
 

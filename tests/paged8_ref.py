@@ -6,8 +6,12 @@ Values.  code * 2^(b - 127): exact in 64 bits, and in the 32 that appended rows 
 Bounds: paged_ref.py's, with these terms in the place of its.
 score: a code is exact as an f16 or bf16 operand and a scale is a power of two, so
   the products err as those of a 16-bit cache do; one factor more, exactly.
-weights as factors of V: bf16 parts, half a step 2^-8 each.  Two are kept (2^-16),
-  of 16-bit rows in tiles of 128 rows one (2^-8).  bf16 has f32's range: no absolute term but where a value leaves it.
+weights as factors of V: in tiles of 16 rows (decode) bf16 parts, half a step 2^-8 each:
+  of f32 rows three (2^-24; 2^-22 is allowed), of others two (2^-16).  In tiles of 128
+  rows as a 16-bit cache's: f32 rows two of f16 (2^-22), others one of their own type;
+  f16 parts have steps of 2^-24, 2^-25 of a weight whose largest is 2^8 or more, times
+  the n values of V; and values are in units of the largest scale, in f16, whose steps
+  are 2^-24 of it: half a step of each value, the weights' sum being 1.
 """
 import numpy as np
 
@@ -113,13 +117,21 @@ class Pool:
         return tuple(CODE[self.code[w, page, :, at]] * scale(self.scale[w, page, :, at // 16])[..., None]
                      for w in range(2))
 
+    def top(self, s, n):
+        """The largest scale of the values of the first n positions."""
+        page, at = self.table[s, np.arange(n) // self.ps], np.arange(n) % self.ps
+        return float(np.nanmax(scale(self.scale[1, page, :, at // 16]), initial=0.0))
+
     def fill(self, rng, s, n, std=1.0):
         if n > 0:
             self.append(s, 0, *(rng.standard_normal((2, n, self.hk, self.d)) * std).astype(np.float32))
 
 
-def bound(out, A, B, n, D, act, tiles):
+def bound(out, A, B, V, top, n, D, act, tiles):
+    """V: the largest |v|, top: the largest scale of v, of the n keys."""
     d = ((D + 10) * A + 4) * U
-    w = 2.0 ** -8 if tiles and act != F32 else 2.0 ** -16
+    w = 2.0 ** -22 if act == F32 else HALF[act] if tiles else 2.0 ** -16
     tol = (2 * (d + n * U) + 16 * U + w) * B + TINY[R.BF16]
+    if tiles and act != R.BF16:
+        tol = tol + n * 2.0 ** -33 * V + 2.0 ** -25 * top
     return tol + (0 if act == F32 else HALF[act] * (np.abs(out) + tol + TINY[act]))

@@ -92,8 +92,9 @@ class Case:
             k, v = self.pool.get(s, int(self.kv[s]))
             pos = int(self.kv[s]) - n + np.arange(n)
             qs = q[r0:r0 + n, :w].reshape(n, self.H, self.D)
-            want, A, B, _ = R.attend(qs, k, v, pos, scale)
-            tol = P.bound(want, A, B, max(1, int(self.kv[s])), self.D, self.act, not self.decode)
+            want, A, B, V = R.attend(qs, k, v, pos, scale)
+            tol = P.bound(want, A, B, V, self.pool.top(s, int(self.kv[s])), max(1, int(self.kv[s])), self.D, self.act,
+                          not self.decode)
             g = got[r0:r0 + n, :w].reshape(want.shape)
             gone = np.argwhere(~np.isfinite(g))
             assert not len(gone), (s, gone[:3])
