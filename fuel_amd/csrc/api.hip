@@ -1586,7 +1586,7 @@ int paged8_attention(const char* who, frq_device* dev, const frq_paged_kv8* kv, 
     PagedKv8 c{};
     frq_paged_kv shape;
     if ((rc = paged8_args(who, kv, b, n_heads, dtype, &shape, &c, &a.rows))) return rc;
-    const bool rows16 = pg_kind(c, a.rows, (int)n_heads, (int)kv->head_dim, 1) == PG_ROWS16;
+    const bool rows16 = pg_kind(c, a.rows, (int)n_heads, (int)kv->head_dim) == PG_ROWS16;
     if (rows16 ? !paged8_rows16_fits(c, a.rows, (int)n_heads, (int)kv->head_dim)
                : !paged_prefill_fits(c, a.rows, (int)n_heads))
         return fail(FRQ_UNSUPPORTED, "%s: rows=%zu n_seqs=%zu of up to %d tokens", who, b->rows, b->n_seqs, a.rows.cap);
@@ -1710,8 +1710,8 @@ size_t frq_paged8_attention_workspace(const frq_paged_kv8* kv, const frq_paged_b
     PagedRows r;
     if (paged8_args("paged8_attention_workspace", kv, b, n_heads, GGML_F32, &shape, &k, &r)) return 0;
     const int heads = (int)n_heads, hd = (int)kv->head_dim;
-    return pg_kind(k, r, heads, hd, 1) == PG_ROWS16 ? paged8_rows16_work_bytes(k, r, heads, hd)
-                                                    : paged_prefill_work_bytes(k, r, heads, hd, 1);
+    return pg_kind(k, r, heads, hd) == PG_ROWS16 ? paged8_rows16_work_bytes(k, r, heads, hd)
+                                                 : paged_prefill_work_bytes(k, r, heads, hd);
 }
 
 int frq_paged8_attention_decode(frq_device* dev, const frq_paged_kv8* kv, const frq_paged_batch* b, int dtype,

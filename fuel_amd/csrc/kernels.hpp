@@ -301,10 +301,9 @@ hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAtten
 hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, long tiles,
                              int tile_rows, int rows, int grp, void* out, int ldo, hipStream_t s);
 // paged_prefill.hip: many rows a sequence, 128-row tiles (work of
-// paged_prefill_work_bytes(), size: bytes of a cached value); fits: the workgroups
-// are a grid.
+// paged_prefill_work_bytes()); fits: the workgroups are a grid.
 bool paged_prefill_fits(const PagedKv& kv, const PagedRows& r, int n_heads);
-size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size = 2);
+size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
 hipError_t launch_paged_prefill(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 
 // paged8.hip: the same over an 8-bit cache (paged8.hpp; `kv` of the arguments is not

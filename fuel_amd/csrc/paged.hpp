@@ -58,7 +58,8 @@ inline long pg_tiles_bound(const PagedRows& r, int grp, int tile_rows) {
 //   CUT     26 + n128 K / 15000       (the second launch and the pieces' bytes)
 // Over 420 such batches the choice is 1.6 % slower than the fastest of the three in
 // the mean, at worst by half (the host knows the rows of a batch and its longest
-// sequence, not how they go together).  Of 32 heads over 8, bf16: 128 rows after
+// sequence, not how they go together).  Over an 8-bit cache, 60 such batches: 0.3 %, at
+// worst by half.  Of 32 heads over 8, bf16: 128 rows after
 // 600: 22 / 18 / 27 (ROWS16 / TILES / CUT), 300 after 600: 41 / 20 / 35, 300 after
 // 4096: 155 / 64 / 52, 1500 after 600: 248 / 55 / 79.
 enum PagedKind { PG_ROWS16, PG_TILES, PG_CUT };
@@ -69,16 +70,16 @@ enum PagedKind { PG_ROWS16, PG_TILES, PG_CUT };
 // longer ones whole tiles gain up to 10 % where all are as long as the longest
 // and there is one for every CU, and lose more where they are not.)
 constexpr int PG_WHOLE_KEYS = 1024;
-inline bool pg_whole(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size) {
+inline bool pg_whole(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     const long tiles = pg_tiles_bound(r, n_heads / kv.kv_heads, 16) * kv.kv_heads;
     return (long)r.cap * hd <= (tiles >= 128 ? 65536 : 32768);
 }
-inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size = 2) {
+inline PagedKind pg_kind(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
     if (!r.row_start) return PG_ROWS16;
     const int grp = n_heads / kv.kv_heads;
     const double k = r.cap, n16 = (double)pg_tiles_bound(r, grp, 16) * kv.kv_heads,
                  n128 = (double)pg_tiles_bound(r, grp, 128) * kv.kv_heads;
-    const double rows16 = (pg_whole(kv, r, n_heads, hd, size) ? 8 : 12) + n16 * k / 20000;
+    const double rows16 = (pg_whole(kv, r, n_heads, hd) ? 8 : 12) + n16 * k / 20000;
     const double tiles = 10 + 0.034 * k * (n128 > 256 ? n128 / 512 : 0.5);
     const double cut = r.cap <= 1 << 24 && n128 <= 4096 ? 26 + n128 * k / 15000 : 1e30;  // (its units are an int)
     if (rows16 <= tiles && rows16 <= cut) return PG_ROWS16;

@@ -661,7 +661,7 @@ hipError_t prefill_launch(const PagedAttendArgs& p, const typename X::Cache& c, 
     const T* q = static_cast<const T*>(p.q);
     T* out = static_cast<T*>(p.out);
     const long tiles = pg_tiles_bound(p.rows, grp, PF_ROWS) * c.kv_heads;
-    if (pg_kind(c, p.rows, p.n_heads, X::DIM, X::BYTES ? 1 : 2) != PG_CUT) {
+    if (pg_kind(c, p.rows, p.n_heads, X::DIM) != PG_CUT) {
         const bool few = tiles <= PF_FEW;
         const auto kernel = few ? paged_prefill_kernel<X, 2, false> : paged_prefill_kernel<X, 1, false>;
         const long wgs = few ? pg_tiles_bound(p.rows, grp, PF_ROWS / 2) * c.kv_heads : tiles;
@@ -706,8 +706,8 @@ bool paged_prefill_fits(const PagedKv& kv, const PagedRows& r, int n_heads) {
     return pg_tiles_bound(r, n_heads / kv.kv_heads, PF_ROWS) * kv.kv_heads <= PG_GRID;
 }
 
-size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd, int size) {
-    if (pg_kind(kv, r, n_heads, hd, size) != PG_CUT) return 0;
+size_t paged_prefill_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd) {
+    if (pg_kind(kv, r, n_heads, hd) != PG_CUT) return 0;
     return PG_WGS * (2 * pg_slot(PF_ROWS, hd) * sizeof(float) + sizeof(PgJoin));
 }
 

@@ -281,7 +281,7 @@ inline Rows16Plan rows16_plan(const PagedKv& kv, const PagedRows& r, int n_heads
     const int grp = n_heads / kv.kv_heads;
     const long tiles = pg_tiles_bound(r, grp, 16) * kv.kv_heads;
     Rows16Plan p;
-    p.unit = pg_whole(kv, r, n_heads, hd, size) ? PG_WHOLE_KEYS : PD_UNIT;
+    p.unit = pg_whole(kv, r, n_heads, hd) ? PG_WHOLE_KEYS : PD_UNIT;
     const long units = tiles * (r.cap > p.unit ? ((long)r.cap + p.unit - 1) / p.unit : 1);
     p.cut = r.cap > p.unit;
     const int most = PG_WGS / 2 * pg_resident(hd, size);
