@@ -49,6 +49,11 @@ constexpr int PF_WAVES = 4;
 constexpr int PF_ROWS = 32 * PF_WAVES;
 constexpr int PF_KEYS = 64;
 constexpr float PF_LOW = 8.0f;
+// Values of an 8-bit cache as f16: in units of 2^-P8_UP of the largest scale, where 448
+// is 57344, and the least code, 2^-9, of a scale P8_SPREAD smaller is 2^-24, f16's least.
+constexpr int P8_UP = 7, P8_SPREAD = 22;
+// Of weights times values as they are: 2^30 keys' sum stays within f32's range.
+constexpr float P8_FAR = -38.0f;
 
 typedef float pf_f16 __attribute__((ext_vector_type(16)));
 typedef short pf_s4 __attribute__((ext_vector_type(4)));
@@ -147,9 +152,11 @@ struct Tile8 {
         for (int a = 0; a < 4; a++) t.top = max(t.top, __builtin_amdgcn_readlane(most, g0 + a));
         return t;
     }
-    // The operand that makes values of group a's codes, in units of 2^(top - 127).
+    // The byte of the scale that values of f16 are in units of, and the operand that
+    // makes them of group a's codes.
+    __device__ __forceinline__ int unit() const { return top - P8_UP; }
     __device__ __forceinline__ float v_relative(int a) const {
-        return p8_operand(v[a] == 255 ? 255 : max(v[a] - top + 127, 0));
+        return p8_operand(v[a] == 255 ? 255 : max(v[a] - unit() + P8_ONE, 0));
     }
 };
 
@@ -260,10 +267,11 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         // (keys of bf16 carry their scale, so only keys of f16 need it at their scores)
         constexpr bool SCALED = std::is_same<E, __bf16>::value;
         using T8 = Tile8<SCALED ? PASS : 2 * NA, SCALED ? PR / 16 : 1, PASS, PR / 16>;
-        // (values of f16 are in units of the largest scale so far: within its range)
+        // (values of f16 are in units of the largest scale so far)
         constexpr bool RELATIVE = X::BYTES && X::F16;
         T8 raw, cur;
-        int unit = 0;  // the byte of the scale that o is in units of
+        int unit = 0;    // the byte of the scale that o is in units of
+        int least = 255;  // RELATIVE: the least scale byte of v of this wavefront's rows that are not all 0
         const int group = wave * (1024 / HD) >> 4;  // of this wavefront's rows in a pass (PR / 16 a pass)
         const int br = (int)threadIdx.x / (HD / 16), bp = (int)threadIdx.x % (HD / 16);
         const uint32_t boff = 16 * (threadIdx.x & 63) + (HD == 128 ? 1024 * (wave & 1) : 0);  // in its group
@@ -324,6 +332,10 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             uint8_t *k = s_k[t & 1], *v = s_v[t & 1];
 #pragma unroll
             for (int i = 0; i < PASS; i++) {
+                if (RELATIVE && raw.v[i] < least) {
+                    const uint32_t any = (rv[i][0] | rv[i][1] | rv[i][2] | rv[i][3]) & 0x7f7f7f7fu;
+                    if (__any(any)) least = raw.v[i];
+                }
                 const float ku = SCALED ? p8_operand(raw.k[i]) : 1.0f, vu = RELATIVE ? raw.v_relative(i) : p8_operand(raw.v[i]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -399,7 +411,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 }
         }
 
-        const auto walk = [&](auto again) {
+        const auto walk = [&](auto again, bool far) {
             constexpr bool AGAIN = decltype(again)::value;
 #pragma unroll
             for (int d = 0; d < X::DT; d++)
@@ -407,7 +419,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
             m = peak = PG_LEAST;
             l = 0.0f;
-            unit = 0;
+            unit = far ? P8_ONE : 0;
             for (int t = t0; t < tiles; t++) {
                 const int j0 = t * PF_KEYS;
                 // tile t landed, in every wavefront, and tile t - 1 is read
@@ -437,21 +449,21 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 const int jw = j0 + key0;  // this wavefront's first key
                 if (jw > last) continue;
 
-                if (RELATIVE && t8.top != unit) {
-                    const float f = __builtin_amdgcn_ldexpf(1.0f, unit - t8.top);
-                    unit = t8.top;
+                if (RELATIVE && t8.unit() != unit && !(AGAIN && far)) {
+                    const float f = __builtin_amdgcn_ldexpf(1.0f, unit - t8.unit());
+                    unit = t8.unit();
 #pragma unroll
                     for (int d = 0; d < X::DT; d++) o[d] *= f;
                 }
                 const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
                 const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
-                if (AGAIN && pf_odd<X, 64 / KW>(kt, vt, (X::BYTES ? t8.nan : bad) >> (key0 >> 4))) {
+                if (AGAIN && (far || pf_odd<X, 64 / KW>(kt, vt, (X::BYTES ? t8.nan : bad) >> (key0 >> 4)))) {
                     if (!__all(pg_all_nan(o)))
                         pg_plain<typename X::Cells, T, HD, 2>(
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
-                            min(jw + 32 * NA, last + 1), X::SHIFT, h == 0, [&](int i) { return 8 * i + 4 * h; },
+                            min(jw + 32 * NA, last + 1), far ? P8_FAR : X::SHIFT, h == 0, [&](int i) { return 8 * i + 4 * h; },
                             [&](int i, int e, float f, float p, float v) {
-                                if (RELATIVE) v = __builtin_amdgcn_ldexpf(v, 127 - unit);
+                                if (RELATIVE) v = __builtin_amdgcn_ldexpf(v, P8_ONE - unit);
                                 o[i / 4][4 * (i % 4) + e] = fmaf(p, v, o[i / 4][4 * (i % 4) + e] * f);
                             },
                             m, l);
@@ -564,23 +576,28 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                     }
             }
         };
-        walk(std::false_type{});
+        walk(std::false_type{}, false);
         // Infinite or NaN sums: the same keys once more, tiles that hold such values
         // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 7.7,
         // all NaN 7.2, with one infinite value in every 16 keys, the worst there is, 205.
-        if (__builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)))) {
+        // Values whose scales lie so far apart that not all were exact: all keys one after
+        // another.  (A row may see none of the large ones, or give them no weight.)
+        bool far = false;
+        if constexpr (RELATIVE)
+            far = __builtin_amdgcn_readfirstlane(__syncthreads_or(t0 < tiles && raw.top - least > P8_SPREAD));
+        if (far || __builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)))) {
             first_tile();
-            walk(std::true_type{});
+            walk(std::true_type{}, far);
         }
         l += pf_other_half(l);
         if constexpr (RELATIVE) {  // as values; l of 0.5 .. 1, so that no o is past the values themselves
             const int ex = l > 0.0f && l < __builtin_inff() ? __builtin_amdgcn_frexp_expf(l) : 0;
             l = __builtin_amdgcn_ldexpf(l, -ex);
-            m += ex;
+            m += ex + (far ? X::SHIFT - P8_FAR : 0.0f);
 #pragma unroll
             for (int d = 0; d < X::DT; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] = __builtin_amdgcn_ldexpf(o[d][i], unit - 127 - ex);
+                for (int i = 0; i < 16; i++) o[d][i] = __builtin_amdgcn_ldexpf(o[d][i], unit - P8_ONE - ex);
         }
         if constexpr (KW == 2) {  // the two that share rows
             static_assert(16 * X::DT * 64 * 4 * RW <= sizeof s_k, "the sums of half the wavefronts");

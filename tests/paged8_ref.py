@@ -10,8 +10,7 @@ weights as factors of V: in tiles of 16 rows (decode) bf16 parts, half a step 2^
   of f32 rows three (2^-24; 2^-22 is allowed), of others two (2^-16).  In tiles of 128
   rows as a 16-bit cache's: f32 rows two of f16 (2^-22), others one of their own type;
   f16 parts have steps of 2^-24, 2^-25 of a weight whose largest is 2^8 or more, times
-  the n values of V; and values are in units of the largest scale, in f16, whose steps
-  are 2^-24 of it: half a step of each value, the weights' sum being 1.
+  the n values of V.
 """
 import numpy as np
 
@@ -117,21 +116,16 @@ class Pool:
         return tuple(CODE[self.code[w, page, :, at]] * scale(self.scale[w, page, :, at // 16])[..., None]
                      for w in range(2))
 
-    def top(self, s, n):
-        """The largest scale of the values of the first n positions."""
-        page, at = self.table[s, np.arange(n) // self.ps], np.arange(n) % self.ps
-        return float(np.nanmax(scale(self.scale[1, page, :, at // 16]), initial=0.0))
-
     def fill(self, rng, s, n, std=1.0):
         if n > 0:
             self.append(s, 0, *(rng.standard_normal((2, n, self.hk, self.d)) * std).astype(np.float32))
 
 
-def bound(out, A, B, V, top, n, D, act, tiles):
-    """V: the largest |v|, top: the largest scale of v, of the n keys."""
+def bound(out, A, B, V, n, D, act, tiles):
+    """V: the largest |v| of the n keys."""
     d = ((D + 10) * A + 4) * U
     w = 2.0 ** -22 if act == F32 else HALF[act] if tiles else 2.0 ** -16
     tol = (2 * (d + n * U) + 16 * U + w) * B + TINY[R.BF16]
     if tiles and act != R.BF16:
-        tol = tol + n * 2.0 ** -33 * V + 2.0 ** -25 * top
+        tol = tol + n * 2.0 ** -33 * V
     return tol + (0 if act == F32 else HALF[act] * (np.abs(out) + tol + TINY[act]))

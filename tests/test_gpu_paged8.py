@@ -93,8 +93,7 @@ class Case:
             pos = int(self.kv[s]) - n + np.arange(n)
             qs = q[r0:r0 + n, :w].reshape(n, self.H, self.D)
             want, A, B, V = R.attend(qs, k, v, pos, scale)
-            tol = P.bound(want, A, B, V, self.pool.top(s, int(self.kv[s])), max(1, int(self.kv[s])), self.D, self.act,
-                          not self.decode)
+            tol = P.bound(want, A, B, V, max(1, int(self.kv[s])), self.D, self.act, not self.decode)
             g = got[r0:r0 + n, :w].reshape(want.shape)
             gone = np.argwhere(~np.isfinite(g))
             assert not len(gone), (s, gone[:3])

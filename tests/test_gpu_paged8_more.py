@@ -199,3 +199,38 @@ def test_overlapping_ranges_end(dev, act):
         F.paged_append(c.kvc, c.batch, act, H, None, k, k, None)
         for code, was in zip(c.cells[:2], c.pool.code):  # pages but the tables'
             np.testing.assert_array_equal(code.numpy()[1:], was[1:])
+
+
+# 16-row tiles, 64-row tiles, 128-row tiles, cut 128-row tiles
+@pytest.mark.parametrize("act", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", [
+    (4, 2, 128, [60, 0], [9, 30]), (32, 2, 128, [0, 30], [170, 60]), (20, 20, 64, [0, 70, 0], [330, 260, 130]),
+    (32, 2, 128, [2200, 2000, 0], [150, 100, 40])])
+@pytest.mark.parametrize("power", [12, 24, 45, 110])
+def test_values_of_later_positions(dev, act, H, hk, D, past, new, power):
+    """Values of a sequence's last positions 2^power times the others': no row before
+    them loses anything, nor do blocks of zeros before them count."""
+    say("later positions", act, H, D, past, power)
+    rng = seed(26, act, H, D, power)
+    c = Case(dev, rng, act, H, hk, D, 16, past, new, fill=False)
+    cut = [int(k) - n // 2 for k, n in zip(c.kv, new)]
+    for s, n in enumerate(c.kv):
+        k, v = rng.standard_normal((2, n, hk, D)).astype(np.float32)
+        v[cut[s]:] *= np.float32(2.0 ** power)
+        if past[s]:
+            v[:20] = 0
+        c.pool.append(s, 0, k, v)
+    c.upload()
+    c.run()
+    got, q = c.got(), R.from_bits(R.to_bits(c.q, act), act)
+    for s, n in enumerate(new):
+        r0 = int(c.start[s])
+        k, v = c.pool.get(s, int(c.kv[s]))
+        pos = int(c.kv[s]) - n + np.arange(n)
+        want, A, B, _ = R.attend(q[r0:r0 + n].reshape(n, H, D), k, v, pos, c.scale)
+        V = np.maximum.accumulate(np.abs(v).max((1, 2)))[pos][:, None, None]  # of the keys that the row sees
+        tol = P.bound(want, A, B, V, int(c.kv[s]), D, act, True)
+        err = np.abs(got[r0:r0 + n].reshape(want.shape) - want)
+        ok = slice(0, n - n // 2) if act == F16 else slice(None)  # (f16 holds no results of the others)
+        bad = np.argwhere(~(err[ok] <= tol[ok]))
+        assert not len(bad), (s, bad[:3], err[ok].max())
