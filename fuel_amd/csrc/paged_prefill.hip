@@ -21,7 +21,7 @@
 // keys, N(0, 1), differ by less.
 // 16-bit activations: p is rounded to the cache's type for the second product
 // (a relative 2^-11 or 2^-8 of each weight at most, the output's own rounding;
-// the sum l takes p as it is).  A second part, as the 16-row kernel keeps, costs
+// the sum l takes p as it is), over an 8-bit cache to the rows' type.  A second part, as the 16-row kernel keeps, costs
 // half as many matrix instructions again, which are the bound here: a prompt of
 // 16384 2.78 ms instead of 2.04, 17 ragged ones 0.196 instead of 0.159, for an
 // output 0.0015 of it from 64 bits instead of 0.0020 (bf16; f16 0.0002, 0.0003).
@@ -35,6 +35,19 @@
 // turn at the matrix pipe, S^T of the next tile under this one's softmax, wave
 // priorities, eight wavefronts on 256 rows, three tiles in LDS, three wavefronts a
 // SIMD (spills).
+//
+// 8-bit caches.  Codes cannot go to LDS by DMA, they have to be 16-bit operands there:
+// the tile after next is loaded to registers, and decoded into the LDS that the barrier
+// has just freed, before the products.
+//   bf16 rows        codes times scales are bf16 numbers: K and V as values
+//   f16 and f32 rows f16 holds a code but not every scale: K's is a factor of its 16
+//                    keys' scores, V is in units of the largest scale so far, exact
+//                    within 2^P8_SPREAD of it; o follows that unit
+// One prompt of 12288, 32 heads over 8 of 128, bf16: 1.26 ms, 0.98 PFLOP/s, as over a
+// 16-bit cache; 17 of 20 .. 1500 f16 rows 0.158 ms, 0.61 PFLOP/s; two chunks of f32 rows
+// after 6000 .. 8000 cached 0.212 ms.  No faster: decoding between the two products
+// (spills), the sums of products apart in more registers, a part of a weight by
+// truncation (1 %).
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
@@ -271,7 +284,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         constexpr bool RELATIVE = X::BYTES && X::F16;
         T8 raw, cur;
         int unit = 0;    // the byte of the scale that o is in units of
-        int least = 255;  // RELATIVE: the least scale byte of v of this wavefront's rows that are not all 0
+        int least = 255;  // RELATIVE: the least scale byte of v, but for 0, that of blocks of zeros
         const int group = wave * (1024 / HD) >> 4;  // of this wavefront's rows in a pass (PR / 16 a pass)
         const int br = (int)threadIdx.x / (HD / 16), bp = (int)threadIdx.x % (HD / 16);
         const uint32_t boff = 16 * (threadIdx.x & 63) + (HD == 128 ? 1024 * (wave & 1) : 0);  // in its group
@@ -285,6 +298,13 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             id0 = j0;
             if constexpr (X::BYTES) {
                 gr.template load<HD>(c, table, head, j0, sq.kv);
+                if constexpr (RELATIVE) {
+                    const bool keys = j0 + 16 * lane < min(sq.kv, tiles * PF_KEYS) && !((gr.none >> lane) & 1);
+                    int v = keys && gr.v_scale ? gr.v_scale : 255;
+#pragma unroll
+                    for (int d = 1; d < 64; d *= 2) v = min(v, __shfl_xor(v, d));
+                    least = min(least, __builtin_amdgcn_readfirstlane(v));
+                }
                 return;
             }
             const int j = j0 + 16 * lane;
@@ -332,10 +352,6 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             uint8_t *k = s_k[t & 1], *v = s_v[t & 1];
 #pragma unroll
             for (int i = 0; i < PASS; i++) {
-                if (RELATIVE && raw.v[i] < least) {
-                    const uint32_t any = (rv[i][0] | rv[i][1] | rv[i][2] | rv[i][3]) & 0x7f7f7f7fu;
-                    if (__any(any)) least = raw.v[i];
-                }
                 const float ku = SCALED ? p8_operand(raw.k[i]) : 1.0f, vu = RELATIVE ? raw.v_relative(i) : p8_operand(raw.v[i]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
@@ -411,7 +427,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 }
         }
 
-        const auto walk = [&](auto again, bool far) {
+        const auto walk = [&](auto again, uint32_t far) {
             constexpr bool AGAIN = decltype(again)::value;
 #pragma unroll
             for (int d = 0; d < X::DT; d++)
@@ -457,7 +473,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 }
                 const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
                 const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
-                if (AGAIN && (far || pf_odd<X, 64 / KW>(kt, vt, (X::BYTES ? t8.nan : bad) >> (key0 >> 4)))) {
+                if (AGAIN && pf_odd<X, 64 / KW>(kt, vt, ((X::BYTES ? t8.nan : bad) | far) >> (key0 >> 4))) {
                     if (!__all(pg_all_nan(o)))
                         pg_plain<typename X::Cells, T, HD, 2>(
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
@@ -576,15 +592,14 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                     }
             }
         };
-        walk(std::false_type{}, false);
+        walk(std::false_type{}, 0);
         // Infinite or NaN sums: the same keys once more, tiles that hold such values
         // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 7.7,
         // all NaN 7.2, with one infinite value in every 16 keys, the worst there is, 205.
         // Values whose scales lie so far apart that not all were exact: all keys one after
         // another.  (A row may see none of the large ones, or give them no weight.)
-        bool far = false;
-        if constexpr (RELATIVE)
-            far = __builtin_amdgcn_readfirstlane(__syncthreads_or(t0 < tiles && raw.top - least > P8_SPREAD));
+        uint32_t far = 0;  // all groups of a tile
+        if constexpr (RELATIVE) far = t0 < tiles && raw.top - least > P8_SPREAD ? 15 : 0;
         if (far || __builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)))) {
             first_tile();
             walk(std::true_type{}, far);

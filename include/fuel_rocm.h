@@ -444,19 +444,23 @@ typedef struct frq_paged_kv8 {
  * older rows under a NaN scale become NaN.  Positions of the block behind the
  * appended rows are no part of the cache any more: a sequence whose end was moved
  * back may be appended to, its later rows are not kept.  Two rows must not lie in the
- * same block of a page but those of one sequence; nothing of k and v is appended by
- * a batch whose sequences have more than `rows` rows together. */
+ * same block of a page but those of one sequence; which rows of k and v a batch
+ * appends whose sequences have more than `rows` rows together is not defined. */
 int frq_paged8_append(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype, size_t n_heads,
                       const void *q_dev, size_t ldq, const void *k_dev, size_t ldk, const void *v_dev, size_t ldv,
                       const float *rope_cos_dev, const float *rope_sin_dev, size_t rope_rows, void *q_out_dev,
                       size_t ldqo);
 /* frq_paged_attention_workspace, _decode and _prefill over such a cache, dtype
  * FRQ_F32, FRQ_F16 or FRQ_BF16.  Codes and scales are taken as the values that they
- * stand for; scores, softmax and sums are f32.  f32 rows of q are multiplied in parts
- * that hold them to 2^-22.  A softmax weight is held to 2^-16 for the product with V,
- * with 16-bit rows in batches of many rows, as the sizes of the structs have it, to 2^-8
- * (their sum is not rounded).  NaN as frq_paged_batch has it; a code times its scale
- * past f32's range is infinite. */
+ * stand for; scores, softmax and sums are f32 (a score is formed in units of the key's
+ * scale first: there too it has to lie in f32's range).  f32 rows of q are multiplied
+ * in parts that hold them to 2^-22.  For the product with V a softmax weight is held to
+ * 2^-22 with f32 rows, to 2^-16 with others; in batches of many rows, as the sizes of
+ * the structs have it, with f16 rows to 2^-11 and with bf16 rows to 2^-8, and with f32
+ * and f16 rows to 2^-33 of the row's largest, if that is more (their sum is not
+ * rounded).  Such a batch of f32 or f16 rows takes many times as long where the scales
+ * of a sequence's values that are not all 0 differ by more than 2^22.  NaN as
+ * frq_paged_batch has it; a code times its scale past f32's range is infinite. */
 size_t frq_paged8_attention_workspace(const frq_paged_kv8 *kv, const frq_paged_batch *batch, size_t n_heads);
 int frq_paged8_attention_decode(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype,
                                 size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,
