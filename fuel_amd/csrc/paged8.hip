@@ -14,11 +14,12 @@
 // exactly, so that no weight has to carry a scale.  f32 rows: q in two parts of f16,
 // 16-bit rows as they are; weights in two parts of bf16, to 2^-16 of each (V's codes
 // are 2^-4 of what was appended), for f32 rows in three, to f32's own precision: the
-// third costs 2 % (64 sequences of up to 9851, f32, 82 us).
+// third costs 1 % (96 sequences of up to 7942, f32, 82 us).
 // Bound by HBM and some 10 us beside it: the lookup and the first keys, the join.  32
-// heads over 8 of 128: one sequence of 199999, 410 MB, 75 us (70 with the loads
-// alone); 64 of up to 9851, 333 MB, 82 (68 alone); dims of 64, 128 sequences of up to
-// 2489, 132 MB, 36 (32 alone).  One of 700: 10 us, 7 of them the two launches' start.
+// heads over 8 of 128: one sequence of 200002, 410 MB, 75 us (70 with the loads
+// alone); 96 of up to 7942, 333 MB, 82 (68 alone); 64 heads over 8 of 64, 128 of 307 ..
+// 2489, 132 MB, 36 (32 alone).  One of 901, 32 KV heads: 10 us, 7 of them the two
+// launches' start.
 // No faster: blocks of 64 keys, three workgroups a CU for dims of 128, the odd blocks'
 // code out of line.
 #include <hip/hip_runtime.h>

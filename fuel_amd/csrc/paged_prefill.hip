@@ -43,11 +43,12 @@
 //   f16 and f32 rows f16 holds a code but not every scale: K's is a factor of its 16
 //                    keys' scores, V is in units of the largest scale so far, exact
 //                    within 2^P8_SPREAD of it; o follows that unit
-// One prompt of 12288, 32 heads over 8 of 128, bf16: 1.26 ms, 0.98 PFLOP/s, as over a
-// 16-bit cache; 17 of 20 .. 1500 f16 rows 0.158 ms, 0.61 PFLOP/s; two chunks of f32 rows
-// after 6000 .. 8000 cached 0.212 ms.  No faster: decoding between the two products
-// (spills), the sums of products apart in more registers, a part of a weight by
-// truncation (1 %).
+// One prompt of 12345, 32 heads over 8 of 128, bf16: 1.23 - 1.27 ms, 1.0 PFLOP/s (beside
+// a 16-bit cache's kernel, 24 % more VALU instructions and bank conflicts of a tenth of
+// its time, as the decoded rows are written); 15 of 66 .. 1562, f16, 0.16 ms, 0.61
+// PFLOP/s; 322 and 451 rows of 32 KV heads that see 4628 and 6620 keys, f32, 0.218 ms.
+// No faster: decoding between the two products (spills), the sums of products apart in
+// more registers; a weight's first part by truncation 1 %.
 #include <hip/hip_runtime.h>
 
 #include "common.hpp"
