@@ -218,7 +218,7 @@ def test_a_server_of_captured_steps(dev, act, H, hk, D):
                 q = R.from_bits(R.to_bits(R.rotate(q, cos[at], sin[at]), act), act)
                 keys, values = pool.get(s, int(state[0][s]))
                 want, A, B, V = R.attend(q, keys, values, at, scale)
-                tol = P.bound(want, A, B, V, pool.top(s, int(state[0][s])), int(state[0][s]), D, act, True)
+                tol = P.bound(want, A, B, V, int(state[0][s]), D, act, True)
                 assert (np.abs(out[lo:hi].reshape(want.shape) - want) <= tol).all(), (t, s)
         rt.graph_destroy(graph)
     finally:
