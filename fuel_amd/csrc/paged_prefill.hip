@@ -601,7 +601,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         // another.  (A row may see none of the large ones, or give them no weight.)
         uint32_t far = 0;  // all groups of a tile
         if constexpr (RELATIVE) far = t0 < tiles && raw.top - least > P8_SPREAD ? 15 : 0;
-        if (far || __builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)))) {
+        const bool odd = __builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)));  // (the last tile is read)
+        if (far || odd) {
             first_tile();
             walk(std::true_type{}, far);
         }
