@@ -598,7 +598,8 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 7.7,
         // all NaN 7.2, with one infinite value in every 16 keys, the worst there is, 205.
         // Values whose scales lie so far apart that not all were exact: all keys one after
-        // another.  (A row may see none of the large ones, or give them no weight.)
+        // another.  (A row may see none of the large ones, or give them no weight.)  322 and
+        // 451 rows of f32 that see 4628 and 6620 keys 0.22 ms, so 6.9; 4000 of f16 0.2, so 14.
         uint32_t far = 0;  // all groups of a tile
         if constexpr (RELATIVE) far = t0 < tiles && raw.top - least > P8_SPREAD ? 15 : 0;
         const bool odd = __builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)));  // (the last tile is read)
