@@ -207,7 +207,8 @@ struct Rows16 {
     __device__ void plain(const PagedKv& c, const int* table, int head, const T* x, float scale, int j0, int j1) {
         const int g = (threadIdx.x & 63) >> 4;
         pg_plain<PgCells<E, HD>, T, HD, 4>(
-            c, table, head, x, scale, limit, j0, j1, P::TOP, g == 0, [&](int i) { return 4 * (VW * g + i); },
+            c, table, head, x, scale, limit, j0, j1, [](float x) { return x; }, P::TOP, g == 0,
+            [&](int i) { return 4 * (VW * g + i); },
             [&](int i, int e, float f, float p, float v) {
                 const int t = (4 * i + e) % VW, k = (4 * i + e) / VW;
                 o[t][k] = fmaf(p, v, o[t][k] * f);

@@ -243,12 +243,12 @@ struct PgCells {
 // an infinite or NaN value come here.  SHARE lanes, 64 / SHARE apart, hold a row of
 // HD dims; a lane's are RUNS runs of 4, run i from dim(i) on.  x: the row's q (from
 // memory: in the registers there is room for the kernels' own loops only); own_l:
-// whether l is the lane's; a weight is 2^shift at most; add(i, e, f, p, v): sum e of
-// run i becomes f times itself and p v.
-template <class Cells, class T, int HD, int SHARE, class Cache, class Dim, class Add>
+// whether l is the lane's; score s has the weight 2^(s - m + shift), m the largest
+// base_of(s); add(i, e, f, p, v): sum e of run i becomes f times itself and p v.
+template <class Cells, class T, int HD, int SHARE, class Cache, class Base, class Dim, class Add>
 __device__ __forceinline__ void pg_plain(const Cache& c, const int* table, int head, const T* x, float scale,
-                                         int limit, int j0, int j1, float shift, bool own_l, Dim dim, Add add,
-                                         float& m, float& l) {
+                                         int limit, int j0, int j1, Base base_of, float shift, bool own_l, Dim dim,
+                                         Add add, float& m, float& l) {
     constexpr int RUNS = HD / SHARE / 4, KEYS = 4;  // keys at a time: q is read once for them
     const float factor = scale * 1.4426950408889634f;
 #pragma unroll 1
@@ -274,7 +274,7 @@ __device__ __forceinline__ void pg_plain(const Cache& c, const int* table, int h
 #pragma unroll
             for (int d = 64 / SHARE; d < 64; d *= 2) s[u] += __shfl_xor(s[u], d);
             if (none) s[u] = pg_nan();
-            if (j + u <= limit) mn = fmaxf(mn, s[u]);
+            if (j + u <= limit) mn = fmaxf(mn, base_of(s[u]));
         }
         if (j > limit) continue;
         const float f = __builtin_amdgcn_exp2f(m - mn);

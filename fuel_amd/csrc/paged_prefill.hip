@@ -117,7 +117,14 @@ struct PrefillTile {
     static constexpr int DIM = HD, NP = PARTS;
     static constexpr bool F16 = std::is_same<E, _Float16>::value;
     // (f16 parts of an f32 weight: as many of its digits as f16's range holds)
-    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, SHIFT = PgElem<E>::TOP - LAZY;
+    static constexpr float LAZY = WIDE && F16 ? 0.0f : 7.0f, TOP = PgElem<E>::TOP, SHIFT = TOP - LAZY;
+    // Score s has the weight 2^(s - base), base that of the running maximum m: m - SHIFT,
+    // up to f32's steps.  From 2^24 on those are 2 and more; of f16 the base is never below
+    // m - SHIFT, since a weight of 2^16 is infinite there.
+    __device__ static __forceinline__ float base_of(float m) {
+        const float b = m - SHIFT;
+        return F16 && m - b > SHIFT ? fmaf(fabsf(m), 0x1p-23f, b) : b;
+    }
     static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;
     static constexpr int RPI = 512 / HD, NI = TILE / 1024;  // rows a DMA instruction, instructions a tile
@@ -264,7 +271,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         if constexpr (CUT) tiles = min(tiles, t0 + m_units);
 
         pf_f16 o[X::DT];
-        float m, l, peak;  // peak: the largest score so far
+        float base, l, peak;  // peak: the largest score so far
 
         // DMA: instruction i of this wavefront takes rows ((i PF_WAVES + wave) RPI) .. of
         // a tile, all in one group of 16 keys.  Source offsets of the lane within it:
@@ -434,7 +441,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             for (int d = 0; d < X::DT; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
-            m = peak = PG_LEAST;
+            base = peak = PG_LEAST;
             l = 0.0f;
             unit = far ? P8_ONE : 0;
             for (int t = t0; t < tiles; t++) {
@@ -478,13 +485,14 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                     if (!__all(pg_all_nan(o)))
                         pg_plain<typename X::Cells, T, HD, 2>(
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
-                            min(jw + 32 * NA, last + 1), far ? P8_FAR : X::SHIFT, h == 0, [&](int i) { return 8 * i + 4 * h; },
+                            min(jw + 32 * NA, last + 1), [](float x) { return X::base_of(x); },
+                            far ? P8_FAR - X::SHIFT : 0.0f, h == 0, [&](int i) { return 8 * i + 4 * h; },
                             [&](int i, int e, float f, float p, float v) {
                                 if (RELATIVE) v = __builtin_amdgcn_ldexpf(v, P8_ONE - unit);
                                 o[i / 4][4 * (i % 4) + e] = fmaf(p, v, o[i / 4][4 * (i % 4) + e] * f);
                             },
-                            m, l);
-                    peak = fmaxf(peak, m);
+                            base, l);
+                    peak = fmaxf(peak, base + X::SHIFT);
                     continue;
                 }
                 pf_f16 st[NA];
@@ -537,24 +545,24 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                     top = fmaxf(top, pf_other_half(top)) * factor;
                 }
                 peak = fmaxf(peak, top);
-                const float low = X::F16 ? fmaxf(top, peak - PG_DROP) : m;
-                if (__any(top > m + X::LAZY || low < m - PF_LOW)) {
-                    const float mn = fmaxf(top, low < m - PF_LOW ? low : m);
-                    const float f = __builtin_amdgcn_exp2f(m - mn);  // (0 or 1 where nothing was seen before)
-                    m = mn;
+                const float low = X::F16 ? fmaxf(top, peak - PG_DROP) : 0.0f;
+                const bool drop = X::F16 && low < base + (X::SHIFT - PF_LOW);
+                if (__any(top - base > X::TOP || drop)) {
+                    const float to = drop ? X::base_of(low) : fmaxf(base, X::base_of(top));
+                    const float f = __builtin_amdgcn_exp2f(base - to);  // (0 or 1 where nothing was seen before)
+                    base = to;
                     l *= f;
 #pragma unroll
                     for (int d = 0; d < X::DT; d++) o[d] *= f;
                 }
                 // (fmaf: one operation less a weight.  Of scores past 2^30 it leaves what the
                 // maximum was rounded by, which can be a weight that is infinite.)
-                const float ms = m - X::SHIFT;
 #pragma unroll
                 for (int a = 0; a < NA; a++)
 #pragma unroll
                     for (int i = 0; i < 16; i++)
-                        st[a][i] = AGAIN ? st[a][i] * fac[2 * a + (i >> 3)] - ms
-                                         : fmaf(st[a][i], fac[2 * a + (i >> 3)], -ms);
+                        st[a][i] = AGAIN ? st[a][i] * fac[2 * a + (i >> 3)] - base
+                                         : fmaf(st[a][i], fac[2 * a + (i >> 3)], -base);
                 if (mask) {  // (again: a factor of 0 would make NaN of -inf)
 #pragma unroll
                     for (int a = 0; a < NA; a++)
@@ -611,7 +619,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         if constexpr (RELATIVE) {  // as values; l of 0.5 .. 1, so that no o is past the values themselves
             const int ex = l > 0.0f && l < __builtin_inff() ? __builtin_amdgcn_frexp_expf(l) : 0;
             l = __builtin_amdgcn_ldexpf(l, -ex);
-            m += ex + (far ? X::SHIFT - P8_FAR : 0.0f);
+            base += ex + (far ? X::SHIFT - P8_FAR : 0.0f);
 #pragma unroll
             for (int d = 0; d < X::DT; d++)
 #pragma unroll
@@ -626,14 +634,14 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 for (int d = 0; d < X::DT; d++)
 #pragma unroll
                     for (int i = 0; i < 16; i++) s_o[64 * (16 * d + i)] = o[d][i];
-                s_m[32 * w + n] = m;
+                s_m[32 * w + n] = base;
                 s_l[32 * w + n] = l;
             }
             __syncthreads();
             if (!key0) {
-                const float m2 = s_m[32 * w + n], mn = fmaxf(m, m2);
-                const float f = __builtin_amdgcn_exp2f(m - mn), f2 = __builtin_amdgcn_exp2f(m2 - mn);
-                m = mn;
+                const float other = s_m[32 * w + n], to = fmaxf(base, other);
+                const float f = __builtin_amdgcn_exp2f(base - to), f2 = __builtin_amdgcn_exp2f(other - to);
+                base = to;
                 l = l * f + s_l[32 * w + n] * f2;
 #pragma unroll
                 for (int d = 0; d < X::DT; d++)
@@ -664,7 +672,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                         *reinterpret_cast<pg_f4*>(dst + 32 * d + 8 * g) =
                             pg_f4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
                 if (h == 0) {
-                    slot[ROWS * HD + 32 * w + n] = m;
+                    slot[ROWS * HD + 32 * w + n] = base;
                     slot[ROWS * HD + ROWS + 32 * w + n] = l;
                 }
             }

@@ -1,0 +1,71 @@
+"""Paged attention of scores so large that f32 has steps of 1 and more there: keys
+whose scores are equal weigh the same, in whichever tile, walk or piece of a row they
+are, over 16-bit and 8-bit caches.
+
+Every q is 2^12 in its first dim and 0 elsewhere, every key 2^12 in that dim, so that all
+products are exact and all scores are the same number: the results are the means of
+the values that a row sees, with the bounds of paged_ref.py and paged8_ref.py for A = 0
+(nothing is lost where equal scores are subtracted)."""
+import numpy as np
+import pytest
+
+import paged8_ref as P
+import paged_ref as R
+import test_gpu_paged as W
+import test_gpu_paged8 as W8
+from paged_ref import BF16, F16, F32
+from test_gpu_paged import say, seed
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [(F32, F16), (F16, F16), (F32, BF16), (BF16, BF16), (F32, 8), (F16, 8), (BF16, 8)]
+POWERS = [20, 24, 25, 26, 27, 28, 29, 31, 90]  # of the scores, in natural units
+
+
+def case(dev, rng, act, cache, H, hk, D, past, new, decode):
+    """A case of equal keys: keys, then values, of each sequence."""
+    if cache == 8:
+        c = W8.Case(dev, rng, act, H, hk, D, 16, past, new, decode=decode, fill=False)
+    else:
+        c = W.Case(dev, rng, act, cache, H, hk, D, 16, past, new, decode=decode)
+    for s, n in enumerate(c.kv):
+        k, v = np.zeros((n, hk, D), np.float32), rng.standard_normal((n, hk, D)).astype(np.float32)
+        k[:, :, 0] = 2.0 ** 12
+        if cache == 8:
+            c.pool.append(s, 0, k, v)
+        else:
+            c.pool.put(s, np.arange(n), k, v)
+    c.q[:] = 0
+    c.q[:, ::D] = 2.0 ** 12
+    return c
+
+
+def means(c, s):
+    """The means of what each row of sequence s sees, their bounds, and the rows' results."""
+    n, r0, D = c.new[s], int(c.start[s]), c.D
+    _, v = c.pool.get(s, int(c.kv[s]))
+    pos = int(c.kv[s]) - n + np.arange(n)
+    want, A, B, V = R.attend(np.zeros((n, c.H, D)), np.zeros_like(v), np.nan_to_num(v), pos, 1.0)
+    keys = int(c.kv[s])
+    if isinstance(c, W8.Case):
+        tol = P.bound(want, A, B, V, keys, D, c.act, not c.decode)
+    else:
+        tol = R.bound(want, A, B, V, keys, D, c.act, c.cache, not c.decode)
+    return want, tol, c.got()[r0:r0 + n, :c.H * D].reshape(want.shape), v, pos
+
+
+# decode cut; 16-row tiles whole; 128-row tiles
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", [
+    (4, 2, 128, [2299, 39], [1, 1]), (4, 2, 128, [60, 0], [9, 30]), (20, 20, 64, [0, 3] * 7, [130, 71] * 7)])
+def test_equal_scores(dev, act, cache, H, hk, D, past, new):
+    rng = seed(50, act, cache, H, D)
+    c = case(dev, rng, act, cache, H, hk, D, past, new, new[0] == 1)
+    c.upload()
+    for power in POWERS:
+        say("equal scores", act, cache, H, D, past, power)
+        c.run(2.0 ** (power - 24))
+        for s in range(len(new)):
+            want, tol, got, _, _ = means(c, s)
+            bad = np.argwhere(~(np.abs(got - want) <= tol))
+            assert not len(bad), (power, s, bad[:3], got[tuple(bad[0])], want[tuple(bad[0])])
