@@ -297,9 +297,9 @@ bool paged_rows16_fits(const PagedKv& kv, const PagedRows& r, int n_heads, int h
 size_t paged_rows16_work_bytes(const PagedKv& kv, const PagedRows& r, int n_heads, int hd);
 hipError_t launch_paged_rows16(int kv_dtype, int dtype, int hd, const PagedAttendArgs& p, hipStream_t s);
 // The pieces of cut tiles that wgs workgroups left (paged.hpp), up to `rows` rows
-// a tile, into the output.
+// a tile, into the output.  normalized: o is (pg_exponent).
 hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, long tiles,
-                             int tile_rows, int rows, int grp, void* out, int ldo, hipStream_t s);
+                             int tile_rows, int rows, int grp, bool normalized, void* out, int ldo, hipStream_t s);
 // paged_prefill.hip: many rows a sequence, 128-row tiles (work of
 // paged_prefill_work_bytes()); fits: the workgroups are a grid.
 bool paged_prefill_fits(const PagedKv& kv, const PagedRows& r, int n_heads);

@@ -330,7 +330,7 @@ struct Rows16 {
 // of such threads as there is room for with every so many-th piece each, PJ_STEP
 // pieces a step, whose loads are one memory round trip.
 constexpr int PJ_WG = 256;
-template <class T, int HD, int PJ_STEP>
+template <class T, int HD, int PJ_STEP, bool NORMALIZED>
 __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restrict__ joins, int records,
                                                            const float* __restrict__ part, int tile_rows, int wg_rows,
                                                            int grp, T* __restrict__ out, int ldo) {
@@ -375,17 +375,22 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
             }
 #pragma unroll
             for (int i = 0; i < PJ_STEP; i++) mn = fmaxf(mn, m[i]);
-            const float f = __builtin_amdgcn_exp2f(M - mn);
+            const float f = __builtin_amdgcn_exp2f(M - mn), was = L;
             M = mn;
             L *= f;
-            O *= f;
+            float e[PJ_STEP];
+#pragma unroll
+            for (int i = 0; i < PJ_STEP; i++) {
+                e[i] = __builtin_amdgcn_exp2f(m[i] - mn);
+                L = fmaf(l[i], w + i * groups <= j.last ? e[i] : 0.0f, L);
+            }
+            O *= pg_factor<NORMALIZED>(f, was, L);
 #pragma unroll
             for (int i = 0; i < PJ_STEP; i++) {
                 const bool add = w + i * groups <= j.last;
-                const float e = __builtin_amdgcn_exp2f(m[i] - mn);
-                L = fmaf(l[i], add ? e : 0.0f, L);
+                const float x = pg_factor<NORMALIZED>(e[i], l[i], L);
 #pragma unroll
-                for (int k = 0; k < 4; k++) O[k] = add ? fmaf(o[i][k], e, O[k]) : O[k];  // (o may be infinite)
+                for (int k = 0; k < 4; k++) O[k] = add ? fmaf(o[i][k], x, O[k]) : O[k];  // (o may be infinite)
             }
         }
         s_o[threadIdx.x] = O;
@@ -400,13 +405,14 @@ __global__ __launch_bounds__(PJ_WG) void paged_join_kernel(const PgJoin* __restr
     for (int i = 0; i < groups; i++) mx = fmaxf(mx, s_m[i * rows + x]);
     L = 0.0f;
     O = pg_f4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < groups; i++) L = fmaf(s_l[i * rows + x], __builtin_amdgcn_exp2f(s_m[i * rows + x] - mx), L);
     for (int i = 0; i < groups; i++) {
-        const float e = __builtin_amdgcn_exp2f(s_m[i * rows + x] - mx);
-        L = fmaf(s_l[i * rows + x], e, L);
+        const float e = pg_factor<NORMALIZED>(__builtin_amdgcn_exp2f(s_m[i * rows + x] - mx), s_l[i * rows + x], L);
         const pg_f4 o = s_o[(i * rows + x) * TH + d];
 #pragma unroll
         for (int k = 0; k < 4; k++) O[k] = fmaf(o[k], e, O[k]);
     }
+    L = pg_divisor<NORMALIZED>(L);
     const int at = (unsigned)(j.i0 + r) / (unsigned)grp;
     const size_t to = j.row0 + at, h = j.head * grp + (j.i0 + r - at * grp);
     T y[4];
@@ -544,11 +550,12 @@ struct AppendCall {
 // have one, finding it costs more: 18.2 -> 23.5).  Tiles of 16 rows in many pieces
 // each, a row a workgroup: 2 sequences of 29561, 128 pieces, 28.9 -> 22.7 us a whole
 // call; one of 131071, 8 KV heads, 64 pieces, 92.6 -> 91.2.
-template <class T, int HD>
+template <class T, int HD, bool NORMALIZED>
 hipError_t join(const PgJoin* joins, const float* part, int wgs, long tiles, int tile_rows, int rows, int grp,
                 void* out, int ldo, hipStream_t s) {
     const bool few = tiles <= wgs / 4;
-    const auto kernel = tile_rows == 16 || few ? paged_join_kernel<T, HD, 8> : paged_join_kernel<T, HD, 2>;
+    const auto kernel = tile_rows == 16 || few ? paged_join_kernel<T, HD, 8, NORMALIZED>
+                                                : paged_join_kernel<T, HD, 2, NORMALIZED>;
     const int wg_rows = tile_rows == 16 && tiles <= wgs / 32 ? 1 : 4, y = (rows + wg_rows - 1) / wg_rows;
     const int x = few && wgs * y > 2048 ? (int)tiles : wgs;
     hipLaunchKernelGGL(kernel, dim3(x, y), dim3(PJ_WG), 0, s, joins, wgs, part, tile_rows, wg_rows, grp,
@@ -586,10 +593,13 @@ hipError_t launch_paged_append(int kv_dtype, int dtype, int hd, const PagedAppen
 }
 
 hipError_t launch_paged_join(int dtype, int hd, const PgJoin* joins, const float* part, int wgs, long tiles,
-                             int tile_rows, int rows, int grp, void* out, int ldo, hipStream_t s) {
-    const auto run = dtype == GGML_F32   ? (hd == 64 ? join<float, 64> : join<float, 128>)
-                     : dtype == GGML_F16 ? (hd == 64 ? join<_Float16, 64> : join<_Float16, 128>)
-                                         : (hd == 64 ? join<__bf16, 64> : join<__bf16, 128>);
+                             int tile_rows, int rows, int grp, bool normalized, void* out, int ldo, hipStream_t s) {
+    const auto run =
+        dtype == GGML_F32 && normalized   ? (hd == 64 ? join<float, 64, true> : join<float, 128, true>)
+        : dtype == GGML_F32               ? (hd == 64 ? join<float, 64, false> : join<float, 128, false>)
+        : dtype == GGML_F16 && normalized ? (hd == 64 ? join<_Float16, 64, true> : join<_Float16, 128, true>)
+        : dtype == GGML_F16               ? (hd == 64 ? join<_Float16, 64, false> : join<_Float16, 128, false>)
+                                          : (hd == 64 ? join<__bf16, 64, false> : join<__bf16, 128, false>);
     return run(joins, part, wgs, tiles, tile_rows, rows, grp, out, ldo, s);
 }
 

@@ -98,7 +98,8 @@ constexpr long PG_GRID = (1L << 24) - 1;
 
 // Cut tiles.  Workgroups that share the keys of a tile of `rows` query rows
 // leave slots of floats in the workspace, two a workgroup: o [rows][hd]
-// (unnormalized), m [rows], l [rows]; and each a record of what is to be joined.
+// (unnormalized, or as pg_exponent() has it), m [rows], l [rows]; and each a record of
+// what is to be joined.
 constexpr size_t pg_slot(int rows, int hd) { return (size_t)rows * hd + 2 * rows; }
 struct PgJoin {
     int rows;        // of the tile that begins in the workgroup's range and goes on past it; 0: none
@@ -183,6 +184,22 @@ constexpr float PG_LEAST = -__FLT_MAX__;
 // f32's range (2^15 a weight, 2^16 a value, 2^30 keys), and what is lost is below
 // 2^-PG_DROP of what f32 sums keep.
 constexpr float PG_DROP = 40.0f;
+
+// Normalized sums: o is the sum of weights times values over 2^pg_exponent(l), l the sum of
+// the weights, so that no o is past the values themselves.  (The exponent apart, not in
+// the maximum: f32 does not hold a maximum of 2^24 and the exponent.)  Where pieces are
+// put together, the factor of one's o, f that of its l, and what o is divided by.
+__device__ __forceinline__ int pg_exponent(float l) {
+    return l > 0.0f && l < __builtin_inff() ? __builtin_amdgcn_frexp_expf(l) : 0;
+}
+template <bool NORMALIZED>
+__device__ __forceinline__ float pg_factor(float f, float l, float all) {
+    return NORMALIZED ? __builtin_amdgcn_ldexpf(f, pg_exponent(l) - pg_exponent(all)) : f;
+}
+template <bool NORMALIZED>
+__device__ __forceinline__ float pg_divisor(float l) {
+    return NORMALIZED ? __builtin_amdgcn_ldexpf(l, -pg_exponent(l)) : l;
+}
 
 // Whether an infinite or NaN value is among a lane's sums.
 template <int N, class V>

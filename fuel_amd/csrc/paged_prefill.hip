@@ -616,10 +616,9 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             walk(std::true_type{}, far);
         }
         l += pf_other_half(l);
-        if constexpr (RELATIVE) {  // as values; l of 0.5 .. 1, so that no o is past the values themselves
-            const int ex = l > 0.0f && l < __builtin_inff() ? __builtin_amdgcn_frexp_expf(l) : 0;
-            l = __builtin_amdgcn_ldexpf(l, -ex);
-            base += ex + (far ? X::SHIFT - P8_FAR : 0.0f);
+        if constexpr (RELATIVE) {  // o as values, normalized
+            const int ex = pg_exponent(l);
+            if (far) l = __builtin_amdgcn_ldexpf(l, (int)(X::SHIFT - P8_FAR));
 #pragma unroll
             for (int d = 0; d < X::DT; d++)
 #pragma unroll
@@ -642,16 +641,18 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 const float other = s_m[32 * w + n], to = fmaxf(base, other);
                 const float f = __builtin_amdgcn_exp2f(base - to), f2 = __builtin_amdgcn_exp2f(other - to);
                 base = to;
-                l = l * f + s_l[32 * w + n] * f2;
+                const float l2 = s_l[32 * w + n], all = l * f + l2 * f2;
+                const float fo = pg_factor<RELATIVE>(f, l, all), fo2 = pg_factor<RELATIVE>(f2, l2, all);
+                l = all;
 #pragma unroll
                 for (int d = 0; d < X::DT; d++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) o[d][i] = fmaf(s_o[64 * (16 * d + i)], f2, o[d][i] * f);
+                    for (int i = 0; i < 16; i++) o[d][i] = fmaf(s_o[64 * (16 * d + i)], fo2, o[d][i] * fo);
             }
         }
         if (key0 == 0 && i0 + 32 * w + n < rows) {
             if (!CUT || whole) {
-                const float inv = sq.bad ? pg_nan() : limit < 0 ? 0.0f : 1.0f / l;  // (o is 0 in the first two)
+                const float inv = sq.bad ? pg_nan() : limit < 0 ? 0.0f : 1.0f / pg_divisor<RELATIVE>(l);  // (o is 0 in the first two)
                 T* dst = out + (size_t)row * ldo + (size_t)qh * HD + 4 * h;
 #pragma unroll
                 for (int d = 0; d < X::DT; d++)
@@ -718,7 +719,8 @@ hipError_t prefill_launch(const PagedAttendArgs& p, const typename X::Cache& c, 
                        p.ldq, p.scale, out, p.ldo, part, joins);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    return launch_paged_join(pg_dtype<T>(), X::DIM, joins, part, PG_WGS, tiles, PF_ROWS, PF_ROWS, grp, p.out, p.ldo, s);
+    return launch_paged_join(pg_dtype<T>(), X::DIM, joins, part, PG_WGS, tiles, PF_ROWS, PF_ROWS, grp,
+                             X::BYTES && X::F16, p.out, p.ldo, s);
 }
 
 struct PrefillCall {

@@ -327,7 +327,7 @@ hipError_t rows16_launch(const PagedAttendArgs& p, const typename A::Cache& c, h
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !pl.cut) return e;
     return launch_paged_join(pg_dtype<T>(), A::DIM, joins, part, pl.wgs, pg_tiles_bound(p.rows, grp, 16) * c.kv_heads,
-                             16, p.rows.row_start || grp > 16 ? 16 : grp, grp, p.out, p.ldo, s);
+                             16, p.rows.row_start || grp > 16 ? 16 : grp, grp, false, p.out, p.ldo, s);
 }
 
 }  // namespace frq

@@ -69,3 +69,13 @@ def test_equal_scores(dev, act, cache, H, hk, D, past, new):
             want, tol, got, _, _ = means(c, s)
             bad = np.argwhere(~(np.abs(got - want) <= tol))
             assert not len(bad), (power, s, bad[:3], got[tuple(bad[0])], want[tuple(bad[0])])
+
+
+# 64-row tiles, the keys of a tile in two halves; cut 128-row tiles
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", [
+    (20, 20, 64, [0, 70, 0], [330, 260, 130]), (32, 2, 128, [0, 30], [170, 60]),
+    (32, 2, 128, [2200, 2000, 0], [150, 100, 40]), (40, 2, 64, [2200, 2000], [150, 140])])
+def test_equal_scores_in_pieces(dev, act, cache, H, hk, D, past, new):
+    """Pieces of few and of many keys: each counts by its keys."""
+    test_equal_scores(dev, act, cache, H, hk, D, past, new)
