@@ -42,7 +42,8 @@
 //   bf16 rows        codes times scales are bf16 numbers: K and V as values
 //   f16 and f32 rows f16 holds a code but not every scale: K's is a factor of its 16
 //                    keys' scores, V is in units of the largest scale so far, exact
-//                    within 2^P8_SPREAD of it; o follows that unit
+//                    within 2^P8_SPREAD of it; o follows that unit.  Where scales differ
+//                    by more, once more with V as bf16 values
 // One prompt of 12345, 32 heads over 8 of 128, bf16: 1.23 - 1.27 ms, 1.0 PFLOP/s (beside
 // a 16-bit cache's kernel, 24 % more VALU instructions and bank conflicts of a tenth of
 // its time, as the decoded rows are written); 15 of 66 .. 1562, f16, 0.16 ms, 0.61
@@ -66,8 +67,9 @@ constexpr float PF_LOW = 8.0f;
 // Values of an 8-bit cache as f16: in units of 2^-P8_UP of the largest scale, where 448
 // is 57344, and the least code, 2^-9, of a scale P8_SPREAD smaller is 2^-24, f16's least.
 constexpr int P8_UP = 7, P8_SPREAD = 22;
-// Of weights times values as they are: 2^30 keys' sum stays within f32's range.
-constexpr float P8_FAR = -38.0f;
+// What weights of values as they are are smaller by than those of values in such units: 2^30
+// keys' sum of them, 2^-31 at most, stays within f32's range.
+constexpr float P8_DOWN = PgElem<__bf16>::TOP - PgElem<_Float16>::TOP;
 
 typedef float pf_f16 __attribute__((ext_vector_type(16)));
 typedef short pf_s4 __attribute__((ext_vector_type(4)));
@@ -137,13 +139,13 @@ struct PrefillTile {
 
 // Whether KEYS rows of K and V from kt and vt on hold an infinite or NaN value, or
 // a page of them is none.  Wave-uniform.
-template <class X, int KEYS>
+template <class X, class V, int KEYS>
 __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uint32_t bad) {
     bool any = bad & ((1u << KEYS / 16) - 1);
     for (int i = 16 * (threadIdx.x & 63); i < KEYS * X::ROW; i += 1024) {
         const pg_u4 k = *reinterpret_cast<const pg_u4*>(kt + i), v = *reinterpret_cast<const pg_u4*>(vt + i);
 #pragma unroll
-        for (int w = 0; w < 4; w++) any |= pg_word_odd<typename X::Elem>(k[w]) || pg_word_odd<typename X::Elem>(v[w]);
+        for (int w = 0; w < 4; w++) any |= pg_word_odd<typename X::Elem>(k[w]) || pg_word_odd<V>(v[w]);
     }
     return __any(any);
 }
@@ -349,7 +351,9 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 rv[i] = *reinterpret_cast<const P8Global<pg_u4>*>(p8_base(c.v, at) + boff);
             }
         };
-        auto decode8 = [&](int t) {
+        auto decode8 = [&](int t, auto again) {
+            constexpr bool VALUES = RELATIVE && decltype(again)::value;
+            using V = typename std::conditional<VALUES, __bf16, E>::type;
             if (t * PF_KEYS + PF_KEYS > sq.kv || raw.bad) {  // rows of V that are no keys hold anything
 #pragma unroll
                 for (int i = 0; i < PASS; i++) {
@@ -360,22 +364,22 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
             uint8_t *k = s_k[t & 1], *v = s_v[t & 1];
 #pragma unroll
             for (int i = 0; i < PASS; i++) {
-                const float ku = SCALED ? p8_operand(raw.k[i]) : 1.0f, vu = RELATIVE ? raw.v_relative(i) : p8_operand(raw.v[i]);
+                const float ku = SCALED ? p8_operand(raw.k[i]) : 1.0f, vu = RELATIVE && !VALUES ? raw.v_relative(i) : p8_operand(raw.v[i]);
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     *reinterpret_cast<v8*>(k + i * PR * X::ROW + (bk ^ (16 * e))) =
                         p8_eight<E>(rk[i][2 * e], rk[i][2 * e + 1], ku);
-                    *reinterpret_cast<v8*>(v + i * PR * X::ROW + (bv ^ (16 * e))) =
-                        p8_eight<E>(rv[i][2 * e], rv[i][2 * e + 1], vu);
+                    *reinterpret_cast<typename PgElem<V>::v8*>(v + i * PR * X::ROW + (bv ^ (16 * e))) =
+                        p8_eight<V>(rv[i][2 * e], rv[i][2 * e + 1], vu);
                 }
             }
             cur = raw;
         };
-        auto first_tile = [&] {
+        auto first_tile = [&](auto again) {
             fetch_ids(t0 * PF_KEYS);
             if constexpr (X::BYTES) {
                 fetch8(t0);
-                decode8(t0);
+                decode8(t0, again);
                 if (t0 + 1 < tiles) fetch8(t0 + 1);
             } else {
                 issue(t0);
@@ -388,7 +392,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
         const uint32_t vbase = (4 * h + vr) * X::ROW +
                                16 * ((2 * ((lane >> 4) & 1) + ((lane >> 1) & 1)) ^ X::vswz(vr)) + 8 * (lane & 1);
 
-        if (t0 < tiles) first_tile();
+        if (t0 < tiles) first_tile(std::false_type{});
 
         // Q^T, the B operand: dims 16 t + 8 h + e of row n (negated for a negative
         // scale: the maximum is taken of scores with a positive factor)
@@ -435,15 +439,19 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 }
         }
 
-        const auto walk = [&](auto again, uint32_t far) {
-            constexpr bool AGAIN = decltype(again)::value;
+        const auto walk = [&](auto again) {
+            constexpr bool AGAIN = decltype(again)::value, VALUES = RELATIVE && AGAIN;
+            using V = typename std::conditional<VALUES, __bf16, E>::type;  // of V and of the weights
+            using v8v = typename PgElem<V>::v8;
+            constexpr int NW = !VALUES ? X::NP : X::WIDE ? 3 : 2;  // parts of a weight
+            constexpr float DOWN = VALUES ? P8_DOWN : 0.0f;        // what weights are smaller by
 #pragma unroll
             for (int d = 0; d < X::DT; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
             base = peak = PG_LEAST;
             l = 0.0f;
-            unit = far ? P8_ONE : 0;
+            unit = VALUES ? P8_ONE : 0;
             for (int t = t0; t < tiles; t++) {
                 const int j0 = t * PF_KEYS;
                 // tile t landed, in every wavefront, and tile t - 1 is read
@@ -457,7 +465,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 if (X::BYTES) {
                     if (t + 1 < tiles) {  // (not among the products: the registers do not hold both)
                         __builtin_amdgcn_sched_barrier(0);
-                        decode8(t + 1);
+                        decode8(t + 1, again);
                         if (t + 2 < tiles) fetch8(t + 2);
                         __builtin_amdgcn_sched_barrier(0);
                     }
@@ -473,7 +481,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 const int jw = j0 + key0;  // this wavefront's first key
                 if (jw > last) continue;
 
-                if (RELATIVE && t8.unit() != unit && !(AGAIN && far)) {
+                if (RELATIVE && !VALUES && t8.unit() != unit) {
                     const float f = __builtin_amdgcn_ldexpf(1.0f, unit - t8.unit());
                     unit = t8.unit();
 #pragma unroll
@@ -481,14 +489,13 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 }
                 const uint8_t* kt = s_k[t & 1] + key0 * X::ROW;
                 const uint8_t* vt = s_v[t & 1] + key0 * X::ROW;
-                if (AGAIN && pf_odd<X, 64 / KW>(kt, vt, ((X::BYTES ? t8.nan : bad) | far) >> (key0 >> 4))) {
+                if (AGAIN && pf_odd<X, V, 64 / KW>(kt, vt, (X::BYTES ? t8.nan : bad) >> (key0 >> 4))) {
                     if (!__all(pg_all_nan(o)))
                         pg_plain<typename X::Cells, T, HD, 2>(
                             c, table, head, q + (size_t)row * ldq + (size_t)qh * HD, scale, limit, jw,
                             min(jw + 32 * NA, last + 1), [](float x) { return X::base_of(x); },
-                            far ? P8_FAR - X::SHIFT : 0.0f, h == 0, [&](int i) { return 8 * i + 4 * h; },
+                            DOWN, h == 0, [&](int i) { return 8 * i + 4 * h; },
                             [&](int i, int e, float f, float p, float v) {
-                                if (RELATIVE) v = __builtin_amdgcn_ldexpf(v, P8_ONE - unit);
                                 o[i / 4][4 * (i % 4) + e] = fmaf(p, v, o[i / 4][4 * (i % 4) + e] * f);
                             },
                             base, l);
@@ -546,9 +553,10 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 }
                 peak = fmaxf(peak, top);
                 const float low = X::F16 ? fmaxf(top, peak - PG_DROP) : 0.0f;
-                const bool drop = X::F16 && low < base + (X::SHIFT - PF_LOW);
+                const bool drop = X::F16 && !VALUES && low < base + (X::SHIFT - PF_LOW);
                 if (__any(top - base > X::TOP || drop)) {
-                    const float to = drop ? X::base_of(low) : fmaxf(base, X::base_of(top));
+                    float to = X::base_of(drop ? low : top);
+                    if (!drop) to = fmaxf(base, to);
                     const float f = __builtin_amdgcn_exp2f(base - to);  // (0 or 1 where nothing was seen before)
                     base = to;
                     l *= f;
@@ -561,7 +569,7 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                 for (int a = 0; a < NA; a++)
 #pragma unroll
                     for (int i = 0; i < 16; i++)
-                        st[a][i] = AGAIN ? st[a][i] * fac[2 * a + (i >> 3)] - base
+                        st[a][i] = AGAIN ? st[a][i] * fac[2 * a + (i >> 3)] - base + DOWN
                                          : fmaf(st[a][i], fac[2 * a + (i >> 3)], -base);
                 if (mask) {  // (again: a factor of 0 would make NaN of -inf)
 #pragma unroll
@@ -570,18 +578,18 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                         for (int i = 0; i < 16; i++)
                             if (jw + 32 * a + (i & 3) + 8 * (i >> 2) + 4 * h > limit) st[a][i] = -__builtin_inff();
                 }
-                v8 pp[X::NP][2 * NA];
+                v8v pp[NW][2 * NA];
 #pragma unroll
                 for (int a = 0; a < NA; a++)
 #pragma unroll
                     for (int i = 0; i < 16; i += 2) {
                         typedef float f2 __attribute__((ext_vector_type(2)));
-                        using v2 = typename PgElem<E>::v2;
+                        using v2 = typename PgElem<V>::v2;
                         f2 rest{__builtin_amdgcn_exp2f(st[a][i]), __builtin_amdgcn_exp2f(st[a][i + 1])};
                         l += rest[0];
                         l += rest[1];
 #pragma unroll
-                        for (int p = 0; p < X::NP; p++) {
+                        for (int p = 0; p < NW; p++) {
                             const v2 h = __builtin_convertvector(rest, v2);
                             pp[p][2 * a + (i >> 3)][i & 7] = h[0];
                             pp[p][2 * a + (i >> 3)][(i & 7) + 1] = h[1];
@@ -595,30 +603,31 @@ __global__ __launch_bounds__(64 * PF_WAVES, 2) void paged_prefill_kernel(typenam
                     for (int d = 0; d < X::DT; d++) {
                         const uint8_t* at = vt + 16 * k * X::ROW + (vbase ^ (64 * d));
                         const pf_s4 lo = pf_read_tr(at), hi = pf_read_tr(at + 8 * X::ROW);
-                        const v8 vf = __builtin_bit_cast(v8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+                        const v8v vf = __builtin_bit_cast(v8v, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 #pragma unroll
-                        for (int p = X::NP - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
+                        for (int p = NW - 1; p >= 0; p--) o[d] = pf_mfma(vf, pp[p][k], o[d]);
                     }
             }
         };
-        walk(std::false_type{}, 0);
+        walk(std::false_type{});
         // Infinite or NaN sums: the same keys once more, tiles that hold such values
         // one key after another.  A prompt of 16384: 2.2 ms, with one infinite value 7.7,
         // all NaN 7.2, with one infinite value in every 16 keys, the worst there is, 205.
-        // Values whose scales lie so far apart that not all were exact: all keys one after
-        // another.  (A row may see none of the large ones, or give them no weight.)  322 and
-        // 451 rows of f32 that see 4628 and 6620 keys 0.22 ms, so 6.9; 4000 of f16 0.2, so 14.
-        uint32_t far = 0;  // all groups of a tile
-        if constexpr (RELATIVE) far = t0 < tiles && raw.top - least > P8_SPREAD ? 15 : 0;
-        const bool odd = __builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)));  // (the last tile is read)
-        if (far || odd) {
-            first_tile();
-            walk(std::true_type{}, far);
+        // Values whose scales lie so far apart that not all were exact as f16 (a row may see
+        // none of the large ones, or give them no weight): once more as well, with V as bf16
+        // values, exact of any scale, and weights in parts of bf16, three for f32 rows, two
+        // for f16.  322 and 451 rows of f32 that see 4628 and 6620 keys 0.21 ms, so 0.46; 4000
+        // of f16, 32 heads over 8, 0.19, so 0.58; 512 after 8000 0.13, so 0.34.
+        bool twice = __builtin_amdgcn_readfirstlane(__syncthreads_or(pg_odd(o)));  // (the last tile is read)
+        if constexpr (RELATIVE) twice = twice || (t0 < tiles && raw.top - least > P8_SPREAD);
+        if (twice) {
+            first_tile(std::true_type{});
+            walk(std::true_type{});
         }
         l += pf_other_half(l);
         if constexpr (RELATIVE) {  // o as values, normalized
             const int ex = pg_exponent(l);
-            if (far) l = __builtin_amdgcn_ldexpf(l, (int)(X::SHIFT - P8_FAR));
+            if (twice) l = __builtin_amdgcn_ldexpf(l, (int)-P8_DOWN);
 #pragma unroll
             for (int d = 0; d < X::DT; d++)
 #pragma unroll

@@ -458,8 +458,9 @@ int frq_paged8_append(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_
  * 2^-22 with f32 rows, to 2^-16 with others; in batches of many rows, as the sizes of
  * the structs have it, with f16 rows to 2^-11 and with bf16 rows to 2^-8, and with f32
  * and f16 rows to 2^-33 of the row's largest, if that is more (their sum is not
- * rounded).  Such a batch of f32 or f16 rows takes 30 to 70 times as long where the
- * scales of a sequence's values, but for 2^-127, differ by more than 2^22.  NaN as
+ * rounded).  Such a batch of f32 or f16 rows walks its keys twice, and takes two to three
+ * times as long, where the scales of a sequence's values, but for 2^-127, differ by more
+ * than 2^22; a weight is held to 2^-22 with f32 rows then, to 2^-16 with f16.  NaN as
  * frq_paged_batch has it; a code times its scale past f32's range is infinite. */
 size_t frq_paged8_attention_workspace(const frq_paged_kv8 *kv, const frq_paged_batch *batch, size_t n_heads);
 int frq_paged8_attention_decode(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype,
