@@ -69,7 +69,9 @@ __device__ __forceinline__ bool p8_word_nan(uint32_t w) {
 
 // 64 groups of 16 keys, lane i the one at position j0 + 16 i: where its rows are in
 // the pools, its scales, and which groups' page is none (those and the ones behind
-// the sequence's end lead to page 0).
+// the sequence's end lead to page 0).  Keys whose codes may stand for more than f32
+// holds have a NaN scale here: products with their codes do not make infinities of
+// them, and what is NaN is taken key by key, as it is.
 struct P8Groups {
     uint32_t off_lo, off_hi;
     int k_scale, v_scale;
@@ -83,6 +85,7 @@ struct P8Groups {
         none = __ballot(off);
         const size_t row = ((page * c.kv_heads + head) << c.log_ps) + in;
         k_scale = c.k_scale[row >> 4];
+        if (k_scale > P8_TOP) k_scale = 255;
         v_scale = c.v_scale[row >> 4];
         off_lo = (uint32_t)(row * HD);
         off_hi = (uint32_t)(row * HD >> 32);

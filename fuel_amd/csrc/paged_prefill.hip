@@ -154,7 +154,7 @@ __device__ __forceinline__ bool pf_odd(const uint8_t* kt, const uint8_t* vt, uin
 // of k's NK groups from k0 on, KSTEP apart, and of v's NV groups from v0 on, VSTEP apart
 // (2^0 for groups without keys, so that what is cleared stays 0), which groups' page is none,
 // which have a page that is none or a NaN scale of k (their keys are NaN), and the
-// largest scale byte of v up to this tile.
+// largest scale byte of v up to this tile, but for those above P8_TOP.
 template <int NK, int KSTEP, int NV, int VSTEP>
 struct Tile8 {
     int k[NK], v[NV];
@@ -170,16 +170,16 @@ struct Tile8 {
         for (int a = 0; a < NK; a++) t.k[a] = __builtin_amdgcn_readlane(ks, g0 + k0 + KSTEP * a);
 #pragma unroll
         for (int a = 0; a < NV; a++) t.v[a] = __builtin_amdgcn_readlane(vs, g0 + v0 + VSTEP * a);
-        const int most = keys && vs < 255 ? vs : 0;
+        const int most = keys && vs <= P8_TOP ? vs : 0;
 #pragma unroll
         for (int a = 0; a < 4; a++) t.top = max(t.top, __builtin_amdgcn_readlane(most, g0 + a));
         return t;
     }
     // The byte of the scale that values of f16 are in units of, and the operand that
-    // makes them of group a's codes.
+    // makes them of group a's codes (NaN of those that may stand for more than f32 holds).
     __device__ __forceinline__ int unit() const { return top - P8_UP; }
     __device__ __forceinline__ float v_relative(int a) const {
-        return p8_operand(v[a] == 255 ? 255 : max(v[a] - unit() + P8_ONE, 0));
+        return p8_operand(v[a] > P8_TOP ? 255 : max(v[a] - unit() + P8_ONE, 0));
     }
 };
 

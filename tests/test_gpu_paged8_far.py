@@ -1,5 +1,6 @@
-"""8-bit paged attention of values whose scales lie far apart: what rows of every type
-keep of them, and what such a batch costs beside one of scales that are alike."""
+"""8-bit paged attention of values whose scales lie far apart, and of codes that stand for
+more than f32 holds: what rows of every type make of them, and what such a batch costs
+beside one of scales that are alike."""
 import time
 
 import numpy as np
@@ -88,3 +89,111 @@ def test_scales_far_apart_cost_a_second_walk(dev, act, H, hk, past, new):
         times.append(best / 4)
     say("   us", [round(1e6 * t, 1) for t in times])
     assert times[1] < 6 * times[0]
+
+
+BIG = float(np.finfo(np.float32).max)
+# (position from the end, scale byte, code, dim): infinite from 2^128 on
+PAST = [(5, 254, 0x7e, 3), (5, 254, 0x01, 4), (40, 247, 0x78, 5), (40, 247, 0x77, 6), (41, 247, 0xf8, 7), (70, 250, 0xfe, 8),
+        (70, 250, 0x58, 9), (71, 250, 0x3f, 10), (100, 246, 0x7e, 11), (5, 254, 0xb1, 12), (41, 247, 0xf8, 3)]
+
+
+def plant(c, s, w):
+    """PAST in k (0) or v (1) of sequence s, their blocks zeros beside them."""
+    n, done = int(c.kv[s]), set()
+    for back, b, code, d in PAST:
+        j = n - back
+        if j < 0:
+            continue
+        page, i = c.pool.table[s, j // 16], j % 16
+        if j // 16 not in done:
+            c.pool.code[w, page] = 0
+            c.pool.scale[w, page] = b
+            done.add(j // 16)
+        if c.pool.scale[w, page, 0, 0] == b:
+            c.pool.code[w, page, :, i, d] = code
+
+
+def in_f32(x):
+    return np.where(np.abs(x) > BIG, np.sign(x) * np.inf, x)
+
+
+@pytest.mark.parametrize("act", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", KINDS + [(4, 2, 128, [599, 2300], [1, 1]), (4, 2, 64, [599, 80], [1, 1])])
+@pytest.mark.parametrize("power", [0, 118])
+def test_values_past_f32(dev, act, H, hk, D, past, new, power):
+    """Infinite where a code times its scale is, for the rows that see it, beside values of
+    2^power."""
+    say("values past f32", act, H, D, past, power)
+    rng = seed(62, act, H, D)
+    c = Case(dev, rng, act, H, hk, D, 16, past, new, decode=new == [1, 1], fill=False)
+    for s, n in enumerate(c.kv):
+        k, v = rng.standard_normal((2, n, hk, D)).astype(np.float32)
+        c.pool.append(s, 0, k, v * np.float32(2.0 ** power))
+        plant(c, s, 1)
+    c.upload()
+    c.run()
+    for s, n in enumerate(new):
+        r0, kv = int(c.start[s]), int(c.kv[s])
+        k, v = c.pool.get(s, kv)
+        v = in_f32(v)
+        pos = kv - n + np.arange(n)
+        q = R.from_bits(R.to_bits(c.q, act), act)[r0:r0 + n, :H * D].reshape(n, H, D)
+        inf = np.isinf(v)
+        want, A, B, _ = R.attend(q, k, np.where(inf, 0, v), pos, c.scale)
+        V = np.maximum.accumulate(np.abs(np.where(inf, 0, v)).max((1, 2)))[pos][:, None, None]
+        tol = P.bound(want, A, B, V, kv, D, act, not c.decode)
+        with np.errstate(invalid="ignore"):
+            for j, g, d in np.argwhere(inf):
+                want[pos >= j, g * H // hk:(g + 1) * H // hk, d] += v[j, g, d]
+        got = c.got()[r0:r0 + n, :H * D].reshape(want.shape)
+        most = 65520.0 if act == F16 else BIG
+        with np.errstate(invalid="ignore"):
+            past_it = np.abs(want) - tol > most  # (f16 holds no more; infinities)
+            near = ~past_it & (np.abs(want) + tol > most)
+        np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
+        np.testing.assert_array_equal(got[past_it], np.where(want[past_it] > 0, np.inf, -np.inf))
+        fine = ~past_it & ~near & ~np.isnan(want)
+        bad = np.argwhere(fine & ~(np.abs(got - want) <= tol))
+        assert not len(bad), (s, bad[:3], len(bad))
+
+
+@pytest.mark.parametrize("act", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", KINDS + [(4, 2, 128, [599, 2300], [1, 1]), (4, 2, 64, [599, 80], [1, 1])])
+def test_keys_past_f32(dev, act, H, hk, D, past, new):
+    """Infinite keys: no weight where q is below zero in their infinite dim, NaN for rows that see
+    one and are above zero or zero there."""
+    say("keys past f32", act, H, D, past)
+    rng = seed(63, act, H, D)
+    c = Case(dev, rng, act, H, hk, D, 16, past, new, decode=new == [1, 1])
+    c.q = c.q.reshape(c.rows, H, D)
+    sign = np.where(np.arange(H) % 3 < 2, -1.0, np.where(np.arange(H) % 2, 0.0, 1.0)).astype(np.float32)
+    c.q[:, :, 3:13] = sign[:, None] * (np.abs(c.q[:, :, 3:13]) + 0.25)
+    c.q = c.q.reshape(c.rows, H * D)
+    ats = [(5, 3, 0x7e), (40, 5, 0x78), (70, 8, 0x7e)]  # each an infinity above zero
+    for s in range(len(new)):
+        for back, d, code in ats:
+            j = int(c.kv[s]) - back
+            if j < 0:
+                continue
+            page, i = c.pool.table[s, j // 16], j % 16
+            c.pool.code[0, page] = 0
+            c.pool.scale[0, page] = 254 if back == 5 else 247 if back == 40 else 251
+            c.pool.code[0, page, :, i, d] = code
+    c.upload()
+    c.run()
+    for s, n in enumerate(new):
+        r0, kv = int(c.start[s]), int(c.kv[s])
+        k, v = c.pool.get(s, kv)
+        inf = (np.abs(k) > BIG).any((1, 2))
+        left = np.flatnonzero(~inf)
+        pos = kv - n + np.arange(n)
+        q = R.from_bits(R.to_bits(c.q, act), act)[r0:r0 + n].reshape(n, H, D)
+        at = np.searchsorted(left, pos, side="right") - 1  # the last of those left that a row sees
+        want, A, B, V = R.attend(q, k[left], v[left], at, c.scale)
+        tol = P.bound(want, A, B, V, kv, D, act, not c.decode)
+        sees = (np.flatnonzero(inf)[None] <= pos[:, None]).any(1)
+        got = c.got()[r0:r0 + n].reshape(want.shape)
+        nan = sees[:, None] & ((sign >= 0)[None] | (at < 0)[:, None])  # (scores of -inf alone: 0 / 0)
+        np.testing.assert_array_equal(np.isnan(got).all(2), nan)
+        bad = np.argwhere(~nan[..., None] & ~(np.abs(got - want) <= tol))
+        assert not len(bad), (s, bad[:3], len(bad))
