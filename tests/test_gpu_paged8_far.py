@@ -40,10 +40,10 @@ def check(c, s, most=np.inf):
 
 @pytest.mark.parametrize("act", TYPES)
 @pytest.mark.parametrize("H,hk,D,past,new", KINDS + [(4, 2, 128, [599, 2300], [1, 1]), (4, 2, 64, [599, 80], [1, 1])])
-@pytest.mark.parametrize("low,high", [(-60, 12), (-20, 5), (-8, 60)])
+@pytest.mark.parametrize("low,high", [(-60, 12), (-20, 5), (-8, 60), (110, 120), (-80, -60)])
 def test_values_far_apart(dev, act, H, hk, D, past, new, low, high):
     """Every block of values 2^low .. 2^high in size, some of zeros: within f16's range, within
-    what f16 holds of the largest, and past f16's range."""
+    what f16 holds of the largest, past f16's range, near f32's end, below f16's least."""
     say("values far apart", act, H, D, past, low, high)
     rng = seed(60, act, H, D, low + 100)
     c = Case(dev, rng, act, H, hk, D, 16, past, new, fill=False, decode=new == [1, 1])
