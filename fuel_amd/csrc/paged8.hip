@@ -477,13 +477,14 @@ struct Append8Row {
 
 // Workgroups below q_wgs: `parts` to a packed row, chunks of its q as paged_append_kernel
 // takes them.  The others: a wavefront takes 16 rows of codes, four lanes a row,
-//   NARROW      the same position of up to 16 heads of k and v: a row a wavefront, the
-//               first of a block's rows works all of them, one after another
+//   NARROW      the same position of up to 16 heads of k and v, a row a wavefront: up to
+//               A8_FEW new rows in a block are worked by the first one's, one after another,
+//               the heads of more by all of them, each head's rows as below
 //   otherwise   the up to 16 rows of a block, of one head of k or v
 // Bound by HBM for many rows (11166 of f32, 32 heads over 8 of 128: 482 MB in 99 us,
 // 4.9 TB/s, as a copy), by four memory round trips for few: the row's sequence (two),
 // its page, its block's scale.
-constexpr int A8_WG = 256;
+constexpr int A8_WG = 256, A8_FEW = 4, A8_SHORT = 3;
 template <class T, int HD, bool NARROW>
 __global__ __launch_bounds__(A8_WG) void paged8_append_kernel(PagedKv8 c, PagedRows b, int n_heads, int q_wgs, int parts,
                                                               const T* q, int ldq, const T* __restrict__ k, int ldk,
@@ -545,30 +546,100 @@ __global__ __launch_bounds__(A8_WG) void paged8_append_kernel(PagedKv8 c, PagedR
         first = max(x.kv - x.n, 0);
         return x.n && !x.bad ? max(first, cs ? min(x.kv, rope_rows) : x.kv) : first;
     };
-    int s, head, lo, hi;  // sequence, head, and the block's positions [lo, hi) that are new
-    bool value, mine;
+    int s, lo, hi;  // sequence, and the block's positions [lo, hi) that are new
     PgSeq sq;
-    R x;
-    const auto row_of = [&](int pos) {
+    const auto row_of = [&](int pos, int head, bool value) {
         return (value ? v : k) + (size_t)(sq.row0 + pos - (sq.kv - sq.n)) * (value ? ldv : ldk) + head * HD + i;
     };
+    const auto turn = [&](R& x, int pos, bool value) {
+        const bool t = cs && !value;
+        x.turn(t ? cs + (size_t)pos * HD + i : nullptr, sn + (t ? (size_t)pos * HD + i : 0));
+    };
+    // the block's first cache row of a head, from page 0's
+    size_t row = 0;
+    const auto find = [&] {
+        bool none;
+        const int j0 = lo & ~15, page = pg_page(c, b.table + (size_t)s * b.max_pages, j0, sq.kv, none);
+        row = ((size_t)page * c.kv_heads << c.log_ps) + (j0 & ((1 << c.log_ps) - 1));
+        return !none;
+    };
+    // the scale that rows of at most amax and older ones under `was` get
+    const auto scale_of = [&](float amax, int was) {
+        const int byte = p8_scale_of(amax);
+        return lo & 15 && was != 255 ? max(was, byte) : byte;
+    };
+    // The block's rows of one head of k or v, four lanes a row.
+    const auto by_rows = [&](int head, bool value) {
+        const int j0 = lo & ~15, pos = j0 + sub;
+        const bool mine = pos >= lo && pos < hi;
+        const size_t at = row + ((size_t)head << c.log_ps);
+        uint8_t* codes = static_cast<uint8_t*>(value ? c.v : c.k) + at * HD + i;
+        uint8_t* scale = (value ? c.v_scale : c.k_scale) + (at >> 4);
+        R x;
+        x.load(row_of(mine ? pos : lo, head, value));
+        const int was = lo > j0 ? *scale : 0;
+        turn(x, mine ? pos : lo, value);
+        float amax = x.most();  // (of the other lanes: lo's)
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
+        const int byte = scale_of(amax, was);
+        if (sub < lo - j0 && byte != was) R::again(codes + sub * HD, was, byte);
+        if (mine) x.put(codes + sub * HD, byte);
+        if (lane == 0) *scale = (uint8_t)byte;
+    };
     if constexpr (NARROW) {
-        const int waves = (2 * c.kv_heads + 15) >> 4, row = (unsigned)at / (unsigned)waves;
-        if (row >= b.rows) return;
-        const int unit = 16 * (at - row * waves) + sub;
-        mine = unit < 2 * c.kv_heads;
-        value = unit >= c.kv_heads;
-        head = mine ? unit - (value ? c.kv_heads : 0) : 0;
-        x.load((value ? v : k) + (size_t)row * (value ? ldv : ldk) + head * HD + i);  // (most often the only row)
-        s = pg_row_seq(b, row);
+        const int waves = (2 * c.kv_heads + 15) >> 4, packed = (unsigned)at / (unsigned)waves;
+        if (packed >= b.rows) return;
+        const int unit0 = 16 * (at - packed * waves), unit = unit0 + sub;
+        const bool mine = unit < 2 * c.kv_heads, value = unit >= c.kv_heads;
+        const int head = mine ? unit - (value ? c.kv_heads : 0) : 0;
+        R x;
+        x.load((value ? v : k) + (size_t)packed * (value ? ldv : ldk) + head * HD + i);  // (most often the only row)
+        s = pg_row_seq(b, packed);
         if (s < 0) return;
         sq = pg_seq(b, s);
-        if (row < sq.row0 || row >= sq.row0 + sq.n) return;
-        lo = sq.kv - sq.n + (row - sq.row0);
+        if (packed < sq.row0 || packed >= sq.row0 + sq.n) return;
+        const int pos = sq.kv - sq.n + (packed - sq.row0);
         int first;
         const int end = ends(sq, first);
-        if (lo < first || lo >= end || (lo > first && (lo & 15))) return;
-        hi = min((lo | 15) + 1, end);
+        if (pos < first || pos >= end) return;
+        lo = max(pos & ~15, first);
+        hi = min((pos | 15) + 1, end);
+        if (hi - lo > A8_FEW) {
+            // (row_start may decrease: rows of the block that are found in other sequences do no part)
+            if (pg_row_seq(b, packed - (pos - lo)) != s) return;
+            const bool all = pg_row_seq(b, packed + (hi - 1 - pos)) == s;
+            if ((!all && pos != lo) || !find()) return;
+            for (int u = unit0 + (all ? pos - lo : 0); u < min(unit0 + 16, 2 * c.kv_heads); u += all ? hi - lo : 1)
+                by_rows(u < c.kv_heads ? u : u - c.kv_heads, u >= c.kv_heads);
+            return;
+        }
+        if (pos != lo || !find()) return;
+        const int j0 = lo & ~15;
+        const size_t at0 = row + ((size_t)head << c.log_ps);
+        uint8_t* codes = static_cast<uint8_t*>(value ? c.v : c.k) + at0 * HD + i;
+        uint8_t* scale = (value ? c.v_scale : c.k_scale) + (at0 >> 4);
+        const int was = lo > j0 ? *scale : 0;
+        turn(x, lo, value);
+        float amax = x.most();
+        for (int p = lo + 1; p < hi; p++) {
+            x.load(row_of(p, head, value));
+            turn(x, p, value);
+            amax = fmaxf(amax, x.most());
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 1));
+        amax = fmaxf(amax, __shfl_xor(amax, 2));
+        if (!mine) return;
+        const int byte = scale_of(amax, was);
+        if (byte != was)
+            for (int r = 0; r < lo - j0; r++) R::again(codes + r * HD, was, byte);
+        for (int p = hi - 1;; p--) {  // (the last one's is at hand)
+            x.put(codes + (p - j0) * HD, byte);
+            if (p == lo) break;
+            x.load(row_of(p - 1, head, value));
+            turn(x, p - 1, value);
+        }
+        if ((lane & 3) == 0) *scale = (uint8_t)byte;
     } else {
         const auto blocks = [&](const PgSeq& x) {
             int first;
@@ -576,69 +647,23 @@ __global__ __launch_bounds__(A8_WG) void paged8_append_kernel(PagedKv8 c, PagedR
             return end > first ? ((end - 1) >> 4) - (first >> 4) + 1 : 0;
         };
         PgUnits<decltype(blocks)> pu(b, blocks);
-        const int unit = (unsigned)at / (unsigned)(2 * c.kv_heads);
+        const int unit = (unsigned)at / (unsigned)(2 * c.kv_heads), of = at - unit * 2 * c.kv_heads;
         if (unit >= pu.total) return;
         int u, first;
         s = pu.find(unit, u);
         sq = pu.get(s);
-        value = (at - unit * 2 * c.kv_heads) & 1;
-        head = (at - unit * 2 * c.kv_heads) >> 1;
         const int end = ends(sq, first), j = ((first >> 4) + u) << 4;
         lo = max(j, first);
         hi = min(j + 16, end);
-        mine = j + sub >= lo && j + sub < hi;
-        x.load(row_of(mine ? j + sub : lo));
+        if (find()) by_rows(of >> 1, of & 1);
     }
-    const int j0 = lo & ~15;
-    bool none;
-    const int page = pg_page(c, b.table + (size_t)s * b.max_pages, j0, sq.kv, none);
-    if (none) return;
-    const size_t row = (((size_t)page * c.kv_heads + head) << c.log_ps) + (j0 & ((1 << c.log_ps) - 1));
-    uint8_t* codes = static_cast<uint8_t*>(value ? c.v : c.k) + row * HD + i;
-    uint8_t* scale = (value ? c.v_scale : c.k_scale) + (row >> 4);
-    const int was = lo > j0 ? *scale : 0;
-    const auto turn = [&](int pos) {
-        const bool t = cs && !value;
-        x.turn(t ? cs + (size_t)pos * HD + i : nullptr, sn + (t ? (size_t)pos * HD + i : 0));
-    };
-    float amax = 0.0f;
-    if constexpr (NARROW) {
-        turn(lo);
-        amax = x.most();
-        for (int pos = lo + 1; pos < hi; pos++) {
-            x.load(row_of(pos));
-            turn(pos);
-            amax = fmaxf(amax, x.most());
-        }
-    } else {
-        turn(mine ? j0 + sub : lo);
-        amax = x.most();  // (of the other lanes: lo's)
-    }
-#pragma unroll
-    for (int d = 1; d < (NARROW ? 4 : 64); d *= 2) amax = fmaxf(amax, __shfl_xor(amax, d));
-    if (NARROW && !mine) return;
-    int byte = p8_scale_of(amax);
-    if (lo > j0) {  // older rows
-        byte = was == 255 ? byte : max(was, byte);
-        if (byte != was)
-            for (int r = NARROW ? 0 : sub; r < lo - j0; r += NARROW ? 1 : 16) R::again(codes + r * HD, was, byte);
-    }
-    if constexpr (NARROW) {
-        for (int pos = hi - 1;; pos--) {  // (the last one's is at hand)
-            x.put(codes + (pos - j0) * HD, byte);
-            if (pos == lo) break;
-            x.load(row_of(pos - 1));
-            turn(pos - 1);
-        }
-    } else if (mine) {
-        x.put(codes + sub * HD, byte);
-    }
-    if (NARROW ? (lane & 3) == 0 : lane == 0) *scale = (uint8_t)byte;
 }
 
-// Few rows a sequence: NARROW (256 sequences of one row each, 8 KV heads: 5.7 us, 9.4
-// otherwise; a block's rows one after another, up to 16, take it longer then).
-inline bool append8_narrow(const PagedRows& r) { return !r.row_start || r.rows <= 2l * r.n_seqs; }
+// Few rows a sequence: NARROW.  us, NARROW / otherwise, 32 KV heads of 128, bf16 rows: 256
+// sequences of one row 7.7 / 28, of three 13 / 29, 1024 of three 30 / 397, one of 256 beside
+// 255 of one 10 / 29 (27 where all of a block's rows are worked by the first one's
+// wavefront); but 64 of four 9.6 / 7.5, one of 500 11 / 7.5.
+inline bool append8_narrow(const PagedRows& r) { return !r.row_start || r.rows <= (long)A8_SHORT * r.n_seqs; }
 
 struct Append8Call {
     const PagedAppendArgs& p;
