@@ -6,7 +6,8 @@
 //   2^e, the least for which its largest |value| is at most 448 * 2^e
 // (e from -127 to 120).  Rows that join older ones in their block take the block's
 // scale, or raise it: then the older codes are rounded once more, exactly but for
-// those that fall below the least normal number, 2^-14.8 of the block's largest.
+// those that fall below the least normal number, 2^-6 in units of the new scale: 2^-13.8
+// of the block's largest, which is above 224 of them.
 //
 // Attention: as paged.hip's 16-row tiles, 32 keys at a time.  K's codes go to the
 // matrix pipe as f16 (bf16 for bf16 rows) without their scale, exactly; a group of

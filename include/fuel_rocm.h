@@ -438,9 +438,9 @@ typedef struct frq_paged_kv8 {
  * rows of a head that lie in one block of 16 positions get the least scale, 2^-127 to
  * 2^120, under which their largest finite magnitude is at most 448, or the block's
  * present one, if older rows are in the block and theirs is larger; each value the
- * nearest code (ties to even).  Where the scale grows the older rows' codes are
- * rounded to it once more (exactly, but for values below 2^-14 of the block's
- * largest).  Infinite and NaN values become NaN codes and take no part in the scale;
+ * nearest code (ties to even; under 2^120 one of at most 240, whose value f32 holds).
+ * Where the scale grows the older rows' codes are rounded to it once more (exactly, but
+ * for values below 2^-6 times the new scale, 2^-13.8 of the block's largest).  Infinite and NaN values become NaN codes and take no part in the scale;
  * older rows under a NaN scale become NaN.  Positions of the block behind the
  * appended rows are no part of the cache any more: a sequence whose end was moved
  * back may be appended to, its later rows are not kept.  Two rows must not lie in the
