@@ -440,10 +440,11 @@ typedef struct frq_paged_kv8 {
  * present one, if older rows are in the block and theirs is larger; each value the
  * nearest code (ties to even; under 2^120 one of at most 240, whose value f32 holds).
  * Where the scale grows the older rows' codes are rounded to it once more (exactly, but
- * for values below 2^-6 times the new scale, 2^-13.8 of the block's largest).  Infinite and NaN values become NaN codes and take no part in the scale;
- * older rows under a NaN scale become NaN.  Positions of the block behind the
- * appended rows are no part of the cache any more: a sequence whose end was moved
- * back may be appended to, its later rows are not kept.  Two rows must not lie in the
+ * for values below 2^-6 times the new scale, 2^-13.8 of the block's largest).
+ * Infinite and NaN values become NaN codes and take no part in the scale; older rows
+ * under a NaN scale become NaN.  Positions of the block behind the appended rows are no
+ * part of the cache any more: a sequence whose end was moved back may be appended to,
+ * its later rows are not kept.  Two rows must not lie in the
  * same block of a page but those of one sequence; which rows of k and v a batch
  * appends whose sequences have more than `rows` rows together is not defined. */
 int frq_paged8_append(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype, size_t n_heads,
@@ -460,8 +461,10 @@ int frq_paged8_append(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_
  * and f16 rows to 2^-33 of the row's largest, if that is more (their sum is not
  * rounded).  Such a batch of f32 or f16 rows walks its keys twice, and takes two to three
  * times as long, where the scales of a sequence's values, but for 2^-127, differ by more
- * than 2^22; a weight is held to 2^-22 with f32 rows then, to 2^-16 with f16.  NaN as
- * frq_paged_batch has it; a code times its scale past f32's range is infinite. */
+ * than 2^22; a weight is held to 2^-22 with f32 rows then, to 2^-16 with f16.  Weights are
+ * taken so small that sums of f32's largest values stay finite: a value's part in a
+ * result is held to 2^-111, also where it is less.  NaN as frq_paged_batch has it; a
+ * code times its scale past f32's range is infinite. */
 size_t frq_paged8_attention_workspace(const frq_paged_kv8 *kv, const frq_paged_batch *batch, size_t n_heads);
 int frq_paged8_attention_decode(frq_device *dev, const frq_paged_kv8 *kv, const frq_paged_batch *batch, int dtype,
                                 size_t n_heads, const void *q_dev, size_t ldq, float scale, void *work_dev,

@@ -197,3 +197,27 @@ def test_keys_past_f32(dev, act, H, hk, D, past, new):
         np.testing.assert_array_equal(np.isnan(got).all(2), nan)
         bad = np.argwhere(~nan[..., None] & ~(np.abs(got - want) <= tol))
         assert not len(bad), (s, bad[:3], len(bad))
+
+
+@pytest.mark.parametrize("act", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", KINDS + [(4, 2, 128, [599, 2300], [1, 1])])
+def test_values_of_2_to_the_minus_100(dev, act, H, hk, D, past, new):
+    """Weights are 2^-31 at most where V is taken as values, 2^-38 or more of a row's largest: each
+    product may lose a step of f32's least, 2^-149, which is 2^-111 of the result."""
+    say("tiny values", act, H, D, past)
+    rng = seed(64, act, H, D)
+    c = Case(dev, rng, act, H, hk, D, 16, past, new, decode=new == [1, 1], fill=False)
+    for s, n in enumerate(c.kv):
+        k, v = rng.standard_normal((2, n, hk, D)).astype(np.float32)
+        c.pool.append(s, 0, k, v * np.float32(2.0 ** -100))
+    c.upload()
+    c.run()
+    for s, n in enumerate(new):
+        r0, kv = int(c.start[s]), int(c.kv[s])
+        k, v = c.pool.get(s, kv)
+        pos = kv - n + np.arange(n)
+        q = R.from_bits(R.to_bits(c.q, act), act)[r0:r0 + n, :H * D].reshape(n, H, D)
+        want, A, B, V = R.attend(q, k, v, pos, c.scale)
+        tol = P.bound(want, A, B, V, kv, D, act, not c.decode) + kv * 2.0 ** -111
+        got = c.got()[r0:r0 + n, :H * D].reshape(want.shape)
+        assert (np.abs(got - want) <= tol).all()
