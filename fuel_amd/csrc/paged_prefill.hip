@@ -21,9 +21,9 @@
 // keys, N(0, 1), differ by less.
 // 16-bit activations: p is rounded to the cache's type for the second product
 // (a relative 2^-11 or 2^-8 of each weight at most, the output's own rounding;
-// the sum l takes p as it is), over an 8-bit cache to the rows' type.  A second part, as the 16-row kernel keeps, costs
-// half as many matrix instructions again, which are the bound here: a prompt of
-// 16384 2.78 ms instead of 2.04, 17 ragged ones 0.196 instead of 0.159, for an
+// the sum l takes p as it is), over an 8-bit cache to the rows' type.  A second part,
+// as the 16-row kernel keeps, costs half as many matrix instructions again, which are
+// the bound here: a prompt of 16384 2.78 ms instead of 2.04, 17 ragged ones 0.196 instead of 0.159, for an
 // output 0.0015 of it from 64 bits instead of 0.0020 (bf16; f16 0.0002, 0.0003).
 // f32 activations: q and p in parts that keep f32's precision.
 // One prompt of 16384, 32 heads over 8 of 128, bf16: 2.0 ms, 1.10 PFLOP/s, where a
@@ -47,7 +47,9 @@
 // One prompt of 12345, 32 heads over 8 of 128, bf16: 1.23 - 1.27 ms, 1.0 PFLOP/s (beside
 // a 16-bit cache's kernel, 24 % more VALU instructions and bank conflicts of a tenth of
 // its time, as the decoded rows are written); 15 of 66 .. 1562, f16, 0.16 ms, 0.61
-// PFLOP/s; 322 and 451 rows of 32 KV heads that see 4628 and 6620 keys, f32, 0.218 ms.
+// PFLOP/s; 322 and 451 rows of 32 KV heads that see 6620 and 4628 keys, f32, 0.217 ms.
+// In equal ranges (CUT), 512 rows after 8000, f32 0.20, f16 0.12, bf16 0.11 (f16 over 16
+// bits 0.10): there dims of 128 spill, 89, 57 and 46 registers.
 // No faster: decoding between the two products (spills), the sums of products apart in
 // more registers; a weight's first part by truncation 1 %.
 #include <hip/hip_runtime.h>
