@@ -127,7 +127,7 @@ struct PrefillTile {
     // m - SHIFT, since a weight of 2^16 is infinite there.
     __device__ static __forceinline__ float base_of(float m) {
         const float b = m - SHIFT;
-        return F16 && m - b > SHIFT ? fmaf(fabsf(m), 0x1p-23f, b) : b;
+        return F16 && m - b > SHIFT ? fmaf(fabsf(m), 0x1.8p-24f, b) : b;  // (a step up)
     }
     static constexpr int KS = HD / 16, DT = HD / 32;   // steps of S^T, dim tiles of O^T
     static constexpr int ROW = 2 * HD, TILE = PF_KEYS * ROW;

@@ -41,8 +41,8 @@ def case(dev, rng, act, cache, H, hk, D, past, new, decode):
 
 
 def means(c, s):
-    """The means of what each row of sequence s sees, their bounds, and the rows' results."""
-    n, r0, D = c.new[s], int(c.start[s]), c.D
+    """The means of what each row of sequence s sees, their bounds, and the rows' positions."""
+    n, D = c.new[s], c.D
     _, v = c.pool.get(s, int(c.kv[s]))
     pos = int(c.kv[s]) - n + np.arange(n)
     want, A, B, V = R.attend(np.zeros((n, c.H, D)), np.zeros_like(v), np.nan_to_num(v), pos, 1.0)
@@ -51,7 +51,7 @@ def means(c, s):
         tol = P.bound(want, A, B, V, keys, D, c.act, not c.decode)
     else:
         tol = R.bound(want, A, B, V, keys, D, c.act, c.cache, not c.decode)
-    return want, tol, c.got()[r0:r0 + n, :c.H * D].reshape(want.shape), v, pos
+    return want, tol, pos
 
 
 # decode cut; 16-row tiles whole; 128-row tiles
@@ -62,11 +62,13 @@ def test_equal_scores(dev, act, cache, H, hk, D, past, new):
     rng = seed(50, act, cache, H, D)
     c = case(dev, rng, act, cache, H, hk, D, past, new, new[0] == 1)
     c.upload()
+    exact = [means(c, s) for s in range(len(new))]
     for power in POWERS:
         say("equal scores", act, cache, H, D, past, power)
         c.run(2.0 ** (power - 24))
-        for s in range(len(new)):
-            want, tol, got, _, _ = means(c, s)
+        out = c.got()
+        for s, (want, tol, _) in enumerate(exact):
+            got = out[c.start[s]:c.start[s] + c.new[s], :H * D].reshape(want.shape)
             bad = np.argwhere(~(np.abs(got - want) <= tol))
             assert not len(bad), (power, s, bad[:3], got[tuple(bad[0])], want[tuple(bad[0])])
 
@@ -79,3 +81,34 @@ def test_equal_scores(dev, act, cache, H, hk, D, past, new):
 def test_equal_scores_in_pieces(dev, act, cache, H, hk, D, past, new):
     """Pieces of few and of many keys: each counts by its keys."""
     test_equal_scores(dev, act, cache, H, hk, D, past, new)
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("H,hk,D,past,new", [
+    (4, 2, 128, [60, 0], [9, 30]), (20, 20, 64, [0, 3] * 7, [130, 71] * 7), (20, 20, 64, [0, 70, 0], [330, 260, 130]),
+    (32, 2, 128, [2200, 2000, 0], [150, 100, 40])])
+def test_equal_scores_beside_nan(dev, act, cache, H, hk, D, past, new):
+    """A NaN in one dim of a value that the later half of a sequence's rows see: its tile's keys are
+    taken one after another, and weigh as those of the others do."""
+    rng = seed(51, act, cache, H, D)
+    c = case(dev, rng, act, cache, H, hk, D, past, new, False)
+    at = [int(k) - n // 2 for k, n in zip(c.kv, new)]
+    for s, j in enumerate(at):
+        page, i = c.pool.table[s, j // 16], j % 16
+        if cache == 8:
+            c.pool.code[1, page, :, i, 1] = P.NAN
+        else:
+            c.pool.v[page, :, i, 1] = R.NAN[cache]
+    c.upload()
+    exact = [means(c, s) for s in range(len(new))]
+    for power in POWERS:
+        say("equal scores beside NaN", act, cache, H, D, past, power)
+        c.run(2.0 ** (power - 24))
+        out = c.got()
+        for s, (want, tol, pos) in enumerate(exact):
+            got = out[c.start[s]:c.start[s] + c.new[s], :H * D].reshape(want.shape)
+            nan = np.zeros(want.shape, bool)
+            nan[pos >= at[s], :, 1] = True
+            np.testing.assert_array_equal(np.isnan(got), nan)
+            bad = np.argwhere(~nan & ~(np.abs(got - want) <= tol))
+            assert not len(bad), (power, s, bad[:3], got[tuple(bad[0])], want[tuple(bad[0])])
